@@ -115,6 +115,15 @@ SIGNATURES = {
     "bf_concretize_finalize": (I32, [P, P, I32, I64, P, P, P, P, F32, I32, P, P, P]),
     "bf_alpha_from_crown": (I32, [P, P, I64, P, P]),
     "bf_domain_status": (I32, [P, I64, I64, P, F32, F32, P, P]),
+    "bf_embed_rows": (I32, [P, I64, I64, P, I32, I64, I64, F32, I32, P, P]),
+    "bf_embed_grad_workspace": (I64, [I64, I64, I64]),
+    "bf_embed_grad": (I32, [P, I64, I32, P, I32, I64, I64, I64, F32, I32, I32, P, P, P]),
+    "bf_policy_loss_workspace": (I64, [I64, I64, I64, I32]),
+    "bf_policy_loss": (I32, [P, I32, I64, I64, I64, I64, I64, P, I32, P, P, P, I64, I64, P, F32, F32, F32, F64, I32, F32,
+                             P, P, P, P, P]),
+    "bf_preference_loss_workspace": (I64, [I64, I64, I64, I32]),
+    "bf_preference_loss": (I32, [P, I32, I64, I64, I64, P, I32, P, P, I64, F32, F32, F32, P, P, P, P, P, P]),
+    "bf_adamw_multi": (I32, [I32, P, P, P, I32, I32, P, P, P, P, P, F64, F64, F64, F64, F64, I64, F32, P, P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,0 +1,69 @@
+// Shared device helpers of the training operators (bf_train_*.hip): element types and their
+// vector loads, token reads, workgroup reductions.
+#pragma once
+
+#include "bf_common.h"
+
+#include <cstring>
+
+namespace bf {
+
+// Element type codes of the training entry points.
+enum : int { TE_F32 = 0, TE_BF16 = 1, TE_F16 = 2 };
+
+inline bool elem_ok(int code) { return code >= TE_F32 && code <= TE_F16; }
+inline int elem_bytes(int code) { return code == TE_F32 ? 4 : 2; }
+
+// Calls f(T()) with the element type of a code that elem_ok has passed.
+template <class F>
+inline int with_elem(int code, F f) {
+  switch (code) {
+    case TE_F32: return f(float());
+    case TE_BF16: return f(__bf16());
+    default: return f(_Float16());
+  }
+}
+
+// N elements at any alignment of T, as fp32.  The copy is one access of up to 16 bytes (gfx950
+// reads and writes global memory at any alignment), so a row of odd length or a view that
+// starts anywhere takes the same path as an aligned one.
+template <class T, int N>
+struct Pack {
+  T v[N];
+};
+
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  Pack<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// Element `i` of a token array of 4- or 8-byte integers; a value that no vocabulary of fewer
+// than 2^31 entries holds becomes the nearest 32-bit one, so its sign and its being too large stay.
+__device__ __forceinline__ int load_token(const void* tokens, int bytes, int64_t i) {
+  if (bytes == 4) return static_cast<const int*>(tokens)[i];
+  const int64_t t = static_cast<const int64_t*>(tokens)[i];
+  return t > 0x7fffffffLL ? 0x7fffffff : t < -0x7fffffffLL ? -0x7fffffff : (int)t;
+}
+
+// Sum over a workgroup of WAVES waves, in a fixed order; `red` holds WAVES floats.
+template <int WAVES>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum(v);
+  if constexpr (WAVES == 1) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) s += red[w];
+  return s;
+}
+
+}  // namespace bf

@@ -599,6 +599,70 @@ int bf_split_certificate(const float* rows, int64_t row_ld, const float* bias, c
 int bf_domain_status(const float* lb, int64_t D, int64_t S, const int* infeasible, float threshold, float tol,
                      int* status, hipStream_t stream);
 
+/* ---- training of token networks ------------------------------------------------
+ * What stands at both ends of a token network's training step, and its weights' update.  No
+ * counterpart in the reference, which bounds networks and does not train them.
+ * Element types are given by code: 0 fp32, 1 bf16, 2 fp16.  Token arrays hold 4- or 8-byte integers
+ * (token_bytes).  Rows may start at any address that is a multiple of their element's size. */
+
+/* out[i, :] = scale * table[tokens[i], :] (fp32 product, rounded once), i < count, out dense [count, dim];
+ * a negative token gives zeros, one past the table NaN. */
+int bf_embed_rows(const void* table, int64_t table_ld, int64_t vocab, const void* tokens, int token_bytes,
+                  int64_t count, int64_t dim, float scale, int elem, void* out, hipStream_t stream);
+
+/* The table's gradient: out[v, :] = scale * the sum of grad[i, :] over the tokens i of value v, in fp32 in
+ * the order of i (the same bits on every call); out dense [vocab, dim], of grad's type or fp32.
+ * accumulate (fp32 out): the sums are added to out and rows without a token are not touched.
+ * Tokens outside [0, vocab) take no part.  Workspace in floats. */
+int64_t bf_embed_grad_workspace(int64_t count, int64_t vocab, int64_t dim);
+int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* tokens, int token_bytes, int64_t count,
+                  int64_t vocab, int64_t dim, float scale, int out_elem, int accumulate, void* out, float* workspace,
+                  hipStream_t stream);
+
+/* Clipped policy loss with a KL term against a reference, and its gradient.  Logits [B, T, V], row
+ * (b, t) at b * ld_b + t * ld_t; tokens, old_logp, ref_logp (NULL: no KL term) and mask (bytes; NULL: all
+ * ones) dense [B, T]; advantage (b, t) at b * adv_b + t * adv_t.  With p the log-probability of a row's token at
+ * the temperature, r = exp(p - old), A the advantage, d = ref - p:
+ *   term = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight (exp(d) - d - 1)
+ *   loss = sum of weight * term, weight = 1 / live rows, or with by_sequence 1 / (live rows of the sequence *
+ *   sequences with a live row).
+ * A row is live unless it is masked or its token negative; other rows are not read, and their logp and
+ * gradient are 0.  A token past the vocabulary gives NaN.  A row of equal terms min takes the unclipped one's
+ * gradient.  stats[4]: loss, sum of weight * (-min(...)), of weight * KL, of weight where the clip is active.
+ * grad (optional): grad_scale * dloss/dlogits, dense [B, T, V], of the logits' type. */
+int64_t bf_policy_loss_workspace(int64_t B, int64_t T, int64_t V, int elem);
+int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V, int64_t ld_b, int64_t ld_t,
+                   const void* tokens, int token_bytes, const float* old_logp, const float* ref_logp,
+                   const float* advantages, int64_t adv_b, int64_t adv_t, const void* mask, float clip_low,
+                   float clip_high, float kl_weight, double temperature, int by_sequence, float grad_scale, float* logp,
+                   float* stats, void* grad, float* workspace, hipStream_t stream);
+
+/* Preference loss of `pairs` chosen and rejected responses, and its gradient.  Logits [N, V] with row
+ * stride ld; response k holds rows offsets[k] .. offsets[k + 1] - 1 (offsets [2 * pairs + 1], ascending; a response may
+ * be empty), the chosen ones first, then the rejected in the same order.  With s the sum of logp - ref_logp
+ * over a response's rows: rewards [2 * pairs] = beta * s, h = reward chosen - reward rejected,
+ *   loss = mean over pairs of -(1 - smoothing) log sigma(h) - smoothing log sigma(-h).
+ * Rows of no response and rows of a negative token take no part (logp and gradient 0).  grad
+ * (optional): grad_scale * dloss/dlogits, dense [N, V], of the logits' type. */
+int64_t bf_preference_loss_workspace(int64_t N, int64_t V, int64_t pairs, int elem);
+int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64_t ld, const void* tokens,
+                       int token_bytes, const float* ref_logp, const int64_t* offsets, int64_t pairs, float beta,
+                       float smoothing, float grad_scale, float* logp, float* rewards, float* loss, void* grad,
+                       float* workspace, hipStream_t stream);
+
+/* One AdamW step (decoupled weight decay, torch.optim.AdamW's formula) over `count` weights; host arrays of
+ * device pointers and element counts.  Weights and gradients each of one type; the moments m and v of all tensors
+ * in one array each, tensor k from the element on that is the sum over the tensors before it of their sizes rounded
+ * up to 128.  Without scales m and v are fp32; with them (fp32, one per 128 elements) bytes: m and
+ * sqrt(v) as float8 e4m3 numbers to be multiplied by their scale (bf_train_adamw.hip says how they are
+ * rounded), padding included, which has to be zero before the first step.  master (optional): fp32
+ * copies of the weights in the same layout, which are stepped; the weights are then written only.
+ * The gradient is multiplied by grad_scale, and by *grad_scale_dev where that is given. */
+int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_t* n, int p_elem, int g_elem, void* m,
+                   void* v, float* m_scale, float* v_scale, float* master, double lr, double beta1, double beta2,
+                   double eps, double weight_decay, int64_t step, float grad_scale, const float* grad_scale_dev,
+                   hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
