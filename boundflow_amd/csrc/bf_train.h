@@ -52,6 +52,24 @@ __device__ __forceinline__ int load_token(const void* tokens, int bytes, int64_t
   return t > 0x7fffffffLL ? 0x7fffffff : t < -0x7fffffffLL ? -0x7fffffff : (int)t;
 }
 
+// Max over the 64 lanes of a wave by the DPP steps of wave_sum (a lane that a step leaves unwritten
+// meets its own value), returned to every lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {
+  const int x = __float_as_int(v);
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(x, x, CTRL, ROWS, 0xf, false)));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+  v = dpp_max<0xb1, 0xf>(v);
+  v = dpp_max<0x4e, 0xf>(v);
+  v = dpp_max<0x141, 0xf>(v);
+  v = dpp_max<0x140, 0xf>(v);
+  v = dpp_max<0x142, 0xa>(v);
+  v = dpp_max<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
 // Sum over a workgroup of WAVES waves, in a fixed order; `red` holds WAVES floats.
 template <int WAVES>
 __device__ __forceinline__ float block_sum(float v, float* red) {

@@ -295,6 +295,176 @@ __global__ __launch_bounds__(LOSS_THREADS) void policy_rows_kernel(const T* __re
   if (threadIdx.x == 0) sums[blockIdx.x] = make_float4(policy, kl, outside, 0.f);
 }
 
+// Sixteen bytes of logits as they are.  as_floats keeps the compiler from holding on to the fp32 values of a
+// row between its two uses, which would take twice the registers that the row does.
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+
+template <class T, int VEC>
+__device__ __forceinline__ void as_floats(Words& w, float (&z)[VEC]) {
+  asm volatile("" : "+v"(w));
+  Pack<T, VEC> x;
+  __builtin_memcpy(&x, &w, sizeof(x));
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) z[e] = (float)x.v[e];
+}
+
+// base: the same in the whole workgroup (scalar registers); at: the thread's bytes
+__device__ __forceinline__ Words load_words(const void* base, uint32_t at) {
+  Words w;
+  __builtin_memcpy(&w, static_cast<const char*>(base) + at, sizeof(w));
+  return w;
+}
+
+// A workgroup's row in registers: vector k * THREADS + tid of 16 bytes in x[k], and of the elements
+// past the last whole vector the tid-th in `rest`.
+template <class T, int THREADS, int NV>
+struct HeldRow {
+  static constexpr int VEC = 16 / sizeof(T), WAVES = THREADS / 64, STEP = THREADS * 16;
+  Words x[NV];
+  float rest;
+
+  static __device__ __forceinline__ uint32_t at() { return threadIdx.x * 16u; }
+  static __device__ __forceinline__ bool has(int k, int vecs) { return k * THREADS + (int)threadIdx.x < vecs; }
+
+  __device__ __forceinline__ void load(int k, const T* row, int vecs) {
+    if (has(k, vecs)) x[k] = load_words(reinterpret_cast<const char*>(row) + k * STEP, at());
+  }
+  __device__ __forceinline__ void load_rest(const T* row, int vecs, int V) {
+    const int e = vecs * VEC + (int)threadIdx.x;
+    if (e < V) rest = (float)row[e];
+  }
+
+  // (K, sum) of the row's softmax, the same in every thread; `red` holds WAVES pairs
+  __device__ __forceinline__ float2 softmax(int vecs, int V, float c, float2* red) {
+    float K = -__builtin_inff(), s = 0.f, z[VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (has(k, vecs)) {
+        as_floats<T>(x[k], z);
+        add_terms(K, s, z, c);
+      }
+    if (vecs * VEC + (int)threadIdx.x < V) {
+      const float one[1] = {rest};
+      add_terms(K, s, one, c);
+    }
+    const float Kw = wave_max(K);
+    s = wave_sum(moved(s, K, Kw));
+    if constexpr (WAVES == 1) return make_float2(Kw, s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(Kw, s);
+    __syncthreads();
+    K = red[0].x;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) K = fmaxf(K, red[w].x);
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += moved(red[w].y, red[w].x, K);
+    return make_float2(K, s);
+  }
+};
+
+// What a workgroup writes for a row: its gradient, or zeros.
+enum : int { ROW_ZEROS, ROW_TERMS, ROW_LOWEST };
+
+// g (onehot(t) - softmax) of vector k, written; q = -g / sum.  `how` is the same in the whole workgroup.
+template <class T, int THREADS, int NV>
+__device__ __forceinline__ void write_gradient(HeldRow<T, THREADS, NV>& h, int k, int vecs, T* out, int how, float c,
+                                               float K, float q, float g, int t) {
+  constexpr int VEC = HeldRow<T, THREADS, NV>::VEC;
+  if (!h.has(k, vecs)) return;
+  float f[VEC];
+  if (how == ROW_TERMS) {
+    as_floats<T>(h.x[k], f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = exp2_fast(fmaf(f[e], c, -K)) * q;
+  } else if (how == ROW_LOWEST) {
+    as_floats<T>(h.x[k], f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = f[e] > -__builtin_inff() ? q : 0.f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+  }
+  const int d = t - (k * THREADS + (int)threadIdx.x) * VEC;
+  if (d >= 0 && d < VEC)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] += d == e ? g : 0.f;
+  Pack<T, VEC> y;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) y.v[e] = (T)f[e];
+  __builtin_memcpy(reinterpret_cast<char*>(out) + k * HeldRow<T, THREADS, NV>::STEP + h.at(), &y, sizeof(y));
+}
+
+// The whole loss of a row in one pass over its logits.  A workgroup holds a row in registers, reduces its
+// softmax, forms the row's term and writes the gradient; as each vector's gradient is stored, the same
+// vector of the workgroup's next row is loaded into its registers, so that loads are in flight while
+// gradients are formed and stored.  Every logit is read once and every gradient written once.
+template <class T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict__ logits, LogitRows rows, PolicyArgs a,
+                                                             const float* __restrict__ weight,
+                                                             float* __restrict__ logp, T* __restrict__ grad,
+                                                             float4* __restrict__ sums) {
+  using Held = HeldRow<T, THREADS, NV>;
+  __shared__ float2 red[2][Held::WAVES];
+  const int N = (int)(a.B * a.T), V = (int)rows.V, vecs = V / Held::VEC;
+  const float c = a.c;
+  Held h;
+  int n = blockIdx.x;
+  bool live = n < N && live_row(a.mask, a.tokens, a.token_bytes, n);
+  const T* row = logits + (n < N ? rows.offset(n) : 0);
+  if (live) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) h.load(k, row, vecs);
+    h.load_rest(row, vecs, V);
+  }
+  float policy = 0.f, kl = 0.f, outside = 0.f;
+  // two buffers, by turns of the rows that use them: before one is filled again, every wave has passed the barrier
+  // of the row in between, and so has read it
+  int buf = 0;
+  while (n < N) {
+    const int next = n + (int)gridDim.x;
+    const bool next_live = next < N && live_row(a.mask, a.tokens, a.token_bytes, next);
+    const T* next_row = logits + (next < N ? rows.offset(next) : 0);
+    float lp = 0.f, K = 0.f, q = 0.f, g = 0.f;
+    int t = -1, how = ROW_ZEROS;
+    if (live) {
+      t = load_token(a.tokens, a.token_bytes, n);
+      const float zt = t < V ? (float)row[t] : 0.f;
+      const float2 soft = h.softmax(vecs, V, c, red[buf]);
+      buf ^= 1;
+      K = soft.x;
+      const float arg = K == kLowK ? (zt > -__builtin_inff() ? 0.f : zt) : fmaf(zt, c, -K);
+      lp = t < V ? (arg - log2_fast(soft.y)) * kLn2 : __int_as_float(0x7fc00000);
+      const PolicyRow r = policy_row(a, n, lp);
+      const float w = weight[div_rows(n, a.T, true)];
+      policy += w * r.policy;
+      kl += w * r.kl;
+      outside += w * r.outside;
+      g = w * r.g * a.inv_t * a.grad_scale;
+      q = -g / soft.y;
+      how = __builtin_amdgcn_readfirstlane(g == 0.f ? ROW_ZEROS : K == kLowK ? ROW_LOWEST : ROW_TERMS);
+      if (how == ROW_ZEROS) t = -1;
+    }
+    if (threadIdx.x == 0) logp[n] = lp;
+    T* out = grad + (int64_t)n * V;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (grad) write_gradient(h, k, vecs, out, how, c, K, q, g, t);
+      if (next_live) h.load(k, next_row, vecs);
+      // the loads stay behind the stores of their registers' old contents, in which no copy of the row is made
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (grad) {
+      const int e = vecs * Held::VEC + (int)threadIdx.x;
+      if (e < V) out[e] = (T)(how == ROW_ZEROS ? 0.f : term(h.rest, c, K) * q + (t == e ? g : 0.f));
+    }
+    if (next_live) h.load_rest(next_row, vecs, V);
+    n = next;
+    live = next_live;
+    row = next_row;
+  }
+  if (threadIdx.x == 0) sums[blockIdx.x] = make_float4(policy, kl, outside, 0.f);
+}
+
 // stats: loss, policy term, KL, clipped share
 __global__ __launch_bounds__(LOSS_THREADS) void policy_stats_kernel(const float4* __restrict__ sums, int64_t count,
                                                                     float kl_weight, float* __restrict__ stats) {
@@ -414,6 +584,13 @@ static Parts row_parts(int64_t N, int64_t V, int elem) {
   return p;
 }
 
+// The row kernel's workgroup for V logits: the smallest that holds a row, or 0 where none does
+// (rows of 65536 fp32 or 131072 16-bit logits and more).
+static int row_threads(int64_t V, int elem) {
+  const int64_t vecs = V / (16 / elem_bytes(elem));
+  return vecs <= 256 ? 64 : vecs <= 1024 ? 256 : vecs <= 4096 ? 512 : vecs <= 16384 ? 1024 : 0;
+}
+
 static bool rows_fit(int64_t N, int64_t V) { return V < (1LL << 30) && N < (1LL << 24); }
 
 }  // namespace bf
@@ -422,11 +599,17 @@ using namespace bf;
 
 extern "C" {
 
-// coef [N] float4, part [N * parts] float2, sums float4 per 256 rows, weight [B]
+// the sums of the row kernel's workgroups, or of 256 rows each
+static int64_t sum_groups(int64_t N) {
+  const int64_t parts = ceil_div(N, LOSS_THREADS), groups = N < 4096 ? N : 4096;
+  return parts > groups ? parts : groups;
+}
+
+// coef [N] float4, part [N * parts] float2, sums float4, weight [B]
 int64_t bf_policy_loss_workspace(int64_t B, int64_t T, int64_t V, int elem) {
   if (!elem_ok(elem) || B < 0 || T < 0 || V <= 0) return 0;
   const int64_t N = B * T;
-  return 4 * N + 2 * N * row_parts(N, V, elem).count + 4 * ceil_div(N, LOSS_THREADS) + B;
+  return 4 * N + 2 * N * row_parts(N, V, elem).count + 4 * sum_groups(N) + B;
 }
 
 int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V, int64_t ld_b, int64_t ld_t,
@@ -457,7 +640,7 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   float4* coef = reinterpret_cast<float4*>(workspace);
   float4* sums = coef + N;
   const int64_t blocks = ceil_div(N, LOSS_THREADS);
-  float2* part = reinterpret_cast<float2*>(sums + blocks);
+  float2* part = reinterpret_cast<float2*>(sums + sum_groups(N));
   float* weight = reinterpret_cast<float*>(part + N * p.count);
   if (N * p.count >= (1LL << 31)) {
     set_error("bf_policy_loss: %lld rows of %lld logits are too many", (long long)N, (long long)V);
@@ -466,6 +649,29 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   if (N > 0) {
     hipLaunchKernelGGL(policy_weights_kernel, dim3(1), dim3(WEIGHT_THREADS), 0, stream, a, weight);
     BF_LAUNCH_CHECK("policy_weights_kernel");
+    const int threads = row_threads(V, elem);
+    if (threads && N >= 256) {
+      // as many workgroups as the device holds; each goes through its rows
+      const int64_t most = 256 * (threads == 64 ? 16 : threads == 256 ? 6 : threads == 512 ? 2 : 1);
+      const int64_t groups = N < most ? N : most;
+      const int rc = with_elem(elem, [&](auto e) -> int {
+        using E = decltype(e);
+        auto run = [&](auto kernel) -> int {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3((unsigned)threads), 0, stream,
+                             static_cast<const E*>(logits), rows, a, weight, logp, static_cast<E*>(grad), sums);
+          BF_LAUNCH_CHECK("policy_row_kernel");
+          return BF_OK;
+        };
+        return threads == 64    ? run(policy_row_kernel<E, 64, 4>)
+               : threads == 256 ? run(policy_row_kernel<E, 256, 4>)
+               : threads == 512 ? run(policy_row_kernel<E, 512, 8>)
+                                : run(policy_row_kernel<E, 1024, 16>);
+      });
+      if (rc != BF_OK) return rc;
+      hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(LOSS_THREADS), 0, stream, sums, groups, kl_weight, stats);
+      BF_LAUNCH_CHECK("policy_stats_kernel");
+      return BF_OK;
+    }
     const int rc = with_elem(elem, [&](auto e) -> int {
       using E = decltype(e);
       const E* x = static_cast<const E*>(logits);
