@@ -9,57 +9,42 @@
 // Preference loss (bf_preference_loss): with s = sum over a response's rows of p_t - ref,
 //   L = mean over pairs of -(1 - e) log sigma(h) - e log sigma(-h),   h = beta (s_chosen - s_rejected).
 //
-// Exponentials are taken in base 2 of c z, c = log2(e) / temperature, against a whole number
-// K >= max(c z): the argument c z - K is one fused multiply-add of the logit (rounded once), and
-// moving a sum from one K to a larger one is a multiplication by a power of two, which is exact.
+// A softmax is held as (M, s): the largest logit M, and s = sum of 2^(c (z - M)), c = log2(e) / temperature.
+// The difference of two logits is exact or rounded by a share of itself, so rows of any magnitude
+// (masks of -1e9 or of the type's lowest value, which fill a whole row now and then) keep the accuracy of
+// their differences; a row of -inf alone has no distribution, and a NaN or +inf makes its row NaN.
 
 #include "bf_train.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace bf {
 
 constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kFloor = -3.4028234663852886e38f;   // M of no logits: the lowest fp32, so that -inf - M is -inf
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
-// Logits below -2^126 (a type's lowest value in a mask, say) count in rows that have nothing else:
-// those are uniform over what is not -inf, as the difference of equal logits says.  In base 2 they
-// would overflow, so they have a K of their own.  A row of -inf alone has no distribution (NaN).
-constexpr float kLowest = -8.507059173023462e37f;    // -2^126
-constexpr float kLowK = -1.7014118346046923e38f;     // -2^127: against any other K its terms are 0
+// 2^(c (z - M))
+__device__ __forceinline__ float term(float z, float c, float M) { return exp2_fast((z - M) * c); }
 
-// Adds 2^(c z - K) over N logits to the sum s at K, raising K where a logit needs it.
+// (M, s) with N more logits
 template <int N>
-__device__ __forceinline__ void add_terms(float& K, float& s, const float (&z)[N], float c) {
-  float m = z[0];
+__device__ __forceinline__ void add_terms(float& M, float& s, const float (&z)[N], float c) {
+  float m = M;
 #pragma unroll
-  for (int k = 1; k < N; ++k) m = fmaxf(m, z[k]);
-  if (m < kLowest) {
-    const float K1 = m > -__builtin_inff() ? fmaxf(K, kLowK) : K;
-    K = K1;   // from -inf, where s is 0 (or NaN)
+  for (int k = 0; k < N; ++k) m = fmaxf(m, z[k]);
+  s *= term(M, c, m);
+  M = m;
 #pragma unroll
-    for (int k = 0; k < N; ++k) s += z[k] != z[k] ? z[k] : K == kLowK && z[k] > -__builtin_inff() ? 1.f : 0.f;
-    return;
-  }
-  const float K1 = fmaxf(K, ceilf(m * c));
-  if (K1 != K) {
-    s = K > kLowK ? s * __builtin_amdgcn_exp2f(K - K1) : s != s ? s : 0.f;
-    K = K1;
-  }
-#pragma unroll
-  for (int k = 0; k < N; ++k) s += __builtin_amdgcn_exp2f(fmaf(z[k], c, -K));
+  for (int k = 0; k < N; ++k) s += term(z[k], c, m);
 }
 
-// s 2^from as a multiple of 2^to, to >= from; a sum of nothing (from is -inf) stays nothing
-__device__ __forceinline__ float moved(float s, float from, float to) {
-  return from == to ? s : s * exp2_fast(from - to);
-}
-
-// 2^(c z - K)
-__device__ __forceinline__ float term(float z, float c, float K) {
-  return K == kLowK ? (z > -__builtin_inff() ? 1.f : 0.f) : exp2_fast(fmaf(z, c, -K));
+// the log-probability of a logit z
+__device__ __forceinline__ float log_prob(float z, float c, float M, float s) {
+  return ((z - M) * c - log2_fast(s)) * kLn2;
 }
 
 // Rows of logits: row n is logits + (n / T) ld_b + (n % T) ld_t.
@@ -74,26 +59,46 @@ struct LogitRows {
 
 // a row that takes part: not masked, and its token not negative
 __device__ __forceinline__ bool live_row(const uint8_t* mask, const void* tokens, int token_bytes, int64_t n) {
-  return (mask == nullptr || mask[n]) && load_token(tokens, token_bytes, n) >= 0;
+  const bool shown = mask == nullptr || mask[n];
+  const int t = load_token(tokens, token_bytes, n);   // both loads under way together
+  return shown & (t >= 0);
 }
 
 constexpr int LOSS_THREADS = 256, LOSS_WAVES = LOSS_THREADS / 64;
 
+// (M, s) over a workgroup of WAVES waves, the same in every thread; `red` holds WAVES pairs and is
+// written before the barrier that it has, and read after it.
+template <int WAVES>
+__device__ __forceinline__ float2 block_softmax(float M, float s, float c, float2* red) {
+  float m = wave_max(M);
+  s = wave_sum(s * term(M, c, m));
+  if constexpr (WAVES == 1) return make_float2(m, s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(m, s);
+  __syncthreads();
+  m = red[0].x;
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) m = fmaxf(m, red[w].x);
+  s = 0.f;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) s += red[w].y * term(red[w].x, c, m);
+  return make_float2(m, s);
+}
+
 // ---------------------------------------------------------------------------
-// (K, sum of 2^(c z - K)) of a part of a row.  Workgroup = (row, part of `chunk` elements).
+// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements).
 template <class T>
 __global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows,
                                                                     const void* __restrict__ tokens, int token_bytes,
                                                                     const uint8_t* __restrict__ mask, float c, int parts,
                                                                     int64_t chunk, float2* __restrict__ part) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ float red_k[LOSS_WAVES], red_s[LOSS_WAVES];
+  __shared__ float2 red[LOSS_WAVES];
   const int64_t n = blockIdx.x / (unsigned)parts;
   const int q = (int)(blockIdx.x % (unsigned)parts);
   if (!live_row(mask, tokens, token_bytes, n)) return;
   const T* row = logits + rows.offset(n);
   const int64_t from = q * chunk, to = min(from + chunk, rows.V);
-  float K = -__builtin_inff(), s = 0.f;
+  float M = kFloor, s = 0.f;
   for (int64_t d = from + threadIdx.x * VEC; d < to; d += LOSS_THREADS * VEC) {
     float z[VEC];
     if (d + VEC <= to) {
@@ -104,61 +109,38 @@ __global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __r
 #pragma unroll
       for (int k = 0; k < VEC; ++k) z[k] = d + k < to ? (float)row[d + k] : -__builtin_inff();
     }
-    add_terms(K, s, z, c);
+    add_terms(M, s, z, c);
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float K2 = __shfl_xor(K, d), s2 = __shfl_xor(s, d), K1 = fmaxf(K, K2);
-    s = moved(s, K, K1) + moved(s2, K2, K1);
-    K = K1;
-  }
-  if ((threadIdx.x & 63) == 0) {
-    red_k[threadIdx.x >> 6] = K;
-    red_s[threadIdx.x >> 6] = s;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < LOSS_WAVES; ++w) {
-      const float K1 = fmaxf(K, red_k[w]);
-      s = moved(s, K, K1) + moved(red_s[w], red_k[w], K1);
-      K = K1;
-    }
-    part[blockIdx.x] = make_float2(K, s);
-  }
+  const float2 x = block_softmax<LOSS_WAVES>(M, s, c, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = x;
 }
 
-// A row's softmax: K, s over its parts, and the log-probability of its token.
+// A row's softmax over its parts, and the log-probability of its token.
 struct RowSoftmax {
-  float K, s, logp;
+  float M, s, logp;
 };
 
 template <class T>
 __device__ __forceinline__ RowSoftmax row_softmax(const T* logits, const LogitRows& rows, int64_t n, int t,
                                                   const float2* part, int parts, float c) {
   RowSoftmax r;
-  r.K = -__builtin_inff();
+  r.M = kFloor;
   r.s = 0.f;
   for (int q = 0; q < parts; ++q) {
     const float2 x = part[n * parts + q];
-    const float K1 = fmaxf(r.K, x.x);
-    r.s = moved(r.s, r.K, K1) + moved(x.y, x.x, K1);
-    r.K = K1;
+    const float m = fmaxf(r.M, x.x);
+    r.s = r.s * term(r.M, c, m) + x.y * term(x.x, c, m);
+    r.M = m;
   }
   // a token past the vocabulary shows as NaN
-  if ((int64_t)t >= rows.V) {
-    r.logp = __int_as_float(0x7fc00000);
-    return r;
-  }
-  const float z = (float)logits[rows.offset(n) + t];
-  const float x = r.K == kLowK ? (z > -__builtin_inff() ? 0.f : z) : fmaf(z, c, -r.K);
-  r.logp = (x - log2_fast(r.s)) * kLn2;
+  r.logp = (int64_t)t < rows.V ? log_prob((float)logits[rows.offset(n) + t], c, r.M, r.s) : __int_as_float(0x7fc00000);
   return r;
 }
 
-// What the gradient of a row needs: dlogits = 2^(c z - K) * q (+ g at the token).
+// What the gradient of a row needs: dlogits = 2^(c (z - M)) * q (+ g at the token).
 // A row with g = 0 gets zeros and its logits are not read.
 __device__ __forceinline__ float4 row_gradient(const RowSoftmax& r, float g) {
-  return make_float4(r.K, -g / r.s, g, 0.f);
+  return make_float4(r.M, -g / r.s, g, 0.f);
 }
 
 template <class T>
@@ -215,28 +197,45 @@ struct PolicyArgs {
 constexpr int WEIGHT_THREADS = 1024, WEIGHT_WAVES = WEIGHT_THREADS / 64;
 
 // weight[b]: 1 / live rows (of all, or with by_sequence of the sequence times the sequences that have
-// any).  One workgroup, a wave per sequence.
+// any).  One workgroup, a row a thread; the sequences are taken WEIGHT_HELD at a time, whose counts lie in LDS.
+constexpr int WEIGHT_HELD = 4096;
+
 __global__ __launch_bounds__(WEIGHT_THREADS) void policy_weights_kernel(PolicyArgs a, float* __restrict__ weight) {
+  __shared__ int held[WEIGHT_HELD];
   __shared__ float red[WEIGHT_WAVES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float total = 0.f, some = 0.f;   // of a wave's sequences, in lane 0
-  for (int64_t b = wave; b < a.B; b += WEIGHT_WAVES) {
-    int live = 0;
-    for (int64_t t = lane; t < a.T; t += 64) live += live_row(a.mask, a.tokens, a.token_bytes, b * a.T + t);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) live += __shfl_xor(live, d);
-    if (lane == 0) {
-      weight[b] = (float)live;
-      total += (float)live;
-      some += live > 0 ? 1.f : 0.f;
+  const int lane = threadIdx.x & 63;
+  const unsigned T = (unsigned)a.T;
+  float total = 0.f, some = 0.f;
+  for (int64_t b0 = 0; b0 < a.B; b0 += WEIGHT_HELD) {
+    const int B = (int)(a.B - b0 < WEIGHT_HELD ? a.B - b0 : WEIGHT_HELD);
+    for (int b = threadIdx.x; b < B; b += WEIGHT_THREADS) held[b] = 0;
+    __syncthreads();
+    const unsigned rows = B * T;
+    for (unsigned i0 = threadIdx.x - lane; i0 < rows; i0 += WEIGHT_THREADS) {   // 64 rows a wave
+      const unsigned i = i0 + lane, b = i / T;
+      const bool in = i < rows && live_row(a.mask, a.tokens, a.token_bytes, b0 * T + i);
+      const unsigned first = __builtin_amdgcn_readfirstlane(b);
+      if (__ballot(i < rows && b != first) == 0) {
+        const int found = __popcll(__ballot(in));
+        if (lane == 0) atomicAdd(&held[first], found);
+      } else if (in) {
+        atomicAdd(&held[b], 1);
+      }
     }
+    __syncthreads();
+    for (int b = threadIdx.x; b < B; b += WEIGHT_THREADS) {
+      weight[b0 + b] = (float)held[b];   // read again by the same thread
+      total += (float)held[b];
+      some += held[b] ? 1.f : 0.f;
+    }
+    __syncthreads();
   }
   const float all = block_sum<WEIGHT_WAVES>(a.by_sequence ? some : total, red);
-  __syncthreads();   // weight[] is written by the waves' first lanes
-  for (int64_t b = threadIdx.x; b < a.B; b += WEIGHT_THREADS) {
-    const float live = weight[b];
-    weight[b] = live > 0.f ? 1.f / (a.by_sequence ? live * all : all) : 0.f;
-  }
+  for (int64_t b0 = 0; b0 < a.B; b0 += WEIGHT_HELD)
+    for (int64_t b = b0 + threadIdx.x; b < a.B && b < b0 + WEIGHT_HELD; b += WEIGHT_THREADS) {
+      const float live = weight[b];
+      weight[b] = live > 0.f ? 1.f / (a.by_sequence ? live * all : all) : 0.f;
+    }
 }
 
 struct PolicyRow {
@@ -244,23 +243,28 @@ struct PolicyRow {
 };
 
 // A live row's terms and dL/dp_t, before its weight.
-__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& a, int64_t n, float logp) {
+__device__ __forceinline__ PolicyRow policy_term(float logp, float old, float ref, bool has_ref, float A, float low,
+                                                 float high, float kl_weight) {
   PolicyRow r;
-  const int64_t b = div_rows(n, a.T, n < (1LL << 31) && a.T < (1LL << 31));
-  const float A = a.advantages[b * a.adv_b + (n - b * a.T) * a.adv_t];
-  const float ratio = expf(logp - a.old_logp[n]);
-  const float plain = ratio * A, clipped = fminf(fmaxf(ratio, a.low), a.high) * A;
+  const float ratio = expf(logp - old);
+  const float plain = ratio * A, clipped = fminf(fmaxf(ratio, low), high) * A;
   const bool out = clipped < plain;   // the clipped side is the smaller: a constant, without a gradient
   r.policy = out ? -clipped : -plain;
   r.outside = out ? 1.f : 0.f;
   r.g = out ? 0.f : -plain;
   r.kl = 0.f;
-  if (a.ref_logp) {
-    const float apart = a.ref_logp[n] - logp, e = expm1f(apart);
+  if (has_ref) {
+    const float apart = ref - logp, e = expm1f(apart);
     r.kl = e - apart;
-    r.g -= a.kl_weight * e;
+    r.g -= kl_weight * e;
   }
   return r;
+}
+
+__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& a, int64_t n, float logp) {
+  const int64_t b = div_rows(n, a.T, n < (1LL << 31) && a.T < (1LL << 31));
+  return policy_term(logp, a.old_logp[n], a.ref_logp ? a.ref_logp[n] : 0.f, a.ref_logp != nullptr,
+                     a.advantages[b * a.adv_b + (n - b * a.T) * a.adv_t], a.low, a.high, a.kl_weight);
 }
 
 // One thread per row: its gradient's coefficients, and the workgroup's share of the sums.
@@ -308,159 +312,198 @@ __device__ __forceinline__ void as_floats(Words& w, float (&z)[VEC]) {
   for (int e = 0; e < VEC; ++e) z[e] = (float)x.v[e];
 }
 
-// base: the same in the whole workgroup (scalar registers); at: the thread's bytes
-__device__ __forceinline__ Words load_words(const void* base, uint32_t at) {
-  Words w;
-  __builtin_memcpy(&w, static_cast<const char*>(base) + at, sizeof(w));
-  return w;
+// A value that is the same in every lane, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float uniform(float x) { return __int_as_float(uniform(__float_as_int(x))); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return ((int64_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x);
 }
 
-// A workgroup's row in registers: vector k * THREADS + tid of 16 bytes in x[k], and of the elements
-// past the last whole vector the tid-th in `rest`.
-template <class T, int THREADS, int NV>
+// A workgroup's row in registers: vector k * THREADS + tid of 16 bytes in x[k], and of the elements past the
+// last whole vector the tid-th in `rest`.  The first FULL steps are whole in every row that the kernel takes.
+template <class T, int THREADS, int NV, int FULL>
 struct HeldRow {
-  static constexpr int VEC = 16 / sizeof(T), WAVES = THREADS / 64, STEP = THREADS * 16;
+  static constexpr int VEC = 16 / sizeof(T), WAVES = THREADS / 64;
   Words x[NV];
   float rest;
 
-  static __device__ __forceinline__ uint32_t at() { return threadIdx.x * 16u; }
-  static __device__ __forceinline__ bool has(int k, int vecs) { return k * THREADS + (int)threadIdx.x < vecs; }
-
-  __device__ __forceinline__ void load(int k, const T* row, int vecs) {
-    if (has(k, vecs)) x[k] = load_words(reinterpret_cast<const char*>(row) + k * STEP, at());
+  static __device__ __forceinline__ bool has(int k, int vecs) {
+    return k < FULL || k * THREADS + (int)threadIdx.x < vecs;
   }
-  __device__ __forceinline__ void load_rest(const T* row, int vecs, int V) {
-    const int e = vecs * VEC + (int)threadIdx.x;
-    if (e < V) rest = (float)row[e];
+  // Loads are never skipped: with a branch around them the compiler waits for every access at every turn.  Threads
+  // past the row's end load its last vector (element) again, and of a row that is not to be read (`read` 0) every
+  // thread loads the first, one cache line.
+  __device__ __forceinline__ void load(int k, const T* row, int read, int vecs) {
+    const int lane = k < FULL ? (int)threadIdx.x : min((int)threadIdx.x, vecs - 1 - k * THREADS);
+    // a step that begins past the row's end lies before it by as much: lane is negative there
+    const char* at = reinterpret_cast<const char*>(row) + read * (k * THREADS * 16);
+    __builtin_memcpy(&x[k], k < FULL ? at + (uint32_t)(read * lane * 16) : at + read * lane * 16, 16);
   }
-
-  // (K, sum) of the row's softmax, the same in every thread; `red` holds WAVES pairs
-  __device__ __forceinline__ float2 softmax(int vecs, int V, float c, float2* red) {
-    float K = -__builtin_inff(), s = 0.f, z[VEC];
+  __device__ __forceinline__ void load_rest(const T* row, int read, int vecs, int V) {
+    rest = (float)row[(uint32_t)(read * min(vecs * VEC + (int)threadIdx.x, V - 1))];
+  }
+  // (M, s) of the thread with vector k, or with its element past the vectors
+  __device__ __forceinline__ void add(int k, int vecs, float c, float& M, float& s) {
+    float z[VEC];
+    as_floats<T>(x[k], z);
+    if (has(k, vecs)) add_terms(M, s, z, c);
+  }
+  __device__ __forceinline__ void add_rest(int vecs, int V, float c, float& M, float& s) {
+    const float one[1] = {rest};
+    if (vecs * VEC + (int)threadIdx.x < V) add_terms(M, s, one, c);
+  }
+  // q 2^(c (z - M)) of vector k; zeros where `keep` is 0, whatever the vector holds (else it is ~0)
+  __device__ __forceinline__ void store(int k, T* out, int vecs, float c, float M, float q, uint32_t keep) {
+    float f[VEC];
+    as_floats<T>(x[k], f);
+    Pack<T, VEC> y;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-      if (has(k, vecs)) {
-        as_floats<T>(x[k], z);
-        add_terms(K, s, z, c);
-      }
-    if (vecs * VEC + (int)threadIdx.x < V) {
-      const float one[1] = {rest};
-      add_terms(K, s, one, c);
-    }
-    const float Kw = wave_max(K);
-    s = wave_sum(moved(s, K, Kw));
-    if constexpr (WAVES == 1) return make_float2(Kw, s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(Kw, s);
-    __syncthreads();
-    K = red[0].x;
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) K = fmaxf(K, red[w].x);
-    s = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += moved(red[w].y, red[w].x, K);
-    return make_float2(K, s);
+    for (int e = 0; e < VEC; ++e) y.v[e] = (T)(term(f[e], c, M) * q);
+    Words w;
+    __builtin_memcpy(&w, &y, 16);
+    w &= keep;
+    store_words(k, out, vecs, w);
+  }
+  static __device__ __forceinline__ void store_words(int k, T* out, int vecs, Words w) {
+    if (has(k, vecs))
+      __builtin_memcpy(reinterpret_cast<char*>(out) + k * THREADS * 16 + threadIdx.x * 16u, &w, 16);
   }
 };
 
-// What a workgroup writes for a row: its gradient, or zeros.
-enum : int { ROW_ZEROS, ROW_TERMS, ROW_LOWEST };
-
-// g (onehot(t) - softmax) of vector k, written; q = -g / sum.  `how` is the same in the whole workgroup.
-template <class T, int THREADS, int NV>
-__device__ __forceinline__ void write_gradient(HeldRow<T, THREADS, NV>& h, int k, int vecs, T* out, int how, float c,
-                                               float K, float q, float g, int t) {
-  constexpr int VEC = HeldRow<T, THREADS, NV>::VEC;
-  if (!h.has(k, vecs)) return;
-  float f[VEC];
-  if (how == ROW_TERMS) {
-    as_floats<T>(h.x[k], f);
+// The loop over a row's vectors: vector k's gradient is formed and stored (GRAD), the same vector of the next row
+// is loaded into its registers, and a vector that was loaded LAG steps before is added to the next row's (M, s).
+template <bool GRAD, class T, int THREADS, int NV, int FULL>
+__device__ __forceinline__ void row_step(HeldRow<T, THREADS, NV, FULL>& h, T* out, const T* next_row, int next_live,
+                                         int vecs, int V, float c, float Mr, float q, uint32_t keep, float& M,
+                                         float& s) {
+  constexpr int LAG = (NV + 1) / 2;
+  const int e = vecs * h.VEC + (int)threadIdx.x;
+  if (GRAD && e < V) out[e] = (T)(keep ? term(h.rest, c, Mr) * q : 0.f);
+  h.load_rest(next_row, next_live, vecs, V);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = exp2_fast(fmaf(f[e], c, -K)) * q;
-  } else if (how == ROW_LOWEST) {
-    as_floats<T>(h.x[k], f);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = f[e] > -__builtin_inff() ? q : 0.f;
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+  for (int k = 0; k < NV + LAG; ++k) {
+    if (k < NV) {
+      if (GRAD) h.store(k, out, vecs, c, Mr, q, keep);
+      h.load(k, next_row, next_live, vecs);
+    }
+    if (k >= LAG) h.add(k - LAG, vecs, c, M, s);
+    // loads stay behind the stores of their registers' old contents: the row is held once
+    __builtin_amdgcn_sched_barrier(0);
   }
-  const int d = t - (k * THREADS + (int)threadIdx.x) * VEC;
-  if (d >= 0 && d < VEC)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] += d == e ? g : 0.f;
-  Pack<T, VEC> y;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) y.v[e] = (T)f[e];
-  __builtin_memcpy(reinterpret_cast<char*>(out) + k * HeldRow<T, THREADS, NV>::STEP + h.at(), &y, sizeof(y));
+  h.add_rest(vecs, V, c, M, s);
 }
 
-// The whole loss of a row in one pass over its logits.  A workgroup holds a row in registers, reduces its
-// softmax, forms the row's term and writes the gradient; as each vector's gradient is stored, the same
-// vector of the workgroup's next row is loaded into its registers, so that loads are in flight while
-// gradients are formed and stored.  Every logit is read once and every gradient written once.
-template <class T, int THREADS, int NV>
+// A row's scalars, fetched a row before they are needed.
+struct PolicyScalars {
+  int n, t, live;
+  float old, ref, A, w;
+};
+
+__device__ __forceinline__ PolicyScalars policy_scalars(const PolicyArgs& a, const float* weight, int n, int N) {
+  PolicyScalars r;
+  r.n = n;
+  r.live = 0;
+  r.t = -1;
+  r.old = r.ref = r.A = r.w = 0.f;
+  if (n < N) {
+    const unsigned b = (unsigned)n / (unsigned)a.T;
+    r.t = load_token(a.tokens, a.token_bytes, n);
+    r.live = (a.mask == nullptr || a.mask[n]) & (r.t >= 0);
+    r.old = a.old_logp[n];
+    r.ref = a.ref_logp ? a.ref_logp[n] : 0.f;
+    r.A = a.advantages[b * a.adv_b + (n - b * (unsigned)a.T) * a.adv_t];
+    r.w = weight[b];
+  }
+  return r;
+}
+
+// The same in scalar registers, once they have arrived.
+__device__ __forceinline__ PolicyScalars uniform(const PolicyScalars& x) {
+  return {uniform(x.n), uniform(x.t), uniform(x.live), uniform(x.old), uniform(x.ref), uniform(x.A), uniform(x.w)};
+}
+
+// The whole loss of a row in one pass over its logits.  A workgroup holds a row in registers: its softmax is
+// there when the row before has been written, the row's term follows, and row_step writes the gradient
+// while it reads the next row and sums its softmax.  Loads, stores and exponentials are under way together, and
+// what is left between two rows is LAG vectors, a reduction and the term.
+//
+// Each turn of the grid takes as many rows as it has workgroups, the workgroups moved on by `stride` from
+// turn to turn: the rows that padding masks stand at the same places of every sequence, and without it a
+// workgroup would meet them at every turn or at none.
+template <bool GRAD, class T, int THREADS, int NV, int FULL>
 __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict__ logits, LogitRows rows, PolicyArgs a,
                                                              const float* __restrict__ weight,
                                                              float* __restrict__ logp, T* __restrict__ grad,
-                                                             float4* __restrict__ sums) {
-  using Held = HeldRow<T, THREADS, NV>;
+                                                             float4* __restrict__ sums, unsigned stride) {
+  using Held = HeldRow<T, THREADS, NV, FULL>;
   __shared__ float2 red[2][Held::WAVES];
   const int N = (int)(a.B * a.T), V = (int)rows.V, vecs = V / Held::VEC;
   const float c = a.c;
+  unsigned place = blockIdx.x, first = 0;   // of the workgroup in the turn, and the turn's first row
+  const auto next_turn = [&] {
+    first += gridDim.x;
+    place += stride;
+    if (place >= gridDim.x) place -= gridDim.x;
+    return (int)(first + place);
+  };
   Held h;
-  int n = blockIdx.x;
-  bool live = n < N && live_row(a.mask, a.tokens, a.token_bytes, n);
-  const T* row = logits + (n < N ? rows.offset(n) : 0);
-  if (live) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) h.load(k, row, vecs);
-    h.load_rest(row, vecs, V);
-  }
+  // the first row from x on that takes part; those that do not get their zeros here.  The loop below goes from one
+  // such row to the next, in one piece: a branch in it that leaves the row's registers alone would have the
+  // compiler keep two sets of them.
+  const auto settled = [&](PolicyScalars x) {
+    while (x.n < N && !x.live) {
+      const PolicyScalars after = policy_scalars(a, weight, next_turn(), N);
+      if (threadIdx.x == 0) logp[x.n] = 0.f;
+      if (GRAD) {
+        T* out = grad + (int64_t)x.n * V;
+        const int e = vecs * Held::VEC + (int)threadIdx.x;
+        if (e < V) out[e] = (T)0.f;
+        for (int k = 0; k < NV; ++k)
+          if (k * THREADS + (int)threadIdx.x < vecs) Held::store_words(k, out, vecs, Words{0u, 0u, 0u, 0u});
+      }
+      x = uniform(after);
+    }
+    return x;
+  };
+  PolicyScalars here = settled(uniform(policy_scalars(a, weight, (int)place, N)));
+  PolicyScalars after = policy_scalars(a, weight, next_turn(), N);
+  const T* row = logits + (here.n < N ? uniform(rows.offset(here.n)) : 0);
+  float M = kFloor, s = 0.f;   // of the thread, for the row that it holds
+  if (here.n < N) row_step<false>(h, grad, row, 1, vecs, V, c, 0.f, 0.f, 0u, M, s);
+  float zt = uniform(here.n < N && here.t < V ? (float)row[here.t] : 0.f);
   float policy = 0.f, kl = 0.f, outside = 0.f;
-  // two buffers, by turns of the rows that use them: before one is filled again, every wave has passed the barrier
-  // of the row in between, and so has read it
+  // two buffers, by turns: before one is filled again, every wave has passed the barrier of the row in between, and
+  // so has read it
   int buf = 0;
-  while (n < N) {
-    const int next = n + (int)gridDim.x;
-    const bool next_live = next < N && live_row(a.mask, a.tokens, a.token_bytes, next);
-    const T* next_row = logits + (next < N ? rows.offset(next) : 0);
-    float lp = 0.f, K = 0.f, q = 0.f, g = 0.f;
-    int t = -1, how = ROW_ZEROS;
-    if (live) {
-      t = load_token(a.tokens, a.token_bytes, n);
-      const float zt = t < V ? (float)row[t] : 0.f;
-      const float2 soft = h.softmax(vecs, V, c, red[buf]);
-      buf ^= 1;
-      K = soft.x;
-      const float arg = K == kLowK ? (zt > -__builtin_inff() ? 0.f : zt) : fmaf(zt, c, -K);
-      lp = t < V ? (arg - log2_fast(soft.y)) * kLn2 : __int_as_float(0x7fc00000);
-      const PolicyRow r = policy_row(a, n, lp);
-      const float w = weight[div_rows(n, a.T, true)];
-      policy += w * r.policy;
-      kl += w * r.kl;
-      outside += w * r.outside;
-      g = w * r.g * a.inv_t * a.grad_scale;
-      q = -g / soft.y;
-      how = __builtin_amdgcn_readfirstlane(g == 0.f ? ROW_ZEROS : K == kLowK ? ROW_LOWEST : ROW_TERMS);
-      if (how == ROW_ZEROS) t = -1;
+  while (here.n < N) {
+    const PolicyScalars then = settled(uniform(after));
+    after = policy_scalars(a, weight, next_turn(), N);
+    const T* next_row = logits + (then.n < N ? uniform(rows.offset(then.n)) : 0);
+    const float zt_next = then.live && then.t < V ? (float)next_row[then.t] : 0.f;
+    const float2 soft = block_softmax<Held::WAVES>(M, s, c, red[buf]);
+    buf ^= 1;
+    // the same in every thread, and in scalar registers for the loop
+    const float Mr = uniform(soft.x);
+    const float lp = here.t < V ? log_prob(zt, c, Mr, soft.y) : __int_as_float(0x7fc00000);
+    const PolicyRow r = policy_term(lp, here.old, here.ref, a.ref_logp != nullptr, here.A, a.low, a.high, a.kl_weight);
+    policy += here.w * r.policy;
+    kl += here.w * r.kl;
+    outside += here.w * r.outside;
+    const float g = here.w * r.g * a.inv_t * a.grad_scale, q = uniform(-g / soft.y);
+    const uint32_t keep = uniform(g == 0.f ? 0 : -1);
+    if (threadIdx.x == 0) logp[here.n] = lp;
+    T* out = grad + (int64_t)here.n * V;
+    M = kFloor;
+    s = 0.f;
+    row_step<GRAD>(h, out, next_row, then.live, vecs, V, c, Mr, q, keep, M, s);
+    // the token's own element, by the thread that wrote its vector
+    if (GRAD && keep && here.t < V) {
+      const int v = here.t / Held::VEC;
+      if ((int)threadIdx.x == (v < vecs ? v % THREADS : here.t - vecs * Held::VEC))
+        out[here.t] = (T)(term(zt, c, Mr) * q + g);
     }
-    if (threadIdx.x == 0) logp[n] = lp;
-    T* out = grad + (int64_t)n * V;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      if (grad) write_gradient(h, k, vecs, out, how, c, K, q, g, t);
-      if (next_live) h.load(k, next_row, vecs);
-      // the loads stay behind the stores of their registers' old contents, in which no copy of the row is made
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (grad) {
-      const int e = vecs * Held::VEC + (int)threadIdx.x;
-      if (e < V) out[e] = (T)(how == ROW_ZEROS ? 0.f : term(h.rest, c, K) * q + (t == e ? g : 0.f));
-    }
-    if (next_live) h.load_rest(next_row, vecs, V);
-    n = next;
-    live = next_live;
-    row = next_row;
+    here = then;
+    zt = uniform(zt_next);
   }
   if (threadIdx.x == 0) sums[blockIdx.x] = make_float4(policy, kl, outside, 0.f);
 }
@@ -526,7 +569,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void preference_pairs_kernel(
         const RowSoftmax x = row_softmax(logits, rows, n, t, part, parts, c);
         lp = x.logp;
         s += lp - a.ref_logp[n];
-        coef[n] = make_float4(x.K, x.s, 0.f, 0.f);
+        coef[n] = make_float4(x.M, x.s, 0.f, 0.f);
       }
       logp[n] = lp;
     }
@@ -584,11 +627,33 @@ static Parts row_parts(int64_t N, int64_t V, int elem) {
   return p;
 }
 
-// The row kernel's workgroup for V logits: the smallest that holds a row, or 0 where none does
-// (rows of 65536 fp32 or 131072 16-bit logits and more).
-static int row_threads(int64_t V, int elem) {
-  const int64_t vecs = V / (16 / elem_bytes(elem));
-  return vecs <= 256 ? 64 : vecs <= 1024 ? 256 : vecs <= 4096 ? 512 : vecs <= 16384 ? 1024 : 0;
+// The row kernel's workgroup for rows of `vecs` whole vectors, handed to f as (threads, vectors a thread, steps that
+// are whole in every such row) at compile time; 0 where no workgroup holds a row (131072 16-bit or 65536 fp32
+// logits and more) or a row has no whole vector.
+template <class F>
+static int with_row_group(int64_t vecs, F f) {
+  using std::integral_constant;
+#define BF_ROW_GROUP(threads, nv, least) \
+  if (vecs <= (threads) * (nv))          \
+  return f(integral_constant<int, threads>(), integral_constant<int, nv>(), integral_constant<int, (least) / (threads)>())
+  if (vecs < 1) return 0;
+  BF_ROW_GROUP(64, 1, 0);
+  BF_ROW_GROUP(64, 2, 64);
+  BF_ROW_GROUP(64, 4, 128);
+  BF_ROW_GROUP(256, 2, 256);
+  BF_ROW_GROUP(256, 4, 512);
+  BF_ROW_GROUP(512, 3, 1024);
+  BF_ROW_GROUP(512, 4, 1536);
+  BF_ROW_GROUP(512, 6, 2048);
+  BF_ROW_GROUP(512, 8, 3072);
+  BF_ROW_GROUP(1024, 6, 4096);
+  BF_ROW_GROUP(1024, 8, 6144);
+  BF_ROW_GROUP(1024, 10, 8192);
+  BF_ROW_GROUP(1024, 12, 10240);
+  BF_ROW_GROUP(1024, 14, 12288);
+  BF_ROW_GROUP(1024, 16, 14336);
+#undef BF_ROW_GROUP
+  return 0;
 }
 
 static bool rows_fit(int64_t N, int64_t V) { return V < (1LL << 30) && N < (1LL << 24); }
@@ -649,28 +714,31 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   if (N > 0) {
     hipLaunchKernelGGL(policy_weights_kernel, dim3(1), dim3(WEIGHT_THREADS), 0, stream, a, weight);
     BF_LAUNCH_CHECK("policy_weights_kernel");
-    const int threads = row_threads(V, elem);
-    if (threads && N >= 256) {
-      // as many workgroups as the device holds; each goes through its rows
-      const int64_t most = 256 * (threads == 64 ? 16 : threads == 256 ? 6 : threads == 512 ? 2 : 1);
-      const int64_t groups = N < most ? N : most;
+    if (N >= 256) {
+      int64_t groups = 0;
       const int rc = with_elem(elem, [&](auto e) -> int {
         using E = decltype(e);
-        auto run = [&](auto kernel) -> int {
-          hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3((unsigned)threads), 0, stream,
-                             static_cast<const E*>(logits), rows, a, weight, logp, static_cast<E*>(grad), sums);
+        return with_row_group(V / (16 / (int)sizeof(E)), [&](auto threads, auto nv, auto full) -> int {
+          // as many workgroups as the device holds; each goes through its rows
+          constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value;
+          const int64_t most = 256 * (TH == 64 ? 16 : TH == 256 ? 6 : TH == 512 ? 2 : 1);
+          groups = N < most ? N : most;
+          auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(TH), 0, stream, static_cast<const E*>(logits), rows, a,
+                               weight, logp, static_cast<E*>(grad), sums, (unsigned)(groups * 0.6180339887498949));
+          };
+          if (grad) launch(policy_row_kernel<true, E, TH, NV, decltype(full)::value>);
+          else launch(policy_row_kernel<false, E, TH, NV, decltype(full)::value>);
           BF_LAUNCH_CHECK("policy_row_kernel");
           return BF_OK;
-        };
-        return threads == 64    ? run(policy_row_kernel<E, 64, 4>)
-               : threads == 256 ? run(policy_row_kernel<E, 256, 4>)
-               : threads == 512 ? run(policy_row_kernel<E, 512, 8>)
-                                : run(policy_row_kernel<E, 1024, 16>);
+        });
       });
       if (rc != BF_OK) return rc;
-      hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(LOSS_THREADS), 0, stream, sums, groups, kl_weight, stats);
-      BF_LAUNCH_CHECK("policy_stats_kernel");
-      return BF_OK;
+      if (groups) {
+        hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(LOSS_THREADS), 0, stream, sums, groups, kl_weight, stats);
+        BF_LAUNCH_CHECK("policy_stats_kernel");
+        return BF_OK;
+      }
     }
     const int rc = with_elem(elem, [&](auto e) -> int {
       using E = decltype(e);
