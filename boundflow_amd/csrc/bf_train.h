@@ -70,6 +70,19 @@ __device__ __forceinline__ float wave_max(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// Max and sum over the 16 lanes of a row, by the first four of those steps, returned to each of them.
+__device__ __forceinline__ float row16_max(float v) {
+  return dpp_max<0x140, 0xf>(dpp_max<0x141, 0xf>(dpp_max<0x4e, 0xf>(dpp_max<0xb1, 0xf>(v))));
+}
+
+__device__ __forceinline__ float row16_sum(float v) {
+  v += __builtin_amdgcn_update_dpp(0.f, v, 0xb1, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0.f, v, 0x4e, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0.f, v, 0x141, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0.f, v, 0x140, 0xf, 0xf, false);
+  return v;
+}
+
 // Sum over a workgroup of WAVES waves, in a fixed order; `red` holds WAVES floats.
 template <int WAVES>
 __device__ __forceinline__ float block_sum(float v, float* red) {

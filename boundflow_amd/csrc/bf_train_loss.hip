@@ -85,104 +85,6 @@ __device__ __forceinline__ float2 block_softmax(float M, float s, float c, float
 }
 
 // ---------------------------------------------------------------------------
-// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements).
-template <class T>
-__global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows,
-                                                                    const void* __restrict__ tokens, int token_bytes,
-                                                                    const uint8_t* __restrict__ mask, float c, int parts,
-                                                                    int64_t chunk, float2* __restrict__ part) {
-  constexpr int VEC = 16 / sizeof(T);
-  __shared__ float2 red[LOSS_WAVES];
-  const int64_t n = blockIdx.x / (unsigned)parts;
-  const int q = (int)(blockIdx.x % (unsigned)parts);
-  if (!live_row(mask, tokens, token_bytes, n)) return;
-  const T* row = logits + rows.offset(n);
-  const int64_t from = q * chunk, to = min(from + chunk, rows.V);
-  float M = kFloor, s = 0.f;
-  for (int64_t d = from + threadIdx.x * VEC; d < to; d += LOSS_THREADS * VEC) {
-    float z[VEC];
-    if (d + VEC <= to) {
-      const Pack<T, VEC> x = load_pack<T, VEC>(row + d);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) z[k] = (float)x.v[k];
-    } else {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) z[k] = d + k < to ? (float)row[d + k] : -__builtin_inff();
-    }
-    add_terms(M, s, z, c);
-  }
-  const float2 x = block_softmax<LOSS_WAVES>(M, s, c, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = x;
-}
-
-// A row's softmax over its parts, and the log-probability of its token.
-struct RowSoftmax {
-  float M, s, logp;
-};
-
-template <class T>
-__device__ __forceinline__ RowSoftmax row_softmax(const T* logits, const LogitRows& rows, int64_t n, int t,
-                                                  const float2* part, int parts, float c) {
-  RowSoftmax r;
-  r.M = kFloor;
-  r.s = 0.f;
-  for (int q = 0; q < parts; ++q) {
-    const float2 x = part[n * parts + q];
-    const float m = fmaxf(r.M, x.x);
-    r.s = r.s * term(r.M, c, m) + x.y * term(x.x, c, m);
-    r.M = m;
-  }
-  // a token past the vocabulary shows as NaN
-  r.logp = (int64_t)t < rows.V ? log_prob((float)logits[rows.offset(n) + t], c, r.M, r.s) : __int_as_float(0x7fc00000);
-  return r;
-}
-
-// What the gradient of a row needs: dlogits = 2^(c (z - M)) * q (+ g at the token).
-// A row with g = 0 gets zeros and its logits are not read.
-__device__ __forceinline__ float4 row_gradient(const RowSoftmax& r, float g) {
-  return make_float4(r.M, -g / r.s, g, 0.f);
-}
-
-template <class T>
-__global__ __launch_bounds__(LOSS_THREADS) void loss_grad_kernel(const T* __restrict__ logits, LogitRows rows,
-                                                                 const void* __restrict__ tokens, int token_bytes,
-                                                                 float c, int parts, int64_t chunk,
-                                                                 const float4* __restrict__ coef, T* __restrict__ grad) {
-  constexpr int VEC = 16 / sizeof(T);
-  const int64_t n = blockIdx.x / (unsigned)parts;
-  const int q = (int)(blockIdx.x % (unsigned)parts);
-  const T* row = logits + rows.offset(n);
-  T* out = grad + n * rows.V;
-  const float4 f = coef[n];
-  const int64_t t = load_token(tokens, token_bytes, n);
-  const int64_t from = q * chunk, to = min(from + chunk, rows.V);
-  const bool read = f.z != 0.f;
-  for (int64_t d = from + threadIdx.x * VEC; d < to; d += LOSS_THREADS * VEC) {
-    if (d + VEC <= to) {
-      Pack<T, VEC> x;
-      if (read) {
-        x = load_pack<T, VEC>(row + d);
-        float y[VEC];
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) y[k] = term((float)x.v[k], c, f.x) * f.y;
-        if (t >= d && t < d + VEC)
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) y[k] += t == d + k ? f.z : 0.f;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) x.v[k] = (T)y[k];
-      } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) x.v[k] = (T)0.f;
-      }
-      store_pack(out + d, x);
-    } else {
-      for (int64_t e = d; e < to; ++e)
-        out[e] = (T)(read ? term((float)row[e], c, f.x) * f.y + (t == e ? f.z : 0.f) : 0.f);
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
 // Policy loss
 
 struct PolicyArgs {
@@ -194,48 +96,60 @@ struct PolicyArgs {
   int token_bytes, by_sequence;
 };
 
-constexpr int WEIGHT_THREADS = 1024, WEIGHT_WAVES = WEIGHT_THREADS / 64;
+// weight[b]: 1 / live rows (of all, or with by_sequence of the sequence times the sequences that have any), by one
+// workgroup.  The sequences are taken WEIGHT_HELD at a time, whose counts lie in `held` (LDS); a thread has the
+// flags of eight rows under way at once.
+constexpr int WEIGHT_HELD = 2048, WEIGHT_THREADS = 1024;
 
-// weight[b]: 1 / live rows (of all, or with by_sequence of the sequence times the sequences that have
-// any).  One workgroup, a row a thread; the sequences are taken WEIGHT_HELD at a time, whose counts lie in LDS.
-constexpr int WEIGHT_HELD = 4096;
-
-__global__ __launch_bounds__(WEIGHT_THREADS) void policy_weights_kernel(PolicyArgs a, float* __restrict__ weight) {
-  __shared__ int held[WEIGHT_HELD];
-  __shared__ float red[WEIGHT_WAVES];
-  const int lane = threadIdx.x & 63;
+template <int THREADS>
+__device__ __forceinline__ void policy_weights(const PolicyArgs& a, float* weight, int* held, float* red) {
+  constexpr int AT_ONCE = 8;
   const unsigned T = (unsigned)a.T;
   float total = 0.f, some = 0.f;
   for (int64_t b0 = 0; b0 < a.B; b0 += WEIGHT_HELD) {
     const int B = (int)(a.B - b0 < WEIGHT_HELD ? a.B - b0 : WEIGHT_HELD);
-    for (int b = threadIdx.x; b < B; b += WEIGHT_THREADS) held[b] = 0;
+    for (int b = threadIdx.x; b < B; b += THREADS) held[b] = 0;
     __syncthreads();
     const unsigned rows = B * T;
-    for (unsigned i0 = threadIdx.x - lane; i0 < rows; i0 += WEIGHT_THREADS) {   // 64 rows a wave
-      const unsigned i = i0 + lane, b = i / T;
-      const bool in = i < rows && live_row(a.mask, a.tokens, a.token_bytes, b0 * T + i);
-      const unsigned first = __builtin_amdgcn_readfirstlane(b);
-      if (__ballot(i < rows && b != first) == 0) {
-        const int found = __popcll(__ballot(in));
-        if (lane == 0) atomicAdd(&held[first], found);
-      } else if (in) {
-        atomicAdd(&held[b], 1);
+    for (unsigned i0 = threadIdx.x; i0 < rows + threadIdx.x; i0 += AT_ONCE * THREADS) {
+      bool in[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const unsigned i = i0 + u * THREADS;
+        in[u] = i < rows && live_row(a.mask, a.tokens, a.token_bytes, b0 * T + i);
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const unsigned i = i0 + u * THREADS, b = min(i, rows - 1) / T;
+        const uint64_t found = __ballot(in[u]);
+        const unsigned lo = __builtin_amdgcn_readfirstlane(b), hi = __builtin_amdgcn_readlane(b, 63);
+        if (lo == hi) {   // a wave's 64 rows are mostly one sequence's
+          if ((threadIdx.x & 63) == 0 && found) atomicAdd(&held[lo], __popcll(found));
+        } else if (in[u]) {
+          atomicAdd(&held[b], 1);
+        }
       }
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < B; b += WEIGHT_THREADS) {
+    for (int b = threadIdx.x; b < B; b += THREADS) {
       weight[b0 + b] = (float)held[b];   // read again by the same thread
       total += (float)held[b];
       some += held[b] ? 1.f : 0.f;
     }
     __syncthreads();
   }
-  const float all = block_sum<WEIGHT_WAVES>(a.by_sequence ? some : total, red);
+  const float all = block_sum<THREADS / 64>(a.by_sequence ? some : total, red);
   for (int64_t b0 = 0; b0 < a.B; b0 += WEIGHT_HELD)
-    for (int64_t b = b0 + threadIdx.x; b < a.B && b < b0 + WEIGHT_HELD; b += WEIGHT_THREADS) {
+    for (int64_t b = b0 + threadIdx.x; b < a.B && b < b0 + WEIGHT_HELD; b += THREADS) {
       const float live = weight[b];
       weight[b] = live > 0.f ? 1.f / (a.by_sequence ? live * all : all) : 0.f;
     }
+}
+
+__global__ __launch_bounds__(WEIGHT_THREADS) void policy_weights_kernel(PolicyArgs a, float* weight) {
+  __shared__ int held[WEIGHT_HELD];
+  __shared__ float red[WEIGHT_THREADS / 64];
+  policy_weights<WEIGHT_THREADS>(a, weight, held, red);
 }
 
 struct PolicyRow {
@@ -261,42 +175,46 @@ __device__ __forceinline__ PolicyRow policy_term(float logp, float old, float re
   return r;
 }
 
-__device__ __forceinline__ PolicyRow policy_row(const PolicyArgs& a, int64_t n, float logp) {
-  const int64_t b = div_rows(n, a.T, n < (1LL << 31) && a.T < (1LL << 31));
-  return policy_term(logp, a.old_logp[n], a.ref_logp ? a.ref_logp[n] : 0.f, a.ref_logp != nullptr,
-                     a.advantages[b * a.adv_b + (n - b * a.T) * a.adv_t], a.low, a.high, a.kl_weight);
+// stats: loss, policy term, KL, clipped share
+__device__ __forceinline__ void write_stats(float policy, float kl, float outside, float kl_weight, float* stats) {
+  stats[0] = policy + kl_weight * kl;
+  stats[1] = policy;
+  stats[2] = kl;
+  stats[3] = outside;
 }
 
-// One thread per row: its gradient's coefficients, and the workgroup's share of the sums.
-template <class T>
-__global__ __launch_bounds__(LOSS_THREADS) void policy_rows_kernel(const T* __restrict__ logits, LogitRows rows,
-                                                                   PolicyArgs a, const float2* __restrict__ part,
-                                                                   int parts, const float* __restrict__ weight,
-                                                                   float* __restrict__ logp, float4* __restrict__ coef,
-                                                                   float4* __restrict__ sums) {
-  __shared__ float red[LOSS_WAVES];
-  const int64_t n = (int64_t)blockIdx.x * LOSS_THREADS + threadIdx.x, N = a.B * a.T;
-  float policy = 0.f, kl = 0.f, outside = 0.f;
-  if (n < N) {
-    float lp = 0.f;
-    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live_row(a.mask, a.tokens, a.token_bytes, n)) {
-      const RowSoftmax x = row_softmax(logits, rows, n, load_token(a.tokens, a.token_bytes, n), part, parts, a.c);
-      const PolicyRow r = policy_row(a, n, x.logp);
-      const float w = weight[div_rows(n, a.T, n < (1LL << 31) && a.T < (1LL << 31))];
-      lp = x.logp;
-      policy = w * r.policy;
-      kl = w * r.kl;
-      outside = w * r.outside;
-      f = row_gradient(x, w * r.g * a.inv_t * a.grad_scale);
-    }
-    logp[n] = lp;
-    coef[n] = f;
+// Sums of three values over a workgroup, in a fixed order, in the first thread.
+template <int WAVES>
+__device__ __forceinline__ float3 block_sum3(float x, float y, float z, float4* red) {
+  x = wave_sum(x);
+  y = wave_sum(y);
+  z = wave_sum(z);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float4(x, y, z, 0.f);
+  __syncthreads();
+  float3 r = make_float3(0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    r.x += red[w].x;
+    r.y += red[w].y;
+    r.z += red[w].z;
   }
-  policy = block_sum<LOSS_WAVES>(policy, red);
-  kl = block_sum<LOSS_WAVES>(kl, red);
-  outside = block_sum<LOSS_WAVES>(outside, red);
-  if (threadIdx.x == 0) sums[blockIdx.x] = make_float4(policy, kl, outside, 0.f);
+  return r;
+}
+
+constexpr int STATS_THREADS = 512;
+
+__global__ __launch_bounds__(STATS_THREADS) void policy_stats_kernel(const float4* __restrict__ sums, int64_t count,
+                                                                     float kl_weight, float* __restrict__ stats) {
+  __shared__ float4 red[STATS_THREADS / 64];
+  float policy = 0.f, kl = 0.f, outside = 0.f;
+  for (int64_t i = threadIdx.x; i < count; i += STATS_THREADS) {
+    const float4 x = sums[i];
+    policy += x.x;
+    kl += x.y;
+    outside += x.z;
+  }
+  const float3 r = block_sum3<STATS_THREADS / 64>(policy, kl, outside, red);
+  if (threadIdx.x == 0) write_stats(r.x, r.y, r.z, kl_weight, stats);
 }
 
 // Sixteen bytes of logits as they are.  as_floats keeps the compiler from holding on to the fp32 values of a
@@ -508,24 +426,257 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
   if (threadIdx.x == 0) sums[blockIdx.x] = make_float4(policy, kl, outside, 0.f);
 }
 
-// stats: loss, policy term, KL, clipped share
-__global__ __launch_bounds__(LOSS_THREADS) void policy_stats_kernel(const float4* __restrict__ sums, int64_t count,
-                                                                    float kl_weight, float* __restrict__ stats) {
-  __shared__ float red[LOSS_WAVES];
-  float policy = 0.f, kl = 0.f, outside = 0.f;
-  for (int64_t i = threadIdx.x; i < count; i += LOSS_THREADS) {
-    policy += sums[i].x;
-    kl += sums[i].y;
-    outside += sums[i].z;
+// ---------------------------------------------------------------------------
+// Rows in parts: few rows, so that a workgroup each would leave the device idle, or rows that no workgroup
+// holds.  One launch sums the parts' softmaxes, the next forms the rows' from them and writes the gradient.
+
+// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements); with `weight` one more makes the policy
+// loss's weights.
+template <class T>
+__global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows,
+                                                                    PolicyArgs a, int64_t N, int parts, int64_t chunk,
+                                                                    float2* __restrict__ part,
+                                                                    float* __restrict__ weight) {
+  constexpr int VEC = 16 / sizeof(T);
+  __shared__ float2 red[LOSS_WAVES];
+  const int64_t n = blockIdx.x / (unsigned)parts;
+  if (n == N) {
+    __shared__ int held[WEIGHT_HELD];
+    __shared__ float sum[LOSS_WAVES];
+    policy_weights<LOSS_THREADS>(a, weight, held, sum);
+    return;
   }
-  policy = block_sum<LOSS_WAVES>(policy, red);
-  kl = block_sum<LOSS_WAVES>(kl, red);
-  outside = block_sum<LOSS_WAVES>(outside, red);
+  const int q = (int)(blockIdx.x % (unsigned)parts);
+  if (!live_row(a.mask, a.tokens, a.token_bytes, n)) return;
+  const T* row = logits + rows.offset(n);
+  const int64_t from = q * chunk, to = min(from + chunk, rows.V);
+  float M = kFloor, s = 0.f;
+  int64_t d = from + threadIdx.x * VEC;
+  for (; d + 3 * LOSS_THREADS * VEC + VEC <= to; d += 4 * LOSS_THREADS * VEC) {   // four loads under way
+    Pack<T, VEC> x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = load_pack<T, VEC>(row + d + u * LOSS_THREADS * VEC);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float z[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) z[k] = (float)x[u].v[k];
+      add_terms(M, s, z, a.c);
+    }
+  }
+  for (; d < to; d += LOSS_THREADS * VEC) {
+    float z[VEC];
+    if (d + VEC <= to) {
+      const Pack<T, VEC> x = load_pack<T, VEC>(row + d);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) z[k] = (float)x.v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) z[k] = d + k < to ? (float)row[d + k] : -__builtin_inff();
+    }
+    add_terms(M, s, z, a.c);
+  }
+  const float2 x = block_softmax<LOSS_WAVES>(M, s, a.c, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = x;
+}
+
+// A row's softmax from its parts, by 16 lanes or (ONE part) by each lane for itself, the same in each of them.
+template <bool ONE>
+__device__ __forceinline__ float2 row_softmax(const float2* part, int64_t n, int parts, float c) {
+  if (ONE) return part[n];
+  float M = kFloor, s = 0.f;
+  for (int q = threadIdx.x & 15; q < parts; q += 16) {
+    const float2 x = part[n * parts + q];
+    const float m = fmaxf(M, x.x);
+    s = s * term(M, c, m) + x.y * term(x.x, c, m);
+    M = m;
+  }
+  const float m = row16_max(M);
+  return make_float2(m, row16_sum(s * term(M, c, m)));
+}
+
+// The log-probability of a live row's token; one past the vocabulary shows as NaN.
+template <class T>
+__device__ __forceinline__ float token_logp(const T* logits, const LogitRows& rows, int64_t n, int t, float2 soft,
+                                            float c) {
+  return (int64_t)t < rows.V ? log_prob((float)logits[rows.offset(n) + t], c, soft.x, soft.y)
+                             : __int_as_float(0x7fc00000);
+}
+
+// What the gradient of a row needs: dlogits = 2^(c (z - M)) q (+ g at the token).  A row with g = 0 gets zeros and
+// its logits are not read.
+__device__ __forceinline__ float4 row_gradient(float2 soft, float g) {
+  return make_float4(soft.x, -g / soft.y, g, 0.f);
+}
+
+// The gradient of elements [from, to) of a row, by a workgroup.
+template <class T>
+__device__ __forceinline__ void write_row_gradient(const T* row, T* out, int64_t from, int64_t to, int64_t t, float c,
+                                                   float4 f) {
+  constexpr int VEC = 16 / sizeof(T);
+  const bool read = f.z != 0.f;
+  for (int64_t d = from + threadIdx.x * VEC; d < to; d += LOSS_THREADS * VEC) {
+    if (d + VEC <= to) {
+      Pack<T, VEC> x;
+      if (read) {
+        x = load_pack<T, VEC>(row + d);
+        float y[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) y[k] = term((float)x.v[k], c, f.x) * f.y;
+        if (t >= d && t < d + VEC)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) y[k] += t == d + k ? f.z : 0.f;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x.v[k] = (T)y[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x.v[k] = (T)0.f;
+      }
+      store_pack(out + d, x);
+    } else {
+      for (int64_t e = d; e < to; ++e)
+        out[e] = (T)(read ? term((float)row[e], c, f.x) * f.y + (t == e ? f.z : 0.f) : 0.f);
+    }
+  }
+}
+
+// A live row of the policy loss from its parts: log-probability, terms, and the gradient's coefficients.
+template <bool ONE, class T>
+__device__ __forceinline__ PolicyRow policy_part_row(const T* logits, const LogitRows& rows, const PolicyArgs& a,
+                                                     const float2* part, int parts, int64_t n, int t, float* lp,
+                                                     float2* soft) {
+  const int64_t b = (unsigned)n / (unsigned)a.T;
+  *soft = row_softmax<ONE>(part, n, parts, a.c);
+  *lp = token_logp(logits, rows, n, t, *soft, a.c);
+  return policy_term(*lp, a.old_logp[n], a.ref_logp ? a.ref_logp[n] : 0.f, a.ref_logp != nullptr,
+                     a.advantages[b * a.adv_b + (n - b * a.T) * a.adv_t], a.low, a.high, a.kl_weight);
+}
+
+// Workgroup = (row, part): its gradient; the last one: every row's log-probability, and the sums.
+template <bool ONE, class T>
+__global__ __launch_bounds__(LOSS_THREADS) void policy_part_kernel(const T* __restrict__ logits, LogitRows rows,
+                                                                   PolicyArgs a, int64_t N, int parts, int64_t chunk,
+                                                                   const float2* __restrict__ part,
+                                                                   const float* __restrict__ weight,
+                                                                   float* __restrict__ logp, float* __restrict__ stats,
+                                                                   T* __restrict__ grad) {
+  if (blockIdx.x == gridDim.x - 1) {
+    constexpr int LANES = ONE ? 1 : 16, ROWS = LOSS_THREADS / LANES;   // rows at a time, and lanes of a row
+    __shared__ float4 red[LOSS_WAVES];
+    float policy = 0.f, kl = 0.f, outside = 0.f;
+    for (int64_t n0 = 0; n0 < N; n0 += ROWS) {
+      const int64_t n = n0 + threadIdx.x / LANES;
+      const bool first = threadIdx.x % LANES == 0;
+      if (n >= N) continue;   // 16 lanes together
+      float lp = 0.f;
+      if (live_row(a.mask, a.tokens, a.token_bytes, n)) {
+        float2 soft;
+        const PolicyRow r = policy_part_row<ONE>(logits, rows, a, part, parts, n, load_token(a.tokens, a.token_bytes, n),
+                                                 &lp, &soft);
+        const float w = first ? weight[(unsigned)n / (unsigned)a.T] : 0.f;
+        if (first) {
+          policy += w * r.policy;
+          kl += w * r.kl;
+          outside += w * r.outside;
+        }
+      }
+      if (first) logp[n] = lp;
+    }
+    const float3 r = block_sum3<LOSS_WAVES>(policy, kl, outside, red);
+    if (threadIdx.x == 0) write_stats(r.x, r.y, r.z, a.kl_weight, stats);
+    return;
+  }
+  const int64_t n = blockIdx.x / (unsigned)parts;
+  const int q = (int)(blockIdx.x % (unsigned)parts);
+  const int t = load_token(a.tokens, a.token_bytes, n);
+  float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live_row(a.mask, a.tokens, a.token_bytes, n)) {
+    float lp;
+    float2 soft;
+    const PolicyRow r = policy_part_row<ONE>(logits, rows, a, part, parts, n, t, &lp, &soft);
+    f = row_gradient(soft, weight[(unsigned)n / (unsigned)a.T] * r.g * a.inv_t * a.grad_scale);
+  }
+  write_row_gradient(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V), (int64_t)t,
+                     a.c, f);
+}
+
+// ---------------------------------------------------------------------------
+// Short rows (a controller's few actions, a small vocabulary): LANES lanes a row, 1 or 16, which go over its
+// elements twice (the second time from the caches).  ALONE: one workgroup does everything, weights and sums included, in
+// one launch.
+constexpr int SHORT_ONE = 16, SHORT_MOST = 512;   // the longest rows of one lane, and of sixteen
+
+template <bool ALONE, int LANES, class T>
+__global__ __launch_bounds__(ALONE ? WEIGHT_THREADS : LOSS_THREADS) void policy_short_kernel(
+    const T* __restrict__ logits, LogitRows rows, PolicyArgs a, float* weight, float* __restrict__ logp,
+    float* __restrict__ stats, T* __restrict__ grad, float4* __restrict__ sums) {
+  constexpr int THREADS = ALONE ? WEIGHT_THREADS : LOSS_THREADS, WAVES = THREADS / 64, VEC = LANES == 1 ? 1 : 16 / sizeof(T);
+  __shared__ float4 red[WAVES];
+  if constexpr (ALONE) {
+    __shared__ int held[WEIGHT_HELD];
+    __shared__ float sum[WAVES];
+    policy_weights<THREADS>(a, weight, held, sum);
+    __syncthreads();   // weight[] is read by other threads of the workgroup than wrote it
+  }
+  const int N = (int)(a.B * a.T), V = (int)rows.V, lane = threadIdx.x % LANES;
+  const float c = a.c;
+  float policy = 0.f, kl = 0.f, outside = 0.f;
+  for (int n = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES; n < N; n += gridDim.x * (THREADS / LANES)) {
+    const T* row = logits + rows.offset(n);
+    T* out = grad + (int64_t)n * V;
+    const int t = load_token(a.tokens, a.token_bytes, n);
+    float lp = 0.f, g = 0.f, q = 0.f, M = kFloor, s = 0.f;
+    if (live_row(a.mask, a.tokens, a.token_bytes, n)) {   // the same in a row's lanes
+      const unsigned b = (unsigned)n / (unsigned)a.T;
+      const float old = a.old_logp[n], ref = a.ref_logp ? a.ref_logp[n] : 0.f, w = weight[b];
+      const float A = a.advantages[b * a.adv_b + (n - b * (unsigned)a.T) * a.adv_t];
+      const float zt = t < V ? (float)row[t] : 0.f;
+      for (int d = lane * VEC; d < V; d += LANES * VEC) {
+        float z[VEC];
+        if (d + VEC <= V) {
+          const Pack<T, VEC> x = load_pack<T, VEC>(row + d);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z[e] = (float)x.v[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z[e] = d + e < V ? (float)row[d + e] : -__builtin_inff();
+        }
+        add_terms(M, s, z, c);
+      }
+      if (LANES > 1) {
+        const float m = row16_max(M);
+        s = row16_sum(s * term(M, c, m));
+        M = m;
+      }
+      lp = t < V ? log_prob(zt, c, M, s) : __int_as_float(0x7fc00000);
+      const PolicyRow r = policy_term(lp, old, ref, a.ref_logp != nullptr, A, a.low, a.high, a.kl_weight);
+      if (lane == 0) {
+        policy += w * r.policy;
+        kl += w * r.kl;
+        outside += w * r.outside;
+      }
+      g = w * r.g * a.inv_t * a.grad_scale;
+      q = -g / s;
+    }
+    if (lane == 0) logp[n] = lp;
+    if (grad)
+      for (int d = lane * VEC; d < V; d += LANES * VEC) {
+        if (d + VEC <= V) {
+          Pack<T, VEC> x;
+          if (g != 0.f) x = load_pack<T, VEC>(row + d);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            x.v[e] = (T)(g != 0.f ? term((float)x.v[e], c, M) * q + (t == d + e ? g : 0.f) : 0.f);
+          store_pack(out + d, x);
+        } else {
+          for (int e = d; e < V; ++e) out[e] = (T)(g != 0.f ? term((float)row[e], c, M) * q + (t == e ? g : 0.f) : 0.f);
+        }
+      }
+  }
+  const float3 r = block_sum3<WAVES>(policy, kl, outside, red);
   if (threadIdx.x == 0) {
-    stats[0] = policy + kl_weight * kl;
-    stats[1] = policy;
-    stats[2] = kl;
-    stats[3] = outside;
+    if (ALONE) write_stats(r.x, r.y, r.z, a.kl_weight, stats);
+    else sums[blockIdx.x] = make_float4(r.x, r.y, r.z, 0.f);
   }
 }
 
@@ -545,35 +696,58 @@ struct PreferenceArgs {
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
 
-// One workgroup per pair: the rows' log-probabilities, the responses' sums, the pair's loss, and the
-// rows' gradient coefficients.
-template <class T>
-__global__ __launch_bounds__(LOSS_THREADS) void preference_pairs_kernel(
+// Rows [from, to) of response k.  Offsets are data: whatever they hold, the rows are the batch's.
+__device__ __forceinline__ int2 response_rows(const PreferenceArgs& a, int64_t k) {
+  const int64_t from = min(max(a.offsets[k], (int64_t)0), a.N);
+  return make_int2((int)from, (int)min(max(a.offsets[k + 1], from), a.N));
+}
+
+constexpr int PAIR_THREADS = 1024, PAIR_WAVES = PAIR_THREADS / 64;
+
+// One workgroup per pair: the rows' log-probabilities, the responses' sums, the pair's loss, and the rows' gradient
+// coefficients; one more clears the rows of no response.
+template <bool ONE, class T>
+__global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(
     const T* __restrict__ logits, LogitRows rows, PreferenceArgs a, const float2* __restrict__ part, int parts, float c,
     float* __restrict__ logp, float4* __restrict__ coef, float* __restrict__ rewards, float* __restrict__ losses) {
-  __shared__ float red[LOSS_WAVES];
+  constexpr int LANES = ONE ? 1 : 16, ROWS = PAIR_THREADS / LANES;
+  __shared__ float red[PAIR_WAVES];
   const int64_t pair = blockIdx.x;
+  const int lane = threadIdx.x % LANES;
+  if (pair == a.pairs) {
+    const int from = a.pairs ? response_rows(a, 0).x : (int)a.N;
+    const int to = a.pairs ? response_rows(a, 2 * a.pairs - 1).y : (int)a.N;
+    const int outside = from + (int)a.N - to;
+    for (int i = threadIdx.x; i < outside; i += PAIR_THREADS) {
+      const int n = i < from ? i : i - from + to;
+      logp[n] = 0.f;
+      coef[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    return;
+  }
   float sum[2];
-  int64_t from[2], to[2];
+  int2 of[2];
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    const int64_t k = pair + side * a.pairs;
-    // offsets are data: whatever they hold, the rows read are the batch's
-    from[side] = min(max(a.offsets[k], (int64_t)0), a.N);
-    to[side] = min(max(a.offsets[k + 1], from[side]), a.N);
+    of[side] = response_rows(a, pair + side * a.pairs);
     float s = 0.f;
-    for (int64_t n = from[side] + threadIdx.x; n < to[side]; n += LOSS_THREADS) {
+    for (int n = of[side].x + threadIdx.x / LANES; n < of[side].y; n += ROWS) {
       const int t = load_token(a.tokens, a.token_bytes, n);
+      const float ref = a.ref_logp[n];
       float lp = 0.f;
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);   // s of the row in y, until the pair's g is known
       if (t >= 0) {
-        const RowSoftmax x = row_softmax(logits, rows, n, t, part, parts, c);
-        lp = x.logp;
-        s += lp - a.ref_logp[n];
-        coef[n] = make_float4(x.M, x.s, 0.f, 0.f);
+        const float2 soft = row_softmax<ONE>(part, n, parts, c);
+        lp = token_logp(logits, rows, n, t, soft, c);
+        if (lane == 0) s += lp - ref;
+        f = make_float4(soft.x, soft.y, 1.f, 0.f);
       }
-      logp[n] = lp;
+      if (lane == 0) {
+        logp[n] = lp;
+        coef[n] = f;
+      }
     }
-    sum[side] = block_sum<LOSS_WAVES>(s, red);
+    sum[side] = block_sum<PAIR_WAVES>(s, red);
   }
   const float h = a.beta * sum[0] - a.beta * sum[1];
   const float dh = -((1.f - a.smoothing) * sigmoid(-h) - a.smoothing * sigmoid(h));
@@ -583,29 +757,34 @@ __global__ __launch_bounds__(LOSS_THREADS) void preference_pairs_kernel(
     losses[pair] = -((1.f - a.smoothing) * log_sigmoid(h) + a.smoothing * log_sigmoid(-h));
   }
   const float g = dh * a.beta * a.grad_scale / (float)a.pairs;
+  if (lane) return;
 #pragma unroll
   for (int side = 0; side < 2; ++side)
-    for (int64_t n = from[side] + threadIdx.x; n < to[side]; n += LOSS_THREADS)
-      if (load_token(a.tokens, a.token_bytes, n) >= 0) {   // coef[n]: written by this thread above
-        const float4 f = coef[n];
-        coef[n] = row_gradient(RowSoftmax{f.x, f.y, 0.f}, side ? -g : g);
-      }
+    for (int n = of[side].x + threadIdx.x / LANES; n < of[side].y; n += ROWS) {
+      const float4 f = coef[n];   // written by this thread above
+      if (f.z != 0.f) coef[n] = row_gradient(make_float2(f.x, f.y), side ? -g : g);
+    }
 }
 
-__global__ void preference_clear_kernel(int64_t N, float* __restrict__ logp, float4* __restrict__ coef) {
-  const int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= N) return;
-  logp[n] = 0.f;
-  coef[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-}
-
-__global__ __launch_bounds__(LOSS_THREADS) void preference_loss_kernel(const float* __restrict__ losses, int64_t pairs,
-                                                                       float* __restrict__ loss) {
-  __shared__ float red[LOSS_WAVES];
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < pairs; i += LOSS_THREADS) s += losses[i];
-  s = block_sum<LOSS_WAVES>(s, red);
-  if (threadIdx.x == 0) *loss = pairs ? s / (float)pairs : 0.f;
+// Workgroup = (row, part): its gradient from the row's coefficients; the last one sums the pairs' losses.
+template <class T>
+__global__ __launch_bounds__(LOSS_THREADS) void preference_grad_kernel(const T* __restrict__ logits, LogitRows rows,
+                                                                       PreferenceArgs a, int parts, int64_t chunk, float c,
+                                                                       const float4* __restrict__ coef,
+                                                                       const float* __restrict__ losses,
+                                                                       float* __restrict__ loss, T* __restrict__ grad) {
+  if (blockIdx.x == gridDim.x - 1) {
+    __shared__ float red[LOSS_WAVES];
+    float s = 0.f;
+    for (int64_t i = threadIdx.x; i < a.pairs; i += LOSS_THREADS) s += losses[i];
+    s = block_sum<LOSS_WAVES>(s, red);
+    if (threadIdx.x == 0) *loss = a.pairs ? s / (float)a.pairs : 0.f;
+    return;
+  }
+  const int64_t n = blockIdx.x / (unsigned)parts;
+  const int q = (int)(blockIdx.x % (unsigned)parts);
+  write_row_gradient(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V),
+                     (int64_t)load_token(a.tokens, a.token_bytes, n), c, coef[n]);
 }
 
 // ---------------------------------------------------------------------------
@@ -656,6 +835,9 @@ static int with_row_group(int64_t vecs, F f) {
   return 0;
 }
 
+// Workgroups whose sums are kept.
+constexpr int64_t SUM_GROUPS = 4096;
+
 static bool rows_fit(int64_t N, int64_t V) { return V < (1LL << 30) && N < (1LL << 24); }
 
 }  // namespace bf
@@ -664,17 +846,10 @@ using namespace bf;
 
 extern "C" {
 
-// the sums of the row kernel's workgroups, or of 256 rows each
-static int64_t sum_groups(int64_t N) {
-  const int64_t parts = ceil_div(N, LOSS_THREADS), groups = N < 4096 ? N : 4096;
-  return parts > groups ? parts : groups;
-}
-
-// coef [N] float4, part [N * parts] float2, sums float4, weight [B]
+// sums of the workgroups (row kernel, short rows), or part [N * parts] float2; weight [B]
 int64_t bf_policy_loss_workspace(int64_t B, int64_t T, int64_t V, int elem) {
   if (!elem_ok(elem) || B < 0 || T < 0 || V <= 0) return 0;
-  const int64_t N = B * T;
-  return 4 * N + 2 * N * row_parts(N, V, elem).count + 4 * sum_groups(N) + B;
+  return 4 * SUM_GROUPS + 2 * B * T * row_parts(B * T, V, elem).count + B;
 }
 
 int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V, int64_t ld_b, int64_t ld_t,
@@ -688,79 +863,94 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
              "bf_policy_loss: bad sizes");
   BF_REQUIRE(temperature > 0.0 && clip_low >= 0.f && clip_high >= 0.f, "bf_policy_loss: temperature %g, clip %g, %g",
              temperature, clip_low, clip_high);
-  BF_REQUIRE(stats, "bf_policy_loss: null pointer");
-  const int64_t N = B * T;
-  BF_REQUIRE(N == 0 || (logits && tokens && old_logp && advantages && logp && workspace),
-             "bf_policy_loss: null pointer");
-  if (!rows_fit(N, V) || B >= (1LL << 24) || T >= (1LL << 24)) {
-    set_error("bf_policy_loss: %lld rows of %lld logits: rows below 2^24, logits below 2^30", (long long)N,
+  BF_REQUIRE(stats && workspace, "bf_policy_loss: null pointer");
+  if (!rows_fit(B * T, V) || B >= (1LL << 24) || T >= (1LL << 24)) {
+    set_error("bf_policy_loss: %lld rows of %lld logits: rows below 2^24, logits below 2^30", (long long)(B * T),
               (long long)V);
     return BF_ERANGE;
   }
-  PolicyArgs a{tokens, old_logp, ref_logp, advantages, static_cast<const uint8_t*>(mask), B, T, adv_b, adv_t,
-               1.f - clip_low, 1.f + clip_high, kl_weight, (float)(1.4426950408889634074 / temperature),
-               (float)(1.0 / temperature), grad_scale, token_bytes, by_sequence};
+  const int64_t N = B * T;
+  BF_REQUIRE(N == 0 || (logits && tokens && old_logp && advantages && logp), "bf_policy_loss: null pointer");
+  const PolicyArgs a{tokens, old_logp, ref_logp, advantages, static_cast<const uint8_t*>(mask), B, T, adv_b, adv_t,
+                     1.f - clip_low, 1.f + clip_high, kl_weight, (float)(1.4426950408889634074 / temperature),
+                     (float)(1.0 / temperature), grad_scale, token_bytes, by_sequence};
   const LogitRows rows{T > 0 ? T : 1, ld_b, ld_t, V};
+  float4* sums = reinterpret_cast<float4*>(workspace);
+  float2* part = reinterpret_cast<float2*>(sums + SUM_GROUPS);
   const Parts p = row_parts(N, V, elem);
-  float4* coef = reinterpret_cast<float4*>(workspace);
-  float4* sums = coef + N;
-  const int64_t blocks = ceil_div(N, LOSS_THREADS);
-  float2* part = reinterpret_cast<float2*>(sums + sum_groups(N));
   float* weight = reinterpret_cast<float*>(part + N * p.count);
-  if (N * p.count >= (1LL << 31)) {
-    set_error("bf_policy_loss: %lld rows of %lld logits are too many", (long long)N, (long long)V);
-    return BF_ERANGE;
-  }
-  if (N > 0) {
-    hipLaunchKernelGGL(policy_weights_kernel, dim3(1), dim3(WEIGHT_THREADS), 0, stream, a, weight);
-    BF_LAUNCH_CHECK("policy_weights_kernel");
-    if (N >= 256) {
-      int64_t groups = 0;
-      const int rc = with_elem(elem, [&](auto e) -> int {
-        using E = decltype(e);
-        return with_row_group(V / (16 / (int)sizeof(E)), [&](auto threads, auto nv, auto full) -> int {
-          // as many workgroups as the device holds; each goes through its rows
-          constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value;
-          const int64_t most = 256 * (TH == 64 ? 16 : TH == 256 ? 6 : TH == 512 ? 2 : 1);
-          groups = N < most ? N : most;
-          auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(TH), 0, stream, static_cast<const E*>(logits), rows, a,
-                               weight, logp, static_cast<E*>(grad), sums, (unsigned)(groups * 0.6180339887498949));
-          };
-          if (grad) launch(policy_row_kernel<true, E, TH, NV, decltype(full)::value>);
-          else launch(policy_row_kernel<false, E, TH, NV, decltype(full)::value>);
-          BF_LAUNCH_CHECK("policy_row_kernel");
-          return BF_OK;
-        });
+  const bool shorts = V <= (elem == TE_F32 ? SHORT_MOST / 2 : SHORT_MOST);
+  const int lanes = V <= SHORT_ONE ? 1 : 16;
+  return with_elem(elem, [&](auto e) -> int {
+    using E = decltype(e);
+    const E* x = static_cast<const E*>(logits);
+    E* out = static_cast<E*>(grad);
+    // one workgroup for what takes it four turns at most: a launch, and the gap before it, costs as much as two
+    if (N == 0 || (shorts && N * lanes <= 4 * WEIGHT_THREADS)) {
+      if (lanes == 1)
+        hipLaunchKernelGGL((policy_short_kernel<true, 1, E>), dim3(1), dim3(WEIGHT_THREADS), 0, stream, x, rows, a,
+                           weight, logp, stats, out, sums);
+      else
+        hipLaunchKernelGGL((policy_short_kernel<true, 16, E>), dim3(1), dim3(WEIGHT_THREADS), 0, stream, x, rows, a,
+                           weight, logp, stats, out, sums);
+      BF_LAUNCH_CHECK("policy_short_kernel");
+      return BF_OK;
+    }
+    int64_t groups = 0;
+    auto weights = [&] {
+      hipLaunchKernelGGL(policy_weights_kernel, dim3(1), dim3(WEIGHT_THREADS), 0, stream, a, weight);
+    };
+    if (shorts) {
+      weights();
+      groups = ceil_div(N * lanes, LOSS_THREADS);
+      if (groups > 256 * 8) groups = 256 * 8;
+      if (lanes == 1)
+        hipLaunchKernelGGL((policy_short_kernel<false, 1, E>), dim3((unsigned)groups), dim3(LOSS_THREADS), 0, stream, x,
+                           rows, a, weight, logp, stats, out, sums);
+      else
+        hipLaunchKernelGGL((policy_short_kernel<false, 16, E>), dim3((unsigned)groups), dim3(LOSS_THREADS), 0, stream, x,
+                           rows, a, weight, logp, stats, out, sums);
+      BF_LAUNCH_CHECK("policy_short_kernel");
+    } else if (N >= 256) {
+      const int rc = with_row_group(V / (16 / (int)sizeof(E)), [&](auto threads, auto nv, auto full) -> int {
+        // as many workgroups as the device holds; each goes through its rows
+        constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, FULL = decltype(full)::value;
+        const int64_t most = 256 * (TH == 64 ? 16 : TH == 256 ? 6 : TH == 512 ? 2 : 1);
+        groups = N < most ? N : most;
+        weights();
+        auto launch = [&](auto kernel) {
+          hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(TH), 0, stream, x, rows, a, weight, logp, out, sums,
+                             (unsigned)(groups * 0.6180339887498949));
+        };
+        if (grad) launch(policy_row_kernel<true, E, TH, NV, FULL>);
+        else launch(policy_row_kernel<false, E, TH, NV, FULL>);
+        BF_LAUNCH_CHECK("policy_row_kernel");
+        return BF_OK;
       });
       if (rc != BF_OK) return rc;
-      if (groups) {
-        hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(LOSS_THREADS), 0, stream, sums, groups, kl_weight, stats);
-        BF_LAUNCH_CHECK("policy_stats_kernel");
-        return BF_OK;
-      }
     }
-    const int rc = with_elem(elem, [&](auto e) -> int {
-      using E = decltype(e);
-      const E* x = static_cast<const E*>(logits);
-      hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows,
-                         tokens, token_bytes, a.mask, a.c, p.count, p.chunk, part);
-      BF_LAUNCH_CHECK("loss_partial_kernel");
-      hipLaunchKernelGGL(policy_rows_kernel<E>, dim3((unsigned)blocks), dim3(LOSS_THREADS), 0, stream, x, rows, a, part,
-                         p.count, weight, logp, coef, sums);
-      BF_LAUNCH_CHECK("policy_rows_kernel");
-      if (grad) {
-        hipLaunchKernelGGL(loss_grad_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows,
-                           tokens, token_bytes, a.c, p.count, p.chunk, coef, static_cast<E*>(grad));
-        BF_LAUNCH_CHECK("loss_grad_kernel");
-      }
+    if (groups) {
+      hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(STATS_THREADS), 0, stream, sums, groups, kl_weight, stats);
+      BF_LAUNCH_CHECK("policy_stats_kernel");
       return BF_OK;
-    });
-    if (rc != BF_OK) return rc;
-  }
-  hipLaunchKernelGGL(policy_stats_kernel, dim3(1), dim3(LOSS_THREADS), 0, stream, sums, blocks, kl_weight, stats);
-  BF_LAUNCH_CHECK("policy_stats_kernel");
-  return BF_OK;
+    }
+    if ((N + 1) * p.count >= (1LL << 31)) {
+      set_error("bf_policy_loss: %lld rows of %lld logits are too many", (long long)N, (long long)V);
+      return BF_ERANGE;
+    }
+    hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count + 1)), dim3(LOSS_THREADS), 0, stream, x, rows, a,
+                       N, p.count, p.chunk, part, weight);
+    BF_LAUNCH_CHECK("loss_partial_kernel");
+    const unsigned grid = grad ? (unsigned)(N * p.count + 1) : 1u;
+    if (p.count == 1)
+      hipLaunchKernelGGL((policy_part_kernel<true, E>), dim3(grid), dim3(LOSS_THREADS), 0, stream, x, rows, a, N, p.count,
+                         p.chunk, part, weight, logp, stats, out);
+    else
+      hipLaunchKernelGGL((policy_part_kernel<false, E>), dim3(grid), dim3(LOSS_THREADS), 0, stream, x, rows, a, N,
+                         p.count, p.chunk, part, weight, logp, stats, out);
+    BF_LAUNCH_CHECK("policy_part_kernel");
+    return BF_OK;
+  });
 }
 
 // coef [N] float4, part [N * parts] float2, losses [pairs]
@@ -779,48 +969,43 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
   BF_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, "bf_preference_loss: label smoothing %g", smoothing);
   BF_REQUIRE(loss && (pairs == 0 || (offsets && rewards && workspace)), "bf_preference_loss: null pointer");
   BF_REQUIRE(N == 0 || (logits && tokens && ref_logp && logp && workspace), "bf_preference_loss: null pointer");
-  if (!rows_fit(N, V) || pairs >= (1LL << 24)) {
+  const Parts p = row_parts(N, V, elem);
+  if (!rows_fit(N, V) || pairs >= (1LL << 24) || (N + 1) * p.count >= (1LL << 31)) {
     set_error("bf_preference_loss: %lld rows of %lld logits, %lld pairs: rows and pairs below 2^24, logits below 2^30",
               (long long)N, (long long)V, (long long)pairs);
     return BF_ERANGE;
   }
   const PreferenceArgs a{tokens, ref_logp, offsets, N, pairs, beta, smoothing, grad_scale, token_bytes};
   const LogitRows rows{N > 0 ? N : 1, 0, ld, V};
-  const Parts p = row_parts(N, V, elem);
   const float c = 1.4426950408889634f;
   float4* coef = reinterpret_cast<float4*>(workspace);
   float2* part = reinterpret_cast<float2*>(coef + N);
   float* losses = reinterpret_cast<float*>(part + N * p.count);
-  if (N * p.count >= (1LL << 31)) {
-    set_error("bf_preference_loss: %lld rows of %lld logits are too many", (long long)N, (long long)V);
-    return BF_ERANGE;
-  }
-  const int rc = with_elem(elem, [&](auto e) -> int {
+  return with_elem(elem, [&](auto e) -> int {
     using E = decltype(e);
     const E* x = static_cast<const E*>(logits);
     if (N > 0) {
-      hipLaunchKernelGGL(preference_clear_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, stream, N, logp, coef);
-      BF_LAUNCH_CHECK("preference_clear_kernel");
-      hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows,
-                         tokens, token_bytes, nullptr, c, p.count, p.chunk, part);
+      PolicyArgs all = {};
+      all.tokens = tokens;
+      all.token_bytes = token_bytes;
+      all.c = c;
+      hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows, all,
+                         N, p.count, p.chunk, part, nullptr);
       BF_LAUNCH_CHECK("loss_partial_kernel");
     }
-    if (pairs > 0) {
-      hipLaunchKernelGGL(preference_pairs_kernel<E>, dim3((unsigned)pairs), dim3(LOSS_THREADS), 0, stream, x, rows, a,
-                         part, p.count, c, logp, coef, rewards, losses);
-      BF_LAUNCH_CHECK("preference_pairs_kernel");
-    }
-    if (N > 0 && grad) {
-      hipLaunchKernelGGL(loss_grad_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows,
-                         tokens, token_bytes, c, p.count, p.chunk, coef, static_cast<E*>(grad));
-      BF_LAUNCH_CHECK("loss_grad_kernel");
-    }
+    if (p.count == 1)
+      hipLaunchKernelGGL((preference_pairs_kernel<true, E>), dim3((unsigned)pairs + 1), dim3(PAIR_THREADS), 0, stream, x,
+                         rows, a, part, p.count, c, logp, coef, rewards, losses);
+    else
+      hipLaunchKernelGGL((preference_pairs_kernel<false, E>), dim3((unsigned)pairs + 1), dim3(PAIR_THREADS), 0, stream, x,
+                         rows, a, part, p.count, c, logp, coef, rewards, losses);
+    BF_LAUNCH_CHECK("preference_pairs_kernel");
+    const unsigned grid = grad ? (unsigned)(N * p.count + 1) : 1u;
+    hipLaunchKernelGGL(preference_grad_kernel<E>, dim3(grid), dim3(LOSS_THREADS), 0, stream, x, rows, a, p.count, p.chunk, c,
+                       coef, losses, loss, static_cast<E*>(grad));
+    BF_LAUNCH_CHECK("preference_grad_kernel");
     return BF_OK;
   });
-  if (rc != BF_OK) return rc;
-  hipLaunchKernelGGL(preference_loss_kernel, dim3(1), dim3(LOSS_THREADS), 0, stream, losses, pairs, loss);
-  BF_LAUNCH_CHECK("preference_loss_kernel");
-  return BF_OK;
 }
 
 }  // extern "C"

@@ -17,12 +17,13 @@ No counterpart in the reference, which bounds networks and does not train them.
 
 from __future__ import annotations
 
+import ctypes
 from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import HipError, ptr
+from ._lib import HipError, current_raw_stream
 
 _ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TOKEN_BYTES = {torch.int32: 4, torch.int64: 8}
@@ -30,38 +31,55 @@ _TOKEN_BYTES = {torch.int32: 4, torch.int64: 8}
 MOMENT_BLOCK = 128   # elements of an 8-bit moment that share a scale; every tensor's moments start at a multiple
 
 
-def _device(t: torch.Tensor, name: str) -> None:
+# Every call checks a dozen tensors before a kernel of a few microseconds: the checks are plain
+# attribute reads, and addresses go to the library as numbers (the tensors are this module's
+# callers' or its own locals until the call has enqueued its kernels).
+
+def _current_device(t: torch.Tensor, name: str) -> int:
+    """The device of the call's first tensor, which has to be the current one."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise HipError(f"{name} must be a HIP device tensor (the backend has no CPU path)")
-    if t.get_device() != torch.cuda.current_device():
+    dev = t.get_device()
+    if dev != torch.cuda.current_device():
+        raise HipError(f"{name} is on {t.device}, not on the current device")
+    return dev
+
+
+def _on_device(t: torch.Tensor, dev: int, name: str) -> None:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise HipError(f"{name} must be a HIP device tensor (the backend has no CPU path)")
+    if t.get_device() != dev:
         raise HipError(f"{name} is on {t.device}, not on the current device")
 
 
 def _elem(t: torch.Tensor, name: str) -> int:
-    _device(t, name)
     code = _ELEM.get(t.dtype)
     if code is None:
         raise HipError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
 
 
-def _tokens(t: torch.Tensor, shape, name: str = "tokens") -> Tuple[torch.Tensor, int]:
-    _device(t, name)
+def _tokens(t: torch.Tensor, shape, dev: int) -> Tuple[torch.Tensor, int]:
+    _on_device(t, dev, "tokens")
     size = _TOKEN_BYTES.get(t.dtype)
     if size is None:
-        raise HipError(f"{name} must be int32 or int64, got {t.dtype}")
+        raise HipError(f"tokens must be int32 or int64, got {t.dtype}")
     if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t.contiguous(), size
+        raise ValueError(f"tokens of shape {tuple(t.shape)}, expected {tuple(shape)}")
+    return t if t.is_contiguous() else t.contiguous(), size
 
 
-def _floats(t: torch.Tensor, shape, name: str) -> torch.Tensor:
-    _device(t, name)
+def _floats(t: torch.Tensor, shape, dev: int, name: str) -> torch.Tensor:
+    _on_device(t, dev, name)
     if t.dtype != torch.float32:
         raise HipError(f"{name} must be float32, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _address(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 # ---------------------------------------------------------------------------
@@ -72,15 +90,19 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.
 
     table [vocab, dim], rows contiguous (any row stride); tokens int32 or int64 of any shape.  A
     negative token is padding and gives zeros, one past the table gives NaN."""
+    dev = _current_device(table, "table")
     elem = _elem(table, "table")
-    if table.dim() != 2 or (table.stride(1) != 1 and table.shape[1] > 1) or table.stride(0) < table.shape[1]:
+    if table.dim() != 2:
+        raise HipError(f"table must be [vocab, dim], got {tuple(table.shape)}")
+    vocab, dim = table.shape
+    ld, step = table.stride()
+    if (step != 1 and dim > 1) or ld < dim:
         raise HipError(f"table must be [vocab, dim] with contiguous rows, got {tuple(table.shape)} with strides "
                        f"{table.stride()}")
-    tokens, token_bytes = _tokens(tokens, None)
-    vocab, dim = table.shape
-    out = torch.empty(*tokens.shape, dim, dtype=table.dtype, device=table.device)
-    _lib.call("bf_embed_rows", ptr(table), table.stride(0), vocab, ptr(tokens), token_bytes, tokens.numel(), dim,
-              float(scale), elem, ptr(out), _lib.stream_handle())
+    tokens, token_bytes = _tokens(tokens, None, dev)
+    out = torch.empty((*tokens.shape, dim), dtype=table.dtype, device=table.device)
+    _lib.call("bf_embed_rows", table.data_ptr(), ld, vocab, tokens.data_ptr(), token_bytes, tokens.numel(), dim,
+              float(scale), elem, out.data_ptr(), current_raw_stream(dev))
     return out
 
 
@@ -94,8 +116,11 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
     float32).  With ``accumulate_into`` (float32 [vocab, dim], contiguous) the sums are added to
     it in place and it is returned; rows without a token are not touched.  Tokens outside of
     [0, vocab) take no part."""
+    dev = _current_device(grad, "grad")
     elem = _elem(grad, "grad")
-    tokens, token_bytes = _tokens(tokens, grad.shape[:-1])
+    if grad.dim() < 1:
+        raise ValueError("grad must be [*tokens.shape, dim]")
+    tokens, token_bytes = _tokens(tokens, grad.shape[:-1], dev)
     dim, count, vocab = grad.shape[-1], tokens.numel(), int(vocab)
     if vocab < 0:
         raise ValueError(f"vocab must be >= 0, got {vocab}")
@@ -103,7 +128,7 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
     if (dim > 1 and rows.stride(1) != 1) or (count > 1 and rows.stride(0) < dim):
         rows = rows.contiguous()
     if accumulate_into is not None:
-        _floats(accumulate_into, (vocab, dim), "accumulate_into")
+        _floats(accumulate_into, (vocab, dim), dev, "accumulate_into")
         if not accumulate_into.is_contiguous():
             raise HipError("accumulate_into must be contiguous")
         if dtype not in (None, torch.float32):
@@ -115,9 +140,9 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
             raise ValueError(f"dtype must be {grad.dtype} or float32, got {dtype}")
         out = torch.empty(vocab, dim, dtype=dtype, device=grad.device)
     space = torch.empty(_lib.load().bf_embed_grad_workspace(count, vocab, dim), device=grad.device)
-    _lib.call("bf_embed_grad", ptr(rows), max(rows.stride(0), dim), elem, ptr(tokens), token_bytes, count, vocab, dim,
-              float(scale), _ELEM[out.dtype], int(accumulate_into is not None), ptr(out), ptr(space),
-              _lib.stream_handle())
+    _lib.call("bf_embed_grad", rows.data_ptr(), max(rows.stride(0), dim), elem, tokens.data_ptr(), token_bytes, count,
+              vocab, dim, float(scale), _ELEM[out.dtype], accumulate_into is not None, out.data_ptr(), space.data_ptr(),
+              current_raw_stream(dev))
     if accumulate_into is not None:
         torch.autograd.graph.increment_version(out)
     return out
@@ -147,12 +172,6 @@ class PreferenceLoss(NamedTuple):
     grad_logits: Optional[torch.Tensor]
 
 
-def _rows_of(logits: torch.Tensor) -> torch.Tensor:
-    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
-        raise HipError(f"logits need a contiguous last axis, got strides {logits.stride()}")
-    return logits
-
-
 def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
                 ref_logp: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, clip_low: float = 0.2,
                 clip_high: float = 0.2, kl_weight: float = 0.0, temperature: float = 1.0, reduction: str = "token",
@@ -170,53 +189,56 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
     sequences of each one's mean (``"sequence"``).  A row is live unless it is masked or its token
     is negative; the others are not read, and logp and gradient are 0 there.  A batch without a live
     row has loss 0.  ``grad_logits`` is ``grad_scale`` times the loss's gradient, of the logits' type."""
+    dev = _current_device(logits, "logits")
     elem = _elem(logits, "logits")
-    if logits.dim() not in (2, 3) or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [B, T, V] or [N, V] with V >= 1, got {tuple(logits.shape)}")
+    shape = logits.shape
+    dims = len(shape)
+    if dims not in (2, 3) or shape[-1] < 1:
+        raise ValueError(f"logits must be [B, T, V] or [N, V] with V >= 1, got {tuple(shape)}")
     if reduction not in ("token", "sequence"):
         raise ValueError(f"unknown reduction: {reduction}")
     if not temperature > 0.0:
         raise ValueError(f"temperature must be >0, got {temperature}")
     if not (clip_low >= 0.0 and clip_high >= 0.0):
         raise ValueError(f"clip limits must be >=0, got {clip_low}, {clip_high}")
-    _rows_of(logits)
-    lead = logits.shape[:-1]
-    V = logits.shape[-1]
-    if logits.dim() == 3:
-        B, T = lead
-        ld_b, ld_t = logits.stride(0), logits.stride(1)
-    else:
-        B, T = lead[0], 1
-        ld_b, ld_t = logits.stride(0), 0
-    tokens, token_bytes = _tokens(tokens, lead)
-    old_logp = _floats(old_logp, lead, "old_logp")
+    strides = logits.stride()
+    lead, V = shape[:-1], shape[-1]
+    if strides[-1] != 1 and V > 1:
+        raise HipError(f"logits need a contiguous last axis, got strides {strides}")
+    B, T = (lead[0], lead[1]) if dims == 3 else (lead[0], 1)
+    tokens, token_bytes = _tokens(tokens, lead, dev)
+    old_logp = _floats(old_logp, lead, dev, "old_logp")
     if ref_logp is not None:
-        ref_logp = _floats(ref_logp, lead, "ref_logp")
-    _device(advantages, "advantages")
+        ref_logp = _floats(ref_logp, lead, dev, "ref_logp")
+    _on_device(advantages, dev, "advantages")
     if advantages.dtype != torch.float32:
         raise HipError(f"advantages must be float32, got {advantages.dtype}")
     if advantages.shape == lead:
-        adv_b, adv_t = advantages.stride(0), advantages.stride(1) if logits.dim() == 3 else 0
+        adv = advantages.stride()
+        adv_b, adv_t = (adv[0], adv[1]) if dims == 3 else (adv[0], 0)
     elif advantages.shape == (B,):
         adv_b, adv_t = advantages.stride(0), 0
     else:
         raise ValueError(f"advantages of shape {tuple(advantages.shape)}, expected {tuple(lead)} or ({B},)")
     if mask is not None:
-        _device(mask, "mask")
+        _on_device(mask, dev, "mask")
         if mask.dtype != torch.bool:
             raise HipError(f"mask must be bool, got {mask.dtype}")
         if mask.shape != lead:
             raise ValueError(f"mask of shape {tuple(mask.shape)}, expected {tuple(lead)}")
-        mask = mask.contiguous()
-    dev = logits.device
-    out = torch.empty(4 + B * T, device=dev)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if with_grad else None
-    space = torch.empty(_lib.load().bf_policy_loss_workspace(B, T, V, elem), device=dev)
-    _lib.call("bf_policy_loss", ptr(logits), elem, B, T, V, ld_b, ld_t, ptr(tokens), token_bytes, ptr(old_logp),
-              ptr(ref_logp), ptr(advantages), adv_b, adv_t, ptr(mask), float(clip_low), float(clip_high),
-              float(kl_weight), float(temperature), int(reduction == "sequence"), float(grad_scale), ptr(out[4:]),
-              ptr(out), ptr(grad), ptr(space), _lib.stream_handle())
-    return PolicyLoss(out[:4], out[4:].view(lead), grad)
+        if not mask.is_contiguous():
+            mask = mask.contiguous()
+    # stats, logp and the workspace in one allocation
+    N = B * T
+    out = torch.empty(4 + N + 3 + _lib.load().bf_policy_loss_workspace(B, T, V, elem), device=logits.device)
+    grad = torch.empty(shape, dtype=logits.dtype, device=logits.device) if with_grad else None
+    at = out.data_ptr()
+    _lib.call("bf_policy_loss", logits.data_ptr(), elem, B, T, V, strides[0], strides[1] if dims == 3 else 0,
+              tokens.data_ptr(), token_bytes, old_logp.data_ptr(), _address(ref_logp), advantages.data_ptr(), adv_b, adv_t,
+              _address(mask), float(clip_low), float(clip_high), float(kl_weight), float(temperature),
+              reduction == "sequence", float(grad_scale), at + 16,
+              at, _address(grad), at + 16 + (N + 3) // 4 * 16, current_raw_stream(dev))
+    return PolicyLoss(out[:4], out[4:4 + N].view(lead), grad)
 
 
 def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.Tensor, offsets: torch.Tensor, *,
@@ -233,32 +255,36 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.
         loss = mean over pairs of -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h).
 
     Rows of no response and rows of a negative token take no part (logp and gradient 0)."""
+    dev = _current_device(logits, "logits")
     elem = _elem(logits, "logits")
     if logits.dim() != 2 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [N, V] with V >= 1, got {tuple(logits.shape)}")
-    _rows_of(logits)
+    N, V = logits.shape
+    ld, step = logits.stride()
+    if step != 1 and V > 1:
+        raise HipError(f"logits need a contiguous last axis, got strides {logits.stride()}")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
-    N, V = logits.shape
-    tokens, token_bytes = _tokens(tokens, (N,))
-    ref_logp = _floats(ref_logp, (N,), "ref_logp")
-    _device(offsets, "offsets")
+    tokens, token_bytes = _tokens(tokens, (N,), dev)
+    ref_logp = _floats(ref_logp, (N,), dev, "ref_logp")
+    _on_device(offsets, dev, "offsets")
     if offsets.dtype != torch.int64:
         raise HipError(f"offsets must be int64, got {offsets.dtype}")
     if offsets.dim() != 1 or offsets.numel() % 2 == 0:
         raise ValueError(f"offsets must be [2 * pairs + 1], got {tuple(offsets.shape)}")
-    offsets = offsets.contiguous()
+    if not offsets.is_contiguous():
+        offsets = offsets.contiguous()
     pairs = offsets.numel() // 2
-    dev = logits.device
-    # loss, rewards and logp in one allocation
-    out = torch.empty(1 + 2 * pairs + N, device=dev)
-    logp = out[1 + 2 * pairs:]
-    grad = torch.empty(N, V, dtype=logits.dtype, device=dev) if with_grad else None
-    space = torch.empty(_lib.load().bf_preference_loss_workspace(N, V, pairs, elem), device=dev)
-    _lib.call("bf_preference_loss", ptr(logits), elem, N, V, logits.stride(0), ptr(tokens), token_bytes, ptr(ref_logp),
-              ptr(offsets), pairs, float(beta), float(label_smoothing), float(grad_scale), ptr(logp), ptr(out[1:]),
-              ptr(out), ptr(grad), ptr(space), _lib.stream_handle())
-    return PreferenceLoss(out[0], out[1:1 + 2 * pairs], logp, grad)
+    # loss, rewards, logp and the workspace in one allocation
+    own = 1 + 2 * pairs + N
+    out = torch.empty(own + 3 + _lib.load().bf_preference_loss_workspace(N, V, pairs, elem), device=logits.device)
+    grad = torch.empty((N, V), dtype=logits.dtype, device=logits.device) if with_grad else None
+    at = out.data_ptr()
+    _lib.call("bf_preference_loss", logits.data_ptr(), elem, N, V, ld, tokens.data_ptr(), token_bytes,
+              ref_logp.data_ptr(), offsets.data_ptr(), pairs, float(beta), float(label_smoothing), float(grad_scale),
+              at + 4 + 8 * pairs, at + 4,
+              at, _address(grad), at + (own + 3) // 4 * 16, current_raw_stream(dev))
+    return PreferenceLoss(out[0], out[1:1 + 2 * pairs], out[1 + 2 * pairs:own], grad)
 
 
 # ---------------------------------------------------------------------------
@@ -294,6 +320,7 @@ def adamw_moments(params: Sequence[torch.Tensor], *, bits: int = 32, master: boo
     if not params:
         raise ValueError("no parameters")
     for k, p in enumerate(params):
+        _on_device(p, _current_device(params[0], "params[0]"), f"params[{k}]")
         _elem(p, f"params[{k}]")
     dev = params[0].device
     at = moment_offsets([p.numel() for p in params])
@@ -330,12 +357,15 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
         raise ValueError(f"betas must be in [0, 1) and eps >=0, got {betas}, {eps}")
+    dev = _current_device(params[0], "params[0]")
+    _on_device(grads[0], dev, "grads[0]")
     p_elem, g_elem = _elem(params[0], "params[0]"), _elem(grads[0], "grads[0]")
-    p_type, g_type, dev = params[0].dtype, grads[0].dtype, params[0].device
+    p_type, g_type = params[0].dtype, grads[0].dtype
     sizes, total = [], 0
     for k, (p, g) in enumerate(zip(params, grads)):
-        if p.dtype != p_type or g.dtype != g_type or p.device != dev or g.device != dev:
-            raise HipError(f"params[{k}] and grads[{k}] must be {p_type} and {g_type} on {dev}, as the first are")
+        if p.dtype != p_type or g.dtype != g_type or p.get_device() != dev or g.get_device() != dev:
+            raise HipError(f"params[{k}] and grads[{k}] must be {p_type} and {g_type} on {params[0].device}, as the "
+                           "first are")
         if p.shape != g.shape:
             raise ValueError(f"params[{k}] of shape {tuple(p.shape)}, grads[{k}] of {tuple(g.shape)}")
         if not (p.is_contiguous() and g.is_contiguous()):
@@ -346,30 +376,37 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     m, v, m_scale, v_scale, master = moments
     eight = m_scale is not None or v_scale is not None
     kind = torch.float8_e4m3fn if eight else torch.float32
-    expected = [("m", m, kind, total), ("v", v, kind, total)]
+    _moment(m, "m", kind, total, dev)
+    _moment(v, "v", kind, total, dev)
     if eight:
-        expected += [("m_scale", m_scale, torch.float32, total // MOMENT_BLOCK),
-                     ("v_scale", v_scale, torch.float32, total // MOMENT_BLOCK)]
+        _moment(m_scale, "m_scale", torch.float32, total // MOMENT_BLOCK, dev)
+        _moment(v_scale, "v_scale", torch.float32, total // MOMENT_BLOCK, dev)
     if master is not None:
-        expected.append(("master", master, torch.float32, total))
-    for name, t, want, length in expected:
-        if t is None:
-            raise ValueError(f"moments.{name} is missing")
-        _device(t, f"moments.{name}")
-        if t.dtype != want:
-            raise HipError(f"moments.{name} must be {want}, got {t.dtype}")
-        if t.numel() != length or not t.is_contiguous():
-            raise ValueError(f"moments.{name} must be flat of {length} elements, got {tuple(t.shape)}")
-    factor, factor_dev = grad_scale, None
+        _moment(master, "master", torch.float32, total, dev)
+    factor_dev = None
     if isinstance(grad_scale, torch.Tensor):
-        _device(grad_scale, "grad_scale")
+        _on_device(grad_scale, dev, "grad_scale")
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
             raise HipError("grad_scale must be a float32 scalar")
-        factor, factor_dev = 1.0, grad_scale
-    _lib.call("bf_adamw_multi", len(sizes), _lib.ptr_array(params), _lib.ptr_array(grads), _lib.i64_array(sizes), p_elem,
-              g_elem, ptr(m), ptr(v), ptr(m_scale), ptr(v_scale), ptr(master), float(lr), float(b1), float(b2),
-              float(eps), float(weight_decay), int(step), float(factor), ptr(factor_dev), _lib.stream_handle())
+        factor_dev, grad_scale = grad_scale.data_ptr(), 1.0
+    count = len(sizes)
+    pointers, lengths = ctypes.c_void_p * count, ctypes.c_int64 * count
+    _lib.call("bf_adamw_multi", count, pointers(*[p.data_ptr() for p in params]),
+              pointers(*[g.data_ptr() for g in grads]), lengths(*sizes), p_elem, g_elem, m.data_ptr(), v.data_ptr(),
+              _address(m_scale), _address(v_scale), _address(master), float(lr), float(b1), float(b2), float(eps),
+              float(weight_decay), int(step), float(grad_scale),
+              factor_dev, current_raw_stream(dev))
     torch.autograd.graph.increment_version([*params, *(t for t in moments if t is not None)])
+
+
+def _moment(t: Optional[torch.Tensor], name: str, kind: torch.dtype, length: int, dev: int) -> None:
+    if t is None:
+        raise ValueError(f"moments.{name} is missing")
+    _on_device(t, dev, f"moments.{name}")
+    if t.dtype != kind:
+        raise HipError(f"moments.{name} must be {kind}, got {t.dtype}")
+    if t.numel() != length or not t.is_contiguous():
+        raise ValueError(f"moments.{name} must be flat of {length} elements, got {tuple(t.shape)}")
 
 
 class AdamW:
