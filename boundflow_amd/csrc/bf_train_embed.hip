@@ -43,127 +43,159 @@ __global__ void embed_rows_kernel(const T* __restrict__ table, int64_t ld, int v
 }
 
 // ---------------------------------------------------------------------------
-// Sorting: a stable counting sort in one launch.  Workgroup b owns the tokens [b R, b R + R);
-// it reads every token (a training batch's fit in the L2 of each XCD), counts those below its
-// range, which is where its part of the order begins, and those of each of its values per wave, and
-// places them.  Each of its waves reads a contiguous slice of the tokens, so equal tokens keep
-// their order: slice by slice, and within 64 tokens lane by lane.
-constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64, SORT_RANGE = 512;
+// Sorting: a stable counting sort of the tokens of values [v0, v0 + held), by one workgroup.  It reads every token (a
+// training batch's fit in the L2 of each XCD), counts those of each of its values per wave, and places their
+// positions.  Each wave reads a contiguous slice of the tokens, so equal tokens keep their order: slice by
+// slice, and within 64 tokens lane by lane.  A thread has SORT_HELD tokens under way at once; where that is all
+// of them, they are read once.
+constexpr int SORT_HELD = 16, SORT_RANGE = 512;
 
-inline int sort_range(int64_t vocab) {
-  const int64_t r = ceil_div(vocab, 256);
-  return (int)(r < SORT_RANGE ? r : SORT_RANGE);
-}
+template <int WAVES, int RANGE>
+struct SortSpace {
+  int place[WAVES][RANGE];   // tokens of a value that a wave has, then where its next one goes
+  int sums[WAVES], below[WAVES];
+};
 
-__global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(const void* __restrict__ tokens, int token_bytes,
-                                                                  int count, int vocab, int range,
-                                                                  int* __restrict__ start, int* __restrict__ order) {
-  __shared__ int place[SORT_WAVES][SORT_RANGE];
-  __shared__ int sums[SORT_WAVES], below[SORT_WAVES];
+// f(position, i): token i's position among the range's.  begin(k, position, count): value v0 + k's part of them,
+// called by one thread each; positions count from the number of tokens below v0 (BELOW) or from 0.
+template <int WAVES, int RANGE, bool BELOW, class F, class G>
+__device__ __forceinline__ void sort_range(const void* tokens, int token_bytes, int count, int v0, int held,
+                                           SortSpace<WAVES, RANGE>& s, F f, G begin) {
+  constexpr int THREADS = WAVES * 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int v0 = blockIdx.x * range, held = min(range, vocab - v0);
-  for (int k = tid; k < SORT_WAVES * SORT_RANGE; k += SORT_THREADS) (&place[0][0])[k] = 0;
+  for (int k = tid; k < WAVES * RANGE; k += THREADS) (&s.place[0][0])[k] = 0;
   __syncthreads();
-  const int slice = (int)(ceil_div(count, SORT_THREADS) * 64);
+  const int slice = (count + THREADS - 1) / THREADS * 64;
   const int from = min(wave * slice, count), to = min(from + slice, count);
-  int less = 0;
-  for (int i = from + lane; i < to; i += 64) {
-    const int t = load_token(tokens, token_bytes, i);
-    if (t >= 0 && t < v0) ++less;
-    if (t >= v0 && t < v0 + held) atomicAdd(&place[wave][t - v0], 1);
-  }
+  int t[SORT_HELD];
+  const auto load = [&](int i0) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1) less += __shfl_xor(less, d);
-  if (lane == 0) below[wave] = less;
+    for (int u = 0; u < SORT_HELD; ++u) {
+      const int i = i0 + u * 64 + lane;
+      t[u] = i < to ? load_token(tokens, token_bytes, i) : -1;
+    }
+  };
+  int less = 0;
+  for (int i0 = from; i0 < to; i0 += SORT_HELD * 64) {
+    load(i0);
+#pragma unroll
+    for (int u = 0; u < SORT_HELD; ++u) {
+      if (BELOW && t[u] >= 0 && t[u] < v0) ++less;
+      if (t[u] >= v0 && t[u] < v0 + held) atomicAdd(&s.place[wave][t[u] - v0], 1);
+    }
+  }
+  if (BELOW) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) less += __shfl_xor(less, d);
+    if (lane == 0) s.below[wave] = less;
+  }
   __syncthreads();
-  // thread k < range: the number of tokens of value v0 + k, and its exclusive sum over k
+  // thread k < RANGE: the number of tokens of value v0 + k, and its exclusive sum over k
   int total = 0;
-  if (tid < range)
-    for (int w = 0; w < SORT_WAVES; ++w) total += place[w][tid];
+  if (tid < RANGE)
+    for (int w = 0; w < WAVES; ++w) total += s.place[w][tid];
   int incl = total;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int x = __shfl_up(incl, d);
     if (lane >= d) incl += x;
   }
-  if (lane == 63) sums[wave] = incl;
+  if (lane == 63) s.sums[wave] = incl;
   __syncthreads();
   int base = incl - total;
-  for (int w = 0; w < SORT_WAVES; ++w) {
-    base += below[w];
-    if (w < wave) base += sums[w];
+  for (int w = 0; w < WAVES; ++w) {
+    if (BELOW) base += s.below[w];
+    if (w < wave) base += s.sums[w];
   }
-  if (tid < range) {
-    if (tid < held) start[v0 + tid] = base;
-    if (tid == held - 1 && v0 + held == vocab) start[vocab] = base + total;
-    for (int w = 0; w < SORT_WAVES; ++w) {
-      const int n = place[w][tid];
-      place[w][tid] = base;
+  if (tid < held) begin(tid, base, total);
+  if (tid < RANGE)
+    for (int w = 0; w < WAVES; ++w) {
+      const int n = s.place[w][tid];
+      s.place[w][tid] = base;
       base += n;
     }
-  }
   __syncthreads();
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const int i = i0 + lane;
-    const int t = i < to ? load_token(tokens, token_bytes, i) : -1;
-    const int k = t >= v0 && t < v0 + held ? t - v0 : -1;
-    uint64_t todo = __ballot(k >= 0);
-    while (todo) {   // one value of the 64 tokens at a time
-      const int lead = __ffsll((unsigned long long)todo) - 1;
-      const int k0 = __builtin_amdgcn_readlane(k, lead);
-      const uint64_t same = __ballot(k == k0);
-      if (k == k0) {
-        const int at = place[wave][k0] + __popcll(same & ((1ull << lane) - 1));
-        order[at] = i;
+  for (int i0 = from; i0 < to; i0 += SORT_HELD * 64) {
+    if (slice > SORT_HELD * 64) load(i0);   // else they are still held
+#pragma unroll
+    for (int u = 0; u < SORT_HELD; ++u) {
+      const bool in = t[u] >= v0 && t[u] < v0 + held;
+      uint64_t same = __ballot(in);
+      if (same == 0) continue;
+      // the lanes of this lane's value: those that agree with it in every bit
+      const int k = in ? t[u] - v0 : 0;
+#pragma unroll
+      for (int b = 1; b < RANGE; b <<= 1) {
+        const uint64_t ones = __ballot(k & b);
+        same &= k & b ? ones : ~ones;
       }
-      // the wave's own counter: no other wave touches it, and a wave's LDS accesses keep their order
-      if (lane == lead) place[wave][k0] += __popcll(same);
+      // the counters are the wave's own: no other wave touches them, and a wave's LDS accesses keep their order
+      if (in) {
+        const int at = s.place[wave][k], before = __popcll(same & ((1ull << lane) - 1));
+        f(at + before, i0 + u * 64 + lane);
+        if (before == 0) s.place[wave][k] = at + __popcll(same);
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      todo &= ~same;
     }
   }
 }
 
-// ---------------------------------------------------------------------------
-// Sums.  A value that occurs at most PIECE times is summed by the workgroups of its row; a more
-// frequent one is cut at the multiples of PIECE of the sorted order, every part summed by a
-// workgroup of its own and the parts added in order, so a token that is half of the batch does not
-// leave one workgroup with half of the work.
-constexpr int PIECE = 64;
-constexpr int SUM_THREADS = 256;
+constexpr int SORT_WAVES = 16;
 
+// start[v]: the first place of value v's tokens in order[], start[vocab]: the end
+__global__ __launch_bounds__(SORT_WAVES * 64) void embed_sort_kernel(const void* __restrict__ tokens, int token_bytes,
+                                                                    int count, int vocab, int range,
+                                                                    int* __restrict__ start, int* __restrict__ order) {
+  __shared__ SortSpace<SORT_WAVES, SORT_RANGE> space;
+  const int v0 = blockIdx.x * range, held = min(range, vocab - v0);
+  sort_range<SORT_WAVES, SORT_RANGE, true>(
+      tokens, token_bytes, count, v0, held, space, [&](int at, int i) { order[at] = i; },
+      [&](int k, int at, int n) {
+        start[v0 + k] = at;
+        if (v0 + k == vocab - 1) start[vocab] = at + n;
+      });
+}
+
+// ---------------------------------------------------------------------------
+// Sums.
+
+// acc += rows list[first .. first + n) (lane l holds list[l]), columns d .. d + VEC of each lane; four tokens' rows
+// under way together
 template <class TI, int VEC>
-__device__ __forceinline__ void add_rows(float (&acc)[VEC], const TI* __restrict__ g, int64_t ld, const int* order,
-                                         int from, int to, int d0, int dim) {
-  if (d0 + VEC <= dim) {
-    int p = from;
-    for (; p + 4 <= to; p += 4) {
-      Pack<TI, VEC> x[4];
+__device__ __forceinline__ void add_rows(float (&acc)[VEC], const TI* __restrict__ g, int64_t ld, int list, int first,
+                                         int n, int d, int dim) {
+  const auto load = [&](int p) {
+    const TI* at = g + (int64_t)__builtin_amdgcn_readlane(list, first + p) * ld + d;
+    Pack<TI, VEC> x;
+    if (d + VEC <= dim) {
+      x = load_pack<TI, VEC>(at);
+    } else {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = load_pack<TI, VEC>(g + order[p + u] * ld + d0);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += (float)x[u].v[k];
+      for (int k = 0; k < VEC; ++k) x.v[k] = d + k < dim ? at[k] : (TI)0.f;
     }
-    for (; p < to; ++p) {
-      const Pack<TI, VEC> x = load_pack<TI, VEC>(g + order[p] * ld + d0);
+    return x;
+  };
+  int p = 0;
+  for (; p + 4 <= n; p += 4) {
+    Pack<TI, VEC> x[4];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += (float)x.v[k];
-    }
-  } else {
-    for (int p = from; p < to; ++p)
+    for (int u = 0; u < 4; ++u) x[u] = load(p + u);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        if (d0 + k < dim) acc[k] += (float)g[order[p] * ld + d0 + k];
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += (float)x[u].v[k];
+  }
+  for (; p < n; ++p) {
+    const Pack<TI, VEC> x = load(p);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] += (float)x.v[k];
   }
 }
 
 // `into` (fp32): the sums are added to it, and rows without a token stay as they are.
 template <class TO, int VEC>
-__device__ __forceinline__ void write_row(const float (&acc)[VEC], float scale, bool into, TO* __restrict__ o, int d0,
-                                          int dim) {
-  if (d0 + VEC <= dim) {
+__device__ __forceinline__ void write_row(const float (&acc)[VEC], float scale, bool into, TO* __restrict__ o, int left) {
+  if (left >= VEC) {
     Pack<TO, VEC> y;
     if (into) y = load_pack<TO, VEC>(o);
 #pragma unroll
@@ -172,68 +204,171 @@ __device__ __forceinline__ void write_row(const float (&acc)[VEC], float scale, 
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
-      if (d0 + k < dim) o[k] = (TO)((into ? (float)o[k] : 0.f) + acc[k] * scale);
+      if (k < left) o[k] = (TO)((into ? (float)o[k] : 0.f) + acc[k] * scale);
   }
 }
 
-// Workgroups below `row_groups`: a wave per (row, 64 VEC columns).  The others: one per piece of the
-// sorted order and 256 VEC columns, for the frequent values that cross it; a piece has at most two
-// (one that ends in it and one that begins in it), whose sums go to part[piece][0] and [1].
+// A value that occurs at most PIECE times is summed with the ROWS rows of its workgroup: the starts of all eight come
+// in one load and the positions of all their tokens in another, so a workgroup waits three times and not
+// three times a row.  A more frequent value is cut at the multiples of PIECE of the sorted order, every part
+// summed by a workgroup of its own and the parts added in order, so a token that is half of the batch does not
+// leave one workgroup with half of the work.
+constexpr int SUM_THREADS = 256, SUM_WAVES = SUM_THREADS / 64;
+constexpr int ROWS = 8, PIECE = 64 / ROWS;
+
+// Workgroups below `pieces`: one per piece, for the frequent values that cross it; a piece has at most two (one that
+// ends in it and one that begins in it), whose sums go to part[piece][0] and [1]; owner[piece]: the one that begins.
+// The others: one per ROWS rows.
 template <class TI, class TO, int VEC>
 __global__ __launch_bounds__(SUM_THREADS) void embed_sum_kernel(
     const TI* __restrict__ g, int64_t ld, const void* __restrict__ tokens, int token_bytes,
-    const int* __restrict__ start, const int* __restrict__ order, int vocab, int dim, int wave_chunks, int64_t row_groups,
-    int group_chunks, float scale, int into, TO* __restrict__ out, float* __restrict__ part) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if ((int64_t)blockIdx.x < row_groups) {
-    const int64_t at = (int64_t)blockIdx.x * (SUM_THREADS / 64) + wave;
-    const int64_t v = div_rows(at, wave_chunks, at < (1LL << 31));
-    if (v >= vocab) return;
-    const int d0 = ((int)(at - v * wave_chunks) * 64 + lane) * VEC;
-    const int from = start[v], to = start[v + 1];
-    if (to - from > PIECE || (into && to == from) || d0 >= dim) return;
-    float acc[VEC] = {};
-    add_rows<TI, VEC>(acc, g, ld, order, from, to, d0, dim);
-    write_row<TO, VEC>(acc, scale, into, out + v * dim + d0, d0, dim);
+    const int* __restrict__ start, const int* __restrict__ order, int vocab, int dim, int pieces, float scale, int into,
+    TO* __restrict__ out, int* __restrict__ owner, float* __restrict__ part) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = (dim + 64 * VEC - 1) / (64 * VEC);
+  if ((int)blockIdx.x >= pieces) {
+    const int v0 = ((int)blockIdx.x - pieces) * ROWS;
+    const int v = min(v0 + lane / PIECE, vocab - 1);
+    const int from = start[v], number = start[v + 1] - from;
+    const int list = lane % PIECE < number ? order[from + lane % PIECE] : 0;
+    for (int k = 0; k < ROWS && v0 + k < vocab; ++k) {
+      const int n = __builtin_amdgcn_readlane(number, k * PIECE);
+      if (n > PIECE || (into && n == 0)) continue;
+      TO* row = out + (int64_t)(v0 + k) * dim;
+      for (int c = wave; c < chunks; c += SUM_WAVES) {
+        const int d = (c * 64 + lane) * VEC;
+        float acc[VEC] = {};
+        add_rows<TI, VEC>(acc, g, ld, list, k * PIECE, n, d, dim);
+        write_row<TO, VEC>(acc, scale, into, row + d, dim - d);
+      }
+    }
     return;
   }
-  const int64_t at = (int64_t)blockIdx.x - row_groups;
-  const int piece = (int)(at / group_chunks);
-  const int d0 = ((int)(at % group_chunks) * SUM_THREADS + (int)threadIdx.x) * VEC;
-  const int total = start[vocab], p0 = piece * PIECE, p1 = min(p0 + PIECE, total);
-  if (p0 >= total || d0 >= dim) return;
-  const int first = load_token(tokens, token_bytes, order[p0]), last = load_token(tokens, token_bytes, order[p1 - 1]);
+  const int piece = blockIdx.x, total = start[vocab], p0 = piece * PIECE, p1 = min(p0 + PIECE, total);
+  if (p0 >= total) {
+    if (threadIdx.x == 0) owner[piece] = -1;
+    return;
+  }
+  const int mine = p0 + lane < p1 ? order[p0 + lane] : 0;
+  const int first = load_token(tokens, token_bytes, __builtin_amdgcn_readfirstlane(mine));
+  const int last = load_token(tokens, token_bytes, __builtin_amdgcn_readlane(mine, p1 - 1 - p0));
+  const int first_end = start[first + 1], first_all = first_end - start[first];
+  const int last_from = start[last], last_all = start[last + 1] - last_from;
+  if (threadIdx.x == 0) owner[piece] = last_all > PIECE && last_from >= p0 ? last : -1;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    const int v = side ? last : first;
-    const int from = start[v], to = start[v + 1];
-    if (to - from <= PIECE || (side && first == last)) continue;
-    float acc[VEC] = {};
-    add_rows<TI, VEC>(acc, g, ld, order, max(from, p0), min(to, p1), d0, dim);
-    float* o = part + ((int64_t)piece * 2 + side) * dim + d0;
-    for (int k = 0; k < VEC && d0 + k < dim; ++k) o[k] = acc[k];
+    if ((side ? last_all : first_all) <= PIECE || (side && first == last)) continue;
+    const int from = side ? last_from - p0 : 0, to = side ? p1 - p0 : min(first_end, p1) - p0;
+    float* row = part + ((int64_t)piece * 2 + side) * dim;
+    for (int c = wave; c < chunks; c += SUM_WAVES) {
+      const int d = (c * 64 + lane) * VEC;
+      float acc[VEC] = {};
+      add_rows<TI, VEC>(acc, g, ld, mine, from, to - from, d, dim);
+      write_row<float, VEC>(acc, 1.f, false, row + d, dim - d);
+    }
   }
 }
 
-// One workgroup per piece and 256 columns: where a frequent value begins in the piece, its parts
-// are added in order.
+// Where a frequent value begins in a piece, its parts are added in order, a quarter of them by each quarter of the
+// workgroup and the quarters together.  Workgroup = (JOIN_PIECES pieces, 256 columns).
+constexpr int JOIN_PIECES = 8, JOIN_PARTS = 4, JOIN_COLUMNS = 256;
+
 template <class TO>
-__global__ __launch_bounds__(SUM_THREADS) void embed_join_kernel(const void* __restrict__ tokens, int token_bytes,
-                                                                 const int* __restrict__ start,
-                                                                 const int* __restrict__ order, int vocab, int dim,
-                                                                 int group_chunks, float scale, int into,
-                                                                 TO* __restrict__ out, const float* __restrict__ part) {
-  const int piece = blockIdx.x / group_chunks;
-  const int d = (blockIdx.x % group_chunks) * SUM_THREADS + threadIdx.x;
-  const int total = start[vocab], p0 = piece * PIECE, p1 = min(p0 + PIECE, total);
-  if (p0 >= total || d >= dim) return;
-  const int v = load_token(tokens, token_bytes, order[p1 - 1]);   // a value that begins here reaches its end
-  const int from = start[v], to = start[v + 1];
-  if (to - from <= PIECE || from < p0) return;
-  const int first = load_token(tokens, token_bytes, order[p0]);
-  float acc[1] = {part[((int64_t)piece * 2 + (first == v ? 0 : 1)) * dim + d]};
-  for (int q = piece + 1; q * PIECE < to; ++q) acc[0] += part[(int64_t)q * 2 * dim + d];
-  write_row<TO, 1>(acc, scale, into, out + (int64_t)v * dim + d, d, dim);
+__global__ __launch_bounds__(JOIN_PARTS * JOIN_COLUMNS) void embed_join_kernel(
+    const void* __restrict__ tokens, int token_bytes, const int* __restrict__ start, const int* __restrict__ order, int dim,
+    int pieces, int columns, float scale, int into, const int* __restrict__ owner, TO* __restrict__ out,
+    const float* __restrict__ part) {
+  __shared__ float sums[JOIN_PARTS][JOIN_COLUMNS];
+  const int piece0 = blockIdx.x / (unsigned)columns * JOIN_PIECES, lane = threadIdx.x & 63;
+  const int x = threadIdx.x % JOIN_COLUMNS, quarter = threadIdx.x / JOIN_COLUMNS;
+  const int d = (blockIdx.x % (unsigned)columns) * JOIN_COLUMNS + x;
+  const int mine = lane < JOIN_PIECES && piece0 + lane < pieces ? owner[piece0 + lane] : -1;
+  uint64_t todo = __ballot(mine >= 0);   // the same in every wave
+  while (todo) {
+    const int k = __ffsll((unsigned long long)todo) - 1, piece = piece0 + k;
+    todo &= todo - 1;
+    const int v = __builtin_amdgcn_readlane(mine, k);
+    const int count = (start[v + 1] - 1) / PIECE - piece + 1, each = (count + JOIN_PARTS - 1) / JOIN_PARTS;
+    float acc = 0.f;
+    if (d < dim) {
+      const int end = min((quarter + 1) * each, count);
+      int q = quarter * each;
+      if (q == 0) {   // the value is its first piece's last, and the others' first
+        const int first = load_token(tokens, token_bytes, order[piece * PIECE]);
+        acc = part[((int64_t)piece * 2 + (first == v ? 0 : 1)) * dim + d];
+        q = 1;
+      }
+#pragma unroll 8
+      for (; q < end; ++q) acc += part[(int64_t)(piece + q) * 2 * dim + d];
+    }
+    sums[quarter][x] = acc;
+    __syncthreads();
+    if (quarter == 0 && d < dim) {
+      float sum[1] = {0.f};
+#pragma unroll
+      for (int w = 0; w < JOIN_PARTS; ++w) sum[0] += sums[w][x];
+      write_row<TO, 1>(sum, scale, into, out + (int64_t)v * dim + d, 1);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens: everything in one launch.  A workgroup sorts the tokens of its rows into LDS and sums them, a wave per
+// row; rows of more than FEW_ALONE tokens are taken by all its waves, a part each.
+constexpr int FEW_TOKENS = 2048, FEW_WAVES = 8, FEW_RANGE = 128, FEW_ALONE = 8;
+
+template <class TI, class TO, int VEC>
+__global__ __launch_bounds__(FEW_WAVES * 64) void embed_few_kernel(const TI* __restrict__ g, int64_t ld,
+                                                                  const void* __restrict__ tokens, int token_bytes,
+                                                                  int count, int vocab, int dim, int range, float scale,
+                                                                  int into, TO* __restrict__ out) {
+  __shared__ SortSpace<FEW_WAVES, FEW_RANGE> space;
+  __shared__ int order[FEW_TOKENS], begin[FEW_RANGE], number[FEW_RANGE];
+  __shared__ float sums[2][FEW_WAVES][64 * VEC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunks = (dim + 64 * VEC - 1) / (64 * VEC);
+  const int v0 = blockIdx.x * range, held = min(range, vocab - v0);
+  sort_range<FEW_WAVES, FEW_RANGE, false>(
+      tokens, token_bytes, count, v0, held, space, [&](int at, int i) { order[at] = i; },
+      [&](int k, int at, int n) {
+        begin[k] = at;
+        number[k] = n;
+      });
+  __syncthreads();
+  // (row, chunk of 64 VEC columns) pairs, a wave each
+  for (int x = wave; x < held * chunks; x += FEW_WAVES) {
+    const int k = (unsigned)x / (unsigned)chunks, c = x - k * chunks;
+    const int n = __builtin_amdgcn_readfirstlane(number[k]);
+    if (n > FEW_ALONE || (into && n == 0)) continue;
+    const int list = lane < n ? order[begin[k] + lane] : 0, d = (c * 64 + lane) * VEC;
+    float acc[VEC] = {};
+    add_rows<TI, VEC>(acc, g, ld, list, 0, n, d, dim);
+    write_row<TO, VEC>(acc, scale, into, out + (int64_t)(v0 + k) * dim + d, dim - d);
+  }
+  int buf = 0;
+  for (int k = 0; k < held; ++k) {
+    const int n = number[k];
+    if (n <= FEW_ALONE) continue;   // the same in the whole workgroup
+    const int each = (n + FEW_WAVES - 1) / FEW_WAVES, q1 = min((wave + 1) * each, n);
+    TO* row = out + (int64_t)(v0 + k) * dim;
+    for (int c = 0; c < chunks; ++c, buf ^= 1) {
+      float acc[VEC] = {};
+      for (int q = wave * each; q < q1; q += 64) {
+        const int here = min(64, q1 - q), list = lane < here ? order[begin[k] + q + lane] : 0;
+        add_rows<TI, VEC>(acc, g, ld, list, 0, here, (c * 64 + lane) * VEC, dim);
+      }
+      store_pack(&sums[buf][wave][lane * VEC], reinterpret_cast<const Pack<float, VEC>&>(acc));
+      __syncthreads();   // the other buffer is read before the barrier of the chunk that fills it again
+      for (int x = threadIdx.x; x < 64 * VEC; x += FEW_WAVES * 64) {
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int w = 0; w < FEW_WAVES; ++w) sum[0] += sums[buf][w][x];
+        const int d = c * 64 * VEC + x;
+        if (d < dim) write_row<TO, 1>(sum, scale, into, row + d, 1);
+      }
+    }
+  }
 }
 
 }  // namespace bf
@@ -265,9 +400,9 @@ int bf_embed_rows(const void* table, int64_t table_ld, int64_t vocab, const void
   });
 }
 
-// start[vocab + 1], order[count], then the parts of the frequent values
+// start[vocab + 1], order[count], owner and parts of the pieces; nothing for few tokens
 int64_t bf_embed_grad_workspace(int64_t count, int64_t vocab, int64_t dim) {
-  return (vocab + 1) + count + ceil_div(count, PIECE) * 2 * dim;
+  return count <= FEW_TOKENS ? 0 : (vocab + 1) + count + ceil_div(count, PIECE) * (1 + 2 * dim);
 }
 
 int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* tokens, int token_bytes, int64_t count,
@@ -279,42 +414,48 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
   BF_REQUIRE(!accumulate || out_elem == TE_F32, "bf_embed_grad: sums are added to fp32 alone");
   BF_REQUIRE(vocab >= 0 && count >= 0 && dim >= 0 && grad_ld >= dim, "bf_embed_grad: bad sizes");
   if (vocab == 0 || dim == 0 || (count == 0 && accumulate)) return BF_OK;
-  BF_REQUIRE((count == 0 || (grad && tokens)) && out && workspace, "bf_embed_grad: null pointer");
-  if (vocab >= (1LL << 30) || count >= (1LL << 30) || dim >= (1LL << 30)) {
-    set_error("bf_embed_grad: %lld tokens, %lld values or %lld columns: each below 2^30", (long long)count,
+  BF_REQUIRE((count == 0 || (grad && tokens)) && out && (workspace || count <= FEW_TOKENS),
+             "bf_embed_grad: null pointer");
+  const int64_t pieces = ceil_div(count, PIECE), columns = ceil_div(dim, JOIN_COLUMNS);
+  if (vocab >= (1LL << 30) || count >= (1LL << 30) || dim >= (1LL << 30) || pieces * columns >= (1LL << 31)) {
+    set_error("bf_embed_grad: %lld tokens, %lld values or %lld columns are too many", (long long)count,
               (long long)vocab, (long long)dim);
     return BF_ERANGE;
   }
-  int* start = reinterpret_cast<int*>(workspace);
-  int* order = start + vocab + 1;
-  float* part = reinterpret_cast<float*>(order + count);
-  const int range = sort_range(vocab);
-  hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)ceil_div(vocab, range)), dim3(SORT_THREADS), 0, stream, tokens,
-                     token_bytes, (int)count, (int)vocab, range, start, order);
-  BF_LAUNCH_CHECK("embed_sort_kernel");
   return with_elem(elem, [&](auto ti) -> int {
     using TI = decltype(ti);
     constexpr int VEC = 16 / sizeof(TI);
     auto run = [&](auto to) -> int {
       using TO = decltype(to);
-      const int64_t wave_chunks = ceil_div(dim, 64 * VEC), group_chunks = ceil_div(dim, SUM_THREADS * VEC);
-      const int64_t row_groups = ceil_div(vocab * wave_chunks, SUM_THREADS / 64), pieces = ceil_div(count, PIECE);
-      const int64_t join_chunks = ceil_div(dim, SUM_THREADS);
-      if (row_groups + pieces * group_chunks >= (1LL << 31) || pieces * join_chunks >= (1LL << 31)) {
-        set_error("bf_embed_grad: %lld rows of %lld columns are too many", (long long)vocab, (long long)dim);
-        return BF_ERANGE;
+      const TI* g = static_cast<const TI*>(grad);
+      TO* o = static_cast<TO*>(out);
+      if (count <= FEW_TOKENS) {
+        // two workgroups a CU and more where there are rows for them
+        const int64_t r = ceil_div(vocab, 512);
+        const int range = (int)(r < FEW_RANGE ? r : FEW_RANGE);
+        hipLaunchKernelGGL((embed_few_kernel<TI, TO, VEC>), dim3((unsigned)ceil_div(vocab, range)), dim3(FEW_WAVES * 64), 0,
+                           stream, g, grad_ld, tokens, token_bytes, (int)count, (int)vocab, (int)dim, range, scale,
+                           accumulate, o);
+        BF_LAUNCH_CHECK("embed_few_kernel");
+        return BF_OK;
       }
-      hipLaunchKernelGGL((embed_sum_kernel<TI, TO, VEC>), dim3((unsigned)(row_groups + pieces * group_chunks)),
-                         dim3(SUM_THREADS), 0, stream, static_cast<const TI*>(grad), grad_ld, tokens, token_bytes, start,
-                         order, (int)vocab, (int)dim, (int)wave_chunks, row_groups, (int)group_chunks, scale,
-                         accumulate, static_cast<TO*>(out), part);
+      int* start = reinterpret_cast<int*>(workspace);
+      int* order = start + vocab + 1;
+      int* owner = order + count;
+      float* part = reinterpret_cast<float*>(owner + pieces);
+      const int64_t r = ceil_div(vocab, 256);
+      const int range = (int)(r < SORT_RANGE ? r : SORT_RANGE);
+      hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)ceil_div(vocab, range)), dim3(SORT_WAVES * 64), 0, stream,
+                         tokens, token_bytes, (int)count, (int)vocab, range, start, order);
+      BF_LAUNCH_CHECK("embed_sort_kernel");
+      hipLaunchKernelGGL((embed_sum_kernel<TI, TO, VEC>), dim3((unsigned)(pieces + ceil_div(vocab, ROWS))),
+                         dim3(SUM_THREADS), 0, stream, g, grad_ld, tokens, token_bytes, start, order, (int)vocab, (int)dim,
+                         (int)pieces, scale, accumulate, o, owner, part);
       BF_LAUNCH_CHECK("embed_sum_kernel");
-      if (count > PIECE) {
-        hipLaunchKernelGGL((embed_join_kernel<TO>), dim3((unsigned)(pieces * join_chunks)), dim3(SUM_THREADS), 0,
-                           stream, tokens, token_bytes, start, order, (int)vocab, (int)dim, (int)join_chunks, scale,
-                           accumulate, static_cast<TO*>(out), part);
-        BF_LAUNCH_CHECK("embed_join_kernel");
-      }
+      hipLaunchKernelGGL((embed_join_kernel<TO>), dim3((unsigned)(ceil_div(pieces, JOIN_PIECES) * columns)),
+                         dim3(JOIN_PARTS * JOIN_COLUMNS), 0, stream, tokens, token_bytes, start, order, (int)dim,
+                         (int)pieces, (int)columns, scale, accumulate, owner, o, part);
+      BF_LAUNCH_CHECK("embed_join_kernel");
       return BF_OK;
     };
     return out_elem == TE_F32 ? run(float()) : run(TI());

@@ -139,9 +139,10 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
         if dtype not in (grad.dtype, torch.float32):
             raise ValueError(f"dtype must be {grad.dtype} or float32, got {dtype}")
         out = torch.empty(vocab, dim, dtype=dtype, device=grad.device)
-    space = torch.empty(_lib.load().bf_embed_grad_workspace(count, vocab, dim), device=grad.device)
+    need = _lib.load().bf_embed_grad_workspace(count, vocab, dim)
+    space = torch.empty(need, device=grad.device) if need else None
     _lib.call("bf_embed_grad", rows.data_ptr(), max(rows.stride(0), dim), elem, tokens.data_ptr(), token_bytes, count,
-              vocab, dim, float(scale), _ELEM[out.dtype], accumulate_into is not None, out.data_ptr(), space.data_ptr(),
+              vocab, dim, float(scale), _ELEM[out.dtype], accumulate_into is not None, out.data_ptr(), _address(space),
               current_raw_stream(dev))
     if accumulate_into is not None:
         torch.autograd.graph.increment_version(out)

@@ -61,8 +61,8 @@ def test_entry_points_refuse_bad_arguments(lib):
 
 
 def test_workspaces_grow_with_what_they_hold(lib):
-    assert lib.bf_embed_grad_workspace(0, 10, 4) >= 11
-    assert lib.bf_embed_grad_workspace(1000, 10, 4) >= 11 + 1000 + 2 * (1000 // 64) * 4
+    assert lib.bf_embed_grad_workspace(100, 10, 4) == 0      # few tokens: sorted and summed in one launch, in LDS
+    assert lib.bf_embed_grad_workspace(5000, 10, 4) >= 11 + 5000 + 2 * (5000 // 64) * 4
     assert lib.bf_policy_loss_workspace(2, 3, 100, 0) >= 6 * 6 + 2
     assert lib.bf_policy_loss_workspace(2, 3, 100, 7) == 0
     assert lib.bf_preference_loss_workspace(5, 100, 2, 1) >= 5 * 6 + 2
