@@ -44,6 +44,17 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, N>& r) {
   __builtin_memcpy(p, &r, sizeof(r));
 }
 
+// Sixteen bytes as they are.
+typedef uint32_t Words __attribute__((ext_vector_type(4)));
+
+// Zeros that the compiler does not know for constants: known ones it stores element by element where the
+// address may be unaligned (eight 2-byte stores for one of 16 bytes).
+__device__ __forceinline__ Words zero_words() {
+  uint32_t z = 0;
+  asm volatile("" : "+v"(z));
+  return Words{z, z, z, z};
+}
+
 // Element `i` of a token array of 4- or 8-byte integers; a value that no vocabulary of fewer
 // than 2^31 entries holds becomes the nearest 32-bit one, so its sign and its being too large stay.
 __device__ __forceinline__ int load_token(const void* tokens, int bytes, int64_t i) {

@@ -217,10 +217,8 @@ __global__ __launch_bounds__(STATS_THREADS) void policy_stats_kernel(const float
   if (threadIdx.x == 0) write_stats(r.x, r.y, r.z, kl_weight, stats);
 }
 
-// Sixteen bytes of logits as they are.  as_floats keeps the compiler from holding on to the fp32 values of a
+// as_floats keeps the compiler from holding on to the fp32 values of a
 // row between its two uses, which would take twice the registers that the row does.
-typedef uint32_t Words __attribute__((ext_vector_type(4)));
-
 template <class T, int VEC>
 __device__ __forceinline__ void as_floats(Words& w, float (&z)[VEC]) {
   asm volatile("" : "+v"(w));
@@ -377,7 +375,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
         const int e = vecs * Held::VEC + (int)threadIdx.x;
         if (e < V) out[e] = (T)0.f;
         for (int k = 0; k < NV; ++k)
-          if (k * THREADS + (int)threadIdx.x < vecs) Held::store_words(k, out, vecs, Words{0u, 0u, 0u, 0u});
+          if (k * THREADS + (int)threadIdx.x < vecs) Held::store_words(k, out, vecs, zero_words());
       }
       x = uniform(after);
     }
@@ -517,9 +515,8 @@ __device__ __forceinline__ void write_row_gradient(const T* row, T* out, int64_t
   const bool read = f.z != 0.f;
   for (int64_t d = from + threadIdx.x * VEC; d < to; d += LOSS_THREADS * VEC) {
     if (d + VEC <= to) {
-      Pack<T, VEC> x;
       if (read) {
-        x = load_pack<T, VEC>(row + d);
+        Pack<T, VEC> x = load_pack<T, VEC>(row + d);
         float y[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) y[k] = term((float)x.v[k], c, f.x) * f.y;
@@ -528,11 +525,11 @@ __device__ __forceinline__ void write_row_gradient(const T* row, T* out, int64_t
           for (int k = 0; k < VEC; ++k) y[k] += t == d + k ? f.z : 0.f;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) x.v[k] = (T)y[k];
+        store_pack(out + d, x);
       } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) x.v[k] = (T)0.f;
+        const Words zero = zero_words();
+        __builtin_memcpy(out + d, &zero, 16);
       }
-      store_pack(out + d, x);
     } else {
       for (int64_t e = d; e < to; ++e)
         out[e] = (T)(read ? term((float)row[e], c, f.x) * f.y + (t == e ? f.z : 0.f) : 0.f);
