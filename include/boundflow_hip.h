@@ -603,7 +603,8 @@ int bf_domain_status(const float* lb, int64_t D, int64_t S, const int* infeasibl
  * What stands at both ends of a token network's training step, and its weights' update.  No
  * counterpart in the reference, which bounds networks and does not train them.
  * Element types are given by code: 0 fp32, 1 bf16, 2 fp16.  Token arrays hold 4- or 8-byte integers
- * (token_bytes).  Rows may start at any address that is a multiple of their element's size. */
+ * (token_bytes).  Rows may start at any address that is a multiple of their element's size; workspaces at a
+ * multiple of 16 bytes. */
 
 /* out[i, :] = scale * table[tokens[i], :] (fp32 product, rounded once), i < count, out dense [count, dim];
  * a negative token gives zeros, one past the table NaN. */

@@ -334,6 +334,28 @@ def test_preference_loss(dtype, lengths, V):
         assert alone.grad_logits is None and torch.equal(alone.loss, got.loss)
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 4097), (torch.bfloat16, 8192), (torch.bfloat16, 16391),
+                                     (torch.float16, 33001), (torch.float32, 20003)])
+def test_preference_loss_of_many_long_rows(dtype, V):
+    """Batches of many long rows: responses of very different lengths, empty ones, a pair without a row, rows of no
+    response, padding tokens, and rows that start at odd elements."""
+    for lengths in ([260, 0, 1, 40, 90, 0, 131, 7], [600, 3], [0] * 30 + [5, 250] * 3 + [0] * 30 + [80, 1] * 3):
+        test_preference_loss(dtype, lengths, V)
+        dev = device()
+        s = preference_inputs(lengths, V, dtype, 77, 1, 2)
+        s["tokens"][::7] = -1
+        on = {k: v.to(dev) for k, v in s.items()}
+        r = ref.preference_loss(**s)
+        got = training.preference_loss(**on)
+        tol_lp = logp_tol(s["logits"], V)
+        close(got.logp, r["logp"], tol_lp + 2.0 ** -24 * r["logp"].abs(), "preference logp with padding")
+        assert not got.grad_logits[::7].any() and not got.grad_logits[-2:].any()
+        again = training.preference_loss(**on)
+        assert torch.equal(got.grad_logits, again.grad_logits) and torch.equal(got.rewards, again.rewards)
+        alone = training.preference_loss(**on, with_grad=False)
+        close(alone.rewards, got.rewards.double().cpu(), 0.1 * float(tol_lp.sum()) + 2.0 ** -20, "rewards alone")
+
+
 def test_preference_loss_without_pairs_and_with_offsets_out_of_range():
     dev = device()
     s = preference_inputs([4, 3], 20, torch.float32, 4)
