@@ -104,31 +104,50 @@ struct PolicyArgs {
   int token_bytes, by_sequence;
 };
 
-// weight[b]: 1 / live rows (of all, or with by_sequence of the sequence times the sequences that have any), by one
-// workgroup.  The sequences are taken WEIGHT_HELD at a time, whose counts lie in `held` (LDS); a thread has the
-// flags of eight rows under way at once.
-constexpr int WEIGHT_HELD = 2048, WEIGHT_THREADS = 1024;
+// The rows' weights: 1 / live rows, or with by_sequence 1 / (live rows of the sequence * sequences that have any).  Up to
+// COUNT_GROUPS workgroups count a share of the rows (of the sequences) each; a row's weight is formed from the counts
+// where it is needed.
+constexpr int COUNT_GROUPS = 64, COUNT_HELD = 2048, COUNT_THREADS = 1024;
 
+struct PolicyCounts {
+  float* share;     // [COUNT_GROUPS]: live rows, or sequences that have any, of each workgroup
+  float* live;      // [B], by_sequence: live rows
+  int groups;
+};
+
+// Workgroup `group` of counts.groups; `held` (LDS) holds the counts of COUNT_HELD sequences at a time.  A thread has the
+// flags of eight rows under way at once.
 template <int THREADS>
-__device__ __forceinline__ void policy_weights(const PolicyArgs& a, float* weight, int* held, float* red) {
+__device__ __forceinline__ void policy_count(const PolicyArgs& a, const PolicyCounts& counts, int group, int* held,
+                                             float* red) {
   constexpr int AT_ONCE = 8;
   const unsigned T = (unsigned)a.T;
-  float total = 0.f, some = 0.f;
-  for (int64_t b0 = 0; b0 < a.B; b0 += WEIGHT_HELD) {
-    const int B = (int)(a.B - b0 < WEIGHT_HELD ? a.B - b0 : WEIGHT_HELD);
-    for (int b = threadIdx.x; b < B; b += THREADS) held[b] = 0;
-    __syncthreads();
-    const unsigned rows = B * T;
+  int total = 0;
+  // the group's sequences, or with the rows taken as one, its rows
+  const int64_t all = a.by_sequence ? a.B : a.B * a.T, each = (all + counts.groups - 1) / counts.groups;
+  const int64_t from = min(group * each, all), to = min(from + each, all);
+  for (int64_t b0 = from; b0 < to;) {
+    const int64_t b1 = a.by_sequence ? min(b0 + COUNT_HELD, to) : to;
+    const int64_t row0 = a.by_sequence ? b0 * a.T : b0;
+    const unsigned rows = (unsigned)(a.by_sequence ? (b1 - b0) * a.T : b1 - b0);
+    if (a.by_sequence) {
+      for (int b = threadIdx.x; b < (int)(b1 - b0); b += THREADS) held[b] = 0;
+      __syncthreads();
+    }
     for (unsigned i0 = threadIdx.x; i0 < rows + threadIdx.x; i0 += AT_ONCE * THREADS) {
       bool in[AT_ONCE];
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
         const unsigned i = i0 + u * THREADS;
-        in[u] = i < rows && live_row(a.mask, a.tokens, a.token_bytes, b0 * T + i);
+        in[u] = i < rows && live_row(a.mask, a.tokens, a.token_bytes, row0 + i);
       }
 #pragma unroll
       for (int u = 0; u < AT_ONCE; ++u) {
-        const unsigned i = i0 + u * THREADS, b = min(i, rows - 1) / T;
+        if (!a.by_sequence) {
+          total += in[u];
+          continue;
+        }
+        const unsigned b = min(i0 + u * THREADS, rows - 1) / T;
         const uint64_t found = __ballot(in[u]);
         const unsigned lo = __builtin_amdgcn_readfirstlane(b), hi = __builtin_amdgcn_readlane(b, 63);
         if (lo == hi) {   // a wave's 64 rows are mostly one sequence's
@@ -138,26 +157,36 @@ __device__ __forceinline__ void policy_weights(const PolicyArgs& a, float* weigh
         }
       }
     }
-    __syncthreads();
-    for (int b = threadIdx.x; b < B; b += THREADS) {
-      weight[b0 + b] = (float)held[b];   // read again by the same thread
-      total += (float)held[b];
-      some += held[b] ? 1.f : 0.f;
+    if (a.by_sequence) {
+      __syncthreads();
+      for (int b = threadIdx.x; b < (int)(b1 - b0); b += THREADS) {
+        counts.live[b0 + b] = (float)held[b];
+        total += held[b] ? 1 : 0;
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    b0 = b1;
   }
-  const float all = block_sum<THREADS / 64>(a.by_sequence ? some : total, red);
-  for (int64_t b0 = 0; b0 < a.B; b0 += WEIGHT_HELD)
-    for (int64_t b = b0 + threadIdx.x; b < a.B && b < b0 + WEIGHT_HELD; b += THREADS) {
-      const float live = weight[b];
-      weight[b] = live > 0.f ? 1.f / (a.by_sequence ? live * all : all) : 0.f;
-    }
+  // below 2^24 rows in all: exact
+  const float share = block_sum<THREADS / 64>((float)total, red);
+  if (threadIdx.x == 0) counts.share[group] = share;
 }
 
-__global__ __launch_bounds__(WEIGHT_THREADS) void policy_weights_kernel(PolicyArgs a, float* weight) {
-  __shared__ int held[WEIGHT_HELD];
-  __shared__ float red[WEIGHT_THREADS / 64];
-  policy_weights<WEIGHT_THREADS>(a, weight, held, red);
+__global__ __launch_bounds__(COUNT_THREADS) void policy_count_kernel(PolicyArgs a, PolicyCounts counts) {
+  __shared__ int held[COUNT_HELD];
+  __shared__ float red[COUNT_THREADS / 64];
+  policy_count<COUNT_THREADS>(a, counts, blockIdx.x, held, red);
+}
+
+// The sum of the shares, by a whole wave.
+__device__ __forceinline__ float count_sum(const PolicyCounts& counts) {
+  const int lane = threadIdx.x & 63;
+  return wave_sum(lane < counts.groups ? counts.share[lane] : 0.f);
+}
+
+// A live row's weight; sum: count_sum's
+__device__ __forceinline__ float row_weight(const PolicyArgs& a, const PolicyCounts& counts, unsigned b, float sum) {
+  return 1.f / (a.by_sequence ? counts.live[b] * sum : sum);
 }
 
 struct PolicyRow {
@@ -349,7 +378,7 @@ struct PolicyScalars {
   float old, ref, A, w;
 };
 
-__device__ __forceinline__ PolicyScalars policy_scalars(const PolicyArgs& a, const float* weight, int n, int N) {
+__device__ __forceinline__ PolicyScalars policy_scalars(const PolicyArgs& a, const PolicyCounts& counts, int n, int N) {
   PolicyScalars r;
   r.n = n;
   r.live = 0;
@@ -362,7 +391,7 @@ __device__ __forceinline__ PolicyScalars policy_scalars(const PolicyArgs& a, con
     r.old = a.old_logp[n];
     r.ref = a.ref_logp ? a.ref_logp[n] : 0.f;
     r.A = a.advantages[b * a.adv_b + (n - b * (unsigned)a.T) * a.adv_t];
-    r.w = weight[b];
+    r.w = a.by_sequence ? counts.live[b] : 1.f;   // to be multiplied by the sum, and inverted
   }
   return r;
 }
@@ -382,13 +411,13 @@ __device__ __forceinline__ PolicyScalars uniform(const PolicyScalars& x) {
 // workgroup would meet them at every turn or at none.
 template <bool GRAD, class T, int THREADS, int NV, int FULL>
 __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict__ logits, LogitRows rows, PolicyArgs a,
-                                                             const float* __restrict__ weight,
-                                                             float* __restrict__ logp, T* __restrict__ grad,
+                                                             PolicyCounts counts, float* __restrict__ logp,
+                                                             T* __restrict__ grad,
                                                              float4* __restrict__ sums, unsigned stride) {
   using Held = HeldRow<T, THREADS, NV, FULL>;
   __shared__ float2 red[2][Held::WAVES];
   const int N = (int)(a.B * a.T), V = (int)rows.V;
-  const float c = a.c;
+  const float c = a.c, count = count_sum(counts);
   unsigned place = blockIdx.x, first = 0;   // of the workgroup in the turn, and the turn's first row
   const auto next_turn = [&] {
     first += gridDim.x;
@@ -402,15 +431,15 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
   // compiler keep two sets of them.
   const auto settled = [&](PolicyScalars x) {
     while (x.n < N && !x.live) {
-      const PolicyScalars after = policy_scalars(a, weight, next_turn(), N);
+      const PolicyScalars after = policy_scalars(a, counts, next_turn(), N);
       if (threadIdx.x == 0) logp[x.n] = 0.f;
       if (GRAD) clear_row<T, THREADS>(grad + (int64_t)x.n * V, V);
       x = uniform(after);
     }
     return x;
   };
-  PolicyScalars here = settled(uniform(policy_scalars(a, weight, (int)place, N)));
-  PolicyScalars after = policy_scalars(a, weight, next_turn(), N);
+  PolicyScalars here = settled(uniform(policy_scalars(a, counts, (int)place, N)));
+  PolicyScalars after = policy_scalars(a, counts, next_turn(), N);
   const T* row = logits + (here.n < N ? uniform(rows.offset(here.n)) : 0);
   float M = kFloor, s = 0.f;   // of the thread, for the row that it holds
   RowShape<T> shape(row, V);
@@ -422,7 +451,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
   int buf = 0;
   while (here.n < N) {
     const PolicyScalars then = settled(uniform(after));
-    after = policy_scalars(a, weight, next_turn(), N);
+    after = policy_scalars(a, counts, next_turn(), N);
     const T* next_row = logits + (then.n < N ? uniform(rows.offset(then.n)) : 0);
     const float zt_next = then.live && then.t < V ? (float)next_row[then.t] : 0.f;
     const float2 soft = block_softmax<Held::WAVES>(M, s, c, red[buf]);
@@ -431,10 +460,11 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
     const float Mr = uniform(soft.x);
     const float lp = here.t < V ? log_prob(zt, c, Mr, soft.y) : __int_as_float(0x7fc00000);
     const PolicyRow r = policy_term(lp, here.old, here.ref, a.ref_logp != nullptr, here.A, a.low, a.high, a.kl_weight);
-    policy += here.w * r.policy;
-    kl += here.w * r.kl;
-    outside += here.w * r.outside;
-    const float g = here.w * r.g * a.inv_t * a.grad_scale, q = uniform(-g / soft.y);
+    const float w = 1.f / (here.w * count);
+    policy += w * r.policy;
+    kl += w * r.kl;
+    outside += w * r.outside;
+    const float g = w * r.g * a.inv_t * a.grad_scale, q = uniform(-g / soft.y);
     const uint32_t keep = uniform(g == 0.f ? 0 : -1);
     if (threadIdx.x == 0) logp[here.n] = lp;
     T* out = grad + (int64_t)here.n * V;
@@ -456,20 +486,18 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
 // Rows in parts: few rows, so that a workgroup each would leave the device idle, or rows that no workgroup
 // holds.  One launch sums the parts' softmaxes, the next forms the rows' from them and writes the gradient.
 
-// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements); with `weight` one more makes the policy
-// loss's weights.
+// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements), and for the policy loss one that counts.
 template <class T>
 __global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows,
                                                                     PolicyArgs a, int64_t N, int parts, int64_t chunk,
-                                                                    float2* __restrict__ part,
-                                                                    float* __restrict__ weight) {
+                                                                    float2* __restrict__ part, PolicyCounts counts) {
   constexpr int VEC = 16 / sizeof(T);
   __shared__ float2 red[LOSS_WAVES];
   const int64_t n = blockIdx.x / (unsigned)parts;
   if (n == N) {
-    __shared__ int held[WEIGHT_HELD];
+    __shared__ int held[COUNT_HELD];
     __shared__ float sum[LOSS_WAVES];
-    policy_weights<LOSS_THREADS>(a, weight, held, sum);
+    policy_count<LOSS_THREADS>(a, counts, 0, held, sum);
     return;
   }
   const int q = (int)(blockIdx.x % (unsigned)parts);
@@ -589,10 +617,10 @@ __device__ __forceinline__ PolicyRow policy_part_row(const T* logits, const Logi
 template <bool ONE, class T>
 __global__ __launch_bounds__(LOSS_THREADS) void policy_part_kernel(const T* __restrict__ logits, LogitRows rows,
                                                                    PolicyArgs a, int64_t N, int parts, int64_t chunk,
-                                                                   const float2* __restrict__ part,
-                                                                   const float* __restrict__ weight,
+                                                                   const float2* __restrict__ part, PolicyCounts counts,
                                                                    float* __restrict__ logp, float* __restrict__ stats,
                                                                    T* __restrict__ grad) {
+  const float count = count_sum(counts);
   if (blockIdx.x == gridDim.x - 1) {
     constexpr int LANES = ONE ? 1 : 16, ROWS = LOSS_THREADS / LANES;   // rows at a time, and lanes of a row
     __shared__ float4 red[LOSS_WAVES];
@@ -606,7 +634,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void policy_part_kernel(const T* __re
         float2 soft;
         const PolicyRow r = policy_part_row<ONE>(logits, rows, a, part, parts, n, load_token(a.tokens, a.token_bytes, n),
                                                  &lp, &soft);
-        const float w = first ? weight[(unsigned)n / (unsigned)a.T] : 0.f;
+        const float w = row_weight(a, counts, (unsigned)n / (unsigned)a.T, count);
         if (first) {
           policy += w * r.policy;
           kl += w * r.kl;
@@ -627,7 +655,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void policy_part_kernel(const T* __re
     float lp;
     float2 soft;
     const PolicyRow r = policy_part_row<ONE>(logits, rows, a, part, parts, n, t, &lp, &soft);
-    f = row_gradient(soft, weight[(unsigned)n / (unsigned)a.T] * r.g * a.inv_t * a.grad_scale);
+    f = row_gradient(soft, row_weight(a, counts, (unsigned)n / (unsigned)a.T, count) * r.g * a.inv_t * a.grad_scale);
   }
   write_row_gradient(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V), (int64_t)t,
                      a.c, f);
@@ -635,22 +663,23 @@ __global__ __launch_bounds__(LOSS_THREADS) void policy_part_kernel(const T* __re
 
 // ---------------------------------------------------------------------------
 // Short rows (a controller's few actions, a small vocabulary): LANES lanes a row, 1 or 16, which go over its
-// elements twice (the second time from the caches).  ALONE: one workgroup does everything, weights and sums included, in
+// elements twice (the second time from the caches).  ALONE: one workgroup does everything, counts and sums included, in
 // one launch.
 constexpr int SHORT_ONE = 16, SHORT_MOST = 512;   // the longest rows of one lane, and of sixteen
 
 template <bool ALONE, int LANES, class T>
-__global__ __launch_bounds__(ALONE ? WEIGHT_THREADS : LOSS_THREADS) void policy_short_kernel(
-    const T* __restrict__ logits, LogitRows rows, PolicyArgs a, float* weight, float* __restrict__ logp,
+__global__ __launch_bounds__(ALONE ? COUNT_THREADS : LOSS_THREADS) void policy_short_kernel(
+    const T* __restrict__ logits, LogitRows rows, PolicyArgs a, PolicyCounts counts, float* __restrict__ logp,
     float* __restrict__ stats, T* __restrict__ grad, float4* __restrict__ sums) {
-  constexpr int THREADS = ALONE ? WEIGHT_THREADS : LOSS_THREADS, WAVES = THREADS / 64, VEC = LANES == 1 ? 1 : 16 / sizeof(T);
+  constexpr int THREADS = ALONE ? COUNT_THREADS : LOSS_THREADS, WAVES = THREADS / 64, VEC = LANES == 1 ? 1 : 16 / sizeof(T);
   __shared__ float4 red[WAVES];
   if constexpr (ALONE) {
-    __shared__ int held[WEIGHT_HELD];
+    __shared__ int held[COUNT_HELD];
     __shared__ float sum[WAVES];
-    policy_weights<THREADS>(a, weight, held, sum);
-    __syncthreads();   // weight[] is read by other threads of the workgroup than wrote it
+    policy_count<THREADS>(a, counts, 0, held, sum);
+    __syncthreads();   // the counts are read by other threads of the workgroup than wrote them
   }
+  const float count = count_sum(counts);
   const int N = (int)(a.B * a.T), V = (int)rows.V, lane = threadIdx.x % LANES;
   const float c = a.c;
   float policy = 0.f, kl = 0.f, outside = 0.f;
@@ -661,7 +690,7 @@ __global__ __launch_bounds__(ALONE ? WEIGHT_THREADS : LOSS_THREADS) void policy_
     float lp = 0.f, g = 0.f, q = 0.f, M = kFloor, s = 0.f;
     if (live_row(a.mask, a.tokens, a.token_bytes, n)) {   // the same in a row's lanes
       const unsigned b = (unsigned)n / (unsigned)a.T;
-      const float old = a.old_logp[n], ref = a.ref_logp ? a.ref_logp[n] : 0.f, w = weight[b];
+      const float old = a.old_logp[n], ref = a.ref_logp ? a.ref_logp[n] : 0.f, w = row_weight(a, counts, b, count);
       const float A = a.advantages[b * a.adv_b + (n - b * (unsigned)a.T) * a.adv_t];
       const float zt = t < V ? (float)row[t] : 0.f;
       for (int d = lane * VEC; d < V; d += LANES * VEC) {
@@ -879,10 +908,10 @@ using namespace bf;
 
 extern "C" {
 
-// sums of the workgroups (row kernel, short rows), or part [N * parts] float2; weight [B]
+// sums of the workgroups (row kernel, short rows), or part [N * parts] float2; the counts' shares, and live rows [B]
 int64_t bf_policy_loss_workspace(int64_t B, int64_t T, int64_t V, int elem) {
   if (!elem_ok(elem) || B < 0 || T < 0 || V <= 0) return 0;
-  return 4 * SUM_GROUPS + 2 * B * T * row_parts(B * T, V, elem).count + B;
+  return 4 * SUM_GROUPS + 2 * B * T * row_parts(B * T, V, elem).count + COUNT_GROUPS + B;
 }
 
 int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V, int64_t ld_b, int64_t ld_t,
@@ -911,7 +940,12 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   float4* sums = reinterpret_cast<float4*>(workspace);
   float2* part = reinterpret_cast<float2*>(sums + SUM_GROUPS);
   const Parts p = row_parts(N, V, elem);
-  float* weight = reinterpret_cast<float*>(part + N * p.count);
+  // a workgroup for 4096 rows at least (the counting waits for loads, not on their number)
+  const int64_t shares = by_sequence ? (B < ceil_div(N, 4096) ? B : ceil_div(N, 4096)) : ceil_div(N, 4096);
+  PolicyCounts counts;
+  counts.share = reinterpret_cast<float*>(part + N * p.count);
+  counts.live = counts.share + COUNT_GROUPS;
+  counts.groups = 1;
   const bool shorts = V <= (elem == TE_F32 ? SHORT_MOST / 2 : SHORT_MOST);
   const int lanes = V <= SHORT_ONE ? 1 : 16;
   return with_elem(elem, [&](auto e) -> int {
@@ -919,30 +953,32 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
     const E* x = static_cast<const E*>(logits);
     E* out = static_cast<E*>(grad);
     // one workgroup for what takes it four turns at most: a launch, and the gap before it, costs as much as two
-    if (N == 0 || (shorts && N * lanes <= 4 * WEIGHT_THREADS)) {
+    if (N == 0 || (shorts && N * lanes <= 4 * COUNT_THREADS)) {
       if (lanes == 1)
-        hipLaunchKernelGGL((policy_short_kernel<true, 1, E>), dim3(1), dim3(WEIGHT_THREADS), 0, stream, x, rows, a,
-                           weight, logp, stats, out, sums);
+        hipLaunchKernelGGL((policy_short_kernel<true, 1, E>), dim3(1), dim3(COUNT_THREADS), 0, stream, x, rows, a,
+                           counts, logp, stats, out, sums);
       else
-        hipLaunchKernelGGL((policy_short_kernel<true, 16, E>), dim3(1), dim3(WEIGHT_THREADS), 0, stream, x, rows, a,
-                           weight, logp, stats, out, sums);
+        hipLaunchKernelGGL((policy_short_kernel<true, 16, E>), dim3(1), dim3(COUNT_THREADS), 0, stream, x, rows, a,
+                           counts, logp, stats, out, sums);
       BF_LAUNCH_CHECK("policy_short_kernel");
       return BF_OK;
     }
     int64_t groups = 0;
-    auto weights = [&] {
-      hipLaunchKernelGGL(policy_weights_kernel, dim3(1), dim3(WEIGHT_THREADS), 0, stream, a, weight);
+    PolicyCounts shared = counts;
+    shared.groups = (int)(shares < 1 ? 1 : shares < COUNT_GROUPS ? shares : COUNT_GROUPS);
+    auto count = [&] {
+      hipLaunchKernelGGL(policy_count_kernel, dim3(shared.groups), dim3(COUNT_THREADS), 0, stream, a, shared);
     };
     if (shorts) {
-      weights();
+      count();
       groups = ceil_div(N * lanes, LOSS_THREADS);
       if (groups > 256 * 8) groups = 256 * 8;
       if (lanes == 1)
         hipLaunchKernelGGL((policy_short_kernel<false, 1, E>), dim3((unsigned)groups), dim3(LOSS_THREADS), 0, stream, x,
-                           rows, a, weight, logp, stats, out, sums);
+                           rows, a, shared, logp, stats, out, sums);
       else
         hipLaunchKernelGGL((policy_short_kernel<false, 16, E>), dim3((unsigned)groups), dim3(LOSS_THREADS), 0, stream, x,
-                           rows, a, weight, logp, stats, out, sums);
+                           rows, a, shared, logp, stats, out, sums);
       BF_LAUNCH_CHECK("policy_short_kernel");
     } else if (N >= 256) {
       const int rc = with_row_group(V / (16 / (int)sizeof(E)), [&](auto threads, auto nv, auto full) -> int {
@@ -950,9 +986,9 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
         constexpr int TH = decltype(threads)::value, NV = decltype(nv)::value, FULL = decltype(full)::value;
         const int64_t most = 256 * (TH == 64 ? 16 : TH == 256 ? 6 : TH == 512 ? 2 : 1);
         groups = N < most ? N : most;
-        weights();
+        count();
         auto launch = [&](auto kernel) {
-          hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(TH), 0, stream, x, rows, a, weight, logp, out, sums,
+          hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(TH), 0, stream, x, rows, a, shared, logp, out, sums,
                              (unsigned)(groups * 0.6180339887498949));
         };
         if (grad) launch(policy_row_kernel<true, E, TH, NV, FULL>);
@@ -972,15 +1008,15 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
       return BF_ERANGE;
     }
     hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count + 1)), dim3(LOSS_THREADS), 0, stream, x, rows, a,
-                       N, p.count, p.chunk, part, weight);
+                       N, p.count, p.chunk, part, counts);
     BF_LAUNCH_CHECK("loss_partial_kernel");
     const unsigned grid = grad ? (unsigned)(N * p.count + 1) : 1u;
     if (p.count == 1)
       hipLaunchKernelGGL((policy_part_kernel<true, E>), dim3(grid), dim3(LOSS_THREADS), 0, stream, x, rows, a, N, p.count,
-                         p.chunk, part, weight, logp, stats, out);
+                         p.chunk, part, counts, logp, stats, out);
     else
       hipLaunchKernelGGL((policy_part_kernel<false, E>), dim3(grid), dim3(LOSS_THREADS), 0, stream, x, rows, a, N,
-                         p.count, p.chunk, part, weight, logp, stats, out);
+                         p.count, p.chunk, part, counts, logp, stats, out);
     BF_LAUNCH_CHECK("policy_part_kernel");
     return BF_OK;
   });
@@ -1023,7 +1059,7 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
       all.token_bytes = token_bytes;
       all.c = c;
       hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows, all,
-                         N, p.count, p.chunk, part, nullptr);
+                         N, p.count, p.chunk, part, PolicyCounts{});
       BF_LAUNCH_CHECK("loss_partial_kernel");
     }
     if (p.count == 1)
