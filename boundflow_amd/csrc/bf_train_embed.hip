@@ -268,11 +268,11 @@ __device__ __forceinline__ void sum_row(const TI* __restrict__ g, int64_t ld, in
   }
 }
 
-// A value that occurs at most PIECE times is summed with the ROWS rows of its workgroup: the starts of both come
-// in one load and the positions of all their tokens in another (more rows a workgroup spare waits and lengthen its chain of
-// rows: 8, 4 and 2 rows, 72, 60 and 54 us for the batch of the comment below).  A more frequent value is cut at the multiples of PIECE of the sorted order, every part
-// summed by a workgroup of its own and the parts added in order, so a token that is half of the batch does not
-// leave one workgroup with half of the work.
+// A value that occurs at most PIECE times is summed with the ROWS rows of its workgroup: the starts of both come in one
+// load and the positions of all their tokens in another.  More rows a workgroup spare waits and lengthen its chain of
+// rows: with 8, 4 and 2, 72, 60 and 54 us for 16384 tokens of 32000 values, 4096 bf16 columns.  A more frequent value is
+// cut at the multiples of PIECE of the sorted order, every part summed by a wave of its own and the parts added in
+// order, so a token that is half of the batch does not leave one wave with half of the work.
 constexpr int SUM_THREADS = 256, SUM_WAVES = SUM_THREADS / 64;
 constexpr int ROWS = 2, PIECE = 8;
 
