@@ -63,7 +63,7 @@ __device__ __forceinline__ void sort_range(const void* tokens, int token_bytes, 
                                            SortSpace<WAVES, RANGE>& s, F f, G begin) {
   constexpr int THREADS = WAVES * 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int k = tid; k < WAVES * RANGE; k += THREADS) (&s.place[0][0])[k] = 0;
+  for (int k = lane; k < held; k += 64) s.place[wave][k] = 0;
   __syncthreads();
   const int slice = (count + THREADS - 1) / THREADS * 64;
   const int from = min(wave * slice, count), to = min(from + slice, count);
@@ -92,7 +92,7 @@ __device__ __forceinline__ void sort_range(const void* tokens, int token_bytes, 
   __syncthreads();
   // thread k < RANGE: the number of tokens of value v0 + k, and its exclusive sum over k
   int total = 0;
-  if (tid < RANGE)
+  if (tid < held)
     for (int w = 0; w < WAVES; ++w) total += s.place[w][tid];
   int incl = total;
 #pragma unroll
@@ -108,7 +108,7 @@ __device__ __forceinline__ void sort_range(const void* tokens, int token_bytes, 
     if (w < wave) base += s.sums[w];
   }
   if (tid < held) begin(tid, base, total);
-  if (tid < RANGE)
+  if (tid < held)
     for (int w = 0; w < WAVES; ++w) {
       const int n = s.place[w][tid];
       s.place[w][tid] = base;
@@ -124,8 +124,7 @@ __device__ __forceinline__ void sort_range(const void* tokens, int token_bytes, 
       if (same == 0) continue;
       // the lanes of this lane's value: those that agree with it in every bit
       const int k = in ? t[u] - v0 : 0;
-#pragma unroll
-      for (int b = 1; b < RANGE; b <<= 1) {
+      for (int b = 1; b < held; b <<= 1) {
         const uint64_t ones = __ballot(k & b);
         same &= k & b ? ones : ~ones;
       }
@@ -319,19 +318,19 @@ __global__ __launch_bounds__(SUM_THREADS) void embed_sum_kernel(
 }
 
 // Where a frequent value begins in a piece, its parts are added in order, a quarter of them by each quarter of the
-// workgroup and the quarters together.  Workgroup = (JOIN_PIECES pieces, JOIN_COLUMNS columns, four a thread).
-constexpr int JOIN_PIECES = 8, JOIN_PARTS = 4, JOIN_THREADS = 1024, JOIN_COLUMNS = JOIN_THREADS / JOIN_PARTS * 4;
+// workgroup and the quarters together.  Workgroup = (`each_pieces` pieces, JOIN_COLUMNS columns, four a thread).
+constexpr int JOIN_PARTS = 4, JOIN_THREADS = 1024, JOIN_COLUMNS = JOIN_THREADS / JOIN_PARTS * 4;
 
 template <class TO>
 __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(
     const void* __restrict__ tokens, int token_bytes, const int* __restrict__ start, const int* __restrict__ order, int dim,
-    int pieces, int columns, float scale, int into, const int* __restrict__ owner, TO* __restrict__ out,
+    int pieces, int each_pieces, int columns, float scale, int into, const int* __restrict__ owner, TO* __restrict__ out,
     const float* __restrict__ part) {
   __shared__ float4 sums[JOIN_PARTS][JOIN_COLUMNS / 4];
-  const int piece0 = blockIdx.x / (unsigned)columns * JOIN_PIECES, lane = threadIdx.x & 63;
+  const int piece0 = blockIdx.x / (unsigned)columns * each_pieces, lane = threadIdx.x & 63;
   const int x = threadIdx.x % (JOIN_COLUMNS / 4), quarter = threadIdx.x / (JOIN_COLUMNS / 4);
   const int d = (blockIdx.x % (unsigned)columns) * JOIN_COLUMNS + x * 4;
-  const int mine = lane < JOIN_PIECES && piece0 + lane < pieces ? owner[piece0 + lane] : -1;
+  const int mine = lane < each_pieces && piece0 + lane < pieces ? owner[piece0 + lane] : -1;
   uint64_t todo = __ballot(mine >= 0);   // the same in every wave
   while (todo) {
     const int k = __ffsll((unsigned long long)todo) - 1, piece = piece0 + k;
@@ -442,8 +441,9 @@ int bf_embed_rows(const void* table, int64_t table_ld, int64_t vocab, const void
   BF_REQUIRE(vocab >= 0 && count >= 0 && dim >= 0 && table_ld >= dim, "bf_embed_rows: bad sizes");
   if (count == 0 || dim == 0) return BF_OK;
   BF_REQUIRE((table || vocab == 0) && tokens && out, "bf_embed_rows: null pointer");
-  const int64_t chunks = ceil_div(dim, 16 / elem_bytes(elem)), blocks = ceil_div(count * chunks, 256);
-  if (vocab >= (1LL << 31) || dim >= (1LL << 30) || blocks >= (1LL << 31)) {
+  const bool wide = vocab >= (1LL << 31) || dim >= (1LL << 30) || count >= (1LL << 32);
+  const int64_t chunks = ceil_div(dim, 16 / elem_bytes(elem)), blocks = wide ? 0 : ceil_div(count * chunks, 256);
+  if (wide || blocks >= (1LL << 31)) {
     set_error("bf_embed_rows: %lld tokens of %lld columns from %lld rows are too many", (long long)count,
               (long long)dim, (long long)vocab);
     return BF_ERANGE;
@@ -488,9 +488,11 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
       const TI* g = static_cast<const TI*>(grad);
       TO* o = static_cast<TO*>(out);
       if (count <= FEW_TOKENS) {
-        // two workgroups a CU and more where there are rows for them
-        const int64_t r = ceil_div(vocab, 512);
-        const int range = (int)(r < FEW_RANGE ? r : FEW_RANGE);
+        // Four workgroups a CU and more where there are rows for them, and 16 rows each at most, since the frequent values
+        // are mostly neighbours (1000 tokens of 60000 values, 3800 columns, added: 61 us with 59 rows each, 45
+        // with 16); a larger table is cut less finely, because every workgroup reads every token.
+        const int64_t r = ceil_div(vocab, 1024), most = vocab <= (1 << 17) ? 16 : FEW_RANGE;
+        const int range = (int)(r < most ? r : most);
         hipLaunchKernelGGL((embed_few_kernel<TI, TO, VEC>), dim3((unsigned)ceil_div(vocab, range)), dim3(FEW_WAVES * 64), 0,
                            stream, g, grad_ld, tokens, token_bytes, (int)count, (int)vocab, (int)dim, range, scale,
                            accumulate, o);
@@ -504,7 +506,7 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
       const int64_t r = ceil_div(vocab, 256);
       const int range = (int)(r < SORT_RANGE ? r : SORT_RANGE);
       // The rows without a token are written with the others, or cleared with them while the tokens are sorted,
-      // which writes the others twice: 32000 rows of 4096 bf16 columns, 16384 tokens (a third of the values), 117 us
+      // which writes the others twice: 32000 rows of 4096 bf16 columns, 16384 tokens (a third of the values), 111 us
       // against 104.
       const bool clear = !accumulate && count <= vocab;
       const int64_t groups = ceil_div(vocab, range), bytes = clear ? vocab * dim * (int64_t)sizeof(TO) : 0;
@@ -522,9 +524,11 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
                          dim3(SUM_THREADS), 0, stream, g, grad_ld, tokens, token_bytes, start, order, (int)vocab, (int)dim,
                          (int)pieces, (int)piece_groups, scale, accumulate, accumulate || clear, o, owner, part);
       BF_LAUNCH_CHECK("embed_sum_kernel");
-      hipLaunchKernelGGL((embed_join_kernel<TO>), dim3((unsigned)(ceil_div(pieces, JOIN_PIECES) * columns)),
+      // narrow rows: fewer values one after another; wide ones have workgroups enough
+      const int each_pieces = columns == 1 ? 2 : 8;
+      hipLaunchKernelGGL((embed_join_kernel<TO>), dim3((unsigned)(ceil_div(pieces, each_pieces) * columns)),
                          dim3(JOIN_THREADS), 0, stream, tokens, token_bytes, start, order, (int)dim,
-                         (int)pieces, (int)columns, scale, accumulate, owner, o, part);
+                         (int)pieces, each_pieces, (int)columns, scale, accumulate, owner, o, part);
       BF_LAUNCH_CHECK("embed_join_kernel");
       return BF_OK;
     };

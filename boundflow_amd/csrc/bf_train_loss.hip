@@ -910,7 +910,7 @@ extern "C" {
 
 // sums of the workgroups (row kernel, short rows), or part [N * parts] float2; the counts' shares, and live rows [B]
 int64_t bf_policy_loss_workspace(int64_t B, int64_t T, int64_t V, int elem) {
-  if (!elem_ok(elem) || B < 0 || T < 0 || V <= 0) return 0;
+  if (!elem_ok(elem) || B < 0 || T < 0 || V <= 0 || B >= (1LL << 24) || T >= (1LL << 24) || !rows_fit(B * T, V)) return 0;
   return 4 * SUM_GROUPS + 2 * B * T * row_parts(B * T, V, elem).count + COUNT_GROUPS + B;
 }
 
@@ -926,9 +926,9 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   BF_REQUIRE(temperature > 0.0 && clip_low >= 0.f && clip_high >= 0.f, "bf_policy_loss: temperature %g, clip %g, %g",
              temperature, clip_low, clip_high);
   BF_REQUIRE(stats && workspace, "bf_policy_loss: null pointer");
-  if (!rows_fit(B * T, V) || B >= (1LL << 24) || T >= (1LL << 24)) {
-    set_error("bf_policy_loss: %lld rows of %lld logits: rows below 2^24, logits below 2^30", (long long)(B * T),
-              (long long)V);
+  if (B >= (1LL << 24) || T >= (1LL << 24) || !rows_fit(B * T, V)) {
+    set_error("bf_policy_loss: %lld x %lld rows of %lld logits: rows below 2^24, logits below 2^30", (long long)B,
+              (long long)T, (long long)V);
     return BF_ERANGE;
   }
   const int64_t N = B * T;
@@ -940,8 +940,8 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   float4* sums = reinterpret_cast<float4*>(workspace);
   float2* part = reinterpret_cast<float2*>(sums + SUM_GROUPS);
   const Parts p = row_parts(N, V, elem);
-  // a workgroup for 4096 rows at least (the counting waits for loads, not on their number)
-  const int64_t shares = by_sequence ? (B < ceil_div(N, 4096) ? B : ceil_div(N, 4096)) : ceil_div(N, 4096);
+  // the counting waits for loads: 1024 rows a workgroup, one a thread
+  const int64_t turns = ceil_div(N, COUNT_THREADS), shares = by_sequence && B < turns ? B : turns;
   PolicyCounts counts;
   counts.share = reinterpret_cast<float*>(part + N * p.count);
   counts.live = counts.share + COUNT_GROUPS;
@@ -1024,7 +1024,7 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
 
 // coef [N] float4, part [N * parts] float2, losses [pairs]
 int64_t bf_preference_loss_workspace(int64_t N, int64_t V, int64_t pairs, int elem) {
-  if (!elem_ok(elem) || N < 0 || V <= 0 || pairs < 0) return 0;
+  if (!elem_ok(elem) || N < 0 || V <= 0 || pairs < 0 || !rows_fit(N, V)) return 0;
   return 4 * N + 2 * N * row_parts(N, V, elem).count + pairs;
 }
 
