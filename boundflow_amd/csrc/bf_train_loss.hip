@@ -496,17 +496,17 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
 // with the memory side is the limit).
 
 // (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements), and for the policy loss one that counts.
-template <class T>
-__global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows,
-                                                                    PolicyArgs a, int64_t N, int parts, int64_t chunk,
-                                                                    float2* __restrict__ part, PolicyCounts counts) {
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows, PolicyArgs a,
+                                                          int64_t N, int parts, int64_t chunk,
+                                                          float2* __restrict__ part, PolicyCounts counts) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ float2 red[LOSS_WAVES];
+  __shared__ float2 red[TH / 64];
   const int64_t n = blockIdx.x / (unsigned)parts;
   if (n == N) {
     __shared__ int held[COUNT_HELD];
-    __shared__ float sum[LOSS_WAVES];
-    policy_count<LOSS_THREADS>(a, counts, 0, held, sum);
+    __shared__ float sum[TH / 64];
+    policy_count<TH>(a, counts, 0, held, sum);
     return;
   }
   const int q = (int)(blockIdx.x % (unsigned)parts);
@@ -515,15 +515,15 @@ __global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __r
   const int64_t from = q * chunk, to = min(from + chunk, rows.V);
   float M = kFloor, s = 0.f;
   const int lead = row_lead(row + from);   // chunks are whole vectors: the same in all of them
-  if (lead && threadIdx.x == LOSS_THREADS - 1) {
+  if (lead && threadIdx.x == TH - 1) {
     const float one[1] = {(float)row[from]};
     add_terms(M, s, one, a.c);
   }
   int64_t d = from + lead + threadIdx.x * VEC;
-  for (; d + 3 * LOSS_THREADS * VEC + VEC <= to; d += 4 * LOSS_THREADS * VEC) {   // four loads under way
+  for (; d + 3 * TH * VEC + VEC <= to; d += 4 * TH * VEC) {   // four loads under way
     Pack<T, VEC> x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = load_pack<T, VEC>(row + d + u * LOSS_THREADS * VEC);
+    for (int u = 0; u < 4; ++u) x[u] = load_pack<T, VEC>(row + d + u * TH * VEC);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float z[VEC];
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __r
       add_terms(M, s, z, a.c);
     }
   }
-  for (; d < to; d += LOSS_THREADS * VEC) {
+  for (; d < to; d += TH * VEC) {
     float z[VEC];
     if (d + VEC <= to) {
       const Pack<T, VEC> x = load_pack<T, VEC>(row + d);
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void loss_partial_kernel(const T* __r
     }
     add_terms(M, s, z, a.c);
   }
-  const float2 x = block_softmax<LOSS_WAVES>(M, s, a.c, red);
+  const float2 x = block_softmax<TH / 64>(M, s, a.c, red);
   if (threadIdx.x == 0) part[blockIdx.x] = x;
 }
 
@@ -578,15 +578,15 @@ __device__ __forceinline__ float4 row_gradient(float2 soft, float g) {
 }
 
 // The gradient of elements [from, to) of a row, by a workgroup.
-template <class T>
+template <int TH, class T>
 __device__ __forceinline__ void write_row_gradient(const T* row, T* out, int64_t from, int64_t to, int64_t t, float c,
                                                    float4 f) {
   constexpr int VEC = 16 / sizeof(T);
   const bool read = f.z != 0.f;
   const int lead = row_lead(read ? row + from : out + from);
-  if (lead && threadIdx.x == LOSS_THREADS - 1)
+  if (lead && threadIdx.x == TH - 1)
     out[from] = (T)(read ? term((float)row[from], c, f.x) * f.y + (t == from ? f.z : 0.f) : 0.f);
-  for (int64_t d = from + lead + threadIdx.x * VEC; d < to; d += LOSS_THREADS * VEC) {
+  for (int64_t d = from + lead + threadIdx.x * VEC; d < to; d += TH * VEC) {
     if (d + VEC <= to) {
       if (read) {
         Pack<T, VEC> x = load_pack<T, VEC>(row + d);
@@ -666,7 +666,7 @@ __global__ __launch_bounds__(LOSS_THREADS) void policy_part_kernel(const T* __re
     const PolicyRow r = policy_part_row<ONE>(logits, rows, a, part, parts, n, t, &lp, &soft);
     f = row_gradient(soft, row_weight(a, counts, (unsigned)n / (unsigned)a.T, count) * r.g * a.inv_t * a.grad_scale);
   }
-  write_row_gradient(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V), (int64_t)t,
+  write_row_gradient<LOSS_THREADS>(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V), (int64_t)t,
                      a.c, f);
 }
 
@@ -773,6 +773,11 @@ __device__ __forceinline__ int2 response_rows(const PreferenceArgs& a, int64_t k
   return make_int2((int)from, (int)min(max(a.offsets[k + 1], from), a.N));
 }
 
+// The preference loss gives a row of up to this many vectors a lane to one wave instead of four: 65536 rows of 500 bf16
+// logits 82 us against 156 (what four waves cost is the start of their workgroups), of 2000 175 against 191; from twice
+// that on the four waves are ahead, 4000 in 310 us against 333.
+constexpr int WAVE_VECTORS = 4;
+
 constexpr int PAIR_THREADS = 1024, PAIR_WAVES = PAIR_THREADS / 64;
 
 // One workgroup per pair: the rows' log-probabilities, the responses' sums, the pair's loss, and the rows' gradient
@@ -838,23 +843,23 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(
 }
 
 // Workgroup = (row, part): its gradient from the row's coefficients; the last one sums the pairs' losses.
-template <class T>
-__global__ __launch_bounds__(LOSS_THREADS) void preference_grad_kernel(const T* __restrict__ logits, LogitRows rows,
-                                                                       PreferenceArgs a, int parts, int64_t chunk, float c,
-                                                                       const float4* __restrict__ coef,
-                                                                       const float* __restrict__ losses,
-                                                                       float* __restrict__ loss, T* __restrict__ grad) {
+template <class T, int TH>
+__global__ __launch_bounds__(TH) void preference_grad_kernel(const T* __restrict__ logits, LogitRows rows,
+                                                             PreferenceArgs a, int parts, int64_t chunk, float c,
+                                                             const float4* __restrict__ coef,
+                                                             const float* __restrict__ losses, float* __restrict__ loss,
+                                                             T* __restrict__ grad) {
   if (blockIdx.x == gridDim.x - 1) {
-    __shared__ float red[LOSS_WAVES];
+    __shared__ float red[TH / 64];
     float s = 0.f;
-    for (int64_t i = threadIdx.x; i < a.pairs; i += LOSS_THREADS) s += losses[i];
-    s = block_sum<LOSS_WAVES>(s, red);
+    for (int64_t i = threadIdx.x; i < a.pairs; i += TH) s += losses[i];
+    s = block_sum<TH / 64>(s, red);
     if (threadIdx.x == 0) *loss = a.pairs ? s / (float)a.pairs : 0.f;
     return;
   }
   const int64_t n = blockIdx.x / (unsigned)parts;
   const int q = (int)(blockIdx.x % (unsigned)parts);
-  write_row_gradient(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V),
+  write_row_gradient<TH>(logits + rows.offset(n), grad + n * rows.V, q * chunk, min(q * chunk + chunk, rows.V),
                      (int64_t)load_token(a.tokens, a.token_bytes, n), c, coef[n]);
 }
 
@@ -1016,8 +1021,8 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
       set_error("bf_policy_loss: %lld rows of %lld logits are too many", (long long)N, (long long)V);
       return BF_ERANGE;
     }
-    hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count + 1)), dim3(LOSS_THREADS), 0, stream, x, rows, a,
-                       N, p.count, p.chunk, part, counts);
+    hipLaunchKernelGGL((loss_partial_kernel<E, LOSS_THREADS>), dim3((unsigned)(N * p.count + 1)), dim3(LOSS_THREADS), 0,
+                       stream, x, rows, a, N, p.count, p.chunk, part, counts);
     BF_LAUNCH_CHECK("loss_partial_kernel");
     const unsigned grid = grad ? (unsigned)(N * p.count + 1) : 1u;
     if (p.count == 1)
@@ -1059,6 +1064,7 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
   float4* coef = reinterpret_cast<float4*>(workspace);
   float2* part = reinterpret_cast<float2*>(coef + N);
   float* losses = reinterpret_cast<float*>(part + N * p.count);
+  const bool wave = p.count == 1 && V <= WAVE_VECTORS * 64 * (16 / elem_bytes(elem));
   return with_elem(elem, [&](auto e) -> int {
     using E = decltype(e);
     const E* x = static_cast<const E*>(logits);
@@ -1067,8 +1073,12 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
       all.tokens = tokens;
       all.token_bytes = token_bytes;
       all.c = c;
-      hipLaunchKernelGGL(loss_partial_kernel<E>, dim3((unsigned)(N * p.count)), dim3(LOSS_THREADS), 0, stream, x, rows, all,
-                         N, p.count, p.chunk, part, PolicyCounts{});
+      auto launch = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(N * p.count)), dim3(threads), 0, stream, x, rows, all, N, p.count, p.chunk,
+                           part, PolicyCounts{});
+      };
+      if (wave) launch(loss_partial_kernel<E, 64>, 64);
+      else launch(loss_partial_kernel<E, LOSS_THREADS>, LOSS_THREADS);
       BF_LAUNCH_CHECK("loss_partial_kernel");
     }
     if (p.count == 1)
@@ -1079,8 +1089,12 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
                          rows, a, part, p.count, c, logp, coef, rewards, losses);
     BF_LAUNCH_CHECK("preference_pairs_kernel");
     const unsigned grid = grad ? (unsigned)(N * p.count + 1) : 1u;
-    hipLaunchKernelGGL(preference_grad_kernel<E>, dim3(grid), dim3(LOSS_THREADS), 0, stream, x, rows, a, p.count, p.chunk, c,
-                       coef, losses, loss, static_cast<E*>(grad));
+    auto launch = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, stream, x, rows, a, p.count, p.chunk, c, coef, losses, loss,
+                         static_cast<E*>(grad));
+    };
+    if (wave) launch(preference_grad_kernel<E, 64>, 64);
+    else launch(preference_grad_kernel<E, LOSS_THREADS>, LOSS_THREADS);
     BF_LAUNCH_CHECK("preference_grad_kernel");
     return BF_OK;
   });
