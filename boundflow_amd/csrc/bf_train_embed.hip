@@ -375,21 +375,26 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens: everything in one launch.  A workgroup sorts the tokens of its rows into LDS and sums them, a wave per
-// row; rows of more than FEW_ALONE tokens are taken by all its waves, a part each.
+// Few tokens: everything in one launch.  A workgroup sorts the tokens of its rows into LDS and sums `width` columns of
+// them, a wave per row; rows of more than FEW_ALONE tokens are taken by all its waves, a part each.  Bound by latency:
+// 600 tokens of 1003 values, 129 fp32 columns 9 us (three launches: 23), and by the writing of large tables.
 constexpr int FEW_TOKENS = 2048, FEW_WAVES = 8, FEW_RANGE = 128, FEW_ALONE = 8;
 
 template <class TI, class TO, int VEC>
 __global__ __launch_bounds__(FEW_WAVES * 64) void embed_few_kernel(const TI* __restrict__ g, int64_t ld,
                                                                   const void* __restrict__ tokens, int token_bytes,
-                                                                  int count, int vocab, int dim, int range, float scale,
-                                                                  int into, TO* __restrict__ out) {
+                                                                  int count, int vocab, int dim, int range, int width,
+                                                                  int slices, float scale, int into,
+                                                                  TO* __restrict__ out) {
   __shared__ SortSpace<FEW_WAVES, FEW_RANGE> space;
   __shared__ int order[FEW_TOKENS], begin[FEW_RANGE], number[FEW_RANGE];
   __shared__ float sums[2][FEW_WAVES][64 * VEC];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunks = (dim + 64 * VEC - 1) / (64 * VEC);
-  const int v0 = blockIdx.x * range, held = min(range, vocab - v0);
+  const int v0 = (int)(blockIdx.x / (unsigned)slices) * range, held = min(range, vocab - v0);
+  const int d0 = (int)(blockIdx.x % (unsigned)slices) * width, columns = min(width, dim - d0);
+  const int chunks = (columns + 64 * VEC - 1) / (64 * VEC);
+  g += d0;
+  out += d0;
   sort_range<FEW_WAVES, FEW_RANGE, false>(
       tokens, token_bytes, count, v0, held, space, [&](int at, int i) { order[at] = i; },
       [&](int k, int at, int n) {
@@ -397,24 +402,37 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void embed_few_kernel(const TI* __r
         number[k] = n;
       });
   __syncthreads();
-  for (int k = wave; k < held; k += FEW_WAVES) {
-    const int n = __builtin_amdgcn_readfirstlane(number[k]);
-    if (n > FEW_ALONE || (into && n == 0)) continue;
-    const int list = lane < n ? order[begin[k] + lane] : 0;
-    sum_row<1, TI, TO, VEC>(g, ld, list, 0, n, 0, dim, scale, into, out + (int64_t)(v0 + k) * dim);
+  for (int k0 = 0; k0 < held; k0 += 64) {   // 64 rows' counts at a time, a lane each: one wait for all of them
+    const bool mine = k0 + lane < held;
+    const int n_of = mine ? number[k0 + lane] : 0, begin_of = mine ? begin[k0 + lane] : 0;
+    uint64_t todo = __ballot(mine && (lane & (FEW_WAVES - 1)) == wave && n_of <= FEW_ALONE && !(into && n_of == 0));
+    while (todo) {
+      const int k = __ffsll((unsigned long long)todo) - 1;
+      todo &= todo - 1;
+      const int n = __builtin_amdgcn_readlane(n_of, k), at = __builtin_amdgcn_readlane(begin_of, k);
+      const int list = lane < n ? order[at + lane] : 0;
+      sum_row<1, TI, TO, VEC>(g, ld, list, 0, n, 0, columns, scale, into, out + (int64_t)(v0 + k0 + k) * dim);
+    }
   }
   int buf = 0;
-  for (int k = 0; k < held; ++k) {
-    const int n = number[k];
-    if (n <= FEW_ALONE) continue;   // the same in the whole workgroup
+  uint64_t many = 0;
+  for (int k0 = -64;;) {   // the frequent values, the same in the whole workgroup
+    while (!many) {
+      k0 += 64;
+      if (k0 >= held) return;
+      many = __ballot(k0 + lane < held && number[k0 + lane] > FEW_ALONE);
+    }
+    const int k = k0 + __ffsll((unsigned long long)many) - 1;
+    many &= many - 1;
+    const int n = __builtin_amdgcn_readfirstlane(number[k]);
     const int each = (n + FEW_WAVES - 1) / FEW_WAVES, q1 = min((wave + 1) * each, n);
     TO* row = out + (int64_t)(v0 + k) * dim;
     for (int c = 0; c < chunks; ++c, buf ^= 1) {
       float acc[1][VEC] = {};
       for (int q = wave * each; q < q1; q += 64) {
         const int here = min(64, q1 - q), list = lane < here ? order[begin[k] + q + lane] : 0;
-        if ((c + 1) * 64 * VEC <= dim) add_rows<true, 8, 1>(acc, g, ld, list, 0, here, c, 0, dim);
-        else add_rows<false, 4, 1>(acc, g, ld, list, 0, here, c, 0, dim);
+        if ((c + 1) * 64 * VEC <= columns) add_rows<true, 8, 1>(acc, g, ld, list, 0, here, c, 0, columns);
+        else add_rows<false, 4, 1>(acc, g, ld, list, 0, here, c, 0, columns);
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sums[buf][wave][lane * VEC + e] = acc[0][e];
@@ -424,7 +442,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void embed_few_kernel(const TI* __r
 #pragma unroll
         for (int w = 0; w < FEW_WAVES; ++w) sum[0] += sums[buf][w][x];
         const int d = c * 64 * VEC + x;
-        if (d < dim) write_row<TO, 1>(sum, scale, into, row + d, 1);
+        if (d < columns) write_row<TO, 1>(sum, scale, into, row + d, 1);
       }
     }
   }
@@ -490,14 +508,21 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
       const TI* g = static_cast<const TI*>(grad);
       TO* o = static_cast<TO*>(out);
       if (count <= FEW_TOKENS) {
-        // Four workgroups a CU and more where there are rows for them, and 16 rows each at most, since the frequent values
-        // are mostly neighbours (1000 tokens of 60000 values, 3800 columns, added: 61 us with 59 rows each, 45
-        // with 16); a larger table is cut less finely, because every workgroup reads every token.
-        const int64_t r = ceil_div(vocab, 1024), most = vocab <= (1 << 17) ? 16 : FEW_RANGE;
+        // Four workgroups a CU and more where there is work for them.  The frequent values are mostly neighbours, so a
+        // workgroup with all columns of its rows would be left with most of the sums: it takes a step's columns of
+        // them, or more where that made more than 2048 workgroups, because every one sorts for itself.  2048
+        // tokens of 32000 values, 4096 bf16 columns 75 us (all columns of 16 rows: 120), 1500 of 8000, 768 fp32 columns
+        // 15 (30).
+        int64_t width = 64 * VEC;
+        while (width < dim && ceil_div(vocab, FEW_RANGE) * ceil_div(dim, width) > 2048) width *= 2;
+        const int64_t slices = ceil_div(dim, width), r = ceil_div(vocab * slices, 1024);
+        // pieces of many rows that are all written come in more workgroups: 1000 tokens of 60000 values, 3800 fp16
+        // columns 124 us against 135
+        const int64_t most = !accumulate && slices > 1 ? FEW_RANGE / 2 : FEW_RANGE;
         const int range = (int)(r < most ? r : most);
-        hipLaunchKernelGGL((embed_few_kernel<TI, TO, VEC>), dim3((unsigned)ceil_div(vocab, range)), dim3(FEW_WAVES * 64), 0,
-                           stream, g, grad_ld, tokens, token_bytes, (int)count, (int)vocab, (int)dim, range, scale,
-                           accumulate, o);
+        hipLaunchKernelGGL((embed_few_kernel<TI, TO, VEC>), dim3((unsigned)(ceil_div(vocab, range) * slices)),
+                           dim3(FEW_WAVES * 64), 0, stream, g, grad_ld, tokens, token_bytes, (int)count, (int)vocab,
+                           (int)dim, range, (int)width, (int)slices, scale, accumulate, o);
         BF_LAUNCH_CHECK("embed_few_kernel");
         return BF_OK;
       }

@@ -109,6 +109,13 @@ def test_embed_tokens_grad(dtype, kind, count, vocab, dim):
     assert torch.equal(running.cpu()[untouched], start[untouched])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind,count,vocab,dim", [
+    ("hot", 900, 1003, 1601), ("hot", 2048, 9000, 1100), ("outside", 777, 5000, 1537), ("spread", 800, 70001, 771)])
+def test_embed_tokens_grad_of_few_tokens_in_wide_rows(dtype, kind, count, vocab, dim):
+    test_embed_tokens_grad(dtype, kind, count, vocab, dim)
+
+
 def test_embed_tokens_grad_of_views():
     dev = device()
     g = gen(5)
