@@ -377,7 +377,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void embed_join_kernel(
 // ---------------------------------------------------------------------------
 // Few tokens: everything in one launch.  A workgroup sorts the tokens of its rows into LDS and sums `width` columns of
 // them, a wave per row; rows of more than FEW_ALONE tokens are taken by all its waves, a part each.  Bound by latency:
-// 600 tokens of 1003 values, 129 fp32 columns 9 us (three launches: 23), and by the writing of large tables.
+// 600 tokens of 1003 values, 129 fp32 columns 9.5 us (three launches: 23), and by the writing of large tables.
 constexpr int FEW_TOKENS = 2048, FEW_WAVES = 8, FEW_RANGE = 128, FEW_ALONE = 8;
 
 template <class TI, class TO, int VEC>
