@@ -33,7 +33,8 @@ MOMENT_BLOCK = 128   # elements of an 8-bit moment that share a scale; every ten
 
 # Every call checks a dozen tensors before a kernel of a few microseconds: the checks are plain
 # attribute reads, and addresses go to the library as numbers (the tensors are this module's
-# callers' or its own locals until the call has enqueued its kernels).
+# callers' or its own locals until the call has enqueued its kernels).  What the kernels write in
+# fp32 is allocated as such by name: a program for 16-bit networks may have another default type.
 
 def _current_device(t: torch.Tensor, name: str) -> int:
     """The device of the call's first tensor, which has to be the current one."""
@@ -140,7 +141,7 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
             raise ValueError(f"dtype must be {grad.dtype} or float32, got {dtype}")
         out = torch.empty(vocab, dim, dtype=dtype, device=grad.device)
     need = _lib.load().bf_embed_grad_workspace(count, vocab, dim)
-    space = torch.empty(need, device=grad.device) if need else None
+    space = torch.empty(need, dtype=torch.float32, device=grad.device) if need else None
     _lib.call("bf_embed_grad", rows.data_ptr(), max(rows.stride(0), dim), elem, tokens.data_ptr(), token_bytes, count,
               vocab, dim, float(scale), _ELEM[out.dtype], accumulate_into is not None, out.data_ptr(), _address(space),
               current_raw_stream(dev))
@@ -231,7 +232,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
             mask = mask.contiguous()
     # stats, logp and the workspace in one allocation
     N = B * T
-    out = torch.empty(4 + N + 3 + _lib.load().bf_policy_loss_workspace(B, T, V, elem), device=logits.device)
+    out = torch.empty(4 + N + 3 + _lib.load().bf_policy_loss_workspace(B, T, V, elem), dtype=torch.float32,
+                      device=logits.device)
     grad = torch.empty(shape, dtype=logits.dtype, device=logits.device) if with_grad else None
     at = out.data_ptr()
     _lib.call("bf_policy_loss", logits.data_ptr(), elem, B, T, V, strides[0], strides[1] if dims == 3 else 0,
@@ -278,7 +280,8 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.
     pairs = offsets.numel() // 2
     # loss, rewards, logp and the workspace in one allocation
     own = 1 + 2 * pairs + N
-    out = torch.empty(own + 3 + _lib.load().bf_preference_loss_workspace(N, V, pairs, elem), device=logits.device)
+    out = torch.empty(own + 3 + _lib.load().bf_preference_loss_workspace(N, V, pairs, elem), dtype=torch.float32,
+                      device=logits.device)
     grad = torch.empty((N, V), dtype=logits.dtype, device=logits.device) if with_grad else None
     at = out.data_ptr()
     _lib.call("bf_preference_loss", logits.data_ptr(), elem, N, V, ld, tokens.data_ptr(), token_bytes,
@@ -328,13 +331,14 @@ def adamw_moments(params: Sequence[torch.Tensor], *, bits: int = 32, master: boo
     total = at[-1]
     copies = None
     if master:
-        copies = torch.zeros(total, device=dev)
+        copies = torch.zeros(total, dtype=torch.float32, device=dev)
         for a, p in zip(at, params):
             copies[a:a + p.numel()].copy_(p.detach().reshape(-1))
     if bits == 32:
-        return AdamWMoments(torch.zeros(total, device=dev), torch.zeros(total, device=dev), None, None, copies)
+        m, v = (torch.zeros(total, dtype=torch.float32, device=dev) for _ in range(2))
+        return AdamWMoments(m, v, None, None, copies)
     m, v = (torch.zeros(total, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
-    scales = [torch.zeros(total // MOMENT_BLOCK, device=dev) for _ in range(2)]
+    scales = [torch.zeros(total // MOMENT_BLOCK, dtype=torch.float32, device=dev) for _ in range(2)]
     return AdamWMoments(m, v, scales[0], scales[1], copies)
 
 

@@ -1,0 +1,57 @@
+"""What the training operators allocate, and hand to the library as addresses, without a device: the
+library call is replaced by a recorder, so the tensors can lie on the CPU."""
+
+import pytest
+import torch
+
+from boundflow_amd import _lib, training
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """(tensors allocated, calls made) while the operators run on CPU tensors."""
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built (run python -m boundflow_amd.build)")
+    made, calls = [], []
+    for name in ("empty", "zeros"):
+        def record(*args, real=getattr(torch, name), **kw):
+            made.append(real(*args, **kw))
+            return made[-1]
+        monkeypatch.setattr(torch, name, record)
+    monkeypatch.setattr(training, "_current_device", lambda t, name: -1)
+    monkeypatch.setattr(training, "_on_device", lambda t, dev, name: None)
+    monkeypatch.setattr(training, "current_raw_stream", lambda dev: None)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: calls.append((name, args)))
+    return made, calls
+
+
+@pytest.fixture(params=[torch.bfloat16, torch.float16, torch.float64], ids=str)
+def default_type(request):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(request.param)
+    yield request.param
+    torch.set_default_dtype(before)
+
+
+def fp32(*shape):
+    return torch.ones(*shape, dtype=torch.float32)
+
+
+def test_buffers_are_fp32_whatever_the_default_type(recorded, default_type):
+    """fp32 inputs: everything that a kernel writes is fp32 (token arrays and 8-bit moments aside)."""
+    made, calls = recorded
+    tokens = torch.ones(3000, dtype=torch.int64)
+    training.embed_tokens_grad(fp32(3000, 4), tokens, 5)
+    training.embed_tokens_grad(fp32(3000, 4), tokens, 5, accumulate_into=fp32(5, 4))
+    r = training.policy_loss(fp32(300, 700), tokens[:300], fp32(300), fp32(300))
+    q = training.preference_loss(fp32(30, 70), tokens[:30], fp32(30), torch.tensor([0, 20, 30]))
+    for t in (r.stats, r.loss, r.logp, r.grad_logits, q.loss, q.rewards, q.logp, q.grad_logits):
+        assert t.dtype == torch.float32
+    weights = [fp32(200), fp32(3, 5)]
+    for bits in (32, 8):
+        moments = training.adamw_moments(weights, bits=bits, master=True)
+        training.adamw_step(weights, [fp32(200), fp32(3, 5)], moments, step=1)
+        assert moments.master.dtype == torch.float32
+    assert [name for name, _ in calls] == ["bf_embed_grad"] * 2 + ["bf_policy_loss", "bf_preference_loss"] + \
+        ["bf_adamw_multi"] * 2
+    assert made and all(t.dtype in (torch.float32, torch.uint8) for t in made), [t.dtype for t in made]
