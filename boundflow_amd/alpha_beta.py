@@ -149,7 +149,7 @@ class _AdamGroup:
 def branch_choices(trace: ForwardTrace, batch: int) -> List[Optional[Tuple[str, int]]]:
     """Widest ambiguous neuron per domain (alpha_beta_crown.py:145-182), on the device."""
     dev = next(iter(trace.relu_pre.values())).lower.device if trace.relu_pre else torch.device("cuda")
-    gap = torch.full((batch,), float("-inf"), device=dev)
+    gap = torch.full((batch,), float("-inf"), dtype=torch.float32, device=dev)
     layer = torch.full((batch,), -1, dtype=torch.int32, device=dev)
     idx = torch.zeros(batch, dtype=torch.int32, device=dev)
     names = list(trace.relu_pre.keys())
@@ -167,7 +167,7 @@ def branch_choices(trace: ForwardTrace, batch: int) -> List[Optional[Tuple[str, 
 def branch_tensors(trace: ForwardTrace, batch: int):
     """Device tensors (layer index, neuron index, gap) of the branching rule."""
     dev = next(iter(trace.relu_pre.values())).lower.device
-    gap = torch.full((batch,), float("-inf"), device=dev)
+    gap = torch.full((batch,), float("-inf"), dtype=torch.float32, device=dev)
     layer = torch.full((batch,), -1, dtype=torch.int32, device=dev)
     idx = torch.zeros(batch, dtype=torch.int32, device=dev)
     stream = _lib.stream_handle()
@@ -213,7 +213,7 @@ def _grad_pass(spec: InputSpec, chain: Chain, trace: ForwardTrace, saved: dict, 
         else:
             vec = _bias_map(layer) if layer.bias is not None else None
             vec_ld = 0
-        gt = torch.empty(M, n_out, device=dev)
+        gt = torch.empty(M, n_out, dtype=torch.float32, device=dev)
         if layer.kind == "linear":
             rank1 = (_lib.ptr(G if vec is not None else None), _lib.ptr(vec), vec_ld)
             packed = reverse_takes_parts(M, n_out, n_in, S)
@@ -225,7 +225,7 @@ def _grad_pass(spec: InputSpec, chain: Chain, trace: ForwardTrace, saved: dict, 
                               n_in, S, *rank1, stream)
                 else:
                     wsz = int(_lib.load().bf_gemm_rank1_workspace(M, n_out, n_in))
-                    ws = torch.empty(wsz, device=dev) if wsz else None
+                    ws = torch.empty(wsz, dtype=torch.float32, device=dev) if wsz else None
                     _lib.call("bf_gemm_rank1", _lib.ptr(g), n_in, _lib.ptr(weight), n_in, 1, _lib.ptr(gt), n_out, M,
                               n_out, n_in, S, *rank1, _lib.ptr(ws), wsz, stream)
         else:
@@ -242,11 +242,11 @@ def _grad_pass(spec: InputSpec, chain: Chain, trace: ForwardTrace, saved: dict, 
         name = layer.out_name
         pre = trace.relu_pre[name]
         A_in, a_stride = saved["A_in"][k]
-        ga = torch.empty(B, n_out, device=dev)
-        gb = torch.empty(B, n_out, device=dev)
+        ga = torch.empty(B, n_out, dtype=torch.float32, device=dev)
+        gb = torch.empty(B, n_out, dtype=torch.float32, device=dev)
         a_t, a_ld = alpha.get(name, (None, 0))
         sp, sp_ld = splits.get(name, (None, 0))
-        g_in = torch.empty(M, n_out, device=dev)
+        g_in = torch.empty(M, n_out, dtype=torch.float32, device=dev)
         with _timed("relu_grad", 0.0, 4.0 * (3 * M * n_out + 4 * B * n_out)):
             _lib.call("bf_relu_grad", _lib.ptr(gt), _lib.ptr(A_in), a_stride, B, S, n_out,
                       _lib.ptr(pre.lower.reshape(B, n_out)), _lib.ptr(pre.upper.reshape(B, n_out)), _lib.ptr(a_t),
@@ -425,13 +425,13 @@ def run_alpha_beta_crown_mlp(
     # one optimizer over every alpha (clamped to [0, 1]) and every split multiplier (>= 0)
     adam = _AdamGroup([alpha[n] for n in names] + [beta[n] for n in beta_names],
                       [(0.0, 1.0)] * len(names) + [(0.0, None)] * len(beta_names))
-    best_metric = torch.empty(B, device=dev)
-    best_lb = torch.empty(B, S, device=dev)
+    best_metric = torch.empty(B, dtype=torch.float32, device=dev)
+    best_lb = torch.empty(B, S, dtype=torch.float32, device=dev)
     improved = torch.empty(B, dtype=torch.int32, device=dev)
     best_alpha = {n: alpha[n].clone() for n in names}
     best_beta = {n: beta[n].clone() for n in names}
     best_scalar = None
-    add = {n: torch.empty(B, numel[n], device=dev) for n in beta_names}
+    add = {n: torch.empty(B, numel[n], dtype=torch.float32, device=dev) for n in beta_names}
     beta_args = (_lib.ptr_array([beta[n] for n in beta_names]), _lib.i64_array([p_ld[n] for n in beta_names]),
                  _lib.ptr_array([splits[n][0] for n in beta_names]), _lib.i64_array([splits[n][1] for n in beta_names]),
                  _lib.i64_array([numel[n] for n in beta_names]), B, _lib.ptr_array([add[n] for n in beta_names]))
@@ -474,7 +474,7 @@ def run_alpha_beta_crown_mlp(
         if not per_batch_params:
             for d in (g_alpha, g_beta):
                 for n in names:
-                    r = torch.empty(numel[n], device=dev)
+                    r = torch.empty(numel[n], dtype=torch.float32, device=dev)
                     _lib.call("bf_sum_rows", _lib.ptr(d[n]), B, numel[n], _lib.ptr(r), stream)
                     d[n] = r
         # small parameters: the step takes the best-of copy of this evaluation's parameters with it
@@ -524,24 +524,24 @@ def _optimise_general(module, spec, trace, chain, linear_spec_C, bound, grad, ou
     use_u = objective in ("upper", "gap", "both")
     C = linear_spec_C
     if C is None:
-        C = torch.eye(out_dim, device=dev).unsqueeze(0).expand(B, out_dim, out_dim)
+        C = torch.eye(out_dim, dtype=torch.float32, device=dev).unsqueeze(0).expand(B, out_dim, out_dim)
     C_neg = (-C).contiguous()
     bound_u, grad_u, _ = _evaluator(module, spec, trace, chain, C_neg)
-    ones = torch.ones(M, device=dev)
+    ones = torch.ones(M, dtype=torch.float32, device=dev)
     g_scale = float(np.float32(-1.0)) if per_batch_params else float(np.float32(-1.0) / np.float32(B))
-    G_l = torch.empty(M, device=dev) if use_l else None
-    G_nu = torch.empty(M, device=dev) if use_u else None
-    metric = torch.empty(B, device=dev)
-    best_metric = torch.empty(B, device=dev)
-    best_lb = torch.empty(B, S, device=dev)
-    best_ub = torch.empty(B, S, device=dev)
+    G_l = torch.empty(M, dtype=torch.float32, device=dev) if use_l else None
+    G_nu = torch.empty(M, dtype=torch.float32, device=dev) if use_u else None
+    metric = torch.empty(B, dtype=torch.float32, device=dev)
+    best_metric = torch.empty(B, dtype=torch.float32, device=dev)
+    best_lb = torch.empty(B, S, dtype=torch.float32, device=dev)
+    best_ub = torch.empty(B, S, dtype=torch.float32, device=dev)
     improved = torch.empty(B, dtype=torch.int32, device=dev)
     best_scalar = None
     adam = _AdamGroup([alpha[n] for n in names] + [beta[n] for n in beta_names],
                       [(0.0, 1.0)] * len(names) + [(0.0, None)] * len(beta_names))
     best_alpha = {n: alpha[n].clone() for n in names}
     best_beta = {n: beta[n].clone() for n in names}
-    add = {n: torch.empty(B, numel[n], device=dev) for n in beta_names}
+    add = {n: torch.empty(B, numel[n], dtype=torch.float32, device=dev) for n in beta_names}
     beta_args = (_lib.ptr_array([beta[n] for n in beta_names]), _lib.i64_array([p_ld[n] for n in beta_names]),
                  _lib.ptr_array([splits[n][0] for n in beta_names]), _lib.i64_array([splits[n][1] for n in beta_names]),
                  _lib.i64_array([numel[n] for n in beta_names]), B, _lib.ptr_array([add[n] for n in beta_names]))
@@ -598,7 +598,7 @@ def _optimise_general(module, spec, trace, chain, linear_spec_C, bound, grad, ou
         if not per_batch_params:
             for d in (g_alpha, g_beta):
                 for n in list(d.keys()):
-                    r = torch.empty(numel[n], device=dev)
+                    r = torch.empty(numel[n], dtype=torch.float32, device=dev)
                     _lib.call("bf_sum_rows", _lib.ptr(d[n]), B, numel[n], _lib.ptr(r), stream)
                     d[n] = r
         adam.step([g_alpha[n] for n in names] + [g_beta[n] for n in beta_names], lr, stream)
@@ -694,7 +694,7 @@ def lower_bound_gradients(module, input_spec, *, linear_spec_C, relu_alpha: Dict
                 splits[n] = _broadcast_split(relu_split_state[n].to(dev), B, numel[n])
                 if relu_beta is not None and bool((splits[n][0] != 0).any().item()):
                     b = relu_beta[n].reshape((B, numel[n]) if per_batch_params else (numel[n],)).contiguous()
-                    add[n] = torch.empty(B, numel[n], device=dev)
+                    add[n] = torch.empty(B, numel[n], dtype=torch.float32, device=dev)
                     _lib.call("bf_beta_coeff", _lib.ptr(b), p_ld[n], _lib.ptr(splits[n][0]), splits[n][1], B,
                               numel[n], _lib.ptr(add[n]), stream)
     saved = {"grad_rows": G}
@@ -704,7 +704,7 @@ def lower_bound_gradients(module, input_spec, *, linear_spec_C, relu_alpha: Dict
     if not per_batch_params:
         for d in (g_alpha, g_beta):
             for n in list(d.keys()):
-                r = torch.empty(numel[n], device=dev)
+                r = torch.empty(numel[n], dtype=torch.float32, device=dev)
                 _lib.call("bf_sum_rows", _lib.ptr(d[n]), B, numel[n], _lib.ptr(r), stream)
                 d[n] = r
     return bounds, g_alpha, g_beta

@@ -141,8 +141,8 @@ class _Frontier:
         self.dev = dev
         self.cap = capacity
         self.split = {n: torch.zeros(capacity, k, dtype=torch.int8, device=dev) for n, k in sizes.items()}
-        self.alpha = {n: torch.zeros(capacity, k, device=dev) for n, k in sizes.items()}
-        self.beta = {n: torch.zeros(capacity, k, device=dev) for n, k in sizes.items()}
+        self.alpha = {n: torch.zeros(capacity, k, dtype=torch.float32, device=dev) for n, k in sizes.items()}
+        self.beta = {n: torch.zeros(capacity, k, dtype=torch.float32, device=dev) for n, k in sizes.items()}
         self.free: List[int] = list(range(capacity - 1, -1, -1))
 
     def alloc(self, count: int) -> List[int]:
@@ -499,7 +499,7 @@ class NativeReluSplitBabConfig:
                 or self.max_eval_batch_size < 1 or self.available_memory_bytes < 1 or self.memory_budget_bytes < 1
                 or self.memory_budget_bytes > self.available_memory_bytes):
             raise ValueError("native ReLU-split BaB config is invalid")
-        if not torch.isfinite(torch.tensor(self.threshold)):
+        if not torch.isfinite(torch.tensor(self.threshold, dtype=torch.float32)):
             raise ValueError("native ReLU-split BaB threshold must be finite")
 
 
@@ -633,8 +633,8 @@ def run_native_relu_split_bab(module, input_spec, *, linear_spec_C: torch.Tensor
             width = torch.full((k,), -1.0, device=dev, dtype=torch.float64)
             layer = torch.full((k,), -1, device=dev, dtype=torch.int32)
             idx = torch.zeros(k, device=dev, dtype=torch.int32)
-            blo = torch.zeros(k, device=dev)
-            bhi = torch.zeros(k, device=dev)
+            blo = torch.zeros(k, dtype=torch.float32, device=dev)
+            bhi = torch.zeros(k, dtype=torch.float32, device=dev)
             for li, n in enumerate(names):
                 pre = trace.relu_pre[n]
                 _lib.call("bf_branch_update_native", _lib.ptr(pre.lower.reshape(k, sizes[n])),

@@ -36,7 +36,7 @@ def packed_conv_transpose_weights(W: torch.Tensor, Co: int, Ho: int, Wo: int, Ci
     geo = (Co, Ho, Wo, Ci, KH, KW, sh, sw, ph, pw, Hi, Wi)
 
     def pack():
-        out = torch.empty(int(_lib.load().bf_conv_transpose_packed_floats(*geo)), device=W.device)
+        out = torch.empty(int(_lib.load().bf_conv_transpose_packed_floats(*geo)), dtype=torch.float32, device=W.device)
         _lib.call("bf_conv_transpose_pack_weights", _lib.ptr(W), *geo, _lib.ptr(out), _lib.stream_handle())
         return out
     return derived("conv_t_pack:" + "x".join(str(v) for v in geo), (W if source is None else source,), pack)
@@ -112,10 +112,10 @@ def conv_backward_step(layer, is_first, A_u, A_l, stride, b_u, b_l, B, S, pre_lo
     if not is_first and _lib.load().bf_conv_transpose_hwc_supported(Co, Ho, Wo, Ci, KH, KW, sh, sw, ph, pw, Hi, Wi):
         # the relaxation applied while the transposed convolution stages each row: the relaxed
         # rows reach HBM only when the gradient pass needs them
-        y_u = torch.empty(M, n_in, device=dev) if A_u is not None else None
-        y_l = torch.empty(M, n_in, device=dev) if A_l is not None else None
-        nb_u = torch.empty(M, device=dev) if A_u is not None else None
-        nb_l = torch.empty(M, device=dev) if A_l is not None else None
+        y_u = torch.empty(M, n_in, dtype=torch.float32, device=dev) if A_u is not None else None
+        y_l = torch.empty(M, n_in, dtype=torch.float32, device=dev) if A_l is not None else None
+        nb_u = torch.empty(M, dtype=torch.float32, device=dev) if A_u is not None else None
+        nb_l = torch.empty(M, dtype=torch.float32, device=dev) if A_l is not None else None
         keep_l = torch.empty_like(A_l) if (save is not None and A_l is not None) else None
         packed = packed_conv_transpose_weights(W, Co, Ho, Wo, Ci, KH, KW, sh, sw, ph, pw, Hi, Wi,
                                                source=layer.weight)
@@ -128,10 +128,10 @@ def conv_backward_step(layer, is_first, A_u, A_l, stride, b_u, b_l, B, S, pre_lo
         if save is not None:
             save.setdefault("relaxed", {})[layer.op_index] = keep_l
         return y_u, y_l, nb_u, nb_l, S * n_in, None
-    nb_u = torch.empty(M, device=dev) if A_u is not None else None
-    nb_l = torch.empty(M, device=dev) if A_l is not None else None
-    c_u = torch.empty(M, device=dev) if (A_u is not None and cvec is not None) else None
-    c_l = torch.empty(M, device=dev) if (A_l is not None and cvec is not None) else None
+    nb_u = torch.empty(M, dtype=torch.float32, device=dev) if A_u is not None else None
+    nb_l = torch.empty(M, dtype=torch.float32, device=dev) if A_l is not None else None
+    c_u = torch.empty(M, dtype=torch.float32, device=dev) if (A_u is not None and cvec is not None) else None
+    c_l = torch.empty(M, dtype=torch.float32, device=dev) if (A_l is not None and cvec is not None) else None
     if is_first and cvec is not None and _lib.load().bf_conv_transpose_small_supported(
             Co, Ho, Wo, Ci, KH, KW, sh, sw, ph, pw, Hi, Wi):
         # input layer: relaxation, transposed conv and concretization norm in one pass
@@ -146,8 +146,8 @@ def conv_backward_step(layer, is_first, A_u, A_l, stride, b_u, b_l, B, S, pre_lo
                   _lib.ptr(b_u), _lib.ptr(b_l), _lib.ptr(rA_u), _lib.ptr(rA_l), _lib.ptr(nb_u), _lib.ptr(nb_l),
                   _lib.ptr(c_u), _lib.ptr(c_l), stream)
     if not is_first:
-        y_u = torch.empty(M, n_in, device=dev) if A_u is not None else None
-        y_l = torch.empty(M, n_in, device=dev) if A_l is not None else None
+        y_u = torch.empty(M, n_in, dtype=torch.float32, device=dev) if A_u is not None else None
+        y_l = torch.empty(M, n_in, dtype=torch.float32, device=dev) if A_l is not None else None
         with _timed("conv_transpose", flops, 4.0 * nz * (M * n_out + M * n_in)):
             _lib.call("bf_conv_transpose_rows", _lib.ptr(rA_u), _lib.ptr(rA_l), M, Co, Ho, Wo, _lib.ptr(W), Ci, KH,
                       KW, sh, sw, ph, pw, Hi, Wi, _lib.ptr(y_u), _lib.ptr(y_l), S, None, 0, 0, None, None, None,
@@ -166,12 +166,12 @@ def conv_backward_step(layer, is_first, A_u, A_l, stride, b_u, b_l, B, S, pre_lo
     else:
         rad = None
         eps = float(pert.eps)
-    norm_u = torch.empty(M, device=dev) if A_u is not None else None
-    norm_l = torch.empty(M, device=dev) if A_l is not None else None
+    norm_u = torch.empty(M, dtype=torch.float32, device=dev) if A_u is not None else None
+    norm_l = torch.empty(M, dtype=torch.float32, device=dev) if A_l is not None else None
     h_scale = h_out = None
     if save is not None and save.get("grad_rows") is not None:
         h_scale = call_memo(save, f"h_scale:{eps!r}", lambda: (save["grad_rows"] * (-eps)).contiguous())
-        h_out = torch.empty(M, n_in, device=dev)
+        h_out = torch.empty(M, n_in, dtype=torch.float32, device=dev)
         save["h"] = h_out
         save["cvec"] = cvec
     with _timed("conv_transpose_concretize", flops, 4.0 * nz * M * n_out):
@@ -180,8 +180,8 @@ def conv_backward_step(layer, is_first, A_u, A_l, stride, b_u, b_l, B, S, pre_lo
                   _lib.ptr(norm_l), _lib.ptr(h_scale), _lib.ptr(h_out), stream)
     if save is not None:
         save.setdefault("relaxed", {})[layer.op_index] = rA_l
-    lb = torch.empty(B, S, device=dev) if A_l is not None else None
-    ub = torch.empty(B, S, device=dev) if A_u is not None else None
+    lb = torch.empty(B, S, dtype=torch.float32, device=dev) if A_l is not None else None
+    ub = torch.empty(B, S, dtype=torch.float32, device=dev) if A_u is not None else None
     _lib.call("bf_concretize_finalize", _lib.ptr(norm_u), _lib.ptr(norm_l), 1, M, _lib.ptr(c_u), _lib.ptr(c_l),
               _lib.ptr(nb_u), _lib.ptr(nb_l), eps, norm_p, _lib.ptr(lb), _lib.ptr(ub), stream)
     return None, None, None, None, 0, IntervalState(lower=lb, upper=ub)
@@ -207,17 +207,17 @@ def _input_layer_fused(spec, save, A_u, A_l, b_u, b_l, B, S, M, pre_lo, pre_hi, 
     else:
         rad = None
         eps = float(pert.eps)
-    norm_u = torch.empty(M, device=dev) if A_u is not None else None
-    norm_l = torch.empty(M, device=dev) if A_l is not None else None
+    norm_u = torch.empty(M, dtype=torch.float32, device=dev) if A_u is not None else None
+    norm_l = torch.empty(M, dtype=torch.float32, device=dev) if A_l is not None else None
     h_scale = h_out = None
     if save is not None and save.get("grad_rows") is not None:
         h_scale = call_memo(save, f"h_scale:{eps!r}", lambda: (save["grad_rows"] * (-eps)).contiguous())
-        h_out = torch.empty(M, n_in, device=dev)
+        h_out = torch.empty(M, n_in, dtype=torch.float32, device=dev)
         save["h"] = h_out
         save["cvec"] = cvec
-    rel_l = torch.empty(M, n_out, device=dev) if (save is not None and A_l is not None) else None
-    lb = torch.empty(B, S, device=dev) if A_l is not None else None
-    ub = torch.empty(B, S, device=dev) if A_u is not None else None
+    rel_l = torch.empty(M, n_out, dtype=torch.float32, device=dev) if (save is not None and A_l is not None) else None
+    lb = torch.empty(B, S, dtype=torch.float32, device=dev) if A_l is not None else None
+    ub = torch.empty(B, S, dtype=torch.float32, device=dev) if A_u is not None else None
     with _timed("crown_relu_conv_transpose_concretize", flops,
                 4.0 * nz * (M * n_out + 2 * B * n_out) + (4.0 * M * n_out if rel_l is not None else 0.0)):
         _lib.call("bf_crown_relu_conv_transpose_concretize", _lib.ptr(A_u), _lib.ptr(A_l), B, S, Co, Ho, Wo,

@@ -727,7 +727,8 @@ def crown_backward(
             # C = I: I @ W is W itself, shared by every domain (no contraction needed)
             A_u = W if A_u is not None else None
             A_l = W if A_l is not None else None
-            brow = (bias if bias is not None else torch.zeros(N, device=dev)).repeat(B).contiguous()
+            brow = (bias if bias is not None else
+                    torch.zeros(N, dtype=torch.float32, device=dev)).repeat(B).contiguous()
             b_u = brow if A_u is not None else None
             b_l = brow if A_l is not None else None
             stride = 0
@@ -985,7 +986,7 @@ def _with_upper_add(backward, relu_pre, C, add_l, add_u, B: int, out_dim: int) -
                 f"{tuple(pre.lower.shape)} for {name}")
     if C is None:
         dev = next(iter(relu_pre.values())).lower.device if relu_pre else None
-        C = torch.eye(out_dim, device=dev).unsqueeze(0).expand(B, out_dim, out_dim).contiguous()
+        C = torch.eye(out_dim, dtype=torch.float32, device=dev).unsqueeze(0).expand(B, out_dim, out_dim).contiguous()
     lower = backward(C, add_l, False, True).lower
     neg_add = {k: -v for k, v in add_u.items()}
     upper = -backward(-C, neg_add, False, True).lower

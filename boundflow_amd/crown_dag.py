@@ -425,8 +425,8 @@ def crown_backward_dag(
 
     def like(st: _Rows, cols: int, one: bool):
         """Fresh (A_u, A_l) of [M, cols] for the bounds st carries (one buffer when shared)."""
-        au = torch.empty(M, cols, device=dev) if st.A_u is not None else None
-        al = (au if one else torch.empty(M, cols, device=dev)) if st.A_l is not None else None
+        au = torch.empty(M, cols, dtype=torch.float32, device=dev) if st.A_u is not None else None
+        al = (au if one else torch.empty(M, cols, dtype=torch.float32, device=dev)) if st.A_l is not None else None
         return au, al
 
     def zeros_like_b(st: _Rows):
@@ -444,8 +444,9 @@ def crown_backward_dag(
         nb_u = None if nb_u is None else nb_u.reshape(M)
         nb_l = None if nb_l is None else nb_l.reshape(M)
         apart = cvec is not None or kbias2 is not None
-        c_u = torch.empty(M, device=dev) if (apart and st.A_u is not None) else None
-        c_l = (c_u if one else torch.empty(M, device=dev)) if (apart and st.A_l is not None) else None
+        c_u = torch.empty(M, dtype=torch.float32, device=dev) if (apart and st.A_u is not None) else None
+        c_l = (c_u if one else torch.empty(M, dtype=torch.float32, device=dev)) \
+            if (apart and st.A_l is not None) else None
         A_l_in = None if one else st.A_l
         nz = int(st.A_u is not None) + int(A_l_in is not None)
         reads = 1 if (nz == 2 and ptr_of(st.A_u) == ptr_of(st.A_l)) else nz
@@ -473,7 +474,7 @@ def crown_backward_dag(
     def add_rows(a, b, cols):
         if a is None:
             return None
-        out = torch.empty(M, cols, device=dev) if cols > 1 else torch.empty(M, device=dev)
+        out = torch.empty((M, cols) if cols > 1 else (M,), dtype=torch.float32, device=dev)
         _lib.call("bf_rows_add", _lib.ptr(a), _lib.ptr(b), M, cols, S, None, None, 0, _lib.ptr(out), stream)
         return out
 
@@ -703,8 +704,8 @@ def _concretize(spec: InputSpec, st: _Rows, B: int, S: int) -> IntervalState:
     dev = spec.center.device
     I = int((st.A_u if st.A_u is not None else st.A_l).shape[1])
     center, rad, eps = _input_center_radius(spec, B, I)
-    lb = torch.empty(B, S, device=dev) if st.A_l is not None else None
-    ub = torch.empty(B, S, device=dev) if st.A_u is not None else None
+    lb = torch.empty(B, S, dtype=torch.float32, device=dev) if st.A_l is not None else None
+    ub = torch.empty(B, S, dtype=torch.float32, device=dev) if st.A_u is not None else None
     nz = int(lb is not None) + int(ub is not None)
     with _timed("concretize_dense", 2.0 * nz * B * S * I, 4.0 * nz * B * S * I):
         if ub is not None:
@@ -742,7 +743,7 @@ def lower_grad_pass(module: BFTaskModule, spec: InputSpec, trace: DagTrace, save
     I = int(A_in.shape[1])
     center, rad, eps = _input_center_radius(spec, B, I)
     GA: Dict[str, torch.Tensor] = {}
-    g0 = torch.empty(M, I, device=dev)
+    g0 = torch.empty(M, I, dtype=torch.float32, device=dev)
     with _timed("concretize_dense_grad", 0.0, 4.0 * 3 * M * I):
         _lib.call("bf_concretize_dense_grad", _lib.ptr(A_in), B, S, I, _lib.ptr(center), _lib.ptr(rad), eps,
                   input_norm_p(spec.perturbation), _lib.ptr(G), _lib.ptr(g0), stream)
@@ -760,7 +761,7 @@ def lower_grad_pass(module: BFTaskModule, spec: InputSpec, trace: DagTrace, save
             W = params[op.inputs[1]].contiguous()
             bias = params[op.inputs[2]].contiguous() if len(op.inputs) == 3 else None
             n_out, n_in = int(W.shape[0]), int(W.shape[1])
-            gt = torch.empty(M, n_out, device=dev)
+            gt = torch.empty(M, n_out, dtype=torch.float32, device=dev)
             rank1 = (_lib.ptr(G if bias is not None else None), _lib.ptr(bias), 0)
             packed = reverse_takes_parts(M, n_out, n_in, S)
             weight = weight_parts(params[op.inputs[1]], True) if packed else W
@@ -771,7 +772,7 @@ def lower_grad_pass(module: BFTaskModule, spec: InputSpec, trace: DagTrace, save
                               n_out, n_in, S, *rank1, stream)
                 else:
                     wsz = int(_lib.load().bf_gemm_rank1_workspace(M, n_out, n_in))
-                    ws = torch.empty(wsz, device=dev) if wsz else None
+                    ws = torch.empty(wsz, dtype=torch.float32, device=dev) if wsz else None
                     _lib.call("bf_gemm_rank1", _lib.ptr(GA[x]), n_in, _lib.ptr(weight), n_in, 1, _lib.ptr(gt), n_out, M,
                               n_out, n_in, S, *rank1, _lib.ptr(ws), wsz, stream)
             GA[y] = gt
@@ -783,7 +784,7 @@ def lower_grad_pass(module: BFTaskModule, spec: InputSpec, trace: DagTrace, save
             Co, Ho, Wo = out_shape
             KH, KW = int(W.shape[2]), int(W.shape[3])
             vec = _conv_bias_map(params[op.inputs[2]], out_shape) if len(op.inputs) == 3 else None
-            gt = torch.empty(M, Co * Ho * Wo, device=dev)
+            gt = torch.empty(M, Co * Ho * Wo, dtype=torch.float32, device=dev)
             with _timed("grad_conv", 2.0 * M * Co * Ho * Wo * Ci * KH * KW, 4.0 * (M * Ci * Hi * Wi + M * Co * Ho * Wo)):
                 _lib.call("bf_conv2d_rows", _lib.ptr(GA[x]), 1, M, Ci, Hi, Wi, _lib.ptr(W), 0, Co, KH, KW, sh, sw, ph,
                           pw, Ho, Wo, _lib.ptr(gt), _lib.ptr(G if vec is not None else None), _lib.ptr(vec), 1, 0,
@@ -794,9 +795,9 @@ def lower_grad_pass(module: BFTaskModule, spec: InputSpec, trace: DagTrace, save
             n = _numel(pre.lower.shape[1:])
             a_t, a_ld = alpha.get(x, (None, 0))
             sp, sp_ld = splits.get(x, (None, 0))
-            ga = torch.empty(B, n, device=dev)
-            gb = torch.empty(B, n, device=dev)
-            g_in = torch.empty(M, n, device=dev)
+            ga = torch.empty(B, n, dtype=torch.float32, device=dev)
+            gb = torch.empty(B, n, dtype=torch.float32, device=dev)
+            g_in = torch.empty(M, n, dtype=torch.float32, device=dev)
             with _timed("relu_grad", 0.0, 4.0 * (3 * M * n + 4 * B * n)):
                 _lib.call("bf_relu_grad", _lib.ptr(GA[x]), _lib.ptr(saved["relu_A"][op_index]), S * n, B, S, n,
                           _lib.ptr(pre.lower.reshape(B, n)), _lib.ptr(pre.upper.reshape(B, n)), _lib.ptr(a_t), a_ld,
@@ -814,13 +815,13 @@ def lower_grad_pass(module: BFTaskModule, spec: InputSpec, trace: DagTrace, save
                     if acc is None:
                         acc = GA[name]
                         continue
-                    out = torch.empty(M, n, device=dev)
+                    out = torch.empty(M, n, dtype=torch.float32, device=dev)
                     _lib.call("bf_rows_add", _lib.ptr(acc), _lib.ptr(GA[name]), M, n, S, None, None, 0, _lib.ptr(out),
                               stream)
                     acc = out
                 else:
                     c = params[name].to(device=dev, dtype=torch.float32).reshape(B, n).contiguous()
-                    out = torch.empty(M, n, device=dev)
+                    out = torch.empty(M, n, dtype=torch.float32, device=dev)
                     _lib.call("bf_rows_add", _lib.ptr(acc), None, M, n, S, _lib.ptr(G), _lib.ptr(c), n, _lib.ptr(out),
                               stream)
                     acc = out

@@ -320,8 +320,8 @@ class HipFusedCrownExecutor:
         ph, pw = _pair(request.attrs, "padding", (0, 0))
         kbias = None if bias is None else derived(
             f"conv_bias_map:{Ho}x{Wo}", (bias,), lambda: bias.reshape(Co, 1).expand(Co, Ho * Wo).reshape(-1).contiguous())
-        pu = torch.empty(D, S, Ci, Hi, Wi, device=dev)
-        pl = torch.empty(D, S, Ci, Hi, Wi, device=dev)
+        pu = torch.empty(D, S, Ci, Hi, Wi, dtype=torch.float32, device=dev)
+        pl = torch.empty(D, S, Ci, Hi, Wi, dtype=torch.float32, device=dev)
         flops = 4.0 * M * Co * Ho * Wo * Ci * KH * KW / (sh * sw)
         if _lib.load().bf_conv_transpose_hwc_supported(Co, Ho, Wo, Ci, KH, KW, sh, sw, ph, pw, Hi, Wi):
             wpk = packed_conv_transpose_weights(W, Co, Ho, Wo, Ci, KH, KW, sh, sw, ph, pw, Hi, Wi)
@@ -334,8 +334,8 @@ class HipFusedCrownExecutor:
         # other conv shapes: the relaxation pass (from the interleaved table), then the transposed convolution
         table = torch.empty(D * N * 4, device=dev, dtype=torch.float32)
         _lib.call("bf_relu_relax_table_from_planes", *[_lib.ptr(t) for t in planes], D * N, _lib.ptr(table), st)
-        ru = torch.empty(M, N, device=dev)
-        rl = torch.empty(M, N, device=dev)
+        ru = torch.empty(M, N, dtype=torch.float32, device=dev)
+        rl = torch.empty(M, N, dtype=torch.float32, device=dev)
         with _timed("executor_relu_relax", 0.0, 4.0 * (4 * M * N + 4 * D * N)):
             _lib.call("bf_crown_relu_relax", _lib.ptr(request.A_u), _lib.ptr(request.A_l), S * N, D, S, N,
                       _lib.ptr(table), None, 0, _lib.ptr(kbias), None, None, None, _lib.ptr(ru), _lib.ptr(rl),

@@ -160,7 +160,7 @@ def split_certificate(module, input_spec, relu_split_state: Dict[str, torch.Tens
         # several first layers: their halfspaces in op order, as one row set
         rows = torch.cat([r for _n, r, _b in sources], dim=0)
         if any(b is not None for _n, _r, b in sources):
-            bias = torch.cat([b if b is not None else torch.zeros(int(r.shape[0]), device=dev)
+            bias = torch.cat([b if b is not None else torch.zeros(int(r.shape[0]), dtype=torch.float32, device=dev)
                               for _n, r, b in sources])
         else:
             bias = None

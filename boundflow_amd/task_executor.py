@@ -120,7 +120,7 @@ class HipTaskExecutor:
         dev = center.device
         rows = w.to(torch.float32).contiguous()
         bias = None if b is None else b.to(device=dev, dtype=torch.float32).expand(B, O).contiguous()
-        lo = torch.empty(B, O, device=dev)
+        lo = torch.empty(B, O, dtype=torch.float32, device=dev)
         hi = torch.empty_like(lo)
         c = center.to(torch.float32).contiguous()
         stream = _lib.stream_handle()
@@ -136,9 +136,9 @@ class HipTaskExecutor:
         if int(w.shape[1]) != K:
             raise ValueError(f"linear shape mismatch: x={tuple(in_lo.shape)} weight={tuple(w.shape)}")
         dev = in_lo.device
-        lo = torch.empty(B, N, device=dev)
+        lo = torch.empty(B, N, dtype=torch.float32, device=dev)
         hi = torch.empty_like(lo)
-        ws = torch.empty(int(_lib.load().bf_ibp_linear_workspace(B, K, N)), device=dev)
+        ws = torch.empty(int(_lib.load().bf_ibp_linear_workspace(B, K, N)), dtype=torch.float32, device=dev)
         _lib.call("bf_ibp_linear", _lib.ptr(in_lo), _lib.ptr(in_hi), B, K, kind, eps, 0, _lib.ptr(w.contiguous()),
                   _lib.ptr(None if b is None else b.contiguous()), N, None, 0, _lib.ptr(ws), _lib.ptr(lo),
                   _lib.ptr(hi), None, None, None, _lib.stream_handle())
@@ -149,7 +149,7 @@ class HipTaskExecutor:
         B, O, I = (int(d) for d in w.shape)
         if tuple(iv.lower.shape) != (B, I):
             raise ValueError(f"batched linear shape mismatch: x={tuple(iv.lower.shape)} weight={tuple(w.shape)}")
-        lo = torch.empty(B, O, device=w.device)
+        lo = torch.empty(B, O, dtype=torch.float32, device=w.device)
         hi = torch.empty_like(lo)
         bb = None if b is None else b.expand(B, O).contiguous()
         _lib.call("bf_ibp_batched_linear", _lib.ptr(iv.lower.contiguous()), _lib.ptr(iv.upper.contiguous()), B, I,
@@ -180,9 +180,10 @@ class HipTaskExecutor:
         Ho = (Hi + 2 * ph - KH) // sh + 1
         Wo = (Wi + 2 * pw - KW) // sw + 1
         dev = iv.lower.device
-        lo = torch.empty(B, Co, Ho, Wo, device=dev)
+        lo = torch.empty(B, Co, Ho, Wo, dtype=torch.float32, device=dev)
         hi = torch.empty_like(lo)
-        ws = torch.empty(int(_lib.load().bf_ibp_conv2d_workspace(B, Ci * Hi * Wi, Co * Ho * Wo)), device=dev)
+        ws = torch.empty(int(_lib.load().bf_ibp_conv2d_workspace(B, Ci * Hi * Wi, Co * Ho * Wo)), dtype=torch.float32,
+                         device=dev)
         _lib.call("bf_ibp_conv2d", _lib.ptr(iv.lower.contiguous()), _lib.ptr(iv.upper.contiguous()), B, Ci, Hi, Wi, 0,
                   0.0, 0, _lib.ptr(w.contiguous()), _lib.ptr(None if b is None else b.contiguous()), Co, KH, KW, sh,
                   sw, ph, pw, Ho, Wo, None, 0, _lib.ptr(ws), _lib.ptr(lo), _lib.ptr(hi), None, None,
@@ -202,14 +203,14 @@ class HipTaskExecutor:
     def _elementwise(self, name: str, a: IntervalState, b: IntervalState, shape) -> IntervalState:
         al, au = a.lower.expand(shape).contiguous(), a.upper.expand(shape).contiguous()
         bl, bu = b.lower.expand(shape).contiguous(), b.upper.expand(shape).contiguous()
-        lo = torch.empty(shape, device=al.device)
+        lo = torch.empty(shape, dtype=torch.float32, device=al.device)
         hi = torch.empty_like(lo)
         _lib.call(name, _lib.ptr(al), _lib.ptr(au), _lib.ptr(bl), _lib.ptr(bu), lo.numel(), _lib.ptr(lo),
                   _lib.ptr(hi), _lib.stream_handle())
         return IntervalState(lo, hi)
 
     def _relu(self, iv: IntervalState) -> IntervalState:
-        lo = torch.empty(iv.lower.shape, device=iv.lower.device)
+        lo = torch.empty(iv.lower.shape, dtype=torch.float32, device=iv.lower.device)
         hi = torch.empty_like(lo)
         _lib.call("bf_interval_relu", _lib.ptr(iv.lower.contiguous()), _lib.ptr(iv.upper.contiguous()),
                   lo.numel(), _lib.ptr(lo), _lib.ptr(hi), _lib.stream_handle())
@@ -224,7 +225,7 @@ class HipTaskExecutor:
             if C.shape[0] != iv.lower.shape[0] or C.shape[2] != iv.lower.shape[1]:
                 raise ValueError(f"spec_linear shape mismatch: C={tuple(C.shape)} logits={tuple(iv.lower.shape)}")
         B, S, O = (int(d) for d in C.shape)
-        lo = torch.empty(B, S, device=C.device)
+        lo = torch.empty(B, S, dtype=torch.float32, device=C.device)
         hi = torch.empty_like(lo)
         _lib.call("bf_spec_linear", _lib.ptr(C.contiguous()), _lib.ptr(iv.lower.reshape(B, O).contiguous()),
                   _lib.ptr(iv.upper.reshape(B, O).contiguous()), B, S, O, _lib.ptr(lo), _lib.ptr(hi),
