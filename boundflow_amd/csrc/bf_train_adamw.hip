@@ -26,7 +26,10 @@
 
 #include "bf_train.h"
 
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 
 namespace bf {
 
@@ -207,6 +210,19 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamWTensors a, Ad
   }
 }
 
+// Whether no two of the arrays that a step writes share memory: two workgroups would step such elements at once, in
+// whatever order.  0.02 us of the host for eight arrays, 2.3 us for 305.
+struct Span {
+  uintptr_t from, to;
+};
+
+static bool apart(Span* spans, int count) {
+  std::sort(spans, spans + count, [](const Span& a, const Span& b) { return a.from < b.from; });
+  for (int k = 1; k < count; ++k)
+    if (spans[k].from < spans[k - 1].to) return false;
+  return true;
+}
+
 }  // namespace bf
 
 using namespace bf;
@@ -224,6 +240,33 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
   BF_REQUIRE((m_scale != nullptr) == (v_scale != nullptr), "bf_adamw_multi: one moment has scales, the other none");
   if (count == 0) return BF_OK;
   BF_REQUIRE(p && g && n && m && v, "bf_adamw_multi: null pointer");
+  // All checks come before the first launch: a call that is refused has stepped nothing.
+  constexpr int FEW = 256, OTHERS = 5;
+  Span few[FEW];
+  std::unique_ptr<Span[]> many;
+  if ((int64_t)count + OTHERS > FEW) {
+    many.reset(new (std::nothrow) Span[(size_t)count + OTHERS]);
+    BF_REQUIRE(many, "bf_adamw_multi: no host memory to check %d tensors", count);
+  }
+  Span* spans = many ? many.get() : few;
+  int written = 0;
+  int64_t total = 0;
+  const auto writes = [&](const void* array, int64_t bytes) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(array);
+    if (array && bytes) spans[written++] = Span{from, from + (uintptr_t)bytes};
+  };
+  for (int k = 0; k < count; ++k) {
+    BF_REQUIRE(n[k] >= 0 && (n[k] == 0 || (p[k] && g[k])), "bf_adamw_multi: tensor %d", k);
+    writes(p[k], n[k] * elem_bytes(p_elem));
+    total += ceil_div(n[k], ADAMW_BLOCK) * ADAMW_BLOCK;
+  }
+  writes(m, total * (m_scale ? 1 : 4));
+  writes(v, total * (m_scale ? 1 : 4));
+  writes(m_scale, total / ADAMW_BLOCK * 4);
+  writes(v_scale, total / ADAMW_BLOCK * 4);
+  writes(master, total * 4);
+  BF_REQUIRE(apart(spans, written),
+             "bf_adamw_multi: two of the weights, moments and copies share memory (tied weights are listed once)");
   // scalars in double, rounded once
   AdamWStep c;
   c.m = m;
@@ -248,7 +291,6 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
     memset(&a, 0, sizeof(a));
     int64_t blocks = 0;
     for (int k = base; k < count && k < base + ADAMW_MOST; ++k) {
-      BF_REQUIRE(n[k] >= 0 && (n[k] == 0 || (p[k] && g[k])), "bf_adamw_multi: tensor %d", k);
       if (n[k] == 0) continue;
       a.p[a.count] = p[k];
       a.g[a.count] = g[k];

@@ -348,7 +348,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     """One AdamW step (torch.optim.AdamW's formula) over all ``params``, in place.
 
     ``step`` counts from 1.  params of one type and grads of one type (each float32, bfloat16 or
-    float16), contiguous, pairwise of the same shape.  ``grad_scale`` multiplies every gradient: a
+    float16), contiguous, pairwise of the same shape; weights that share memory are refused (tied
+    ones are listed once, with their gradients' sum).  ``grad_scale`` multiplies every gradient: a
     number, or a float32 scalar tensor on the device (the factor of a clipped norm).  The step is
     computed in fp32 and each weight rounded once; with ``moments.master`` the copies are stepped
     and the weights follow them.  The parameters' versions are raised, so that bound queries remake

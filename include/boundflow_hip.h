@@ -658,6 +658,7 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
  * sqrt(v) as float8 e4m3 numbers to be multiplied by their scale (bf_train_adamw.hip says how they are
  * rounded), padding included, which has to be zero before the first step.  master (optional): fp32
  * copies of the weights in the same layout, which are stepped; the weights are then written only.
+ * No two of the arrays that are written may share memory (refused: two workgroups would step such elements at once).
  * The gradient is multiplied by grad_scale, and by *grad_scale_dev where that is given. */
 int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_t* n, int p_elem, int g_elem, void* m,
                    void* v, float* m_scale, float* v_scale, float* master, double lr, double beta1, double beta2,

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from boundflow_amd import training
+from boundflow_amd._lib import HipError
 from tests.gpu_util import device
 from tests.test_gpu_training import gen, policy_inputs, preference_inputs
 
@@ -46,3 +47,12 @@ def test_results_do_not_depend_on_the_default_type(default):
     finally:
         torch.set_default_dtype(before)
     assert all(a.dtype == b.dtype and torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+def test_adamw_refuses_tied_weights():
+    dev = device()
+    w = torch.ones(300, device=dev)
+    opt = training.AdamW([w, torch.ones(5, device=dev), w])
+    with pytest.raises(HipError, match="share memory"):
+        opt.step([torch.ones(300, device=dev), torch.ones(5, device=dev), torch.ones(300, device=dev)])
+    assert torch.equal(w, torch.ones(300, device=dev)) and not opt.moments.m.any() and opt.t == 0

@@ -1,0 +1,47 @@
+"""What the training operators' entry points refuse before anything is enqueued.  No device call is made."""
+
+import pytest
+import torch
+
+from boundflow_amd import _lib
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built (run python -m boundflow_amd.build)")
+    return _lib.load()
+
+
+def adamw(lib, params, grads, sizes, moments, **kw):
+    """Status of one step over host memory that must not be reached (the call has to be refused)."""
+    args = dict(count=len(sizes), p=_lib.ptr_array(params), g=_lib.ptr_array(grads), n=_lib.i64_array(sizes), p_elem=0,
+                g_elem=0, m=moments[0], v=moments[1], m_scale=None, v_scale=None, master=None, lr=0.1, b1=0.9, b2=0.9,
+                eps=1e-8, wd=0.0, step=1, scale=1.0, scale_dev=None, stream=None)
+    return lib.bf_adamw_multi(*{**args, **kw}.values())
+
+
+@pytest.mark.parametrize("count", [2, 7, 97, 300])
+def test_adamw_refuses_weights_that_share_memory(lib, count):
+    flat = torch.zeros(64 * count)
+    weights = list(flat.view(count, 64))
+    m, v = torch.zeros(128 * count), torch.zeros(128 * count)
+    at = [m.data_ptr(), v.data_ptr()]
+    sizes = [64] * count
+    tied = weights[:-1] + [weights[0]]
+    assert adamw(lib, tied, weights, sizes, at) == 1 and b"share memory" in lib.bf_last_error()
+    # the last of one is the first of another
+    across = weights[:-1] + [flat[63:127]]
+    assert adamw(lib, across, weights, sizes, at) == 1 and b"share memory" in lib.bf_last_error()
+    assert adamw(lib, weights, weights, sizes, [at[0], at[0]]) == 1 and b"share memory" in lib.bf_last_error()
+    assert adamw(lib, weights, weights, sizes, at, master=at[1]) == 1 and b"share memory" in lib.bf_last_error()
+    assert adamw(lib, weights, weights, sizes, [flat.data_ptr(), at[1]]) == 1 and b"share memory" in lib.bf_last_error()
+
+
+def test_adamw_refuses_a_late_tensor_before_it_steps_the_first(lib):
+    """More tensors than a launch takes: the 120th is looked at before the first launch."""
+    weights = list(torch.zeros(120, 64))
+    m, v = torch.zeros(120 * 128), torch.zeros(120 * 128)
+    at = [m.data_ptr(), v.data_ptr()]
+    assert adamw(lib, weights, weights, [64] * 119 + [-1], at) == 1 and b"tensor 119" in lib.bf_last_error()
+    assert adamw(lib, weights, weights[:119] + [None], [64] * 120, at) == 1 and b"tensor 119" in lib.bf_last_error()
