@@ -42,9 +42,10 @@ __device__ __forceinline__ void add_terms(float& M, float& s, const float (&z)[N
   for (int k = 0; k < N; ++k) s += term(z[k], c, m);
 }
 
-// the log-probability of a logit z
-__device__ __forceinline__ float log_prob(float z, float c, float M, float s) {
-  return ((z - M) * c - log2_fast(s)) * kLn2;
+// The log-probability of a logit z.  The difference is not taken through base 2, where that of a mask's value, the
+// type's lowest, would pass the largest fp32.
+__device__ __forceinline__ float log_prob(float z, float inv_t, float M, float s) {
+  return (z - M) * inv_t - log2_fast(s) * kLn2;
 }
 
 // Rows of logits: row n is logits + (n / T) ld_b + (n % T) ld_t.
@@ -462,7 +463,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
     buf ^= 1;
     // the same in every thread, and in scalar registers for the loop
     const float Mr = uniform(soft.x);
-    const float lp = here.t < V ? log_prob(zt, c, Mr, soft.y) : __int_as_float(0x7fc00000);
+    const float lp = here.t < V ? log_prob(zt, a.inv_t, Mr, soft.y) : __int_as_float(0x7fc00000);
     const PolicyRow r = policy_term(lp, here.old, here.ref, a.ref_logp != nullptr, here.A, a.low, a.high, a.kl_weight);
     const float w = 1.f / (here.w * count);
     policy += w * r.policy;
@@ -566,8 +567,8 @@ __device__ __forceinline__ float2 row_softmax(const float2* part, int64_t n, int
 // The log-probability of a live row's token; one past the vocabulary shows as NaN.
 template <class T>
 __device__ __forceinline__ float token_logp(const T* logits, const LogitRows& rows, int64_t n, int t, float2 soft,
-                                            float c) {
-  return (int64_t)t < rows.V ? log_prob((float)logits[rows.offset(n) + t], c, soft.x, soft.y)
+                                            float inv_t) {
+  return (int64_t)t < rows.V ? log_prob((float)logits[rows.offset(n) + t], inv_t, soft.x, soft.y)
                              : __int_as_float(0x7fc00000);
 }
 
@@ -617,7 +618,7 @@ __device__ __forceinline__ PolicyRow policy_part_row(const T* logits, const Logi
                                                      float2* soft) {
   const int64_t b = (unsigned)n / (unsigned)a.T;
   *soft = row_softmax<ONE>(part, n, parts, a.c);
-  *lp = token_logp(logits, rows, n, t, *soft, a.c);
+  *lp = token_logp(logits, rows, n, t, *soft, a.inv_t);
   return policy_term(*lp, a.old_logp[n], a.ref_logp ? a.ref_logp[n] : 0.f, a.ref_logp != nullptr,
                      a.advantages[b * a.adv_b + (n - b * a.T) * a.adv_t], a.low, a.high, a.kl_weight);
 }
@@ -719,7 +720,7 @@ __global__ __launch_bounds__(ALONE ? COUNT_THREADS : LOSS_THREADS) void policy_s
         s = row16_sum(s * term(M, c, m));
         M = m;
       }
-      lp = t < V ? log_prob(zt, c, M, s) : __int_as_float(0x7fc00000);
+      lp = t < V ? log_prob(zt, a.inv_t, M, s) : __int_as_float(0x7fc00000);
       const PolicyRow r = policy_term(lp, old, ref, a.ref_logp != nullptr, A, a.low, a.high, a.kl_weight);
       if (lane == 0) {
         policy += w * r.policy;
@@ -814,7 +815,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);   // s of the row in y, until the pair's g is known
       if (t >= 0) {
         const float2 soft = row_softmax<ONE>(part, n, parts, c);
-        lp = token_logp(logits, rows, n, t, soft, c);
+        lp = token_logp(logits, rows, n, t, soft, 1.f);
         if (lane == 0) s += lp - ref;
         f = make_float4(soft.x, soft.y, 1.f, 0.f);
       }

@@ -6,8 +6,9 @@ import torch
 
 from boundflow_amd import training
 from boundflow_amd._lib import HipError
+from oracle import training_ref as ref
 from tests.gpu_util import device
-from tests.test_gpu_training import gen, policy_inputs, preference_inputs
+from tests.test_gpu_training import check_policy, close, gen, logp_tol, policy_inputs, preference_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +57,29 @@ def test_adamw_refuses_tied_weights():
     with pytest.raises(HipError, match="share memory"):
         opt.step([torch.ones(300, device=dev), torch.ones(5, device=dev), torch.ones(300, device=dev)])
     assert torch.equal(w, torch.ones(300, device=dev)) and not opt.moments.m.any() and opt.t == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,rows", [(5, 6), (301, 6), (4099, 6), (2050, 300)])
+def test_losses_at_tokens_that_a_mask_took_out(dtype, V, rows):
+    """A token whose logit is a mask's value, the type's lowest: its log-probability is about that number, and where
+    the old and the reference policy say the same, the ratio is 1, the KL term 0 and the loss finite."""
+    dev = device()
+    s = policy_inputs(1, rows, V, dtype, 7, True, "none")
+    z, lowest = s["logits"].clone(), torch.finfo(dtype).min
+    picked = torch.arange(0, rows, 2)
+    z[0, picked, s["tokens"][0, picked]] = lowest
+    s["logits"] = z
+    lp = torch.log_softmax(z.double(), -1).gather(-1, s["tokens"][..., None])[..., 0]
+    s["old_logp"], s["ref_logp"] = lp.float(), lp.float()
+    got = check_policy(s, dev, what=f"tokens at the lowest value, {rows} x {V}")
+    assert torch.isfinite(got.logp).all() and torch.isfinite(got.stats).all()
+    q = dict(logits=z[0], tokens=s["tokens"][0], ref_logp=s["ref_logp"][0], offsets=torch.tensor([0, 2, rows]))
+    r = ref.preference_loss(**q)
+    got = training.preference_loss(**to(dev, q))
+    tol = logp_tol(z[0], V) + 2.0 ** -23 * r["logp"].abs()
+    close(got.logp, r["logp"], tol, "preference logp")
+    # rows at a mask's value differ from the reference's by what both are rounded by, 2^-24 of it each
+    moved = 0.1 * tol.sum()
+    close(got.rewards, r["rewards"], moved.expand(2), "preference rewards")
+    assert torch.isfinite(got.loss)
