@@ -831,7 +831,10 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(
   if (threadIdx.x == 0) {
     rewards[pair] = a.beta * sum[0];
     rewards[pair + a.pairs] = a.beta * sum[1];
-    losses[pair] = -((1.f - a.smoothing) * log_sigmoid(h) + a.smoothing * log_sigmoid(-h));
+    // A term of weight 0 is not there: a response at -inf makes h infinite, and 0 * inf would be NaN.
+    const float good = a.smoothing < 1.f ? (1.f - a.smoothing) * log_sigmoid(h) : 0.f;
+    const float bad = a.smoothing > 0.f ? a.smoothing * log_sigmoid(-h) : 0.f;
+    losses[pair] = -(good + bad);
   }
   const float g = dh * a.beta * a.grad_scale / (float)a.pairs;
   if (lane) return;

@@ -1,6 +1,8 @@
 """Edges of the training operators' calls: other default types, numbers at the ends of their range, layouts,
 limits.  Tolerances as in test_gpu_training.py."""
 
+import math
+
 import pytest
 import torch
 
@@ -83,3 +85,27 @@ def test_losses_at_tokens_that_a_mask_took_out(dtype, V, rows):
     moved = 0.1 * tol.sum()
     close(got.rewards, r["rewards"], moved.expand(2), "preference rewards")
     assert torch.isfinite(got.loss)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("smoothing,out", [(0.0, 1), (1.0, 0), (0.1, 1)])
+def test_preference_loss_of_a_response_that_cannot_be(dtype, smoothing, out):
+    """A token at -inf: its response has reward -inf.  Rejected (out = 1), h = inf and -log sigma(h) = 0; the term whose
+    weight is 0 is not there, so the batch's loss is that of the other pair.  With both weights the loss is infinite."""
+    dev = device()
+    s = preference_inputs([3, 2, 2, 4], 40, dtype, 6)
+    want = ref.preference_loss(**s, label_smoothing=smoothing)
+    h = float(want["rewards"][0] - want["rewards"][2])
+    other = math.log1p(math.exp(-h)) if smoothing == 0.0 else math.log1p(math.exp(h))
+    row = {1: 8, 0: 3}[out]     # in the second pair: of its rejected response, or of its chosen one
+    s["logits"][row, s["tokens"][row]] = float("-inf")
+    got = training.preference_loss(**to(dev, s), label_smoothing=smoothing)
+    assert float(got.rewards[1 + 2 * out]) == float("-inf")
+    if smoothing in (0.0, 1.0):
+        # the pair's loss is 0 and so is its gradient
+        assert abs(float(got.loss) - other / 2) < 2.0 ** -18 * (abs(h) + 1)
+        assert not got.grad_logits[[3, 4, 7, 8, 9, 10]].any() and torch.isfinite(got.grad_logits).all()
+    else:
+        assert float(got.loss) == float("inf")
+        # d loss / d h of the second pair is -(0.9 * 0 - 0.1 * 1) = 0.1 for the rejected response at -inf
+        assert got.grad_logits[[3, 4]].any()
