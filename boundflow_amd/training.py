@@ -90,9 +90,14 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.
     """``scale * table[tokens]`` ([*tokens.shape, dim], of the table's type, rounded once).
 
     table [vocab, dim], rows contiguous (any row stride); tokens int32 or int64 of any shape.  A
-    negative token is padding and gives zeros, one past the table gives NaN."""
+    negative token is padding and gives zeros, one past the table gives NaN.  The rows come without a
+    graph: a table that requires grad is refused while gradients are recorded (pass ``table.detach()``),
+    because a ``backward()`` through the network would leave it untrained without an error."""
     dev = _current_device(table, "table")
     elem = _elem(table, "table")
+    if table.requires_grad and torch.is_grad_enabled():
+        raise HipError("table requires grad, but the rows come without a graph: pass table.detach() and get its "
+                       "gradient from embed_tokens_grad")
     if table.dim() != 2:
         raise HipError(f"table must be [vocab, dim], got {tuple(table.shape)}")
     vocab, dim = table.shape

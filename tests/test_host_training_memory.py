@@ -55,3 +55,14 @@ def test_buffers_are_fp32_whatever_the_default_type(recorded, default_type):
     assert [name for name, _ in calls] == ["bf_embed_grad"] * 2 + ["bf_policy_loss", "bf_preference_loss"] + \
         ["bf_adamw_multi"] * 2
     assert made and all(t.dtype in (torch.float32, torch.uint8) for t in made), [t.dtype for t in made]
+
+
+def test_a_table_that_requires_grad_is_refused_where_its_gradient_would_be_lost(recorded):
+    _made, calls = recorded
+    table, tokens = fp32(4, 6).requires_grad_(True), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(_lib.HipError, match="table.detach()"):
+        training.embed_tokens(table, tokens)
+    assert not calls
+    assert training.embed_tokens(table.detach(), tokens).shape == (3, 6)
+    with torch.no_grad():
+        assert training.embed_tokens(table, tokens).shape == (3, 6)
