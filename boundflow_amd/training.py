@@ -102,6 +102,8 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.
         raise HipError(f"table must be [vocab, dim], got {tuple(table.shape)}")
     vocab, dim = table.shape
     ld, step = table.stride()
+    if vocab <= 1:
+        ld = dim      # a single row's stride leads nowhere, and may be anything
     if (step != 1 and dim > 1) or ld < dim:
         raise HipError(f"table must be [vocab, dim] with contiguous rows, got {tuple(table.shape)} with strides "
                        f"{table.stride()}")

@@ -109,3 +109,12 @@ def test_preference_loss_of_a_response_that_cannot_be(dtype, smoothing, out):
         assert float(got.loss) == float("inf")
         # d loss / d h of the second pair is -(0.9 * 0 - 0.1 * 1) = 0.1 for the rejected response at -inf
         assert got.grad_logits[[3, 4]].any()
+
+
+def test_embed_tokens_from_a_table_of_one_row():
+    dev = device()
+    table = torch.randn(6, 1, generator=gen(1)).to(dev).t()
+    tokens = torch.tensor([0, -1, 0, 1], device=dev)
+    got = training.embed_tokens(table, tokens)
+    assert torch.equal(got[0], table[0]) and torch.equal(got[2], table[0])
+    assert not got[1].any() and torch.isnan(got[3]).all()

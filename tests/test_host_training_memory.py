@@ -66,3 +66,12 @@ def test_a_table_that_requires_grad_is_refused_where_its_gradient_would_be_lost(
     assert training.embed_tokens(table.detach(), tokens).shape == (3, 6)
     with torch.no_grad():
         assert training.embed_tokens(table, tokens).shape == (3, 6)
+
+
+def test_a_table_of_one_row_may_have_any_stride(recorded):
+    """[1, dim] as a transposed column has row stride 1: the stride of a single row leads nowhere."""
+    _made, calls = recorded
+    table = fp32(6, 1).t()
+    assert table.stride() == (1, 1)
+    assert training.embed_tokens(table, torch.zeros(3, dtype=torch.int64)).shape == (3, 6)
+    assert calls[0][1][1] >= 6, "the library takes no stride below the width"
