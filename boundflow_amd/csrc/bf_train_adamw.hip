@@ -251,12 +251,17 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
   Span* spans = many ? many.get() : few;
   int written = 0;
   int64_t total = 0;
+  const int chunk = adamw_chunk(m_scale != nullptr);
   const auto writes = [&](const void* array, int64_t bytes) {
     const uintptr_t from = reinterpret_cast<uintptr_t>(array);
     if (array && bytes) spans[written++] = Span{from, from + (uintptr_t)bytes};
   };
   for (int k = 0; k < count; ++k) {
     BF_REQUIRE(n[k] >= 0 && (n[k] == 0 || (p[k] && g[k])), "bf_adamw_multi: tensor %d", k);
+    if (!launch_fits(ceil_div(n[k], chunk), ADAMW_THREADS)) {
+      set_error("bf_adamw_multi: tensor %d of %lld elements is more than a launch takes", k, (long long)n[k]);
+      return BF_ERANGE;
+    }
     writes(p[k], n[k] * elem_bytes(p_elem));
     total += ceil_div(n[k], ADAMW_BLOCK) * ADAMW_BLOCK;
   }
@@ -286,24 +291,22 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
   c.inv_root_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   c.phase = (uint32_t)(uint64_t)step * 0x9E3779B9u;
   int64_t at = 0;
-  for (int base = 0; base < count; base += ADAMW_MOST) {
+  for (int k = 0; k < count;) {
     AdamWTensors a;
     memset(&a, 0, sizeof(a));
     int64_t blocks = 0;
-    for (int k = base; k < count && k < base + ADAMW_MOST; ++k) {
+    for (; k < count && a.count < ADAMW_MOST; ++k) {
       if (n[k] == 0) continue;
+      const int64_t more = ceil_div(n[k], chunk);
+      if (!launch_fits(blocks + more, ADAMW_THREADS)) break;   // a launch takes any one tensor
       a.p[a.count] = p[k];
       a.g[a.count] = g[k];
       a.n[a.count] = n[k];
       a.at[a.count] = at;
       a.first[a.count] = (int)blocks;
       at += ceil_div(n[k], ADAMW_BLOCK) * ADAMW_BLOCK;
-      blocks += ceil_div(n[k], adamw_chunk(m_scale != nullptr));
+      blocks += more;
       ++a.count;
-      if (blocks >= (1LL << 31)) {
-        set_error("bf_adamw_multi: tensor %d brings a launch to 2^31 workgroups or more", k);
-        return BF_ERANGE;
-      }
     }
     if (blocks == 0) continue;
     a.first[a.count] = (int)blocks;

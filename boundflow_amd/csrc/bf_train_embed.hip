@@ -461,19 +461,23 @@ int bf_embed_rows(const void* table, int64_t table_ld, int64_t vocab, const void
   BF_REQUIRE(vocab >= 0 && count >= 0 && dim >= 0 && table_ld >= dim, "bf_embed_rows: bad sizes");
   if (count == 0 || dim == 0) return BF_OK;
   BF_REQUIRE((table || vocab == 0) && tokens && out, "bf_embed_rows: null pointer");
-  const bool wide = vocab >= (1LL << 31) || dim >= (1LL << 30) || count >= (1LL << 32);
-  const int64_t chunks = ceil_div(dim, 16 / elem_bytes(elem)), blocks = wide ? 0 : ceil_div(count * chunks, 256);
-  if (wide || blocks >= (1LL << 31)) {
+  if (vocab >= (1LL << 31) || dim >= (1LL << 30) || count >= (1LL << 32)) {
     set_error("bf_embed_rows: %lld tokens of %lld columns from %lld rows are too many", (long long)count,
               (long long)dim, (long long)vocab);
     return BF_ERANGE;
   }
   return with_elem(elem, [&](auto t) -> int {
     using T = decltype(t);
-    hipLaunchKernelGGL(embed_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, stream,
-                       static_cast<const T*>(table), table_ld, (int)vocab, tokens, token_bytes, count, (int)dim,
-                       (int)chunks, scale, static_cast<T*>(out));
-    BF_LAUNCH_CHECK("embed_rows_kernel");
+    // 64 GiB of rows are a launch each
+    const int64_t chunks = ceil_div(dim, 16 / (int64_t)sizeof(T)), most = ((1LL << 32) - 256) / chunks;
+    for (int64_t i = 0; i < count; i += most) {
+      const int64_t here = count - i < most ? count - i : most;
+      hipLaunchKernelGGL(embed_rows_kernel<T>, dim3((unsigned)ceil_div(here * chunks, 256)), dim3(256), 0, stream,
+                         static_cast<const T*>(table), table_ld, (int)vocab,
+                         static_cast<const char*>(tokens) + i * token_bytes, token_bytes, here, (int)dim, (int)chunks,
+                         scale, static_cast<T*>(out) + i * dim);
+      BF_LAUNCH_CHECK("embed_rows_kernel");
+    }
     return BF_OK;
   });
 }
@@ -495,11 +499,12 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
   BF_REQUIRE((count == 0 || (grad && tokens)) && out && (workspace || count <= FEW_TOKENS),
              "bf_embed_grad: null pointer");
   const int64_t pieces = ceil_div(count, PIECE), columns = ceil_div(dim, JOIN_COLUMNS);
-  if (vocab >= (1LL << 30) || count >= (1LL << 30) || dim >= (1LL << 30) || pieces * columns >= (1LL << 31)) {
+  const auto too_many = [&] {
     set_error("bf_embed_grad: %lld tokens, %lld values or %lld columns are too many", (long long)count,
               (long long)vocab, (long long)dim);
     return BF_ERANGE;
-  }
+  };
+  if (vocab >= (1LL << 30) || count >= (1LL << 30) || dim >= (1LL << 30)) return too_many();
   return with_elem(elem, [&](auto ti) -> int {
     using TI = decltype(ti);
     constexpr int VEC = 16 / sizeof(TI);
@@ -520,9 +525,11 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
         // columns 124 us against 135
         const int64_t most = !accumulate && slices > 1 ? FEW_RANGE / 2 : FEW_RANGE;
         const int range = (int)(r < most ? r : most);
-        hipLaunchKernelGGL((embed_few_kernel<TI, TO, VEC>), dim3((unsigned)(ceil_div(vocab, range) * slices)),
-                           dim3(FEW_WAVES * 64), 0, stream, g, grad_ld, tokens, token_bytes, (int)count, (int)vocab,
-                           (int)dim, range, (int)width, (int)slices, scale, accumulate, o);
+        const int64_t few = ceil_div(vocab, range) * slices;
+        if (!launch_fits(few, FEW_WAVES * 64)) return too_many();
+        hipLaunchKernelGGL((embed_few_kernel<TI, TO, VEC>), dim3((unsigned)few), dim3(FEW_WAVES * 64), 0, stream, g,
+                           grad_ld, tokens, token_bytes, (int)count, (int)vocab, (int)dim, range, (int)width,
+                           (int)slices, scale, accumulate, o);
         BF_LAUNCH_CHECK("embed_few_kernel");
         return BF_OK;
       }
@@ -538,24 +545,23 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
       const bool clear = !accumulate && count <= vocab;
       const int64_t groups = ceil_div(vocab, range), bytes = clear ? vocab * dim * (int64_t)sizeof(TO) : 0;
       const int64_t fills = ceil_div(bytes, FILL_BYTES);
-      if (groups + fills >= (1LL << 31)) {
-        set_error("bf_embed_grad: %lld rows of %lld columns are too many", (long long)vocab, (long long)dim);
-        return BF_ERANGE;
-      }
+      const int64_t piece_groups = ceil_div(pieces, SUM_WAVES);
+      // narrow rows: fewer values one after another; wide ones have workgroups enough
+      const int each_pieces = columns == 1 ? 2 : 8;
+      const int64_t sums = piece_groups + ceil_div(vocab, ROWS), joins = ceil_div(pieces, each_pieces) * columns;
+      if (!launch_fits(groups + fills, SORT_WAVES * 64) || !launch_fits(sums, SUM_THREADS) ||
+          !launch_fits(joins, JOIN_THREADS))
+        return too_many();
       hipLaunchKernelGGL(embed_sort_kernel, dim3((unsigned)(groups + fills)), dim3(SORT_WAVES * 64), 0, stream, tokens,
                          token_bytes, (int)count, (int)vocab, range, (int)groups, start, order, static_cast<char*>(out),
                          bytes);
       BF_LAUNCH_CHECK("embed_sort_kernel");
-      const int64_t piece_groups = ceil_div(pieces, SUM_WAVES);
-      hipLaunchKernelGGL((embed_sum_kernel<TI, TO, VEC>), dim3((unsigned)(piece_groups + ceil_div(vocab, ROWS))),
-                         dim3(SUM_THREADS), 0, stream, g, grad_ld, tokens, token_bytes, start, order, (int)vocab, (int)dim,
-                         (int)pieces, (int)piece_groups, scale, accumulate, accumulate || clear, o, owner, part);
+      hipLaunchKernelGGL((embed_sum_kernel<TI, TO, VEC>), dim3((unsigned)sums), dim3(SUM_THREADS), 0, stream, g,
+                         grad_ld, tokens, token_bytes, start, order, (int)vocab, (int)dim, (int)pieces,
+                         (int)piece_groups, scale, accumulate, accumulate || clear, o, owner, part);
       BF_LAUNCH_CHECK("embed_sum_kernel");
-      // narrow rows: fewer values one after another; wide ones have workgroups enough
-      const int each_pieces = columns == 1 ? 2 : 8;
-      hipLaunchKernelGGL((embed_join_kernel<TO>), dim3((unsigned)(ceil_div(pieces, each_pieces) * columns)),
-                         dim3(JOIN_THREADS), 0, stream, tokens, token_bytes, start, order, (int)dim,
-                         (int)pieces, each_pieces, (int)columns, scale, accumulate, owner, o, part);
+      hipLaunchKernelGGL((embed_join_kernel<TO>), dim3((unsigned)joins), dim3(JOIN_THREADS), 0, stream, tokens,
+                         token_bytes, start, order, (int)dim, (int)pieces, each_pieces, (int)columns, scale, accumulate, owner, o, part);
       BF_LAUNCH_CHECK("embed_join_kernel");
       return BF_OK;
     };

@@ -780,18 +780,18 @@ __device__ __forceinline__ int2 response_rows(const PreferenceArgs& a, int64_t k
 constexpr int WAVE_VECTORS = 4;
 
 constexpr int PAIR_THREADS = 1024, PAIR_WAVES = PAIR_THREADS / 64;
+constexpr int64_t PAIR_GROUPS = 1 << 21;   // workgroups of a launch, one more beside them
 
-// One workgroup per pair: the rows' log-probabilities, the responses' sums, the pair's loss, and the rows' gradient
-// coefficients; one more clears the rows of no response.
+// One workgroup per pair (of more than PAIR_GROUPS pairs, several one after another): the rows' log-probabilities,
+// the responses' sums, the pair's loss, and the rows' gradient coefficients; one more clears the rows of no response.
 template <bool ONE, class T>
 __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(
     const T* __restrict__ logits, LogitRows rows, PreferenceArgs a, const float2* __restrict__ part, int parts, float c,
     float* __restrict__ logp, float4* __restrict__ coef, float* __restrict__ rewards, float* __restrict__ losses) {
   constexpr int LANES = ONE ? 1 : 16, ROWS = PAIR_THREADS / LANES;
   __shared__ float red[PAIR_WAVES];
-  const int64_t pair = blockIdx.x;
-  const int lane = threadIdx.x % LANES;
-  if (pair == a.pairs) {
+  const int lane = threadIdx.x % LANES, groups = (int)gridDim.x - 1;
+  if ((int)blockIdx.x == groups) {
     const int from = a.pairs ? response_rows(a, 0).x : (int)a.N;
     const int to = a.pairs ? response_rows(a, 2 * a.pairs - 1).y : (int)a.N;
     const int outside = from + (int)a.N - to;
@@ -802,48 +802,50 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(
     }
     return;
   }
-  float sum[2];
-  int2 of[2];
+  for (int64_t pair = blockIdx.x; pair < a.pairs; pair += groups) {
+    float sum[2];
+    int2 of[2];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    of[side] = response_rows(a, pair + side * a.pairs);
-    float s = 0.f;
-    for (int n = of[side].x + threadIdx.x / LANES; n < of[side].y; n += ROWS) {
-      const int t = load_token(a.tokens, a.token_bytes, n);
-      const float ref = a.ref_logp[n];
-      float lp = 0.f;
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);   // s of the row in y, until the pair's g is known
-      if (t >= 0) {
-        const float2 soft = row_softmax<ONE>(part, n, parts, c);
-        lp = token_logp(logits, rows, n, t, soft, 1.f);
-        if (lane == 0) s += lp - ref;
-        f = make_float4(soft.x, soft.y, 1.f, 0.f);
+    for (int side = 0; side < 2; ++side) {
+      of[side] = response_rows(a, pair + side * a.pairs);
+      float s = 0.f;
+      for (int n = of[side].x + threadIdx.x / LANES; n < of[side].y; n += ROWS) {
+        const int t = load_token(a.tokens, a.token_bytes, n);
+        const float ref = a.ref_logp[n];
+        float lp = 0.f;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);   // s of the row in y, until the pair's g is known
+        if (t >= 0) {
+          const float2 soft = row_softmax<ONE>(part, n, parts, c);
+          lp = token_logp(logits, rows, n, t, soft, 1.f);
+          if (lane == 0) s += lp - ref;
+          f = make_float4(soft.x, soft.y, 1.f, 0.f);
+        }
+        if (lane == 0) {
+          logp[n] = lp;
+          coef[n] = f;
+        }
       }
-      if (lane == 0) {
-        logp[n] = lp;
-        coef[n] = f;
-      }
+      sum[side] = block_sum<PAIR_WAVES>(s, red);
     }
-    sum[side] = block_sum<PAIR_WAVES>(s, red);
-  }
-  const float h = a.beta * sum[0] - a.beta * sum[1];
-  const float dh = -((1.f - a.smoothing) * sigmoid(-h) - a.smoothing * sigmoid(h));
-  if (threadIdx.x == 0) {
-    rewards[pair] = a.beta * sum[0];
-    rewards[pair + a.pairs] = a.beta * sum[1];
-    // A term of weight 0 is not there: a response at -inf makes h infinite, and 0 * inf would be NaN.
-    const float good = a.smoothing < 1.f ? (1.f - a.smoothing) * log_sigmoid(h) : 0.f;
-    const float bad = a.smoothing > 0.f ? a.smoothing * log_sigmoid(-h) : 0.f;
-    losses[pair] = -(good + bad);
-  }
-  const float g = dh * a.beta * a.grad_scale / (float)a.pairs;
-  if (lane) return;
+    const float h = a.beta * sum[0] - a.beta * sum[1];
+    const float dh = -((1.f - a.smoothing) * sigmoid(-h) - a.smoothing * sigmoid(h));
+    if (threadIdx.x == 0) {
+      rewards[pair] = a.beta * sum[0];
+      rewards[pair + a.pairs] = a.beta * sum[1];
+      // A term of weight 0 is not there: a response at -inf makes h infinite, and 0 * inf would be NaN.
+      const float good = a.smoothing < 1.f ? (1.f - a.smoothing) * log_sigmoid(h) : 0.f;
+      const float bad = a.smoothing > 0.f ? a.smoothing * log_sigmoid(-h) : 0.f;
+      losses[pair] = -(good + bad);
+    }
+    const float g = dh * a.beta * a.grad_scale / (float)a.pairs;
+    if (lane == 0)
 #pragma unroll
-  for (int side = 0; side < 2; ++side)
-    for (int n = of[side].x + threadIdx.x / LANES; n < of[side].y; n += ROWS) {
-      const float4 f = coef[n];   // written by this thread above
-      if (f.z != 0.f) coef[n] = row_gradient(make_float2(f.x, f.y), side ? -g : g);
-    }
+      for (int side = 0; side < 2; ++side)
+        for (int n = of[side].x + threadIdx.x / LANES; n < of[side].y; n += ROWS) {
+          const float4 f = coef[n];   // written by this thread above
+          if (f.z != 0.f) coef[n] = row_gradient(make_float2(f.x, f.y), side ? -g : g);
+        }
+  }
 }
 
 // Workgroup = (row, part): its gradient from the row's coefficients; the last one sums the pairs' losses.
@@ -918,7 +920,8 @@ static int with_row_group(int64_t vecs, F f) {
 // Workgroups whose sums are kept.
 constexpr int64_t SUM_GROUPS = 4096;
 
-static bool rows_fit(int64_t N, int64_t V) { return V < (1LL << 30) && N < (1LL << 24); }
+// The longest launches have a workgroup a row and one more (rows in parts are few); counts of rows stay exact in fp32.
+static bool rows_fit(int64_t N, int64_t V) { return V < (1LL << 30) && launch_fits(N + 1, LOSS_THREADS); }
 
 }  // namespace bf
 
@@ -945,7 +948,7 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
              temperature, clip_low, clip_high);
   BF_REQUIRE(stats && workspace, "bf_policy_loss: null pointer");
   if (B >= (1LL << 24) || T >= (1LL << 24) || !rows_fit(B * T, V)) {
-    set_error("bf_policy_loss: %lld x %lld rows of %lld logits: rows below 2^24, logits below 2^30", (long long)B,
+    set_error("bf_policy_loss: %lld x %lld rows of %lld logits: rows below 2^24 - 1, logits below 2^30", (long long)B,
               (long long)T, (long long)V);
     return BF_ERANGE;
   }
@@ -1021,10 +1024,6 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
       BF_LAUNCH_CHECK("policy_stats_kernel");
       return BF_OK;
     }
-    if ((N + 1) * p.count >= (1LL << 31)) {
-      set_error("bf_policy_loss: %lld rows of %lld logits are too many", (long long)N, (long long)V);
-      return BF_ERANGE;
-    }
     hipLaunchKernelGGL((loss_partial_kernel<E, LOSS_THREADS>), dim3((unsigned)(N * p.count + 1)), dim3(LOSS_THREADS), 0,
                        stream, x, rows, a, N, p.count, p.chunk, part, counts);
     BF_LAUNCH_CHECK("loss_partial_kernel");
@@ -1056,12 +1055,12 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
   BF_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, "bf_preference_loss: label smoothing %g", smoothing);
   BF_REQUIRE(loss && (pairs == 0 || (offsets && rewards && workspace)), "bf_preference_loss: null pointer");
   BF_REQUIRE(N == 0 || (logits && tokens && ref_logp && logp && workspace), "bf_preference_loss: null pointer");
-  const Parts p = row_parts(N, V, elem);
-  if (!rows_fit(N, V) || pairs >= (1LL << 24) || (N + 1) * p.count >= (1LL << 31)) {
-    set_error("bf_preference_loss: %lld rows of %lld logits, %lld pairs: rows and pairs below 2^24, logits below 2^30",
-              (long long)N, (long long)V, (long long)pairs);
+  if (!rows_fit(N, V) || pairs >= (1LL << 24)) {
+    set_error("bf_preference_loss: %lld rows of %lld logits, %lld pairs: rows below 2^24 - 1, pairs below 2^24, logits "
+              "below 2^30", (long long)N, (long long)V, (long long)pairs);
     return BF_ERANGE;
   }
+  const Parts p = row_parts(N, V, elem);
   const PreferenceArgs a{tokens, ref_logp, offsets, N, pairs, beta, smoothing, grad_scale, token_bytes};
   const LogitRows rows{N > 0 ? N : 1, 0, ld, V};
   const float c = 1.4426950408889634f;
@@ -1085,11 +1084,12 @@ int bf_preference_loss(const void* logits, int elem, int64_t N, int64_t V, int64
       else launch(loss_partial_kernel<E, LOSS_THREADS>, LOSS_THREADS);
       BF_LAUNCH_CHECK("loss_partial_kernel");
     }
+    const unsigned pair_grid = (unsigned)(pairs < PAIR_GROUPS ? pairs : PAIR_GROUPS) + 1;
     if (p.count == 1)
-      hipLaunchKernelGGL((preference_pairs_kernel<true, E>), dim3((unsigned)pairs + 1), dim3(PAIR_THREADS), 0, stream, x,
+      hipLaunchKernelGGL((preference_pairs_kernel<true, E>), dim3(pair_grid), dim3(PAIR_THREADS), 0, stream, x,
                          rows, a, part, p.count, c, logp, coef, rewards, losses);
     else
-      hipLaunchKernelGGL((preference_pairs_kernel<false, E>), dim3((unsigned)pairs + 1), dim3(PAIR_THREADS), 0, stream, x,
+      hipLaunchKernelGGL((preference_pairs_kernel<false, E>), dim3(pair_grid), dim3(PAIR_THREADS), 0, stream, x,
                          rows, a, part, p.count, c, logp, coef, rewards, losses);
     BF_LAUNCH_CHECK("preference_pairs_kernel");
     const unsigned grid = grad ? (unsigned)(N * p.count + 1) : 1u;

@@ -9,7 +9,7 @@ import torch
 from boundflow_amd import training
 from boundflow_amd._lib import HipError
 from oracle import training_ref as ref
-from tests.gpu_util import device
+from tests.gpu_util import announce, device
 from tests.test_gpu_training import check_policy, close, gen, logp_tol, policy_inputs, preference_inputs
 
 pytestmark = pytest.mark.gpu
@@ -118,3 +118,44 @@ def test_embed_tokens_from_a_table_of_one_row():
     got = training.embed_tokens(table, tokens)
     assert torch.equal(got[0], table[0]) and torch.equal(got[2], table[0])
     assert not got[1].any() and torch.isnan(got[3]).all()
+
+
+def test_embed_tokens_of_more_rows_than_a_launch_takes():
+    """2^23 + 11 rows of 4096 bf16 columns, 64 GiB: 2^32 vectors of 16 bytes and some."""
+    dev = device()
+    count, dim = (1 << 23) + 11, 4096
+    announce("embedding of 64 GiB")
+    table = torch.randn(50, dim, generator=gen(1)).bfloat16().to(dev)
+    tokens = torch.randint(0, 50, (count,), generator=gen(2)).to(dev)
+    got = training.embed_tokens(table, tokens)
+    for rows in (slice(0, 300), slice(count // 2, count // 2 + 300), slice(count - 300, count)):
+        assert torch.equal(got[rows], table[tokens[rows]])
+    # every row's first and last element
+    for d in (0, dim - 1):
+        assert torch.equal(got[:, d], table[tokens, d])
+
+
+def test_preference_loss_of_more_pairs_than_a_launch_has_workgroups():
+    """Answers of one token, 2^22 + 3 pairs: a workgroup takes several."""
+    dev = device()
+    pairs, V = (1 << 22) + 3, 3
+    N = 2 * pairs
+    announce(f"{pairs} pairs")
+    z = torch.randn(N, V, generator=gen(3))
+    tokens = torch.randint(0, V, (N,), generator=gen(4))
+    ref_logp = -torch.rand(N, generator=gen(5))
+    got = training.preference_loss(z.to(dev), tokens.to(dev), ref_logp.to(dev), torch.arange(N + 1, device=dev), beta=0.5,
+                                   grad_scale=float(pairs))
+    logsm = torch.log_softmax(z.double(), -1)
+    logp = logsm.gather(-1, tokens[:, None])[:, 0]
+    rewards = 0.5 * (logp - ref_logp.double())
+    h = rewards[:pairs] - rewards[pairs:]
+    tol = logp_tol(z, V)
+    close(got.logp, logp, tol + 2.0 ** -24 * logp.abs(), "logp")
+    close(got.rewards, rewards, 0.5 * tol + 2.0 ** -22 * rewards.abs(), "rewards")
+    # 1024 threads sum some 4096 terms each, and then one another's: 4106 roundings at most
+    loss = torch.nn.functional.softplus(-h).mean()
+    close(got.loss, loss, 4200 * 2.0 ** -24 * float(loss) + float(tol.max()), "loss")
+    g = -torch.sigmoid(-h) * 0.5
+    want = torch.cat([g, -g])[:, None] * (torch.nn.functional.one_hot(tokens, V) - logsm.exp())
+    close(got.grad_logits, want, 2.0 ** -20 + 2.0 ** -20 * want.abs(), "gradient")

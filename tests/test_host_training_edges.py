@@ -45,3 +45,21 @@ def test_adamw_refuses_a_late_tensor_before_it_steps_the_first(lib):
     at = [m.data_ptr(), v.data_ptr()]
     assert adamw(lib, weights, weights, [64] * 119 + [-1], at) == 1 and b"tensor 119" in lib.bf_last_error()
     assert adamw(lib, weights, weights[:119] + [None], [64] * 120, at) == 1 and b"tensor 119" in lib.bf_last_error()
+
+
+def test_sizes_that_no_launch_takes_are_refused_before_the_first(lib):
+    """A grid of 2^32 work-items or more is status 3 up front, not a launch that fails behind others."""
+    some = torch.zeros(64)
+    p = some.data_ptr()
+    assert lib.bf_embed_grad(p, 1, 0, p, 8, 3000, 1 << 26, 1, 1.0, 0, 0, p, p, None) == 3   # two values a workgroup
+    assert lib.bf_embed_grad(p, 1, 0, p, 8, 5, (1 << 30) - 1, 1, 1.0, 0, 0, p, p, None) == 3
+    assert lib.bf_embed_grad(p, 8, 0, p, 8, 1 << 29, 9, 8, 1.0, 0, 0, p, p, None) == 3      # the pieces' sums joined
+    rows = (1 << 24) - 1
+    assert lib.bf_policy_loss(p, 0, 1, rows, 700, 0, 700, p, 8, p, None, p, 0, 0, None, 0.2, 0.2, 0.0, 1.0, 0, 1.0, p, p,
+                              p, p, None) == 3
+    assert lib.bf_preference_loss(p, 0, rows, 700, 700, p, 8, p, p, 1, 0.1, 0.0, 1.0, p, p, p, p, p, None) == 3
+    assert lib.bf_preference_loss(p, 0, 5, 700, 700, p, 8, p, p, 1 << 24, 0.1, 0.0, 1.0, p, p, p, p, p, None) == 3
+    assert lib.bf_policy_loss_workspace(1, rows, 700, 0) == 0 and lib.bf_preference_loss_workspace(rows, 700, 1, 0) == 0
+    weights, at = list(torch.zeros(120, 64)), [1 << 60, 2 << 60]
+    assert adamw(lib, weights, weights, [64] * 119 + [1 << 34], at) == 3   # in the second launch
+    assert adamw(lib, weights, weights, [64] * 119 + [1 << 35], at, m_scale=p, v_scale=p) == 3
