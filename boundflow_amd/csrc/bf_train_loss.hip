@@ -920,6 +920,14 @@ static int with_row_group(int64_t vecs, F f) {
 // Workgroups whose sums are kept.
 constexpr int64_t SUM_GROUPS = 4096;
 
+// Short rows of the policy loss, and batches of them that one workgroup takes in four turns at most: a launch, and the
+// gap before it, costs as much as two.
+static bool short_rows(int64_t V, int elem) { return V <= (elem == TE_F32 ? SHORT_MOST / 2 : SHORT_MOST); }
+static int short_lanes(int64_t V) { return V <= SHORT_ONE ? 1 : 16; }
+static bool one_group(int64_t N, int64_t V, int elem) {
+  return N == 0 || (short_rows(V, elem) && N * short_lanes(V) <= 4 * COUNT_THREADS);
+}
+
 // The longest launches have a workgroup a row and one more (rows in parts are few); counts of rows stay exact in fp32.
 static bool rows_fit(int64_t N, int64_t V) { return V < (1LL << 30) && launch_fits(N + 1, LOSS_THREADS); }
 
@@ -929,10 +937,12 @@ using namespace bf;
 
 extern "C" {
 
-// sums of the workgroups (row kernel, short rows), or part [N * parts] float2; the counts' shares, and live rows [B]
+// sums of the workgroups (row kernel, short rows), and part [N * parts] float2 (rows in parts), neither where one
+// workgroup does everything; the counts' shares, and live rows [B]
 int64_t bf_policy_loss_workspace(int64_t B, int64_t T, int64_t V, int elem) {
   if (!elem_ok(elem) || B < 0 || T < 0 || V <= 0 || B >= (1LL << 24) || T >= (1LL << 24) || !rows_fit(B * T, V)) return 0;
-  return 4 * SUM_GROUPS + 2 * B * T * row_parts(B * T, V, elem).count + COUNT_GROUPS + B;
+  const int64_t sums = one_group(B * T, V, elem) ? 0 : 4 * SUM_GROUPS + 2 * B * T * row_parts(B * T, V, elem).count;
+  return sums + COUNT_GROUPS + B;
 }
 
 int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V, int64_t ld_b, int64_t ld_t,
@@ -964,17 +974,16 @@ int bf_policy_loss(const void* logits, int elem, int64_t B, int64_t T, int64_t V
   // the counting waits for loads: 1024 rows a workgroup, one a thread
   const int64_t turns = ceil_div(N, COUNT_THREADS), shares = by_sequence && B < turns ? B : turns;
   PolicyCounts counts;
-  counts.share = reinterpret_cast<float*>(part + N * p.count);
+  const bool alone = one_group(N, V, elem), shorts = short_rows(V, elem);
+  const int lanes = short_lanes(V);
+  counts.share = alone ? workspace : reinterpret_cast<float*>(part + N * p.count);
   counts.live = counts.share + COUNT_GROUPS;
   counts.groups = 1;
-  const bool shorts = V <= (elem == TE_F32 ? SHORT_MOST / 2 : SHORT_MOST);
-  const int lanes = V <= SHORT_ONE ? 1 : 16;
   return with_elem(elem, [&](auto e) -> int {
     using E = decltype(e);
     const E* x = static_cast<const E*>(logits);
     E* out = static_cast<E*>(grad);
-    // one workgroup for what takes it four turns at most: a launch, and the gap before it, costs as much as two
-    if (N == 0 || (shorts && N * lanes <= 4 * COUNT_THREADS)) {
+    if (alone) {
       if (lanes == 1)
         hipLaunchKernelGGL((policy_short_kernel<true, 1, E>), dim3(1), dim3(COUNT_THREADS), 0, stream, x, rows, a,
                            counts, logp, stats, out, sums);

@@ -13,11 +13,11 @@ def recorded(monkeypatch):
     if not _lib.LIB_PATH.exists():
         pytest.skip("library not built (run python -m boundflow_amd.build)")
     made, calls = [], []
-    for name in ("empty", "zeros"):
-        def record(*args, real=getattr(torch, name), **kw):
+    for owner, name in ((torch, "empty"), (torch, "zeros"), (torch.Tensor, "new_empty")):
+        def record(*args, real=getattr(owner, name), **kw):
             made.append(real(*args, **kw))
             return made[-1]
-        monkeypatch.setattr(torch, name, record)
+        monkeypatch.setattr(owner, name, record)
     monkeypatch.setattr(training, "_current_device", lambda t, name: -1)
     monkeypatch.setattr(training, "_on_device", lambda t, dev, name: None)
     monkeypatch.setattr(training, "current_raw_stream", lambda dev: None)
@@ -75,3 +75,23 @@ def test_a_table_of_one_row_may_have_any_stride(recorded):
     assert table.stride() == (1, 1)
     assert training.embed_tokens(table, torch.zeros(3, dtype=torch.int64)).shape == (3, 6)
     assert calls[0][1][1] >= 6, "the library takes no stride below the width"
+
+
+@pytest.mark.parametrize("rows,V", [(4, 5), (4, 70001), (40, 50001), (300, 700), (2100, 9), (3000, 2050), (9000, 520)])
+def test_results_do_not_keep_the_workspace(recorded, rows, V):
+    """A caller that keeps a step's log-probabilities keeps what the results take, and 32 KiB beside them at most."""
+    _made, calls = recorded
+    logits, tokens = torch.zeros(1, V).expand(rows, V), torch.zeros(rows, dtype=torch.int64)
+    r = training.policy_loss(logits, tokens, fp32(rows), fp32(rows), with_grad=False)
+    held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in (r.stats, r.loss, r.logp)}
+    assert sum(held.values()) <= 4 * (4 + rows) + 32768 + 16
+    q = training.preference_loss(logits, tokens, fp32(rows), torch.tensor([0, rows // 2, rows]), with_grad=False)
+    held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in (q.loss, q.rewards, q.logp)}
+    assert sum(held.values()) <= 4 * (3 + rows) + 32768 + 16
+    # what kernels get as their workspace starts at a multiple of 16 bytes of its buffer, and lies within one
+    lib, made = _lib.load(), {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in recorded[0]}
+    for (name, args), need in zip(calls, (lib.bf_policy_loss_workspace(rows, 1, V, 0),
+                                          lib.bf_preference_loss_workspace(rows, V, 1, 0))):
+        space = args[-2]
+        base = max(b for b in made if b <= space)
+        assert (space - base) % 16 == 0 and space + 4 * need <= base + made[base], name
