@@ -496,7 +496,9 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const T* __restrict
 // memory-side cache gained nothing (a third of the traffic from there, the same time: what the XCDs exchange
 // with the memory side is the limit).
 
-// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements), and for the policy loss one that counts.
+// (M, s) of a part of a row.  Workgroup = (row, part of `chunk` elements).  The policy loss, whose workgroups have
+// LOSS_THREADS, launches one more, which counts; the preference loss's short rows, a wave each, do without the LDS of
+// the counts, which would leave a CU 19 of 32 such workgroups (65536 rows of 500 bf16 logits 70 us against 80).
 template <class T, int TH>
 __global__ __launch_bounds__(TH) void loss_partial_kernel(const T* __restrict__ logits, LogitRows rows, PolicyArgs a,
                                                           int64_t N, int parts, int64_t chunk,
@@ -504,11 +506,13 @@ __global__ __launch_bounds__(TH) void loss_partial_kernel(const T* __restrict__ 
   constexpr int VEC = 16 / sizeof(T);
   __shared__ float2 red[TH / 64];
   const int64_t n = blockIdx.x / (unsigned)parts;
-  if (n == N) {
-    __shared__ int held[COUNT_HELD];
-    __shared__ float sum[TH / 64];
-    policy_count<TH>(a, counts, 0, held, sum);
-    return;
+  if constexpr (TH == LOSS_THREADS) {
+    if (n == N) {
+      __shared__ int held[COUNT_HELD];
+      __shared__ float sum[TH / 64];
+      policy_count<TH>(a, counts, 0, held, sum);
+      return;
+    }
   }
   const int q = (int)(blockIdx.x % (unsigned)parts);
   if (!live_row(a.mask, a.tokens, a.token_bytes, n)) return;
@@ -775,8 +779,8 @@ __device__ __forceinline__ int2 response_rows(const PreferenceArgs& a, int64_t k
 }
 
 // The preference loss gives a row of up to this many vectors a lane to one wave instead of four: 65536 rows of 500 bf16
-// logits 82 us against 156 (what four waves cost is the start of their workgroups), of 2000 175 against 191; from twice
-// that on the four waves are ahead, 4000 in 310 us against 333.
+// logits 70 us against 154 (what four waves cost is the start of their workgroups), of 2000 177 against 188; from twice
+// that on the four waves are ahead, 4000 in 305 us against 332.
 constexpr int WAVE_VECTORS = 4;
 
 constexpr int PAIR_THREADS = 1024, PAIR_WAVES = PAIR_THREADS / 64;
