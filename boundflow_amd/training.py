@@ -161,7 +161,7 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
 # Losses
 
 # A loss's small results are views of one buffer, and a workspace of up to this many floats lies behind them: a second
-# allocation takes 1.2 us of the host, and a call on few rows (some 2048 parts of 8 bytes) waits for the host (45
+# allocation takes 1.2 us of the host, and a call on few rows (up to 2048 parts of 8 bytes) waits for the host (45
 # preference rows 20.0 us against 21.0).  A larger one is a buffer of its own, or a caller that keeps a result would keep
 # it too.
 _SHARED_WORKSPACE = 8192

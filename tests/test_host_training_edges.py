@@ -63,3 +63,18 @@ def test_sizes_that_no_launch_takes_are_refused_before_the_first(lib):
     weights, at = list(torch.zeros(120, 64)), [1 << 60, 2 << 60]
     assert adamw(lib, weights, weights, [64] * 119 + [1 << 34], at) == 3   # in the second launch
     assert adamw(lib, weights, weights, [64] * 119 + [1 << 35], at, m_scale=p, v_scale=p) == 3
+
+
+def test_workspaces_hold_what_their_kernels_write(lib):
+    # a first place per value and the end, a place per token; per eight tokens an owner and two rows of sums
+    for count, vocab, dim in ((2049, 1, 1), (5000, 10, 4), (16_384, 32_000, 4096), (20_001, 70_001, 129)):
+        pieces = -(-count // 8)
+        assert lib.bf_embed_grad_workspace(count, vocab, dim) >= vocab + 1 + count + pieces * (1 + 2 * dim)
+    # 64 shares of the counts, live rows per sequence; four sums per workgroup (2048 at most for short rows, 4096 for
+    # held ones); a largest logit and a sum per part of a row
+    for B, T, V, elem, sums, parts in ((64, 16, 5, 0, 0, 0), (5000, 2, 100, 1, 4 * 2048, 0), (8, 600, 700, 2, 4 * 4096, 0),
+                                       (1, 4, 70_001, 0, 0, 2 * 4 * 35), (3, 800, 140_000, 1, 0, 2 * 2400)):
+        assert lib.bf_policy_loss_workspace(B, T, V, elem) >= 64 + B + sums + parts
+    # four coefficients per row, a loss per pair
+    for N, V, pairs, elem, parts in ((45, 50_001, 2, 0, 45 * 25), (9001, 50_001, 16, 1, 9001), (2047, 4099, 3, 2, 2047 * 2)):
+        assert lib.bf_preference_loss_workspace(N, V, pairs, elem) >= 4 * N + 2 * parts + pairs
