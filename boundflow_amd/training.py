@@ -440,7 +440,9 @@ def _moment(t: Optional[torch.Tensor], name: str, kind: torch.dtype, length: int
 
 
 class AdamW:
-    """AdamW over a fixed list of parameters: their moments and the step count around ``adamw_step``."""
+    """AdamW over a fixed list of parameters: their moments and the step count around ``adamw_step``.
+
+    ``moments`` and ``t`` (steps taken) are the whole state: a checkpoint holds both, and is loaded by setting them."""
 
     def __init__(self, params: Sequence[torch.Tensor], *, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, bits: int = 32, master: bool = False):

@@ -159,3 +159,26 @@ def test_preference_loss_of_more_pairs_than_a_launch_has_workgroups():
     g = -torch.sigmoid(-h) * 0.5
     want = torch.cat([g, -g])[:, None] * (torch.nn.functional.one_hot(tokens, V) - logsm.exp())
     close(got.grad_logits, want, 2.0 ** -20 + 2.0 ** -20 * want.abs(), "gradient")
+
+
+@pytest.mark.parametrize("bits,master", [(32, False), (8, True)])
+def test_adamw_goes_on_from_its_saved_state(bits, master, tmp_path):
+    dev = device()
+    g = gen(9)
+    first = [torch.randn(n, generator=g).bfloat16().to(dev) for n in (1000, 7)]
+    grads = [[torch.randn(n, generator=g).bfloat16().to(dev) for n in (1000, 7)] for _ in range(6)]
+    straight = [p.clone() for p in first]
+    opt = training.AdamW(straight, bits=bits, master=master)
+    for k in grads:
+        opt.step(k)
+    broken = [p.clone() for p in first]
+    opt = training.AdamW(broken, bits=bits, master=master)
+    for k in grads[:3]:
+        opt.step(k)
+    torch.save({"params": broken, "moments": tuple(opt.moments), "t": opt.t}, tmp_path / "state.pt")
+    kept = torch.load(tmp_path / "state.pt", weights_only=True)
+    again = training.AdamW(kept["params"], bits=bits, master=master)
+    again.moments, again.t = training.AdamWMoments(*kept["moments"]), kept["t"]
+    for k in grads[3:]:
+        again.step(k)
+    assert all(torch.equal(a, b) for a, b in zip(kept["params"], straight))

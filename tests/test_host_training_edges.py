@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from boundflow_amd import _lib
+from oracle import training_ref as ref
 
 
 @pytest.fixture(scope="module")
@@ -78,3 +79,19 @@ def test_workspaces_hold_what_their_kernels_write(lib):
     # four coefficients per row, a loss per pair
     for N, V, pairs, elem, parts in ((45, 50_001, 2, 0, 45 * 25), (9001, 50_001, 16, 1, 9001), (2047, 4099, 3, 2, 2047 * 2)):
         assert lib.bf_preference_loss_workspace(N, V, pairs, elem) >= 4 * N + 2 * parts + pairs
+
+
+@pytest.mark.parametrize("beta2,steps", [(0.99, 400), (0.999, 1000)])
+def test_phases_keep_a_slow_average_at_every_step(beta2, steps):
+    """sqrt(v) of steady gradients of 0.1 to 1 beside one of a burst of 100 at step 20: within two spacings, a quarter, of
+    the exact one at every step and at both of the usual decays."""
+    level = torch.rand(256, generator=torch.Generator().manual_seed(3), dtype=torch.float64) * 0.9 + 0.1
+    held, v, burst = (torch.zeros(256, dtype=torch.float64) for _ in range(3))
+    burst[::128] = 100.0
+    for t in range(1, steps + 1):
+        g = level + (burst if t == 20 else 0.0 * burst)
+        v = beta2 * v + (1 - beta2) * g * g
+        count, spacing, scale = ref.hold((beta2 * held * held + (1 - beta2) * g * g).sqrt(), ref.phases(256, t), True)
+        held = count.floor() * spacing * scale.repeat_interleave(128)
+        ratio = (held / v.sqrt())[burst == 0]
+        assert 0.75 < float(ratio.min()) and float(ratio.max()) < 1.25, t
