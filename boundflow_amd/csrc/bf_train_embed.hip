@@ -513,7 +513,8 @@ int bf_embed_grad(const void* grad, int64_t grad_ld, int elem, const void* token
       const TI* g = static_cast<const TI*>(grad);
       TO* o = static_cast<TO*>(out);
       if (count <= FEW_TOKENS) {
-        // Four workgroups a CU and more where there is work for them.  The frequent values are mostly neighbours, so a
+        // 1024 workgroups and more where there is work for them (a CU holds three at a time with 16-bit rows and five
+        // with fp32 ones: 46 and 30 KB of LDS).  The frequent values are mostly neighbours, so a
         // workgroup with all columns of its rows would be left with most of the sums: it takes a step's columns of
         // them, or more where that made more than 2048 workgroups, because every one sorts for itself.  2048
         // tokens of 32000 values, 4096 bf16 columns 75 us (all columns of 16 rows: 120), 1500 of 8000, 768 fp32 columns

@@ -893,7 +893,7 @@ static Parts row_parts(int64_t N, int64_t V, int elem) {
 }
 
 // The row kernel's workgroup for rows of `vecs` whole vectors, handed to f as (threads, vectors a thread, steps that
-// are whole in every such row) at compile time; 0 where no workgroup holds a row (131072 16-bit or 65536 fp32
+// are whole in every such row) at compile time; 0 where no workgroup holds a row (131080 16-bit or 65540 fp32
 // logits and more) or a row has no whole vector.
 template <class F>
 static int with_row_group(int64_t vecs, F f) {
