@@ -208,14 +208,14 @@ __device__ __forceinline__ PolicyRow policy_term(float logp, float old, float re
   if (has_ref) {
     const float apart = ref - logp, e = expm1f(apart);
     r.kl = e - apart;
-    r.g -= kl_weight * e;
+    if (kl_weight != 0.f) r.g -= kl_weight * e;   // 0 * inf would be NaN where the exponential overflows
   }
   return r;
 }
 
 // stats: loss, policy term, KL, clipped share
 __device__ __forceinline__ void write_stats(float policy, float kl, float outside, float kl_weight, float* stats) {
-  stats[0] = policy + kl_weight * kl;
+  stats[0] = kl_weight != 0.f ? policy + kl_weight * kl : policy;
   stats[1] = policy;
   stats[2] = kl;
   stats[3] = outside;

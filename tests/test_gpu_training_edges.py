@@ -182,3 +182,22 @@ def test_adamw_goes_on_from_its_saved_state(bits, master, tmp_path):
     for k in grads[3:]:
         again.step(k)
     assert all(torch.equal(a, b) for a, b in zip(kept["params"], straight))
+
+
+@pytest.mark.parametrize("B,T,V", [(1, 6, 5), (2, 40, 300), (2, 5, 4099), (2, 200, 2050)])
+def test_policy_loss_with_a_kl_weight_of_0_at_rows_far_from_the_reference(B, T, V):
+    """exp(ref - p) passes the largest fp32 (the reference has the token 95 and 300 nats above): the KL statistic is inf,
+    and a term of weight 0 is not in the loss or its gradient."""
+    dev = device()
+    s = policy_inputs(B, T, V, torch.float32, 3, True, "none")
+    s["ref_logp"][0, 1] += 95.0
+    s["ref_logp"][-1, 4] += 300.0
+    want = training.policy_loss(**{**to(dev, s), "ref_logp": None})
+    got = training.policy_loss(**to(dev, s), kl_weight=0.0)
+    assert float(got.stats[2]) == float("inf")
+    for k in (0, 1, 3):
+        assert float(got.stats[k]) == float(want.stats[k])
+    assert torch.equal(got.grad_logits, want.grad_logits) and torch.equal(got.logp, want.logp)
+    r = ref.policy_loss(**s)
+    # terms of a few units, each off by some 2^-22 of its row's spread of 30 (logp_tol) and summed in fp32
+    assert abs(float(got.loss) - float(r["stats"][0])) < 1e-4 * (1 + abs(float(r["stats"][0])))
