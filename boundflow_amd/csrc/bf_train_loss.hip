@@ -198,7 +198,8 @@ struct PolicyRow {
 __device__ __forceinline__ PolicyRow policy_term(float logp, float old, float ref, bool has_ref, float A, float low,
                                                  float high, float kl_weight) {
   PolicyRow r;
-  const float ratio = expf(logp - old);
+  float ratio = expf(logp - old);
+  if (A == 0.f && ratio > -kFloor) ratio = -kFloor;   // 0 * inf would be NaN (a NaN stays one)
   const float plain = ratio * A, clipped = fminf(fmaxf(ratio, low), high) * A;
   const bool out = clipped < plain;   // the clipped side is the smaller: a constant, without a gradient
   r.policy = out ? -clipped : -plain;

@@ -201,3 +201,21 @@ def test_policy_loss_with_a_kl_weight_of_0_at_rows_far_from_the_reference(B, T, 
     r = ref.policy_loss(**s)
     # terms of a few units, each off by some 2^-22 of its row's spread of 30 (logp_tol) and summed in fp32
     assert abs(float(got.loss) - float(r["stats"][0])) < 1e-4 * (1 + abs(float(r["stats"][0])))
+
+
+@pytest.mark.parametrize("B,T,V", [(1, 6, 5), (2, 40, 300), (2, 5, 4099), (2, 200, 2050)])
+def test_policy_loss_of_rows_without_an_advantage_far_from_the_old_policy(B, T, V):
+    """exp(p - old) passes the largest fp32 at rows whose advantage is 0: the term is 0, as exp(95) * 0 is."""
+    dev = device()
+    s = policy_inputs(B, T, V, torch.float32, 5, False, "none")
+    s["advantages"][0, 1] = s["advantages"][-1, 4] = 0.0
+    near = ref.policy_loss(**s)
+    s["old_logp"][0, 1] -= 95.0
+    s["old_logp"][-1, 4] -= 300.0
+    r = ref.policy_loss(**s)
+    assert torch.equal(r["stats"], near["stats"])
+    got = training.policy_loss(**to(dev, s))
+    # terms of a few units, each off by some 2^-22 of its row's spread of 30 (logp_tol) and summed in fp32
+    close(got.stats, r["stats"], 1e-4 * (1 + r["stats"].abs()), "stats")
+    assert torch.isfinite(got.grad_logits).all()
+    assert not got.grad_logits[0, 1].any() and not got.grad_logits[-1, 4].any()
