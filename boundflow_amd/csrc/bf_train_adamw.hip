@@ -239,7 +239,7 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
              beta1, beta2, eps);
   BF_REQUIRE((m_scale != nullptr) == (v_scale != nullptr), "bf_adamw_multi: one moment has scales, the other none");
   if (count == 0) return BF_OK;
-  BF_REQUIRE(p && g && n && m && v, "bf_adamw_multi: null pointer");
+  BF_REQUIRE(p && g && n, "bf_adamw_multi: null pointer");
   // All checks come before the first launch: a call that is refused has stepped nothing.
   constexpr int FEW = 256, OTHERS = 5;
   Span few[FEW];
@@ -265,6 +265,8 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
     writes(p[k], n[k] * elem_bytes(p_elem));
     total += ceil_div(n[k], ADAMW_BLOCK) * ADAMW_BLOCK;
   }
+  if (total == 0) return BF_OK;
+  BF_REQUIRE(m && v, "bf_adamw_multi: null pointer");
   writes(m, total * (m_scale ? 1 : 4));
   writes(v, total * (m_scale ? 1 : 4));
   writes(m_scale, total / ADAMW_BLOCK * 4);

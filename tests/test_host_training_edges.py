@@ -95,3 +95,9 @@ def test_phases_keep_a_slow_average_at_every_step(beta2, steps):
         held = count.floor() * spacing * scale.repeat_interleave(128)
         ratio = (held / v.sqrt())[burst == 0]
         assert 0.75 < float(ratio.min()) and float(ratio.max()) < 1.25, t
+
+
+def test_adamw_of_empty_weights_has_nothing_to_do(lib):
+    """Weights without an element, alone, have moments without an address."""
+    assert adamw(lib, [None, None], [None, None], [0, 0], [None, None]) == 0
+    assert adamw(lib, [None], [None], [0], [None, None], m_scale=8, v_scale=8) == 0
