@@ -26,8 +26,32 @@ void set_error(const char* fmt, ...);
     }                                    \
   } while (0)
 
+// A grid counts its work-items in 32 bits, and of a larger one the runtime starts what is left of the number, without an
+// error: bounds would be missing, and nobody told.  Every launch goes through this check; one that does not fit is not
+// made, and the BF_LAUNCH_CHECK that follows it says so.
+inline bool launch_fits(int64_t blocks, int64_t threads) { return blocks < (1LL << 32) / threads; }
+
+inline thread_local bool launch_refused = false;
+
+inline bool may_launch(const dim3& grid, const dim3& block) {
+  const bool fits = launch_fits(grid.x, block.x) && launch_fits(grid.y, block.y) && launch_fits(grid.z, block.z);
+  if (!fits) launch_refused = true;
+  return fits;
+}
+
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...)                                        \
+  do {                                                                                                   \
+    if (::bf::may_launch(grid, block)) (kernel)<<<grid, block, lds, stream>>>(__VA_ARGS__);              \
+  } while (0)
+
 #define BF_LAUNCH_CHECK(what)                                                       \
   do {                                                                              \
+    if (::bf::launch_refused) {                                                     \
+      ::bf::launch_refused = false;                                                 \
+      ::bf::set_error("%s: a launch of 2^32 work-items or more", what);             \
+      return ::bf::BF_ERANGE;                                                       \
+    }                                                                               \
     hipError_t _e = hipGetLastError();                                              \
     if (_e != hipSuccess) {                                                         \
       ::bf::set_error("%s: launch failed: %s", what, hipGetErrorString(_e));        \

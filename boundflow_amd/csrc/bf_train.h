@@ -14,10 +14,6 @@ enum : int { TE_F32 = 0, TE_BF16 = 1, TE_F16 = 2 };
 inline bool elem_ok(int code) { return code >= TE_F32 && code <= TE_F16; }
 inline int elem_bytes(int code) { return code == TE_F32 ? 4 : 2; }
 
-// Whether a launch takes `blocks` workgroups of `threads` (a power of two): a grid counts its work-items in 32 bits, and
-// of a larger one the runtime starts what is left of the number, without an error.
-inline bool launch_fits(int64_t blocks, int threads) { return blocks < (1LL << 32) / threads; }
-
 // Calls f(T()) with the element type of a code that elem_ok has passed.
 template <class F>
 inline int with_elem(int code, F f) {
