@@ -2,7 +2,9 @@
 
 The networks that the bound queries verify are trained, and repaired after a failed query,
 with what is here: the lookup of token rows and its gradient (``embed_tokens``,
-``embed_tokens_grad``), two losses of token logits with their gradients (``policy_loss``,
+``embed_tokens_grad``), dropout with a mask that is made again for its gradient (``dropout``,
+``dropout_grad``), the cross entropy of a head over a vocabulary with its gradients
+(``vocabulary_loss``), two losses of token logits with their gradients (``policy_loss``,
 ``preference_loss``) and the weights' update (``adamw_step``, ``AdamW``).  A token network is
 bounded in embedding space: the looked-up rows are the centre of the input set.
 
@@ -155,6 +157,86 @@ def embed_tokens_grad(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, s
     if accumulate_into is not None:
         torch.autograd.graph.increment_version(out)
     return out
+
+
+# ---------------------------------------------------------------------------
+# Dropout
+
+def _matrix(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(``t`` as rows of its last axis, the rows' stride): a view where its strides allow one, a copy otherwise."""
+    if t.is_contiguous():
+        return t, t.shape[-1] if t.dim() else 1
+    rows = t.reshape(-1, t.shape[-1])
+    if rows.stride(1) != 1 or rows.stride(0) < rows.shape[1]:
+        rows = rows.contiguous()
+    return rows, rows.stride(0)
+
+
+def dropout(x: torch.Tensor, p: float, *, seed: int, counter: Union[int, torch.Tensor] = 0,
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x`` with each element dropped (0) with probability ``p`` and the others divided by 1 - p, added to
+    ``residual`` (of x's shape and type) where there is one; dense, of x's type, rounded once.
+
+    No mask is stored: whether element e is kept (e counts x's elements in their order, whatever its strides) follows from
+    ``seed`` (an integer below 2^64), ``counter`` and e, so ``dropout_grad`` with the same two makes the same mask, and
+    every other counter (below 2^63) an independent one.  A counter that lies on the device (int64, one element) is read
+    when the kernel runs: a captured graph whose counter is raised between replays drops anew.  p counts in steps
+    of 2^-16 (the nearest is taken, in the division too).  The result comes without a graph: an x or residual that
+    requires grad is refused while gradients are recorded."""
+    if residual is not None and isinstance(residual, torch.Tensor) and residual.requires_grad and \
+            torch.is_grad_enabled():
+        raise HipError("residual requires grad, but the sum comes without a graph: pass residual.detach()")
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        raise HipError("x requires grad, but the result comes without a graph: pass x.detach() and get its gradient from "
+                       "dropout_grad")
+    return _dropout(x, "x", p, seed, counter, residual)
+
+
+def dropout_grad(grad: torch.Tensor, p: float, *, seed: int, counter: Union[int, torch.Tensor] = 0) -> torch.Tensor:
+    """Gradient of ``dropout`` with respect to its x, from ``grad`` (of x's shape): the same mask and factor on it.  (With
+    respect to the residual it is grad itself.)"""
+    return _dropout(grad, "grad", p, seed, counter, None)
+
+
+def _dropout(x, name, p, seed, counter, residual) -> torch.Tensor:
+    dev = _current_device(x, name)
+    elem = _elem(x, name)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1], got {p}")
+    if not 0 <= seed < 1 << 64:
+        raise ValueError(f"seed must be in [0, 2^64), got {seed}")
+    at, counter_dev = 0, None
+    if isinstance(counter, torch.Tensor):
+        _on_device(counter, dev, "counter")
+        if counter.dtype != torch.int64 or counter.numel() != 1:
+            raise HipError("counter must be a number or an int64 tensor of one element")
+        counter_dev = counter.data_ptr()
+    else:
+        at = int(counter)
+        if not 0 <= at < 1 << 63:
+            raise ValueError(f"counter must be in [0, 2^63), got {counter}")
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    count = x.numel()
+    if count == 0:
+        if residual is not None:
+            _residual(residual, x, dev)
+        return out
+    rows, ld = _matrix(x)
+    dim = x.shape[-1] if x.dim() else 1
+    more, more_ld = None, 0
+    if residual is not None:
+        _residual(residual, x, dev)
+        more, more_ld = _matrix(residual)
+    _lib.call("bf_dropout", rows.data_ptr(), ld, _address(more), more_ld, elem, count // dim, dim, float(p),
+              seed - (1 << 64) if seed >> 63 else seed, at, counter_dev, out.data_ptr(), current_raw_stream(dev))
+    return out
+
+
+def _residual(residual: torch.Tensor, x: torch.Tensor, dev: int) -> None:
+    _on_device(residual, dev, "residual")
+    if residual.dtype != x.dtype or residual.shape != x.shape:
+        raise ValueError(f"residual must be {x.dtype} of shape {tuple(x.shape)}, got {residual.dtype} of "
+                         f"{tuple(residual.shape)}")
 
 
 # ---------------------------------------------------------------------------
@@ -313,6 +395,94 @@ def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.
               at + 4 + 8 * pairs, at + 4,
               at, _address(grad), space, current_raw_stream(dev))
     return PreferenceLoss(out[0], out[1:1 + 2 * pairs], out[1 + 2 * pairs:own], grad)
+
+
+class VocabularyLoss(NamedTuple):
+    """``logp``: the tokens' log-probabilities (float32, of the tokens' shape); the gradients None where none are made."""
+
+    loss: torch.Tensor
+    logp: torch.Tensor
+    grad_hidden: Optional[torch.Tensor]
+    grad_weight: Optional[torch.Tensor]
+    grad_bias: Optional[torch.Tensor]
+
+
+def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *,
+                    bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                    grad_scale: float = 1.0, with_grad: bool = True,
+                    weight_grad_dtype: Optional[torch.dtype] = None) -> VocabularyLoss:
+    """Softmax cross entropy of a linear head over a vocabulary, with its gradients, without keeping the logits.
+
+    hidden [B, T, D] or [N, D] (a view such as ``states[:, :-1]`` is read in place), weight [V, D] (rows contiguous, any
+    row stride) and bias [V] of one type; tokens and mask (bool) of hidden's leading shape.  With the logits
+    z = (hidden weight^T + bias) / temperature, a token's log-probability is z[token] - log sum exp z, and the loss the mean
+    of its negative over the live rows.  A row is live unless it is masked or its token is negative; the others are
+    not read, and logp and gradient are 0 there.  A batch without a live row has loss 0.  A token past the vocabulary
+    gives NaN.  The gradients are ``grad_scale`` times the loss's, of the inputs' type, the weight's also in float32
+    (``weight_grad_dtype``; ``embed_tokens_grad`` can then add that of a tied table to it).  ``with_grad=False`` gives loss
+    and log-probabilities alone: those that ``policy_loss`` and ``preference_loss`` take as an old or a reference policy's.
+
+    Products of 16-bit inputs are summed in fp32; between them the softmax's gradient is held in the inputs' type
+    (fp32: in 24 bits)."""
+    dev = _current_device(hidden, "hidden")
+    elem = _elem(hidden, "hidden")
+    shape = hidden.shape
+    dims = len(shape)
+    if dims not in (2, 3) or shape[-1] < 1:
+        raise ValueError(f"hidden must be [B, T, D] or [N, D] with D >= 1, got {tuple(shape)}")
+    if not temperature > 0.0:
+        raise ValueError(f"temperature must be >0, got {temperature}")
+    lead, D = shape[:-1], shape[-1]
+    strides = hidden.stride()
+    if strides[-1] != 1 and D > 1:
+        raise HipError(f"hidden needs a contiguous last axis, got strides {strides}")
+    _on_device(weight, dev, "weight")
+    if weight.dtype != hidden.dtype:
+        raise HipError(f"weight must be {hidden.dtype}, as hidden is, got {weight.dtype}")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] != D:
+        raise ValueError(f"weight must be [V, {D}] with V >= 1, got {tuple(weight.shape)}")
+    V = weight.shape[0]
+    ld, step = weight.stride()
+    if V == 1:
+        ld = D        # a single row's stride leads nowhere, and may be anything
+    if (step != 1 and D > 1) or ld < D:
+        raise HipError(f"weight must have contiguous rows, got {tuple(weight.shape)} with strides {weight.stride()}")
+    if bias is not None:
+        _on_device(bias, dev, "bias")
+        if bias.dtype != hidden.dtype:
+            raise HipError(f"bias must be {hidden.dtype}, as hidden is, got {bias.dtype}")
+        if bias.shape != (V,):
+            raise ValueError(f"bias of shape {tuple(bias.shape)}, expected ({V},)")
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+    B, T = (lead[0], lead[1]) if dims == 3 else (lead[0], 1)
+    tokens, token_bytes = _tokens(tokens, lead, dev)
+    if mask is not None:
+        _on_device(mask, dev, "mask")
+        if mask.dtype != torch.bool:
+            raise HipError(f"mask must be bool, got {mask.dtype}")
+        if mask.shape != lead:
+            raise ValueError(f"mask of shape {tuple(mask.shape)}, expected {tuple(lead)}")
+        if not mask.is_contiguous():
+            mask = mask.contiguous()
+    wide = weight.dtype if weight_grad_dtype is None else weight_grad_dtype
+    if wide not in (weight.dtype, torch.float32):
+        raise ValueError(f"weight_grad_dtype must be {weight.dtype} or float32, got {wide}")
+    N = B * T
+    need = _lib.load().bf_vocab_loss_workspace(N, D, V, elem, weight.data_ptr(), ld, with_grad)
+    out = torch.empty(1 + N, dtype=torch.float32, device=hidden.device)      # loss, logp
+    space = torch.empty(need, dtype=torch.float32, device=hidden.device) if need else None
+    grad_hidden = grad_weight = grad_bias = None
+    if with_grad:
+        grad_hidden = hidden.new_empty(shape)
+        grad_weight = torch.empty(V, D, dtype=wide, device=hidden.device)
+        grad_bias = None if bias is None else hidden.new_empty(V)
+    at = out.data_ptr()
+    _lib.call("bf_vocab_loss", hidden.data_ptr(), elem, B, T, D, strides[0], strides[1] if dims == 3 else 0,
+              weight.data_ptr(), V, ld, _address(bias), tokens.data_ptr(), token_bytes, _address(mask), float(temperature),
+              float(grad_scale), at + 4, at, _address(grad_hidden), _address(grad_weight), _ELEM[wide], _address(grad_bias),
+              _address(space), current_raw_stream(dev))
+    return VocabularyLoss(out[0], out[1:1 + N].view(lead), grad_hidden, grad_weight, grad_bias)
 
 
 # ---------------------------------------------------------------------------

@@ -665,6 +665,29 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
                    double eps, double weight_decay, int64_t step, float grad_scale, const float* grad_scale_dev,
                    hipStream_t stream);
 
+/* Softmax cross entropy of a head over a vocabulary, with its gradients; the logits are not kept.  Hidden rows
+ * [B, T, D], row (b, t) at b * ld_b + t * ld_t; weight [V, D] with row stride ld_w, bias [V] (NULL: none) of the same type;
+ * tokens and mask (bytes; NULL: all ones) dense [B, T].  With z = hidden . weight + bias over the temperature:
+ *   logp = z[token] - log(sum of exp(z)),  loss = the mean of -logp over the live rows (0 without one).
+ * A row is live unless it is masked or its token negative; other rows are not read, and their logp and gradient
+ * are 0.  A token past the vocabulary gives NaN.  grad_hidden dense [B, T, D] and grad_bias [V] of the inputs' type,
+ * grad_weight dense [V, D] of that type or fp32: grad_scale * the loss's gradient; all that there are, or none of them (NULL).
+ * Workspace in floats, 16-byte aligned; its size depends on whether the weight can be read as it lies. */
+int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
+                                int with_grad);
+int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
+                  const void* weight, int64_t V, int64_t ld_w, const void* bias, const void* tokens, int token_bytes,
+                  const void* mask, double temperature, float grad_scale, float* logp, float* loss, void* grad_hidden,
+                  void* grad_weight, int grad_weight_elem, void* grad_bias, float* workspace, hipStream_t stream);
+
+/* Dropout: out[e] = (residual[e]) + (u_e >= border ? x[e] / (1 - border / 2^16) : 0) with border = p * 2^16, rounded, in
+ * fp32 and rounded once.  u_e are 16 bits of the Philox 4x32 generator of ten rounds, whose counter is (e / 8,
+ * counter) and whose key is the seed (bf_train_dropout.hip), e = row * dim + column.  x and residual (NULL: none) [rows, dim]
+ * with row strides, out dense.  counter_dev (optional): the counter is read there when the kernel runs. */
+int bf_dropout(const void* x, int64_t x_ld, const void* residual, int64_t residual_ld, int elem, int64_t rows,
+               int64_t dim, double p, int64_t seed, int64_t counter, const int64_t* counter_dev, void* out,
+               hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

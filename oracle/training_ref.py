@@ -127,3 +127,53 @@ def hold(x, phase, root):
     if root:
         count = torch.where((y > 0) & (count < 1), torch.ones((), dtype=torch.float64), count)
     return count.view(-1), spacing.view(-1), scale
+
+
+def vocabulary_loss(hidden, weight, tokens, *, bias=None, mask=None, temperature=1.0, grad_scale=1.0):
+    """dict of loss, logp and the gradients, and what a tolerance needs, all of the live rows (``at``, their places):
+    x, p (softmax), g (the loss's derivative by a row's logits over the temperature) and the magnitudes of the products
+    that make a logit."""
+    lead, D = tokens.shape, hidden.shape[-1]
+    live = tokens >= 0
+    if mask is not None:
+        live = live & mask
+    at = live.reshape(-1).nonzero()[:, 0]
+    x, w, y = hidden.reshape(-1, D)[at].double(), weight.double(), tokens.reshape(-1)[at]
+    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.double()
+    z = torch.mm(x, w.t()) + b
+    size = torch.mm(x.abs(), w.abs().t()) + torch.where(torch.isfinite(b) & (b.abs() < 1e30), b.abs(), 0.0)
+    logsm = torch.log_softmax(z / temperature, 1)
+    rows = torch.arange(at.numel())
+    n = max(at.numel(), 1)
+    logp = torch.zeros(live.numel(), dtype=torch.float64)
+    logp[at] = logsm[rows, y]
+    p = logsm.exp()
+    g = p.clone()
+    g[rows, y] -= 1.0
+    factor = grad_scale / (temperature * n)
+    dx = torch.zeros(live.numel(), D, dtype=torch.float64)
+    dx[at] = torch.mm(g, w) * factor
+    return {"loss": -logp.sum() / n, "logp": logp.view(lead), "hidden": dx.view(hidden.shape),
+            "weight": torch.mm(g.t(), x) * factor, "bias": g.sum(0) * factor, "at": at, "x": x, "w": w, "p": p, "g": g,
+            "z": z, "size": size, "factor": factor}
+
+
+def philox(block, counter, seed):
+    """The eight 16-bit numbers of a block: Philox 4x32 of ten rounds in Python's integers."""
+    low = 0xFFFFFFFF
+    c = [block & low, block >> 32, counter & low, counter >> 32]
+    k = [seed & low, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(b >> 32) ^ c[1] ^ k[0], b & low, (a >> 32) ^ c[3] ^ k[1], a & low]
+        k = [(k[0] + 0x9E3779B9) & low, (k[1] + 0xBB67AE85) & low]
+    return [w >> s & 0xFFFF for w in c for s in (0, 16)]
+
+
+def dropout(x, p, seed, counter=0, residual=None, first=0):
+    """(result, kept), elements counted from ``first`` on (a multiple of 8)."""
+    border = int(p * 65536 + 0.5)
+    drawn = [u for k in range(-(-x.numel() // 8)) for u in philox(first // 8 + k, counter, seed)][:x.numel()]
+    kept = torch.tensor(drawn, dtype=torch.int64).view(x.shape) >= border
+    y = torch.where(kept, x.double() / (1.0 - border / 65536.0 if border < 65536 else 1.0), 0.0)
+    return (y if residual is None else y + residual.double()), kept

@@ -1,0 +1,448 @@
+"""The operators of a supervised step, ``vocabulary_loss`` and ``dropout``, against plain float64 restatements
+(oracle/training_ref.py).
+
+Tolerances are those of the arithmetic.  A logit is a sum of D exact products in fp32 (fp32 inputs: of six part
+products each, what they leave out below 2^-22 of a product): off by at most (6 D + 8) 2^-24 of the sum of their
+magnitudes, as is a gradient's sum over its rows or its vocabulary.  A log-probability is off by what the logits, the exponents' roundings and the sum
+leave.  The softmax's gradient is rounded to the inputs' type between the products (fp32: to three bf16 parts, 2^-24),
+and results are rounded once."""
+
+import math
+
+import pytest
+import torch
+
+from boundflow_amd import training
+from boundflow_amd._lib import HipError
+from oracle import training_ref as ref
+from tests.gpu_util import announce, device
+from tests.test_gpu_training import TINY, TYPES, U, close, gen, logp_tol, rounded
+
+pytestmark = pytest.mark.gpu
+
+
+def head(N, D, V, dtype, seed, *, bias=True, spread=2.0):
+    """Hidden rows, a head and tokens, the tokens' logits raised by different amounts."""
+    g = gen(seed)
+    weight = (torch.randn(V, D, generator=g) * spread / math.sqrt(D)).to(dtype)
+    tokens = torch.randint(0, V, (N,), generator=g)
+    lift = torch.rand(N, 1, generator=g) * (math.log(V) + 2) / spread ** 2
+    hidden = (torch.randn(N, D, generator=g) + lift * weight[tokens].float()).to(dtype)
+    return hidden, weight, tokens, (torch.randn(V, generator=g) * 0.5).to(dtype) if bias else None
+
+
+def tolerances(r, dtype, temperature, V, D):
+    """(of logp per live row, of G per live row and entry)"""
+    count = 6 * D + 8 if dtype == torch.float32 else D + 8
+    dz = (count * 2.0 ** -24 * r["size"]).amax(1) / temperature + 2.0 ** -22 * r["size"].amax(1) * (
+        dtype == torch.float32)
+    tol_lp = 2 * dz + logp_tol(r["z"] / temperature, V)
+    # What is below a type's normal numbers: fp16 holds 2^14 G in steps of 2^-24, so G to 2^-39.  In fp32 a probability below
+    # 2^-126 is 0, and so is each of three bf16 parts (the matrix cores read subnormal bf16 as 0): 4 * 2^-126 in all.
+    extra = 2.0 ** -124 if dtype == torch.float32 else 2.0 ** -39
+    return tol_lp, r["p"] * (tol_lp + 2.0 ** -21)[:, None] + r["g"].abs() * (U[dtype] + 2.0 ** -23) + extra
+
+
+def check(hidden, weight, tokens, *, bias=None, mask=None, temperature=1.0, grad_scale=1.0, wide=None, on=None, what=""):
+    """`on`: the device tensors where their layout is not that of the others."""
+    dev = device()
+    dtype, (V, D) = weight.dtype, weight.shape
+    r = ref.vocabulary_loss(hidden, weight, tokens, bias=bias, mask=mask, temperature=temperature, grad_scale=grad_scale)
+    args = {"hidden": hidden, "weight": weight, "tokens": tokens, "bias": bias, "mask": mask}
+    args = {k: None if v is None else v.to(dev) for k, v in args.items()}
+    args.update(on or {})
+    kw = dict(temperature=temperature, grad_scale=grad_scale)
+    what = f"{what or tuple(hidden.shape)} x {V} {dtype}"
+    got = training.vocabulary_loss(**args, **kw, weight_grad_dtype=wide)
+    tol_lp, tol_g = tolerances(r, dtype, temperature, V, D)
+    flat = torch.zeros(tokens.numel(), dtype=torch.float64)
+    flat[r["at"]] = tol_lp
+    close(got.logp, r["logp"], flat.view(tokens.shape) + 2.0 ** -23 * r["logp"].abs(), f"logp {what}")
+    n = max(r["at"].numel(), 1)
+    close(got.loss, r["loss"], float(tol_lp.sum()) / n + (n / 256 + 16) * 2.0 ** -23 * float(r["logp"].abs().sum()) / n,
+          f"loss {what}")
+    f, g = r["factor"], r["g"].abs()
+    many = 6 if dtype == torch.float32 else 1
+    tol = torch.zeros(tokens.numel(), D, dtype=torch.float64)
+    tol[r["at"]] = f * (torch.mm(tol_g, r["w"].abs()) + (many * V + 8) * 2.0 ** -24 * torch.mm(g, r["w"].abs()))
+    assert got.grad_hidden.dtype == dtype and got.grad_hidden.is_contiguous()
+    close(got.grad_hidden, r["hidden"], tol.view(hidden.shape) + rounded(r["hidden"], dtype), f"grad hidden {what}")
+    tol = f * (torch.mm(tol_g.t(), r["x"].abs()) + (many * n + 8) * 2.0 ** -24 * torch.mm(g.t(), r["x"].abs()))
+    assert got.grad_weight.dtype == (wide or dtype)
+    close(got.grad_weight, r["weight"], tol + rounded(r["weight"], wide or dtype), f"grad weight {what}")
+    if bias is None:
+        assert got.grad_bias is None
+    else:
+        tol = f * (tol_g.sum(0) + (many * n + 8) * 2.0 ** -24 * g.sum(0))
+        close(got.grad_bias, r["bias"], tol + rounded(r["bias"], dtype), f"grad bias {what}")
+    alone = training.vocabulary_loss(**args, **kw, with_grad=False)
+    assert alone[2:] == (None, None, None)
+    assert torch.equal(alone.logp, got.logp) and torch.equal(alone.loss, got.loss), "other bits without gradients"
+    return got
+
+
+SIZES = [(1, 1, 1), (1, 8, 5), (2, 7, 130), (3, 64, 257), (7, 192, 1003), (8, 129, 97), (9, 128, 128), (16, 65, 256),
+         (17, 320, 300), (33, 64, 4099), (64, 256, 129), (65, 1025, 200), (130, 96, 2), (257, 128, 515), (300, 63, 1003)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", SIZES)
+def test_vocabulary_loss(dtype, N, D, V):
+    hidden, weight, tokens, bias = head(N, D, V, dtype, N + D + V)
+    check(hidden, weight, tokens)
+    check(hidden, weight, tokens, bias=bias, temperature=0.7, grad_scale=100.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", [(700, 192, 1500), (1500, 64, 700), (40, 64, 9000), (513, 1100, 520)])
+def test_vocabulary_loss_of_many_tiles(dtype, N, D, V):
+    hidden, weight, tokens, bias = head(N, D, V, dtype, N + D)
+    mask = torch.rand(N, generator=gen(1)) < 0.8
+    check(hidden, weight, tokens, bias=bias, mask=mask, wide=torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["some", "sequence", "first", "empty", "negative"])
+@pytest.mark.parametrize("B,T", [(3, 2), (5, 77)])
+def test_rows_that_do_not_count(dtype, kind, B, T):
+    """Masked rows and rows of a negative token may hold anything, are not read, and get zeros."""
+    dev = device()
+    N, D, V = B * T, 96, 333
+    hidden, weight, tokens, bias = head(N, D, V, dtype, 5)
+    hidden, tokens = hidden.view(B, T, D).clone(), tokens.view(B, T).clone()
+    mask = torch.ones(B, T, dtype=torch.bool)
+    if kind == "some":
+        mask = torch.rand(B, T, generator=gen(2)) < 0.5
+    elif kind == "sequence":
+        mask[0] = False
+    elif kind == "first":
+        mask[:] = False
+        mask[-1, -1] = True
+    elif kind == "empty":
+        mask[:] = False
+    else:
+        tokens[torch.rand(B, T, generator=gen(3)) < 0.4] = -100
+    live = mask & (tokens >= 0)
+    hidden[~live] = float("nan")
+    got = check(hidden, weight, tokens, bias=bias, mask=None if kind == "negative" else mask, what=kind)
+    assert not bool(got.logp.cpu()[~live].any()) and not bool(got.grad_hidden.cpu()[~live].any())
+    if kind == "empty":
+        assert float(got.loss) == 0.0 and not bool(got.grad_weight.any()) and not bool(got.grad_bias.any())
+    small = training.vocabulary_loss(hidden.to(dev), weight.to(dev), tokens.int().to(dev), bias=bias.to(dev),
+                                     mask=None if kind == "negative" else mask.to(dev))
+    for a, b in zip(small, got):
+        assert torch.equal(a, b), "32-bit tokens, other bits"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [6, 100])
+def test_views_are_read_in_place(dtype, N):
+    dev = device()
+    D, V = 72, 140
+    hidden, weight, tokens, bias = head(N, D, V, dtype, 8)
+    whole = torch.full((2, N // 2 + 1, D + 5), float("nan"), dtype=dtype)
+    whole[:, :-1, 3:-2] = hidden.view(2, N // 2, D)
+    table = torch.full((V + 2, D + 9), float("nan"), dtype=dtype)
+    table[1:-1, 7:-2] = weight
+    on = {"hidden": whole.to(dev)[:, :-1, 3:-2], "weight": table.to(dev)[1:-1, 7:-2]}
+    on["bias"] = torch.stack([bias, bias], 1).to(dev)[:, 0]
+    on["tokens"] = torch.stack([tokens, tokens]).t().contiguous().to(dev)[:, 0].view(2, N // 2)
+    check(hidden.view(2, N // 2, D), weight, tokens.view(2, N // 2), bias=bias, on=on, what="views")
+    wide = torch.zeros(V, 2 * 128, dtype=dtype)       # a weight that can be read as it lies, with gaps
+    wide[:, :64] = weight[:, :64]
+    check(hidden[:, :64], weight[:, :64], tokens, on={"weight": wide.to(dev)[:, :64]}, what="rows with gaps")
+    # one hidden row for all, by a stride of 0
+    same = hidden[:1].expand(N, D)
+    check(same, weight, tokens, on={"hidden": hidden[:1].to(dev).expand(N, D)}, what="a repeated row")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [5, 70])
+def test_masked_vocabulary(dtype, N):
+    """-inf and the type's lowest value in the bias take entries out: no probability, no gradient."""
+    hidden, weight, tokens, bias = head(N, 64, 300, dtype, 12)
+    bias[40:170] = float("-inf")
+    bias[200:] = torch.finfo(dtype).min
+    bias[41] = 0.25
+    tokens = torch.where((tokens >= 40) & (tokens < 170) | (tokens >= 200), 41, tokens)
+    got = check(hidden, weight, tokens, bias=bias, what="masked vocabulary")
+    assert not bool(got.grad_weight[42:170].any()) and not bool(got.grad_weight[200:].any())
+    assert not bool(got.grad_bias[42:170].any())
+    bias[:] = torch.finfo(torch.float32).min if dtype == torch.float32 else torch.finfo(dtype).min
+    if dtype != torch.float16:      # 65504 leaves fp32 logits their digits; these leave none, so all are alike
+        dev = device()
+        got = training.vocabulary_loss(hidden.to(dev), weight.to(dev), tokens.to(dev), bias=bias.to(dev))
+        close(got.logp, torch.full((N,), -math.log(300), dtype=torch.float64), 2.0 ** -20, "nothing but the lowest value")
+
+
+@pytest.mark.parametrize("N", [4, 40])
+def test_what_is_not_a_number_shows(N):
+    dev = device()
+    hidden, weight, tokens, bias = (t.to(dev) for t in head(N, 64, 40, torch.float32, 9))
+    late = tokens.clone()
+    late[1] = 40
+    got = training.vocabulary_loss(hidden, weight, late)
+    assert torch.isnan(got.logp[1]) and torch.isnan(got.loss) and torch.isnan(got.grad_hidden[1]).all()
+    assert int(torch.isnan(got.logp).sum()) == 1 and torch.isnan(got.grad_weight).all()
+    late = tokens.clone()
+    late[1] = 1 << 40
+    assert torch.isnan(training.vocabulary_loss(hidden, weight, late).logp[1])
+    for value in (float("nan"), float("inf")):
+        odd = hidden.clone()
+        odd[2, 5] = value
+        got = training.vocabulary_loss(odd, weight, tokens)
+        assert torch.isnan(got.logp[2]) and torch.isnan(got.loss) and torch.isnan(got.grad_hidden[2]).any()
+        assert int(torch.isnan(got.logp).sum()) == 1
+        odd = bias.clone()
+        odd[3] = value
+        got = training.vocabulary_loss(hidden, weight, tokens, bias=odd)
+        assert torch.isnan(got.logp).all()
+    got = training.vocabulary_loss(hidden, weight, tokens, bias=torch.full_like(bias, float("-inf")))
+    assert torch.isnan(got.logp).all()
+
+
+def test_no_rows():
+    dev = device()
+    weight, bias = torch.randn(9, 16, device=dev), torch.randn(9, device=dev)
+    for shape in ((0,), (0, 5), (3, 0)):
+        got = training.vocabulary_loss(torch.zeros(*shape, 16, device=dev), weight,
+                                       torch.zeros(shape, dtype=torch.int64, device=dev), bias=bias)
+        assert float(got.loss) == 0.0 and got.logp.shape == shape and got.grad_hidden.shape == (*shape, 16)
+        assert not bool(got.grad_weight.any()) and not bool(got.grad_bias.any())
+        assert float(training.vocabulary_loss(torch.zeros(*shape, 16, device=dev), weight, torch.zeros(
+            shape, dtype=torch.int64, device=dev), with_grad=False).loss) == 0.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,scale", [(5, 30.0), (90, 30.0)])
+def test_sure_and_far_logits(dtype, N, scale):
+    """Logits of hundreds: probabilities of 1 and of 0."""
+    hidden, weight, tokens, bias = head(N, 64, 500, dtype, 4)
+    check((hidden.float() * scale).to(dtype), weight, tokens, bias=bias, what="far logits")
+
+
+def test_gradients_against_differences():
+    """Along a direction the loss moves as the gradients say: central differences of the oracle-free fp32 loss, whose own
+    error is that of two losses over the step."""
+    dev = device()
+    hidden, weight, tokens, bias = (t.to(dev) for t in head(37, 96, 211, torch.float32, 3))
+    got = training.vocabulary_loss(hidden, weight, tokens, bias=bias, temperature=1.3)
+    loss = lambda h, w, b: float(training.vocabulary_loss(h, w, tokens, bias=b, temperature=1.3,  # noqa: E731
+                                                          with_grad=False).loss)
+    g = torch.Generator(device=dev).manual_seed(1)
+    step = 2.0 ** -6
+    for name, at, grad in (("hidden", 0, got.grad_hidden), ("weight", 1, got.grad_weight), ("bias", 2, got.grad_bias)):
+        d = torch.randn(grad.shape, device=dev, generator=g) * (0.3 if name == "weight" else 1.0)
+        moved = [[t + s * step * d if k == at else t for k, t in enumerate((hidden, weight, bias))] for s in (1, -1)]
+        slope = (loss(*moved[0]) - loss(*moved[1])) / (2 * step)
+        want = float((grad.double() * d.double()).sum())
+        # third derivatives of a mean log-softmax along d are below 2 |dz|^3, dz the logits' own change
+        if name == "hidden":
+            dz = float((d @ weight.t()).abs().max())
+        elif name == "weight":
+            dz = float((hidden @ d.t()).abs().max())
+        else:
+            dz = float(d.abs().max())
+        tol = step ** 2 / 6 * 2 * (2 * dz / 1.3) ** 3 + 2.0 ** -18 / step
+        announce(f"difference along {name}: {slope:.6f} against {want:.6f}, tolerance {tol:.2e}")
+        assert abs(slope - want) <= tol
+
+
+def test_pieces_of_the_vocabulary():
+    """More vocabulary than a piece holds: fp32 rows take 6 bytes of the softmax's gradient and of the packed weight each."""
+    dev = device()
+    N, D, V = 1024, 40, 170_001
+    hidden, weight, tokens, bias = head(N, D, V, torch.float32, 6)
+    mask = torch.rand(N, generator=gen(4)) < 0.6
+    got = training.vocabulary_loss(hidden.to(dev), weight.to(dev), tokens.to(dev), bias=bias.to(dev), mask=mask.to(dev))
+    at = mask.nonzero()[:, 0]
+    n = at.numel()
+    x, w = hidden[at].double().to(dev), weight.double().to(dev)
+    q = torch.log_softmax(torch.mm(x, w.t()) + bias.double().to(dev), 1)
+    rows, y = torch.arange(n, device=dev), tokens[at].to(dev)
+    logp = q[rows, y]
+    g = q.exp_()
+    g[rows, y] -= 1.0
+    size = float(torch.mm(x.abs()[:64], w.abs().t()).max() * 1.5)
+    rel = 2 * ((6 * D + 8) * 2.0 ** -24 + 2.0 ** -22) * size + 2.0 ** -22 * 40 + (V / 256 + 64) * 2.0 ** -24
+    close(got.logp.cpu()[at], logp.cpu(), rel, "logp of pieces")
+    for name, have, want, bound in (
+            ("hidden", got.grad_hidden[at.to(dev)], torch.mm(g, w) / n, torch.mm(g.abs(), w.abs()) / n),
+            ("weight", got.grad_weight, torch.mm(g.t(), x) / n, torch.mm(g.abs().t(), x.abs()) / n),
+            ("bias", got.grad_bias, g.sum(0) / n, g.abs().sum(0) / n)):
+        # sums of up to V terms in fp32: 512 part sums of at most 6 * 512 terms each would be their worst order; 2^-15 holds
+        # (6 V 2^-24 = 2^-4 is the bound of one sum, which the random signs of its roundings stay far below)
+        close(have.cpu(), want.cpu(), (rel + 2.0 ** -15) * bound.cpu() + rounded(want.cpu(), torch.float32), f"grad {name}")
+    assert not bool(got.grad_hidden.cpu()[~mask].any())
+
+
+def test_refusals():
+    dev = device()
+    hidden, weight, tokens, bias = (t.to(dev) for t in head(6, 8, 10, torch.bfloat16, 1))
+    call = training.vocabulary_loss
+    for error, match, args, kw in (
+            (HipError, "weight must be", (hidden, weight.float(), tokens), {}),
+            (ValueError, "weight must be", (hidden, weight[:, :7], tokens), {}),
+            (ValueError, "V >= 1", (hidden, weight[:0], tokens), {}),
+            (HipError, "contiguous rows", (hidden, weight.t().contiguous().t(), tokens), {}),
+            (HipError, "contiguous rows", (hidden, weight[:1].expand(10, 8), tokens), {}),
+            (HipError, "contiguous last axis", (hidden.t().contiguous().t(), weight, tokens), {}),
+            (ValueError, "hidden must be", (hidden[0], weight, tokens[0]), {}),
+            (ValueError, "tokens of shape", (hidden, weight, tokens[:5]), {}),
+            (HipError, "tokens must be", (hidden, weight, tokens.float()), {}),
+            (HipError, "bias must be", (hidden, weight, tokens), {"bias": bias.float()}),
+            (ValueError, "bias of shape", (hidden, weight, tokens), {"bias": bias[:9]}),
+            (HipError, "mask must be", (hidden, weight, tokens), {"mask": tokens}),
+            (ValueError, "mask of shape", (hidden, weight, tokens), {"mask": tokens[:5] > 0}),
+            (ValueError, "temperature", (hidden, weight, tokens), {"temperature": 0.0}),
+            (ValueError, "weight_grad_dtype", (hidden, weight, tokens), {"weight_grad_dtype": torch.float16}),
+            (HipError, "device tensor", (hidden, weight.cpu(), tokens), {}),
+            (HipError, "must be float32", (hidden.double(), weight, tokens), {})):
+        with pytest.raises(error, match=match):
+            call(*args, **kw)
+
+
+# ---------------------------------------------------------------------------
+# dropout
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1,), (), (7,), (8,), (3, 5), (33, 8), (5, 129), (2, 3, 50), (64, 160)])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout(dtype, shape, p):
+    dev = device()
+    g = gen(len(shape) + 3)
+    x, r = torch.randn(shape, generator=g).to(dtype), torch.randn(shape, generator=g).to(dtype)
+    seed, counter = 0xFEDCBA9876543210, (3 << 33) + 5
+    want, kept = ref.dropout(x, p, seed, counter)
+    got = training.dropout(x.to(dev), p, seed=seed, counter=counter)
+    assert got.dtype == dtype and got.shape == x.shape
+    close(got, want, rounded(want, dtype), f"dropout {shape} {p}")
+    assert torch.equal(got.cpu() != 0, kept & (x != 0))
+    assert torch.equal(training.dropout_grad(x.to(dev), p, seed=seed, counter=counter), got)
+    on_device = torch.tensor(counter, device=dev)
+    assert torch.equal(training.dropout(x.to(dev), p, seed=seed, counter=on_device), got)
+    want, _ = ref.dropout(x, p, seed, counter, residual=r)
+    both = training.dropout(x.to(dev), p, seed=seed, counter=counter, residual=r.to(dev))
+    # the sum's rounding in fp32, before that to the type, is of a term that may be larger than the sum
+    close(both, want, rounded(want, dtype) + 2.0 ** -22 * (x.abs().double() / max(1 - p, 0.5) + r.abs().double()),
+          f"dropout and residual {shape} {p}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dropout_of_views(dtype):
+    """The mask follows an element's place in x, not in memory."""
+    dev = device()
+    whole = torch.randn(20, 41, generator=gen(2)).to(dtype).to(dev)
+    kw = dict(seed=5, counter=1)
+    for view in (whole[:, :40], whole[:, 3:], whole[::2], whole.t(), whole[:, ::3], whole[4], whole[:, 7],
+                 whole[:1].expand(9, 41), whole.view(4, 5, 41)[:, 1:, 2:]):
+        want = training.dropout(view.contiguous(), 0.3, **kw)
+        assert torch.equal(training.dropout(view, 0.3, **kw), want)
+        assert torch.equal(training.dropout(view.contiguous(), 0.3, residual=view, **kw),
+                           training.dropout(view, 0.3, residual=view.contiguous(), **kw))
+    assert torch.equal(training.dropout(whole[:0], 0.3, **kw), whole[:0])
+
+
+def test_masks_of_counters_and_seeds():
+    """Shares of kept elements within six standard deviations, of one mask and of both of two."""
+    dev = device()
+    n = 1 << 20
+    x = torch.ones(n, device=dev)
+    masks = [training.dropout(x, 0.25, seed=s, counter=c) != 0 for s, c in ((1, 0), (1, 1), (2, 0), (1, 1 << 32),
+                                                                        (1 << 32, 0))]
+    for i, a in enumerate(masks):
+        share = float(a.float().mean())
+        assert abs(share - 0.75) < 6 * math.sqrt(0.75 * 0.25 / n), share
+        assert abs(float((a[1:] & a[:-1]).float().mean()) - 0.75 ** 2) < 6 * math.sqrt(0.25 / n)
+        for b in masks[:i]:
+            assert abs(float((a & b).float().mean()) - 0.75 ** 2) < 6 * math.sqrt(0.25 / n)
+
+
+def test_dropped_places_may_hold_anything():
+    dev = device()
+    x = torch.randn(4096, generator=gen(3)).to(dev)
+    kept = training.dropout(torch.ones_like(x), 0.5, seed=9) != 0
+    odd = torch.where(kept, x, torch.tensor([float("nan"), float("inf")], device=dev).repeat(2048))
+    assert torch.equal(training.dropout(odd, 0.5, seed=9), training.dropout(x, 0.5, seed=9))
+    assert torch.equal(training.dropout(odd, 1.0, seed=9), torch.zeros_like(x))
+
+
+def test_dropout_of_a_large_tensor():
+    """Past 2^32 elements: the last ones against the oracle."""
+    dev = device()
+    n = (1 << 32) + 1000 * 8 + 3
+    x = torch.ones(n, device=dev, dtype=torch.bfloat16)
+    got = training.dropout(x, 0.5, seed=11, counter=2)
+    for first in (0, (1 << 31) - 64, (1 << 32) - 64, (1 << 32) + 7936):
+        part = got[first:first + 256].cpu()
+        want, _ = ref.dropout(torch.ones(part.numel()), 0.5, 11, 2, first=first)
+        assert torch.equal(part.double(), want), first
+
+
+def test_dropout_refusals():
+    dev = device()
+    x = torch.ones(4, 6, device=dev)
+    for error, match, args, kw in (
+            (ValueError, "p must be", (x, 1.5), {"seed": 1}), (ValueError, "p must be", (x, float("nan")), {"seed": 1}),
+            (ValueError, "seed must be", (x, 0.5), {"seed": -1}), (ValueError, "seed must be", (x, 0.5), {"seed": 1 << 64}),
+            (ValueError, "counter must be", (x, 0.5), {"seed": 1, "counter": -1}),
+            (HipError, "counter must be", (x, 0.5), {"seed": 1, "counter": torch.ones(1, device=dev)}),
+            (HipError, "device tensor", (x, 0.5), {"seed": 1, "counter": torch.ones(1, dtype=torch.int64)}),
+            (ValueError, "residual must be", (x, 0.5), {"seed": 1, "residual": x.half()}),
+            (ValueError, "residual must be", (x, 0.5), {"seed": 1, "residual": x[:3]}),
+            (HipError, "dropout_grad", (x.clone().requires_grad_(True), 0.5), {"seed": 1}),
+            (HipError, "residual requires grad", (x, 0.5), {"seed": 1, "residual": x.clone().requires_grad_(True)}),
+            (HipError, "must be float32", (x.double(), 0.5), {"seed": 1})):
+        with pytest.raises(error, match=match):
+            training.dropout(*args, **kw)
+
+
+# ---------------------------------------------------------------------------
+# streams, graphs, both together
+
+def test_on_another_stream_and_in_a_graph():
+    """A captured step, replayed with other tokens and a raised counter, between eager work: every replay as the eager
+    call."""
+    dev = device()
+    hidden, weight, tokens, bias = (t.to(dev) for t in head(150, 128, 700, torch.bfloat16, 2))
+    counter = torch.zeros((), dtype=torch.int64, device=dev)
+
+    def step():
+        x = training.dropout(hidden, 0.2, seed=3, counter=counter)
+        r = training.vocabulary_loss(x, weight, tokens, bias=bias)
+        return [*r, training.dropout_grad(r.grad_hidden, 0.2, seed=3, counter=counter)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(there, step()):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    seen = []
+    for turn in range(4):
+        counter.fill_(turn)
+        tokens.copy_(torch.randint(-1, 700, (150,), generator=gen(turn)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for a, b in zip(captured, want):
+            assert torch.equal(a, b), turn
+        seen.append(captured[2].clone())
+    assert not torch.equal(seen[0], seen[1])
+
+
+def test_scores_feed_the_other_losses():
+    """log-probabilities without gradients are those that the losses on logits compute."""
+    dev = device()
+    hidden, weight, tokens, bias = (t.to(dev) for t in head(44, 128, 301, torch.float32, 7))
+    scored = training.vocabulary_loss(hidden, weight, tokens, bias=bias, with_grad=False).logp
+    logits = torch.addmm(bias, hidden, weight.t())
+    offsets = torch.tensor([0, 9, 20, 33, 44], device=dev)
+    r = training.preference_loss(logits, tokens, scored, offsets)
+    tol = (2 * 128 * 2.0 ** -24 * float((hidden.abs() @ weight.abs().t()).max() + 3) * 2 + 2.0 ** -17)
+    assert float((r.logp - scored).abs().max()) < tol
+    assert abs(float(r.loss) - math.log(2)) < 0.1 * 24 * tol

@@ -1,0 +1,84 @@
+"""Host side of the operators of a supervised step: what the C entry points refuse before any launch, what their
+workspaces hold, and the generator of the dropout masks as the oracle states it.  No device call is made."""
+
+import pytest
+import torch
+
+from boundflow_amd import _lib, training
+from boundflow_amd._lib import HipError
+from oracle import training_ref as ref
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built (run python -m boundflow_amd.build)")
+    return _lib.load()
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(HipError, match="device tensor"):
+        training.vocabulary_loss(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(HipError, match="device tensor"):
+        training.dropout(torch.zeros(3), 0.5, seed=1)
+
+
+def test_philox_known_answers():
+    """The published test vectors of Philox 4x32 of ten rounds: counters and keys of zeros, of ones and of pi's digits."""
+    def words(counter, key):
+        u = ref.philox(counter[0] | counter[1] << 32, counter[2] | counter[3] << 32, key[0] | key[1] << 32)
+        return [u[2 * k] | u[2 * k + 1] << 16 for k in range(4)]
+
+    ones = 0xFFFFFFFF
+    assert words([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert words([ones] * 4, [ones] * 2) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+    assert words([0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344], [0xA4093822, 0x299F31D0]) == \
+        [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
+
+
+def test_entry_points_refuse_bad_arguments(lib):
+    some = torch.zeros(64)
+    p = some.data_ptr()
+    assert p % 16 == 0
+    loss = lambda **k: lib.bf_vocab_loss(*{**dict(  # noqa: E731
+        hidden=p, elem=0, B=1, T=2, D=4, ld_b=8, ld_t=4, weight=p, V=3, ld_w=4, bias=p, tokens=p, token_bytes=8, mask=None,
+        temperature=1.0, scale=1.0, logp=p, loss=p, dh=p, dw=p, dw_elem=0, db=p, space=p, stream=None), **k}.values())
+    for bad in (dict(elem=5), dict(V=0), dict(D=0), dict(temperature=0.0), dict(temperature=float("nan")), dict(loss=None),
+                dict(token_bytes=1), dict(ld_t=-1), dict(ld_w=3), dict(weight=None), dict(hidden=None), dict(tokens=None),
+                dict(logp=None), dict(space=None), dict(space=p + 4), dict(dw=None), dict(dh=None), dict(db=None),
+                dict(bias=None), dict(dw_elem=1), dict(B=-1)):
+        assert loss(**bad) == 1, bad
+    for far in (dict(T=1 << 24), dict(B=1 << 40, T=1 << 40), dict(V=1 << 31), dict(ld_w=1 << 21),
+                dict(D=1 << 21, ld_w=1 << 21), dict(T=(1 << 23) - 1, V=1 << 29)):
+        assert loss(**far) == 3, far
+    drop = lambda **k: lib.bf_dropout(*{**dict(  # noqa: E731
+        x=p, ld=4, residual=None, r_ld=0, elem=0, rows=2, dim=4, p=0.5, seed=1, counter=0, counter_dev=None, out=p,
+        stream=None), **k}.values())
+    for bad in (dict(elem=3), dict(p=1.5), dict(p=float("nan")), dict(x=None), dict(out=None), dict(rows=-1), dict(ld=3),
+                dict(residual=p, r_ld=3)):
+        assert drop(**bad) == 1, bad
+    assert drop(rows=0) == 0 and drop(dim=0, ld=0) == 0
+    assert drop(rows=1 << 41, dim=8, ld=8) == 3
+
+
+def test_workspaces_hold_what_their_kernels_write(lib):
+    size = lib.bf_vocab_loss_workspace
+    for N, D, V, elem in ((1, 1, 1, 0), (8, 2048, 32000, 1), (1003, 1025, 50001, 2), (2048, 1024, 32000, 0),
+                          (8184, 4096, 128000, 1)):
+        some = 1 << 20        # an address that can be read as it lies
+        alone, grad = size(N, D, V, elem, some, D, 0), size(N, D, V, elem, some, D, 1)
+        assert 0 < alone < grad
+        # a token, a place and statistics per row and tile of the vocabulary; the packed rows
+        parts = 3 if elem == 0 else 1
+        assert 4 * alone >= 8 * N + 2 * parts * N * D
+        # G and the sums of the hidden rows' gradient stay bounded: the logits would be 4 N V
+        assert 4 * (grad - alone) <= (540 << 20) + 16 * 4 * (N + 64) * (D + 64)
+    assert size(0, 4, 4, 0, 0, 4, 1) == 0 and size(4, 4, 4, 7, 0, 4, 1) == 0 and size(1 << 24, 4, 4, 0, 0, 4, 1) == 0
+    # a weight that has to be packed takes more
+    assert size(100, 64, 1000, 1, 1 << 20, 64, 0) < size(100, 64, 1000, 1, (1 << 20) + 2, 64, 0)
+
+
+def test_requires_grad_is_refused_before_the_device_is_asked():
+    x = torch.zeros(3, requires_grad=True)
+    with pytest.raises(HipError, match="dropout_grad"):
+        training.dropout(x, 0.5, seed=1)
