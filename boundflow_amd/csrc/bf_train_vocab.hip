@@ -5,10 +5,11 @@
 //   G_nv   = exp(z_nv / t) / sum - [v = y_n],      s = grad_scale / (t rows)
 //   dx_n   = s sum_v G_nv w_v,   dw_v = s sum_n G_nv x_n,   db_v = s sum_n G_nv
 //
-// The logits are never kept.  A first pass forms them tile by tile and leaves each row's largest logit M and
-// sum of 2^(c (z - M)) per tile, c = log2(e) / t; a second one forms them again, a piece of the vocabulary at a
-// time, and leaves the piece's G in the type of the matrix products (fp32: in three parts), from which
-// the piece's dw and its share of dx are made.
+// The logits are never stored.  A first pass over the vocabulary (vocab_logits_kernel) leaves each row's largest logit and
+// sum of exponentials per tile, and of as much of the vocabulary as the workspace has room for the exponentials in the type
+// of the matrix products (fp32: in three parts).  vocab_softmax_kernel joins the tiles' statistics and makes those exponentials
+// G; dx and dw follow from it (vocab_grads_kernel).  For what has no room, the logits are formed again, a
+// piece at a time, with the statistics known.
 //
 // Rows that count (not masked, token not negative) are gathered first, in their order, and only they are multiplied.
 // Every sum is in fp32 and in a fixed order.
@@ -16,9 +17,6 @@
 #include "bf_vocab_gemm.h"
 
 namespace bf {
-
-typedef VocabTile<4, 2, 2, 4> VocabLarge;
-typedef VocabTile<2, 2, 2, 2> VocabMid;
 
 // ---------------------------------------------------------------------------
 // Rows that count
@@ -101,99 +99,223 @@ __device__ __forceinline__ void pack_chunk(const Pack<T, 8>& x, E* at, int64_t p
   }
 }
 
-// The hidden rows that count, dense and padded with zeros to Dp columns and a multiple of 64 rows (fp32: in parts).
-template <class T, class E>
-__global__ void __launch_bounds__(256) vocab_pack_rows_kernel(const T* __restrict__ hidden, int64_t ld_b, int64_t ld_t,
-                                                              int length, const int* __restrict__ source,
-                                                              const int* __restrict__ live, int D, int Dp,
-                                                              E* __restrict__ out, int64_t part) {
-  const int n = blockIdx.x, rows = *live;
-  if (n >= (rows + 63) / 64 * 64) return;
-  const bool counts = n < rows;
-  const int from = counts ? source[n] : 0;
-  const T* row = hidden + (from / length) * ld_b + (from % length) * ld_t;
-  for (int d = 8 * threadIdx.x; d < Dp; d += 8 * 256)
-    pack_chunk<T, E>(row_chunk(row, d, counts ? D : 0), out + (int64_t)n * Dp + d, part);
-}
+// What the products read, and what rows that do not count get.  Workgroups [0, N): hidden row n to its place among
+// the rows that count, dense and padded with zeros to Dp columns (fp32: in parts), or zeros to its gradient.  [N, N + 64): zeros
+// behind the last row up to a multiple of 64.  The others: rows of a weight that cannot be read as it
+// lies, padded and split alike.  Up to VOCAB_SCAN rows each workgroup counts for itself which rows count, which saves a launch.
+constexpr int VOCAB_SCAN = 1024;
 
-// Rows of a weight that cannot be read as they lie, padded with zeros to Dp columns (fp32: in parts).
-template <class T, class E>
-__global__ void __launch_bounds__(256) vocab_pack_weight_kernel(const T* __restrict__ weight, int64_t ld, int D, int Dp,
-                                                                E* __restrict__ out, int64_t part) {
-  const int64_t v = blockIdx.x;
-  for (int d = 8 * threadIdx.x; d < Dp; d += 8 * 256)
-    pack_chunk<T, E>(row_chunk(weight + v * ld, d, D), out + v * Dp + d, part);
-}
+struct VocabPrepare {
+  const void* hidden;
+  int64_t ld_b, ld_t;
+  int length;
+  const void* tokens;
+  int token_bytes;
+  const uint8_t* mask;
+  int N, D, Dp;
+  int* live;
+  int* source;
+  int* place;
+  int* token;
+  float* logp;
+  void* x;
+  int64_t x_part;
+  void* grad_hidden;        // or null
+  const void* weight;       // rows to be packed, or null
+  int64_t ld_w, weight_rows;
+  void* w;
+  int64_t w_part;
+};
 
-// A row's statistics from those of its tiles, its token's log-probability.  64 rows a workgroup, the tiles over 16 waves.
-__global__ void __launch_bounds__(1024) vocab_rows_stats_kernel(const float2* __restrict__ part, int64_t part_ld, int tiles,
-                                                                const float* __restrict__ chosen,
-                                                                const int* __restrict__ token,
-                                                                const int* __restrict__ source,
-                                                                const int* __restrict__ live, int vocab, float c,
-                                                                float inv_t, float2* __restrict__ row,
-                                                                float* __restrict__ logp) {
-  __shared__ float2 red[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = blockIdx.x * 64 + lane, rows = *live;
-  if ((int)blockIdx.x * 64 >= rows) return;
-  float top = -INFINITY, sum = 0.f;
-  auto join = [&](float2 x) {
-    const float held = fmaxf(top, x.x) == -INFINITY ? 0.f : fmaxf(top, x.x);
-    // a share without a logit above -inf has sum 0, or NaN
-    sum = sum * (top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - held) * c)) +
-          x.y * (x.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x.x - held) * c));
-    top = fmaxf(top, x.x);
-  };
-  if (n < rows)
-    for (int k = wave; k < tiles; k += 16) join(part[k * part_ld + n]);
-  red[wave][lane] = make_float2(top, sum);
-  __syncthreads();
-  if (wave || n >= rows) return;
-  for (int w = 1; w < 16; ++w) join(red[w][lane]);
-  float lp = (chosen[n] - top) * inv_t - logf(sum);
-  float inv = 1.f / sum;
-  if (token[n] >= vocab) lp = inv = __int_as_float(0x7fc00000);   // a token past the vocabulary shows as NaN
-  row[n] = make_float2(top, inv);
-  logp[source[n]] = lp;
-}
-
-// The loss, by one workgroup; and where there is a gradient of the hidden rows, that: the pieces' sums joined, scaled
-// and brought back to their rows, zeros in rows that do not count (workgroup 1 + n does row n).
-template <class T>
-__global__ void __launch_bounds__(256) vocab_finish_kernel(const float* __restrict__ logp, int N,
-                                                           const int* __restrict__ live, const int* __restrict__ place,
-                                                           const float* __restrict__ dx, int64_t dx_split, int64_t dx_ld,
-                                                           int splits, int D, float scale, float* __restrict__ loss,
-                                                           T* __restrict__ grad) {
-  const int rows = max(*live, 1);
-  if (blockIdx.x == 0) {
-    __shared__ float red[4];
-    float sum = 0.f;
-    for (int n = threadIdx.x; n < N; n += 256) sum += logp[n];
-    sum = block_sum<4>(sum, red);
-    if (threadIdx.x == 0) *loss = *live ? -sum / (float)rows : 0.f;
+template <class T, class E, bool SCAN>
+__global__ void __launch_bounds__(256) vocab_prepare_kernel(VocabPrepare p) {
+  const int t = threadIdx.x;
+  if ((int64_t)blockIdx.x >= p.N + 64) {
+    const int64_t at = ((int64_t)blockIdx.x - p.N - 64) * 256 + t;
+    const int chunks = p.Dp / 8;
+    const int64_t v = div_rows(at, chunks, at < (1LL << 31));
+    if (v >= p.weight_rows) return;
+    const int d = 8 * (int)(at - v * chunks);
+    pack_chunk<T, E>(row_chunk((const T*)p.weight + v * p.ld_w, d, p.D), (E*)p.w + v * p.Dp + d, p.w_part);
     return;
   }
-  const int64_t n = blockIdx.x - 1;
-  const int at = place[n];
-  T* out = grad + n * D;
-  const float factor = scale / (float)rows;
-  for (int d = 8 * threadIdx.x; d < D; d += 8 * 256) {
-    Pack<T, 8> y;
-    if (at < 0) {
+  const int n = blockIdx.x;
+  int live, at = -1;
+  if constexpr (SCAN) {
+    __shared__ int sums[4][2];
+    int before = 0, all = 0, mine = -1;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y.v[k] = (T)0.f;
-    } else {
-      float x[8] = {};
-      for (int s = 0; s < splits; ++s) {
-        const Pack<float, 8> more = load_pack<float, 8>(dx + s * dx_split + at * dx_ld + d);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] += more.v[k];
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y.v[k] = (T)(x[k] * factor);
+    for (int k = 0; k < VOCAB_SCAN / 256; ++k) {
+      const int i = 256 * k + t;
+      const int tok = i < p.N && (!p.mask || p.mask[i]) ? load_token(p.tokens, p.token_bytes, i) : -1;
+      before += __popcll(__ballot(tok >= 0 && i < n));
+      all += __popcll(__ballot(tok >= 0));
+      if (i == n) mine = tok;
     }
+    __shared__ int own;
+    if ((t & 63) == 0) {
+      sums[t >> 6][0] = before;
+      sums[t >> 6][1] = all;
+    }
+    if (t == (n & 255)) own = mine;
+    __syncthreads();
+    before = sums[0][0] + sums[1][0] + sums[2][0] + sums[3][0];
+    live = sums[0][1] + sums[1][1] + sums[2][1] + sums[3][1];
+    if (n < p.N && own >= 0) at = before;
+    if (t == 0) {
+      if (n == 0) *p.live = live;
+      if (n < p.N) p.place[n] = at;
+      if (at >= 0) {
+        p.source[at] = n;
+        p.token[at] = own;
+      } else if (n < p.N) {
+        p.logp[n] = 0.f;
+      }
+    }
+  } else {
+    live = *p.live;
+    if (n < p.N) at = p.place[n];
+  }
+  E* x = (E*)p.x;
+  if (n >= p.N) {      // behind the last row that counts
+    at = live + n - p.N;
+    if (at >= (live + 63) / 64 * 64) return;
+    for (int d = 8 * t; d < p.Dp; d += 8 * 256)
+      pack_chunk<T, E>(row_chunk((const T*)nullptr, d, 0), x + (int64_t)at * p.Dp + d, p.x_part);
+  } else if (at >= 0) {
+    const T* row = (const T*)p.hidden + (int64_t)(n / p.length) * p.ld_b + (int64_t)(n % p.length) * p.ld_t;
+    for (int d = 8 * t; d < p.Dp; d += 8 * 256)
+      pack_chunk<T, E>(row_chunk(row, d, p.D), x + (int64_t)at * p.Dp + d, p.x_part);
+  } else if (p.grad_hidden) {
+    T* row = (T*)p.grad_hidden + (int64_t)n * p.D;
+    for (int d = t; d < p.D; d += 256) row[d] = (T)0.f;
+  }
+}
+
+// Rows of a weight alone, for a later piece of the vocabulary.
+template <class T, class E>
+__global__ void __launch_bounds__(256) vocab_pack_weight_kernel(const T* __restrict__ weight, int64_t ld, int64_t rows, int D,
+                                                                int Dp, E* __restrict__ out, int64_t part) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int chunks = Dp / 8;
+  const int64_t v = div_rows(at, chunks, at < (1LL << 31));
+  if (v >= rows) return;
+  const int d = 8 * (int)(at - v * chunks);
+  pack_chunk<T, E>(row_chunk(weight + v * ld, d, D), out + v * Dp + d, part);
+}
+
+// Statistics of the rows that count, from those of their tiles, and G from the exponentials that the first pass left, in
+// place.  A workgroup joins a row's tiles and takes VOCAB_CHUNK of its entries; the first one of a row writes what others
+// read.  The token's entry comes from its log-probability: p - 1 from a rounded p would have no digits left where p is near 1.
+// The others are rounded a second time here (half a step of their type).
+constexpr int VOCAB_CHUNK = 8192;
+
+struct VocabSoftmax {
+  const float2* part;
+  int64_t part_ld;
+  int tiles, tile;            // their number, and the entries of one
+  const float* chosen;
+  const int* token;
+  const int* source;
+  const int* live;
+  int vocab;
+  float c, inv_t;
+  float2* row;
+  float* logp;
+  void* G;                    // or null
+  int64_t ldg, g_part;
+  int held;                   // entries of G
+  int chunks;                 // workgroups of a row
+};
+
+template <class E, bool PARTS>
+__global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
+  const int n = blockIdx.x / p.chunks, chunk = blockIdx.x - n * p.chunks;
+  if (n >= *p.live) return;
+  __shared__ float red[8];
+  const int t = threadIdx.x, wave = t >> 6;
+  const float2* part = p.part + n * p.part_ld;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int k = t; k < p.tiles; k += 256) top = fmaxf(top, part[k].x);
+  top = wave_max(top);
+  if ((t & 63) == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float sum = 0.f;
+#pragma unroll 4
+  for (int k = t; k < p.tiles; k += 256) {
+    const float2 x = part[k];
+    // a tile without a logit above -inf has sum 0, or NaN
+    sum += x.x == -INFINITY ? x.y : x.y * __builtin_amdgcn_exp2f((x.x - top) * p.c);
+  }
+  sum = block_sum<4>(sum, red + 4);
+  const int token = p.token[n];
+  float lp = (p.chosen[n] - top) * p.inv_t - logf(sum);
+  float inv = 1.f / sum;
+  if (token >= p.vocab) lp = inv = __int_as_float(0x7fc00000);   // a token past the vocabulary shows as NaN
+  if (chunk == 0 && t == 0) {
+    p.row[n] = make_float2(top, inv);
+    p.logp[p.source[n]] = lp;
+  }
+  if (!p.G) return;
+  constexpr float SCALE = __is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f;
+  const float at_token = (expf(lp) - 1.f) * SCALE;
+  E* g = (E*)p.G + n * p.ldg;
+#pragma unroll
+  for (int k = 0; k < VOCAB_CHUNK / 2048; ++k) {
+    const int v = chunk * VOCAB_CHUNK + 2048 * k + 8 * t;
+    if (v >= p.held) break;
+    const float factor = __builtin_amdgcn_exp2f((part[v / p.tile].x - top) * p.c) * inv;
+    Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
+#pragma unroll
+    for (int q = 0; q < (PARTS ? VOCAB_PARTS : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part + v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float y = (float)x[0].v[e];
+      if constexpr (PARTS) y = ((float)x[2].v[e] + (float)x[1].v[e]) + y;
+      y = v + e == token ? at_token : y * factor;
+      if constexpr (PARTS) {
+        __bf16 parts[VOCAB_PARTS];
+        split_parts(y, parts);
+#pragma unroll
+        for (int q = 0; q < VOCAB_PARTS; ++q) x[q].v[e] = parts[q];
+      } else {
+        x[0].v[e] = (E)y;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < (PARTS ? VOCAB_PARTS : 1); ++q) store_pack(g + q * p.g_part + v, x[q]);
+  }
+}
+
+// The loss alone.
+__global__ void __launch_bounds__(256) vocab_loss_kernel(const float* __restrict__ logp, int N, const int* __restrict__ live,
+                                                          float* __restrict__ loss) {
+  __shared__ float red[4];
+  vocab_loss<4>(logp, N, *live, loss, red);
+}
+
+// The hidden rows' gradient where it was summed in pieces: joined, scaled and brought back to the rows that count.
+template <class T>
+__global__ void __launch_bounds__(256) vocab_join_kernel(const int* __restrict__ live, const int* __restrict__ place,
+                                                         const float* __restrict__ dx, int64_t dx_split, int64_t dx_ld,
+                                                         int splits, int D, float scale, T* __restrict__ grad) {
+  const int at = place[blockIdx.x];
+  if (at < 0) return;
+  T* out = grad + (int64_t)blockIdx.x * D;
+  const float factor = scale / (float)*live;
+  for (int d = 8 * threadIdx.x; d < D; d += 8 * 256) {
+    float x[8] = {};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const Pack<float, 8> more = load_pack<float, 8>(dx + s * dx_split + at * dx_ld + d);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] += more.v[k];
+    }
+    Pack<T, 8> y;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y.v[k] = (T)(x[k] * factor);
     if (d + 8 <= D) {
       store_pack(out + d, y);
     } else {
@@ -221,10 +343,11 @@ struct VocabPlan {
   int elem, parts;
   bool direct, grad;
   int64_t rows, Dp;          // padded
-  int64_t piece;             // vocabulary of a piece
-  int64_t first;             // vocabulary of a launch of the first pass
-  int64_t stats_tiles;       // tiles of the vocabulary in the first pass
-  int splits;
+  int64_t piece;             // vocabulary of a piece: what G and the packed weight have room for
+  int64_t tiles;             // of the vocabulary in the first pass
+  int logits_tile, grads_tile;
+  int splits;                // of the hidden rows' gradient
+  bool joined;               // it is summed in pieces first
   // bytes from the workspace's start
   int64_t live, source, place, token, chosen, row, part, x, w, g, dx, bytes;
 };
@@ -233,9 +356,16 @@ inline bool vocab_direct(int elem, int64_t D, const void* weight, int64_t ld) {
   return elem != TE_F32 && D % 64 == 0 && ld % 8 == 0 && (uintptr_t)weight % 16 == 0;
 }
 
-constexpr int64_t VOCAB_PIECE_BYTES = 512LL << 20;   // of a piece's G and packed weight
+inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n) {
+  switch (tile) {
+    case VT_LARGE: return ceil_div(m, VocabLarge::BM) * ceil_div(n, VocabLarge::BN);
+    case VT_SLIM: return ceil_div(m, VocabSlim::BM) * ceil_div(n, VocabSlim::BN);
+    default: return ceil_div(m, VocabMid::BM) * ceil_div(n, VocabMid::BN);
+  }
+}
 
-inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld, bool grad) {
+inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld, bool grad,
+                            int64_t room) {
   VocabPlan p;
   p.N = N;
   p.D = D;
@@ -250,16 +380,38 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   const int64_t whole = ceil_div(V, 256) * 256;
   p.piece = whole;
   if (per_token > 0) {
-    p.piece = VOCAB_PIECE_BYTES / per_token / 256 * 256;
+    p.piece = room / per_token / 256 * 256;
     if (p.piece < 256) p.piece = 256;
     if (p.piece > whole) p.piece = whole;
   }
-  p.first = p.direct ? whole : p.piece;
-  p.stats_tiles = ceil_div(V, 128);
+  const int64_t in_piece = p.piece < V ? p.piece : V;
+  // by the whole vocabulary, so that the statistics have the same bits with and without gradients and whatever the room
+  if (N <= VocabSlim::BN) p.logits_tile = VT_SLIM;
+  else if (vocab_tile_count(VT_LARGE, V, N) >= 200) p.logits_tile = VT_LARGE;
+  else p.logits_tile = vocab_tile_count(VT_MID, V, N) > 256 ? VT_MID : VT_DEEP;
+  p.tiles = vocab_tile_count(p.logits_tile, V, 1);
+  p.grads_tile = VT_SLIM;
   p.splits = 1;
+  p.joined = false;
   if (grad) {
-    const int64_t tiles = ceil_div(N, VocabMid::BN) * ceil_div(D, VocabMid::BM);
-    while (p.splits < 16 && tiles * p.splits < 256 && p.splits * 8 * 64 < p.piece) p.splits *= 2;
+    if (N > VocabSlim::BN) {
+      const int64_t large = vocab_tile_count(VT_LARGE, D, N) + vocab_tile_count(VT_LARGE, D, in_piece);
+      const int64_t mid = vocab_tile_count(VT_MID, D, N) + vocab_tile_count(VT_MID, D, in_piece);
+      p.grads_tile = large >= 200 ? VT_LARGE : mid > 256 ? VT_MID : VT_DEEP;
+    }
+    // dx's sums over the vocabulary are cut so that none of them takes longer than a good part of the whole launch
+    const int64_t slots = p.grads_tile == VT_LARGE || p.grads_tile == VT_DEEP ? 256 : 512;
+    const int64_t dx = vocab_tile_count(p.grads_tile, D, N), dw = vocab_tile_count(p.grads_tile, D, in_piece);
+    const int64_t dx_steps = ceil_div(in_piece, 64), dw_steps = ceil_div(N, 64) + 4;
+    int64_t most = (dx * dx_steps + dw * dw_steps) / slots / 3;
+    if (most < 8) most = 8;
+    int64_t splits = ceil_div(dx_steps, most);
+    const int64_t fits = (128LL << 20) / (4 * p.rows * p.Dp);
+    if (splits > fits) splits = fits;
+    if (splits > 32) splits = 32;
+    if (splits < 1) splits = 1;
+    p.splits = (int)splits;
+    p.joined = splits > 1 || p.piece < V;
   }
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -273,23 +425,13 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.token = take(4 * N);
   p.chosen = take(4 * N);
   p.row = take(8 * N);
-  p.part = take(8 * p.stats_tiles * N);
+  p.part = take(8 * p.tiles * N);
   p.x = take(2 * p.parts * p.rows * p.Dp);
   p.w = take(p.direct ? 0 : 2 * p.parts * p.piece * p.Dp);
   p.g = take(grad ? 2 * p.parts * p.rows * p.piece : 0);
-  p.dx = take(grad ? 4 * p.splits * p.rows * p.Dp : 0);
+  p.dx = take(p.joined ? 4 * p.splits * p.rows * p.Dp : 0);
   p.bytes = at;
   return p;
-}
-
-inline bool vocab_large(const VocabArgs& a) {
-  return ceil_div(a.M, VocabLarge::BM) * ceil_div(a.N, VocabLarge::BN) * a.splits >= 256;
-}
-
-template <int MODE, class E, bool PARTS>
-void vocab_gemm(const VocabArgs& a, hipStream_t stream) {
-  if (vocab_large(a)) launch_vocab_gemm<VocabLarge, MODE, E, PARTS>(a, stream);
-  else launch_vocab_gemm<VocabMid, MODE, E, PARTS>(a, stream);
 }
 
 struct VocabCall {
@@ -333,110 +475,169 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   const int64_t x_part = p.rows * p.Dp, w_part = p.piece * p.Dp, g_part = p.rows * p.piece;
   const float c = (float)(1.4426950408889634 / q.temperature), inv_t = (float)(1.0 / q.temperature);
   const float scale = (float)((double)q.grad_scale / q.temperature) / (__is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f);
+  const T* weight = (const T*)q.weight;
+  // Without G in the way the first pass takes a weight that can be read as it lies whole; otherwise the pieces from
+  // the last to the first, whose packed weight and exponentials are then there for the second pass.
+  const int64_t first_piece = p.direct && !p.grad ? ceil_div(p.V, 256) * 256 : p.piece;
+  const int64_t pieces = ceil_div(p.V, first_piece);
+  auto count_of = [&](int64_t k) { return (int)(p.V - k * first_piece < first_piece ? p.V - k * first_piece : first_piece); };
 
-  hipLaunchKernelGGL(vocab_rows_kernel, dim3(1), dim3(1024), 0, stream, q.tokens, q.token_bytes, (const uint8_t*)q.mask,
-                     N, live, source, place, token, q.logp);
-  BF_LAUNCH_CHECK("bf_vocab_loss");
-  hipLaunchKernelGGL((vocab_pack_rows_kernel<T, E>), dim3((unsigned)p.rows), dim3(256), 0, stream, (const T*)q.hidden,
-                     q.ld_b, q.ld_t, (int)q.length, source, live, D, (int)p.Dp, x, x_part);
+  VocabPrepare pre;
+  memset(&pre, 0, sizeof(pre));
+  pre.hidden = q.hidden;
+  pre.ld_b = q.ld_b;
+  pre.ld_t = q.ld_t;
+  pre.length = (int)q.length;
+  pre.tokens = q.tokens;
+  pre.token_bytes = q.token_bytes;
+  pre.mask = (const uint8_t*)q.mask;
+  pre.N = N;
+  pre.D = D;
+  pre.Dp = (int)p.Dp;
+  pre.live = live;
+  pre.source = source;
+  pre.place = place;
+  pre.token = token;
+  pre.logp = q.logp;
+  pre.x = x;
+  pre.x_part = x_part;
+  pre.grad_hidden = q.grad_hidden;
+  if (!p.direct) {
+    pre.weight = weight + (pieces - 1) * first_piece * q.ld_w;
+    pre.ld_w = q.ld_w;
+    pre.weight_rows = count_of(pieces - 1);
+    pre.w = w;
+    pre.w_part = w_part;
+  }
+  const dim3 prepare((unsigned)(N + 64 + ceil_div(pre.weight_rows * (p.Dp / 8), 256)));
+  if (N <= VOCAB_SCAN) {
+    hipLaunchKernelGGL((vocab_prepare_kernel<T, E, true>), prepare, dim3(256), 0, stream, pre);
+  } else {
+    hipLaunchKernelGGL(vocab_rows_kernel, dim3(1), dim3(1024), 0, stream, q.tokens, q.token_bytes, (const uint8_t*)q.mask, N,
+                       live, source, place, token, q.logp);
+    BF_LAUNCH_CHECK("bf_vocab_loss");
+    hipLaunchKernelGGL((vocab_prepare_kernel<T, E, false>), prepare, dim3(256), 0, stream, pre);
+  }
   BF_LAUNCH_CHECK("bf_vocab_loss");
 
   VocabArgs a;
   memset(&a, 0, sizeof(a));
   a.live = live;
-  a.pairs = PARTS ? VOCAB_PAIRS : 1;
   a.elem = p.elem;
+  a.splits = 1;
   a.tokens = token;
   a.c = c;
-  a.part_ld = N;
+  a.part = part;
+  a.part_ld = p.tiles;
   a.chosen = chosen;
   a.row = row;
-  a.splits = 1;
-  const T* weight = (const T*)q.weight;
-  // the weight's rows from v0 on, as the products read them
-  auto weight_rows = [&](int64_t v0, int count) {
+  a.B = x;
+  a.ldb = p.Dp;
+  a.b_part = x_part;
+  a.N = N;
+  a.b_rows = (int)p.rows;
+  a.K = (int)p.Dp;
+  a.ldg = p.piece;
+  a.g_part = g_part;
+  a.g_rows = (int)p.rows;
+  // the weight's rows of a piece, as the products read them
+  auto weight_rows = [&](int64_t v0, int count, bool pack) {
+    a.v0 = (int)v0;
+    a.M = a.a_rows = count;
+    a.bias = q.bias ? (const T*)q.bias + v0 : nullptr;
     if (p.direct) {
       a.A = weight + v0 * q.ld_w;
       a.lda = q.ld_w;
-      a.a_part = 0;
       return;
     }
-    hipLaunchKernelGGL((vocab_pack_weight_kernel<T, E>), dim3((unsigned)count), dim3(256), 0, stream,
-                       weight + v0 * q.ld_w, q.ld_w, D, (int)p.Dp, w, w_part);
+    if (pack)
+      hipLaunchKernelGGL((vocab_pack_weight_kernel<T, E>), dim3((unsigned)ceil_div(count * (p.Dp / 8), 256)), dim3(256), 0,
+                         stream, weight + v0 * q.ld_w, q.ld_w, count, D, (int)p.Dp, w, w_part);
     a.A = w;
     a.lda = p.Dp;
     a.a_part = w_part;
   };
-  auto logits = [&](int64_t v0, int count) {
-    weight_rows(v0, count);
-    a.B = x;
-    a.ldb = p.Dp;
-    a.b_part = x_part;
-    a.M = a.a_rows = count;
-    a.N = N;
-    a.b_rows = (int)p.rows;
-    a.K = a.a_cols = a.b_cols = (int)p.Dp;
-    a.v0 = (int)v0;
-    a.bias = q.bias ? (const T*)q.bias + v0 : nullptr;
-  };
-  int tiles = 0;
-  for (int64_t v0 = 0; v0 < p.V; v0 += p.first) {
-    const int count = (int)(p.V - v0 < p.first ? p.V - v0 : p.first);
-    logits(v0, count);
-    a.part = part + (int64_t)tiles * N;
-    vocab_gemm<VM_STATS, E, PARTS>(a, stream);
+  for (int64_t k = pieces - 1; k >= 0; --k) {
+    weight_rows(k * first_piece, count_of(k), k < pieces - 1);
+    a.G = p.grad && k == 0 ? g : nullptr;
+    vocab_logits<E, PARTS>(p.logits_tile, a, true, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
-    tiles += (int)ceil_div(count, vocab_large(a) ? VocabLarge::BM : VocabMid::BM);
   }
-  hipLaunchKernelGGL(vocab_rows_stats_kernel, dim3((unsigned)ceil_div(N, 64)), dim3(1024), 0, stream, part, (int64_t)N,
-                     tiles, chosen, token, source, live, (int)p.V, c, inv_t, row, q.logp);
-  BF_LAUNCH_CHECK("bf_vocab_loss");
 
-  for (int64_t v0 = 0; p.grad && v0 < p.V; v0 += p.piece) {
-    const int count = (int)(p.V - v0 < p.piece ? p.V - v0 : p.piece);
-    logits(v0, count);
-    a.G = g;
-    a.ldg = p.piece;
-    a.g_part = g_part;
-    a.g_rows = (int)p.rows;
-    vocab_gemm<VM_GRAD, E, PARTS>(a, stream);
+  VocabSoftmax soft;
+  soft.part = part;
+  soft.part_ld = p.tiles;
+  soft.tiles = (int)p.tiles;
+  soft.tile = p.logits_tile == VT_LARGE ? VocabLarge::BM : VocabMid::BM;
+  soft.chosen = chosen;
+  soft.token = token;
+  soft.source = source;
+  soft.live = live;
+  soft.vocab = (int)p.V;
+  soft.c = c;
+  soft.inv_t = inv_t;
+  soft.row = row;
+  soft.logp = q.logp;
+  soft.G = p.grad ? g : nullptr;
+  soft.ldg = p.piece;
+  soft.g_part = g_part;
+  soft.held = p.grad ? (int)(ceil_div(count_of(0), 64) * 64) : 0;
+  soft.chunks = p.grad ? (int)ceil_div(soft.held, VOCAB_CHUNK) : 1;
+  hipLaunchKernelGGL((vocab_softmax_kernel<E, PARTS>), dim3((unsigned)((int64_t)N * soft.chunks)), dim3(256), 0, stream, soft);
+  BF_LAUNCH_CHECK("bf_vocab_loss");
+  if (!p.grad) {
+    hipLaunchKernelGGL(vocab_loss_kernel, dim3(1), dim3(256), 0, stream, q.logp, N, live, q.loss);
     BF_LAUNCH_CHECK("bf_vocab_loss");
+    return BF_OK;
+  }
+
+  for (int64_t k = 0; k < pieces; ++k) {
+    const int64_t v0 = k * first_piece;
+    const int count = count_of(k);
+    weight_rows(v0, count, k > 0);
+    if (k > 0) {
+      a.G = g;
+      vocab_logits<E, PARTS>(p.logits_tile, a, false, stream);
+      BF_LAUNCH_CHECK("bf_vocab_loss");
+    }
     // dx: the weight's rows are k
-    a.B = g;
-    a.ldb = p.piece;
-    a.b_part = g_part;
-    a.M = D;
-    a.N = N;
-    a.K = (int)(ceil_div(count, 64) * 64);
-    a.a_rows = count;
-    a.a_cols = (int)p.Dp;
-    a.b_rows = (int)p.rows;
-    a.splits = p.splits;
-    a.dx = dx;
-    a.dx_split = p.rows * p.Dp;
-    a.dx_ld = p.Dp;
-    a.dx_add = v0 > 0;
-    vocab_gemm<VM_DX, E, PARTS>(a, stream);
-    BF_LAUNCH_CHECK("bf_vocab_loss");
+    VocabArgs b = a;
+    b.B = g;
+    b.ldb = p.piece;
+    b.b_part = g_part;
+    b.M = D;
+    b.K = (int)(ceil_div(count, 64) * 64);
+    b.a_cols = (int)p.Dp;
+    b.splits = p.splits;
+    b.dx = p.joined ? dx : nullptr;
+    b.dx_split = p.rows * p.Dp;
+    b.dx_ld = p.Dp;
+    b.dx_add = k > 0;
+    b.source = source;
+    b.out = q.grad_hidden;
+    b.out_elem = p.elem;
+    b.scale = scale;
     // dw: the hidden rows are k
-    a.splits = 1;
-    a.A = x;
-    a.lda = p.Dp;
-    a.a_part = x_part;
-    a.a_rows = (int)p.rows;
-    a.N = count;
-    a.b_cols = (int)p.piece;
-    a.dw = (char*)q.grad_weight + v0 * D * elem_bytes(q.grad_weight_elem);
-    a.dw_ld = D;
-    a.dw_elem = q.grad_weight_elem;
-    a.db = q.grad_bias ? (T*)q.grad_bias + v0 : nullptr;
-    a.scale = scale;
-    vocab_gemm<VM_DW, E, PARTS>(a, stream);
+    VocabArgs d = b;
+    d.splits = 1;
+    d.dx = nullptr;
+    d.A = x;
+    d.lda = p.Dp;
+    d.a_part = x_part;
+    d.a_rows = (int)p.rows;
+    d.N = count;
+    d.b_cols = (int)p.piece;
+    d.out = (char*)q.grad_weight + v0 * D * elem_bytes(q.grad_weight_elem);
+    d.out_elem = q.grad_weight_elem;
+    d.db = q.grad_bias ? (T*)q.grad_bias + v0 : nullptr;
+    vocab_grads<E, PARTS>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
-  hipLaunchKernelGGL((vocab_finish_kernel<T>), dim3(p.grad ? (unsigned)(1 + N) : 1), dim3(256), 0, stream, q.logp, N, live,
-                     place, dx, p.rows * p.Dp, p.Dp, p.splits, D, scale, q.loss, (T*)q.grad_hidden);
-  BF_LAUNCH_CHECK("bf_vocab_loss");
+  if (p.joined) {
+    hipLaunchKernelGGL((vocab_join_kernel<T>), dim3((unsigned)N), dim3(256), 0, stream, live, place, dx, p.rows * p.Dp, p.Dp,
+                       p.splits, D, scale, (T*)q.grad_hidden);
+    BF_LAUNCH_CHECK("bf_vocab_loss");
+  }
   return BF_OK;
 }
 
@@ -454,19 +655,20 @@ inline bool vocab_sizes_ok(int64_t N, int64_t D, int64_t V, int64_t ld_w) {
 using namespace bf;
 
 extern "C" int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
-                                           int with_grad) {
-  if (!elem_ok(elem) || N <= 0 || D <= 0 || V <= 0 || ld_w < D || !vocab_sizes_ok(N, D, V, ld_w)) return 0;
-  return vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0).bytes / 4;
+                                           int with_grad, int64_t room) {
+  if (!elem_ok(elem) || N <= 0 || D <= 0 || V <= 0 || ld_w < D || room < 0 || !vocab_sizes_ok(N, D, V, ld_w)) return 0;
+  return vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0, room).bytes / 4;
 }
 
 extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
                              const void* weight, int64_t V, int64_t ld_w, const void* bias, const void* tokens,
                              int token_bytes, const void* mask, double temperature, float grad_scale, float* logp,
                              float* loss, void* grad_hidden, void* grad_weight, int grad_weight_elem, void* grad_bias,
-                             float* workspace, hipStream_t stream) {
+                             float* workspace, int64_t room, hipStream_t stream) {
   BF_REQUIRE(elem_ok(elem) && (token_bytes == 4 || token_bytes == 8), "bf_vocab_loss: element type %d, token bytes %d",
              elem, token_bytes);
-  BF_REQUIRE(B >= 0 && T >= 0 && D > 0 && V > 0 && ld_b >= 0 && ld_t >= 0 && ld_w >= D, "bf_vocab_loss: bad sizes");
+  BF_REQUIRE(B >= 0 && T >= 0 && D > 0 && V > 0 && ld_b >= 0 && ld_t >= 0 && ld_w >= D && room >= 0,
+             "bf_vocab_loss: bad sizes");
   BF_REQUIRE(temperature > 0.0, "bf_vocab_loss: temperature %g", temperature);
   BF_REQUIRE(loss, "bf_vocab_loss: null pointer");
   const bool grad = grad_hidden || grad_weight || grad_bias;
@@ -490,7 +692,7 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
     BF_LAUNCH_CHECK("bf_vocab_loss");
     return BF_OK;
   }
-  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, grad);
+  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, grad, room);
   const VocabCall q = {hidden, T, ld_b, ld_t, weight, ld_w, bias, tokens, token_bytes, mask, temperature, grad_scale, logp,
                        loss, grad_hidden, grad_weight, grad_weight_elem, grad_bias, (char*)workspace, stream};
   switch (elem) {

@@ -1,0 +1,9 @@
+// The products of the vocabulary loss for f16.
+#include "bf_vocab_tiles.h"
+
+namespace bf {
+
+template void vocab_logits<_Float16, false>(int, const VocabArgs&, bool, hipStream_t);
+template void vocab_grads<_Float16, false>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
+
+}  // namespace bf

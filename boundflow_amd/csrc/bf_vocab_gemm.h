@@ -32,6 +32,10 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 enum : int { VM_STATS = 0, VM_GRAD = 1, VM_DX = 2, VM_DW = 3 };
 
+// z's tiles end in one of two ways.  VM_STATS: the tile's largest logit and sum of exponentials per token, and where G is
+// given the exponentials themselves, 2^(c (z - the tile's largest)); vocab_softmax_kernel makes them G in place.  VM_GRAD, with the rows'
+// statistics known: G.
+
 constexpr int VOCAB_BK = 64;            // k of a stage
 constexpr int VOCAB_PARTS = 3, VOCAB_PAIRS = 6;
 // fp16 holds G times this: p - [v = y] lies within [-1, 1], and a probability below 2^-24 would be subnormal
@@ -42,43 +46,45 @@ struct VocabArgs {
   const void* B;
   int64_t lda, ldb;          // elements between rows (of M or N with k contiguous, of k otherwise)
   int64_t a_part, b_part;    // elements between the parts of fp32 operands
-  int pairs;                 // 1, or VOCAB_PAIRS for parts
   int M, N, K;               // K a multiple of VOCAB_BK
   int a_rows, b_rows;        // rows of A and B that may be read: later ones give the last one's values
   int a_cols, b_cols;        // of operands with k in their rows: elements of a row that may be read
   const int* live;           // rows of X that count, on the device
   int splits;                // VM_DX: pieces of k, each with sums of its own
+  int elem;                  // of the call's tensors
   // softmax
-  const void* bias;          // [M] or null, of type `elem`
-  int elem;
-  const int* tokens;         // [N] less v0
-  int v0;
+  const void* bias;          // [M] or null
+  const int* tokens;         // [N]
+  int v0;                    // the token that row 0 of A stands for
   float c;                   // log2(e) / temperature
-  float2* part;              // [tiles of M, part_ld]: largest logit and sum of 2^(c (z - it)) over the tile
+  float2* part;              // [N, part_ld]: largest logit and sum of 2^(c (z - it)) over a tile
   int64_t part_ld;
   float* chosen;             // [N] the token's logit
   const float2* row;         // [N] largest logit, 1 / sum
-  // results
-  void* G;                   // [parts, rows, ldg]
+  void* G;                   // [parts, g_rows, ldg], or null (VM_STATS)
   int64_t ldg, g_part;
   int g_rows;
-  float* dx;                 // [splits, dx_rows, dx_ld]
+  // gradients
+  float* dx;                 // [splits, dx_rows, dx_ld], or null: rows are final and go to `out`
   int64_t dx_split, dx_ld;
   int dx_add;                // add to what is there
-  void* dw;                  // [N, dw_ld] of type dw_elem
-  int64_t dw_ld;
-  int dw_elem;
-  void* db;                  // [N] of type `elem`, or null
-  float scale;               // of dw and db, before the division by the rows that count
+  const int* source;         // VM_DX without dx: the row of out that row n is
+  void* out;                 // dense rows of M: VM_DX of type elem, VM_DW of type out_elem
+  int out_elem;
+  void* db;                  // [N] of type elem, or null
+  float scale;               // of out and db, before the division by the rows that count
 };
 
-// Tiles of BM x BN, NWM x NWN waves of 32 FM x 32 FN each.
-template <int FM_, int FN_, int NWM_, int NWN_>
+// Tiles of BM x BN, NWM x NWN waves of 32 FM x 32 FN each; STAGES of LDS, OCC workgroups on a CU.
+template <int FM_, int FN_, int NWM_, int NWN_, int STAGES_, int OCC_>
 struct VocabTile {
-  static constexpr int FM = FM_, FN = FN_, NWM = NWM_, NWN = NWN_;
+  static constexpr int FM = FM_, FN = FN_, NWM = NWM_, NWN = NWN_, STAGES = STAGES_, OCC = OCC_;
   static constexpr int BM = 32 * FM * NWM, BN = 32 * FN * NWN, WAVES = NWM * NWN, NT = 64 * WAVES;
   static constexpr int A_BYTES = BM * VOCAB_BK * 2, B_BYTES = BN * VOCAB_BK * 2;
   static constexpr int STAGE = A_BYTES + B_BYTES;
+  // behind the stages: the bias of the tile's rows, two floats per column from each half of a wave along M
+  static constexpr int BIAS_AT = STAGES * STAGE, RED_AT = BIAS_AT + 4 * BM, LDS = RED_AT + 2 * 4 * 2 * NWM * BN;
+  static_assert(BM * BN * 2 <= STAGES * STAGE, "a tile of G passes through the stages' memory");
 };
 
 // 16 bytes a lane from base + off to LDS at dst + 16 lane, asynchronously (vmcnt counts it)
@@ -108,15 +114,17 @@ struct Vec8<_Float16> {
 //
 // LDS of a stage, in slots of 16 bytes.  k contiguous: row r of 8 slots, slot s holding chunk s ^ (r % 8), so that the
 // 32 lanes which read one chunk of 32 rows meet all banks.  k in rows (TR): row k of SIDE / 8 slots, slot s holding
-// chunk s ^ 4 (k % 4): the four rows of k that 16 lanes read together lie 32 bytes apart.
+// chunk s ^ swap(k): 32 lanes read 64 bytes of four rows of k together, which meet all banks.
 template <bool TR, int SIDE, int WAVES>
 struct VocabOperand {
   static constexpr int COPIES = SIDE * VOCAB_BK * 2 / 1024;     // of 1 KB, one wave each
   static constexpr int PER_WAVE = (COPIES + WAVES - 1) / WAVES;
-  static_assert(!TR || SIDE >= 128, "the slots' permutation spans 16 of them");
+  static_assert(!TR || SIDE >= 64, "the slots' permutation spans 8 of them, or 16");
   static_assert(COPIES % WAVES == 0, "every wave makes the same copies");
   uint32_t off[PER_WAVE];   // bytes from the stage's first k
   int krow[PER_WAVE];       // TR: the row of k that a lane copies
+
+  static __device__ __forceinline__ int swap(int k) { return SIDE >= 128 ? 4 * (k & 3) : 4 * ((k >> 1) & 1); }
 
   // first: the tile's first row (k contiguous) or column (TR)
   __device__ __forceinline__ void set(int wave, int lane, int first, int rows, int cols, int64_t ld) {
@@ -126,7 +134,7 @@ struct VocabOperand {
       if constexpr (TR) {
         constexpr int SLOTS = SIDE / 8;
         const int k = copy * (64 / SLOTS) + lane / SLOTS;
-        int col = first + 8 * ((lane % SLOTS) ^ (4 * (k & 3)));
+        int col = first + 8 * ((lane % SLOTS) ^ swap(k));
         if (col > cols - 8) col = cols - 8;
         krow[j] = k;
         off[j] = (uint32_t)(2 * (k * ld + col));
@@ -138,15 +146,18 @@ struct VocabOperand {
     }
   }
 
-  // `base`: the stage's first k (of the tile's first row); left: rows of k from there on (TR)
-  __device__ __forceinline__ void copy(const char* base, int64_t ld, int left, int wave, uint32_t dst) const {
+  // `base`: the stage's first k (of the tile's first row)
+  __device__ __forceinline__ void copy(const char* base, int wave, uint32_t dst) const {
+#pragma unroll
+    for (int j = 0; j < PER_WAVE; ++j) copy16_to_lds(base, off[j], dst + (wave * PER_WAVE + j) * 1024);
+  }
+
+  // the same of a stage that only `left` rows of k are left for: the last one stands for those that are missing
+  __device__ __forceinline__ void copy_last(const char* base, int64_t ld, int left, int wave, uint32_t dst) const {
 #pragma unroll
     for (int j = 0; j < PER_WAVE; ++j) {
-      uint32_t o = off[j];
-      if constexpr (TR) {
-        if (left < VOCAB_BK && krow[j] >= left) o -= (uint32_t)(2 * (krow[j] - (left - 1)) * ld);
-      }
-      copy16_to_lds(base, o, dst + (wave * PER_WAVE + j) * 1024);
+      const int past = krow[j] - (left - 1);
+      copy16_to_lds(base, off[j] - (past > 0 ? (uint32_t)(2 * past * ld) : 0), dst + (wave * PER_WAVE + j) * 1024);
     }
   }
 
@@ -156,7 +167,7 @@ struct VocabOperand {
     if constexpr (TR) {
       const int g = lane >> 4, i = lane & 15;
       const int k = 16 * kk + 8 * (g >> 1) + (i >> 2), col = side + 16 * (g & 1) + 4 * (i & 3);
-      const int at = k * (2 * SIDE) + (((col >> 3) ^ (4 * (i >> 2))) << 4) + 2 * (col & 7);
+      const int at = k * (2 * SIDE) + (((col >> 3) ^ swap(i >> 2)) << 4) + 2 * (col & 7);
       const lds_char* p = (const lds_char*)stage;
       const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + at));
       const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + at + 4 * (2 * SIDE)));
@@ -193,14 +204,32 @@ __device__ __forceinline__ void split_parts(float x, __bf16 part[VOCAB_PARTS]) {
   }
 }
 
+// The loss, by one workgroup: minus the sum of the log-probabilities (0 in rows that do not count) over the rows that do.
+// 256 threads take it, whatever the workgroup's size, so that it has the same bits with and without gradients.
+template <int WAVES>
+__device__ __forceinline__ void vocab_loss(const float* __restrict__ logp, int rows, int live, float* loss, float* red) {
+  float sum = 0.f;
+  if (threadIdx.x < 256)
+#pragma unroll 8
+    for (int n = threadIdx.x; n < rows; n += 256) sum += logp[n];
+  sum = block_sum<WAVES>(sum, red);
+  if (threadIdx.x == 0) *loss = live ? -sum / (float)live : 0.f;
+}
+
+// Waits until all but the last LEFT of this wave's copies are there.
+template <int LEFT>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
+
+// One tile's sums.  `block` of `share * 8` workgroups: XCD block % 8's share-th of the tiles.
 template <class T, int MODE, class E, bool PARTS>
-__global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
+__device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint32_t block) {
   constexpr bool A_TR = MODE >= VM_DX, B_TR = MODE == VM_DW;
   constexpr int FM = T::FM, FN = T::FN;
   typedef typename Vec8<E>::type V8;
   typedef VocabOperand<A_TR, T::BM, T::WAVES> OpA;
   typedef VocabOperand<B_TR, T::BN, T::WAVES> OpB;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * T::STAGE];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -212,8 +241,8 @@ __global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
   const int ntm = (p.M + T::BM - 1) / T::BM, ntn = (N + T::BN - 1) / T::BN;
   const int splits = MODE == VM_DX ? p.splits : 1;
   const int tiles = ntm * ntn * splits, share = (tiles + 7) / 8;
-  int tile = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= share || tile >= tiles) return;
+  int tile = (int)(block & 7) * share + (int)(block >> 3);
+  if ((int)(block >> 3) >= share || tile >= tiles) return;
   int split = 0;
   if constexpr (MODE == VM_DX) {
     split = tile / (ntm * ntn);
@@ -242,14 +271,15 @@ __global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
   const char *a_at = a_first, *b_at = b_first;
   const uint32_t lds0 = (uint32_t)(uintptr_t)((lds_char*)smem);
   int pair = 0, ks = 0;
-  if constexpr (PARTS) {
-    a_at = a_first + 2 * 2 * p.a_part;   // a2 b0 first
-  }
+  if constexpr (PARTS) a_at = a_first + 2 * 2 * p.a_part;   // a2 b0 first
 
   auto issue = [&](int buffer) {
     const uint32_t dst = lds0 + buffer * T::STAGE;
-    opa.copy(a_at, p.lda, A_TR ? p.a_rows - (k_first + ks) * VOCAB_BK : VOCAB_BK, wave, dst);
-    opb.copy(b_at, p.ldb, B_TR ? p.b_rows - (k_first + ks) * VOCAB_BK : VOCAB_BK, wave, dst + T::A_BYTES);
+    // the weight ends where the vocabulary does; everything else has zeros up to a whole stage
+    const int left = MODE == VM_DX ? p.a_rows - (k_first + ks) * VOCAB_BK : VOCAB_BK;
+    if (left < VOCAB_BK) opa.copy_last(a_at, p.lda, left, wave, dst);
+    else opa.copy(a_at, wave, dst);
+    opb.copy(b_at, wave, dst + T::A_BYTES);
     a_at += a_step;
     b_at += b_step;
     if (++ks == steps) {
@@ -264,6 +294,13 @@ __global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
     }
   };
 
+  float* bias = (float*)(smem + T::BIAS_AT);
+  if constexpr (MODE <= VM_GRAD) {
+    // rows past the vocabulary get logits of -inf; the first barrier of the loop is before the first use
+    for (int m = threadIdx.x; m < T::BM; m += T::NT)
+      bias[m] = m0 + m >= p.M ? -INFINITY : p.bias ? load_elem(p.bias, p.elem, m0 + m) : 0.f;
+  }
+
   const int wm = (wave % T::NWM) * 32 * FM, wn = (wave / T::NWM) * 32 * FN;
   floatx16 acc[FM][FN];
 #pragma unroll
@@ -276,125 +313,222 @@ __global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
   const bool sum_cols = MODE == VM_DW && p.db && tm == 0 && wave % T::NWM == 0;
 #pragma unroll
   for (int j = 0; j < FN; ++j) col_sum[j] = 0.f;
+  // G's column sums, the bias's gradient: every part of G once, beside the first part of X
+  auto column_sums = [&](int s, const V8* x) {
+    if (sum_cols && (!PARTS || (s >= steps && s < 2 * steps) || s >= 4 * steps)) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) col_sum[j] += (float)x[j][e];
+    }
+  };
 
-  if (total > 0) issue(0);
-  for (int s = 0; s < total; ++s) {
-    // this wave's copies of the stage are there, then everyone's; the other buffer's readers are done
+  if constexpr (T::WAVES == 8) {
+    // Two groups of four waves, one wave of each on a SIMD, take turns: while one multiplies what it has in registers
+    // (half a stage, 16 products in 512 cycles) the other reads its next half stage from LDS and starts the copies
+    // of the next stage.  A buffer is written again when the second group has read its last half, and has to be there
+    // three turns later.
+    static_assert(T::STAGES == 2, "two buffers in turn");
+    const bool second = wave >= 4;
+    if (total > 0) issue(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 1 < total) issue((s + 1) & 1);
-    const char* stage = smem + (s & 1) * T::STAGE;
+    if (second) asm volatile("s_barrier" ::: "memory");
+    for (int s = 0; s < total; ++s) {
+      const char* stage = smem + (s & 1) * T::STAGE;
 #pragma unroll
-    for (int kk = 0; kk < VOCAB_BK / 16; ++kk) {
-      V8 a[FM], b[FN];
+      for (int h = 0; h < 2; ++h) {
+        V8 a[2][FM], b[2][FN];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) a[i] = OpA::template read<V8>(stage, wm + 32 * i, kk, lane);
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) b[j] = OpB::template read<V8>(stage + T::A_BYTES, wn + 32 * j, kk, lane);
+          for (int i = 0; i < FM; ++i) a[k][i] = OpA::template read<V8>(stage, wm + 32 * i, 2 * h + k, lane);
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[i], b[j], acc[i][j]);
-      if constexpr (MODE == VM_DW) {
-        // G's column sums, the bias's gradient: every part of G once, beside the first part of X
-        if (sum_cols && (!PARTS || (s >= steps && s < 2 * steps) || s >= 4 * steps)) {
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) col_sum[j] += (float)b[j][e];
+          for (int j = 0; j < FN; ++j) b[k][j] = OpB::template read<V8>(stage + T::A_BYTES, wn + 32 * j, 2 * h + k, lane);
         }
+        if (h == 0 && s + 1 < total) issue((s + 1) & 1);
+        if (h == 1 && second) wait_copies<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[k][i], b[k][j], acc[i][j]);
+          if constexpr (MODE == VM_DW) column_sums(s, b[k]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (h == 1 && !second) wait_copies<0>();
+        asm volatile("s_barrier" ::: "memory");
+      }
+    }
+    if (!second) asm volatile("s_barrier" ::: "memory");
+  } else {
+    // All but one of the stages are under way.
+    constexpr int AHEAD = T::STAGES - 1, COPIES = OpA::PER_WAVE + OpB::PER_WAVE;
+    static_assert((AHEAD - 1) * COPIES < 64, "what vmcnt counts");
+    for (int s = 0; s < AHEAD && s < total; ++s) issue(s);
+    int from = 0, to = AHEAD;   // buffers of stage s and of the stage that is started beside it
+    for (int s = 0; s < total; ++s) {
+      // this wave's copies of the stage are there, then everyone's; the readers of the buffer before it are done
+      if (s + AHEAD <= total) wait_copies<(AHEAD - 1) * COPIES>();
+      else wait_copies<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + AHEAD < total) issue(to);
+      const char* stage = smem + from * T::STAGE;
+      from = from + 1 == T::STAGES ? 0 : from + 1;
+      to = to + 1 == T::STAGES ? 0 : to + 1;
+#pragma unroll
+      for (int kk = 0; kk < VOCAB_BK / 16; ++kk) {
+        V8 a[FM], b[FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) a[i] = OpA::template read<V8>(stage, wm + 32 * i, kk, lane);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) b[j] = OpB::template read<V8>(stage + T::A_BYTES, wn + 32 * j, kk, lane);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[i], b[j], acc[i][j]);
+        if constexpr (MODE == VM_DW) column_sums(s, b);
       }
     }
   }
 
   // C: this lane's column n0 + wn + 32 j + lane % 32, rows m0 + wm + 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4
   const int half = lane >> 5, ln = lane & 31;
-  if constexpr (MODE == VM_STATS) {
-    float* red = (float*)smem;     // [NWM][BN][2]
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (MODE <= VM_GRAD) {
+    float* red = (float*)(smem + T::RED_AT);
+    const int share_of = 2 * (wave % T::NWM) + half;      // of the 2 NWM that hold a column
+    if constexpr (MODE == VM_STATS) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn + 32 * j + ln;
-      const int token = n < N ? p.tokens[n] - p.v0 : -1;
-      float top = -INFINITY;
+      for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn + 32 * j + ln;
+        const int token = n < N ? p.tokens[n] - p.v0 - m0 - wm - 4 * half : -1;   // among this lane's rows
+        float top = -INFINITY, chosen = 0.f;
+        bool found = false;
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int m = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
-          float z = acc[i][j][r];
-          if (p.bias && m < p.M) z += load_elem(p.bias, p.elem, m);
-          if (m >= p.M) z = -INFINITY;
-          if (m == token) p.chosen[n] = z;
-          acc[i][j][r] = z;
-          top = fmaxf(top, z);
-        }
-      const float held = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
+          for (int q = 0; q < 4; ++q) {
+            const float4 b4 = *(const float4*)(bias + wm + 32 * i + 8 * q + 4 * half);
+            const float add[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - held) * p.c);
-      float2 mine = make_float2(top, sum);
-      float* at = red + 2 * ((2 * (wave % T::NWM) + half) * T::BN + wn + 32 * j + ln);
-      at[0] = mine.x;
-      at[1] = mine.y;
-    }
-    __syncthreads();
-    for (int col = threadIdx.x; col < T::BN; col += T::NT) {
-      if (n0 + col >= N) continue;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 2 * T::NWM; ++w) top = fmaxf(top, red[2 * (w * T::BN + col)]);
-      const float held = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 2 * T::NWM; ++w) {
-        const float* at = red + 2 * (w * T::BN + col);
-        // a share without a logit above -inf has no sum, but one that met a NaN has
-        sum += at[1] * (at[0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((at[0] - held) * p.c));
-      }
-      p.part[(int64_t)tm * p.part_ld + n0 + col] = make_float2(top, sum);
-    }
-  } else if constexpr (MODE == VM_GRAD) {
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn + 32 * j + ln;
-      if (n >= p.g_rows) continue;
-      const bool counts = n < N;
-      const int token = counts ? p.tokens[n] - p.v0 : -1;
-      const float2 row = counts ? p.row[n] : make_float2(0.f, 0.f);
-      E* g = (E*)p.G + (int64_t)n * p.ldg;
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = m0 + wm + 32 * i + 8 * q + 4 * half;
-          if (m >= p.ldg) continue;
-          Pack<E, 4> out[PARTS ? VOCAB_PARTS : 1];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = 0.f;
-            if (counts && m + r < p.M) {
-              float z = acc[i][j][4 * q + r];
-              if (p.bias) z += load_elem(p.bias, p.elem, m + r);
-              x = __builtin_amdgcn_exp2f((z - row.x) * p.c) * row.y;
-              if (m + r == token) x -= 1.f;
-            }
-            if constexpr (PARTS) {
-              __bf16 part[VOCAB_PARTS];
-              split_parts(x, part);
-#pragma unroll
-              for (int k = 0; k < VOCAB_PARTS; ++k) out[k].v[r] = part[k];
-            } else {
-              if constexpr (sizeof(E) == 2 && __is_same(E, _Float16)) x *= VOCAB_F16_SCALE;
-              out[0].v[r] = (E)x;
+            for (int r = 0; r < 4; ++r) {
+              const float z = acc[i][j][4 * q + r] + add[r];
+              const bool it = token == 32 * i + 8 * q + r;
+              chosen = it ? z : chosen;
+              found |= it;
+              acc[i][j][4 * q + r] = z;
+              top = fmaxf(top, z);
             }
           }
+        if (found) p.chosen[n] = chosen;
+        red[share_of * T::BN + wn + 32 * j + ln] = top;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-          for (int k = 0; k < (PARTS ? VOCAB_PARTS : 1); ++k) store_pack(g + k * p.g_part + m, out[k]);
+      for (int j = 0; j < FN; ++j) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 2 * T::NWM; ++w) top = fmaxf(top, red[w * T::BN + wn + 32 * j + ln]);
+        const float held = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f((acc[i][j][r] - held) * p.c);
+            acc[i][j][r] = e;
+            sum += e;
+          }
+        red[(2 * T::NWM + share_of) * T::BN + wn + 32 * j + ln] = sum;
+        if (n0 + wn + 32 * j + ln >= N) {
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
         }
+      }
+    } else {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the stages have been read
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn + 32 * j + ln;
+        const bool counts = n < N;
+        const int token = counts ? p.tokens[n] - p.v0 - m0 - wm - 4 * half : -1;
+        const float2 row = counts ? p.row[n] : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4 b4 = *(const float4*)(bias + wm + 32 * i + 8 * q + 4 * half);
+            const float add[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float x = __builtin_amdgcn_exp2f((acc[i][j][4 * q + r] + add[r] - row.x) * p.c) * row.y;
+              if (token == 32 * i + 8 * q + r) x -= 1.f;
+              acc[i][j][4 * q + r] = counts ? x : 0.f;
+            }
+          }
+      }
     }
-  } else if constexpr (MODE == VM_DX) {
+    if (MODE == VM_GRAD || p.G) {
+      // The tile as rows of G: a lane has four neighbours of a row, a wave 32 rows, so it passes through LDS (slot s of
+      // 16 bytes of row n at s ^ n % slots) to be written in whole lines.  fp32: part by part.
+      constexpr int SLOTS = T::BM / 8;
+#pragma unroll 1
+      for (int part = 0; part < (PARTS ? VOCAB_PARTS : 1); ++part) {
+        if (part) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int col = wn + 32 * j + ln;
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              Pack<E, 4> x;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float v = acc[i][j][4 * q + r];
+                if constexpr (__is_same(E, _Float16)) {
+                  x.v[r] = (E)(v * VOCAB_F16_SCALE);
+                } else {
+                  x.v[r] = (E)v;
+                  if constexpr (PARTS) acc[i][j][4 * q + r] = __builtin_isfinite(v) ? v - (float)x.v[r] : 0.f;
+                }
+              }
+              const int slot = ((wm + 32 * i) / 8 + q) ^ (col % SLOTS);
+              *(Pack<E, 4>*)__builtin_assume_aligned(smem + col * (2 * T::BM) + 16 * slot + 8 * half, 8) = x;
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        E* g = (E*)p.G + part * p.g_part + m0;
+#pragma unroll 4
+        for (int at = threadIdx.x; at < T::BN * SLOTS; at += T::NT) {
+          const int col = at / SLOTS, slot = at % SLOTS;
+          if (n0 + col < p.g_rows)
+            *(Words*)(g + (int64_t)(n0 + col) * p.ldg + 8 * slot) =
+                *(const Words*)(smem + col * (2 * T::BM) + 16 * (slot ^ (col % SLOTS)));
+        }
+      }
+    } else {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    if constexpr (MODE == VM_STATS) {
+      for (int col = threadIdx.x; col < T::BN; col += T::NT) {
+        if (n0 + col >= N) continue;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 2 * T::NWM; ++w) {
+          top = fmaxf(top, red[w * T::BN + col]);
+          sum += red[(2 * T::NWM + w) * T::BN + col];
+        }
+        p.part[(n0 + col) * p.part_ld + (p.v0 + m0) / T::BM] = make_float2(top, sum);
+      }
+    }
+  } else if (MODE == VM_DX && p.dx) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = n0 + wn + 32 * j + ln;
@@ -427,28 +561,28 @@ __global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
         if (half == 0 && n < N) store_elem(p.db, p.elem, n, sum * scale);
       }
       if (n >= N) continue;
+      const int64_t row = (int64_t)(MODE == VM_DX ? p.source[n] : n) * p.M;
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int m = m0 + wm + 32 * i + 8 * q + 4 * half;
-          const int64_t at = (int64_t)n * p.dw_ld + m;
           if (m + 4 <= p.M) {
-            if (p.dw_elem == TE_F32) {
+            if (PARTS || p.out_elem == TE_F32) {
               Pack<float, 4> x;
 #pragma unroll
               for (int r = 0; r < 4; ++r) x.v[r] = acc[i][j][4 * q + r] * scale;
-              store_pack((float*)p.dw + at, x);
+              store_pack((float*)p.out + row + m, x);
             } else {
               Pack<E, 4> x;
 #pragma unroll
               for (int r = 0; r < 4; ++r) x.v[r] = (E)(acc[i][j][4 * q + r] * scale);
-              store_pack((E*)p.dw + at, x);
+              store_pack((E*)p.out + row + m, x);
             }
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (m + r < p.M) store_elem(p.dw, p.dw_elem, at + r, acc[i][j][4 * q + r] * scale);
+              if (m + r < p.M) store_elem(p.out, p.out_elem, row + m + r, acc[i][j][4 * q + r] * scale);
           }
         }
     }
@@ -456,10 +590,56 @@ __global__ void __launch_bounds__(T::NT) vocab_gemm_kernel(VocabArgs p) {
 }
 
 template <class T, int MODE, class E, bool PARTS>
-inline void launch_vocab_gemm(const VocabArgs& p, hipStream_t stream) {
-  const int64_t tiles = ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN) * (MODE == VM_DX ? p.splits : 1);
-  const int64_t blocks = 8 * ceil_div(tiles, 8);
-  hipLaunchKernelGGL((vocab_gemm_kernel<T, MODE, E, PARTS>), dim3((unsigned)blocks), dim3(T::NT), 0, stream, p);
+__global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4) vocab_logits_kernel(VocabArgs p) {
+  __shared__ __attribute__((aligned(1024))) char smem[T::LDS];
+  vocab_tile<T, MODE, E, PARTS>(p, smem, blockIdx.x);
 }
+
+// dX and dW of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the CUs that dX's few long
+// ones leave.  dX's come first; the last workgroup takes the loss where `loss` is given.
+template <class T, class E, bool PARTS>
+__global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
+    vocab_grads_kernel(VocabArgs dx, VocabArgs dw, uint32_t dx_blocks, const float* logp, int rows, float* loss) {
+  __shared__ __attribute__((aligned(1024))) char smem[T::RED_AT];
+  if (loss && blockIdx.x + 1 == gridDim.x) vocab_loss<T::WAVES>(logp, rows, *dx.live, loss, (float*)smem);
+  else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, PARTS>(dx, smem, blockIdx.x);
+  else vocab_tile<T, VM_DW, E, PARTS>(dw, smem, blockIdx.x - dx_blocks);
+}
+
+// Workgroups for `tiles` tiles at most, a whole number per XCD.
+inline int64_t vocab_blocks(int64_t tiles) { return 8 * ceil_div(tiles, 8); }
+
+template <class T, class E, bool PARTS>
+inline void launch_vocab_logits(const VocabArgs& p, bool stats, hipStream_t stream) {
+  const dim3 grid((unsigned)vocab_blocks(ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN)));
+  if (stats) hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
+  else hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
+}
+
+template <class T, class E, bool PARTS>
+inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
+                               hipStream_t stream) {
+  const int64_t first = vocab_blocks(ceil_div(dx.M, T::BM) * ceil_div(dx.N, T::BN) * dx.splits);
+  const int64_t all = first + vocab_blocks(ceil_div(dw.M, T::BM) * ceil_div(dw.N, T::BN)) + (loss ? 1 : 0);
+  hipLaunchKernelGGL((vocab_grads_kernel<T, E, PARTS>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
+                     logp, rows, loss);
+}
+
+// Tiles by the size of the problem.
+// Large: the products' rate.  Mid: where Large would leave CUs without a tile.  Slim: up to 64 rows, where the
+// weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU.
+typedef VocabTile<4, 2, 2, 4, 2, 1> VocabLarge;
+typedef VocabTile<2, 2, 2, 2, 2, 2> VocabMid;
+typedef VocabTile<2, 2, 2, 2, 4, 1> VocabDeep;
+typedef VocabTile<1, 2, 4, 1, 3, 2> VocabSlim;
+
+enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3 };
+
+// Defined for each type by a file of its own (bf_vocab_*.hip).
+template <class E, bool PARTS>
+void vocab_logits(int tile, const VocabArgs& p, bool stats, hipStream_t stream);
+template <class E, bool PARTS>
+void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
+                 hipStream_t stream);
 
 }  // namespace bf

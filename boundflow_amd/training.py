@@ -410,7 +410,7 @@ class VocabularyLoss(NamedTuple):
 def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *,
                     bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, temperature: float = 1.0,
                     grad_scale: float = 1.0, with_grad: bool = True,
-                    weight_grad_dtype: Optional[torch.dtype] = None) -> VocabularyLoss:
+                    weight_grad_dtype: Optional[torch.dtype] = None, room: int = 2 << 30) -> VocabularyLoss:
     """Softmax cross entropy of a linear head over a vocabulary, with its gradients, without keeping the logits.
 
     hidden [B, T, D] or [N, D] (a view such as ``states[:, :-1]`` is read in place), weight [V, D] (rows contiguous, any
@@ -422,8 +422,9 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     (``weight_grad_dtype``; ``embed_tokens_grad`` can then add that of a tied table to it).  ``with_grad=False`` gives loss
     and log-probabilities alone: those that ``policy_loss`` and ``preference_loss`` take as an old or a reference policy's.
 
-    Products of 16-bit inputs are summed in fp32; between them the softmax's gradient is held in the inputs' type
-    (fp32: in 24 bits)."""
+    Products of 16-bit inputs are summed in fp32; between them the softmax's gradient is held in the inputs' type (fp32: in
+    24 bits).  ``room`` bytes of it (and of a copy of a weight whose rows cannot be read as they lie) are held at a time, for as
+    many tokens of the vocabulary as fit; the logits of the others are formed twice, which takes up to a third longer."""
     dev = _current_device(hidden, "hidden")
     elem = _elem(hidden, "hidden")
     shape = hidden.shape
@@ -465,11 +466,13 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
             raise ValueError(f"mask of shape {tuple(mask.shape)}, expected {tuple(lead)}")
         if not mask.is_contiguous():
             mask = mask.contiguous()
+    if room < 0:
+        raise ValueError(f"room must be >=0, got {room}")
     wide = weight.dtype if weight_grad_dtype is None else weight_grad_dtype
     if wide not in (weight.dtype, torch.float32):
         raise ValueError(f"weight_grad_dtype must be {weight.dtype} or float32, got {wide}")
     N = B * T
-    need = _lib.load().bf_vocab_loss_workspace(N, D, V, elem, weight.data_ptr(), ld, with_grad)
+    need = _lib.load().bf_vocab_loss_workspace(N, D, V, elem, weight.data_ptr(), ld, with_grad, room)
     out = torch.empty(1 + N, dtype=torch.float32, device=hidden.device)      # loss, logp
     space = torch.empty(need, dtype=torch.float32, device=hidden.device) if need else None
     grad_hidden = grad_weight = grad_bias = None
@@ -481,7 +484,7 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     _lib.call("bf_vocab_loss", hidden.data_ptr(), elem, B, T, D, strides[0], strides[1] if dims == 3 else 0,
               weight.data_ptr(), V, ld, _address(bias), tokens.data_ptr(), token_bytes, _address(mask), float(temperature),
               float(grad_scale), at + 4, at, _address(grad_hidden), _address(grad_weight), _ELEM[wide], _address(grad_bias),
-              _address(space), current_raw_stream(dev))
+              _address(space), room, current_raw_stream(dev))
     return VocabularyLoss(out[0], out[1:1 + N].view(lead), grad_hidden, grad_weight, grad_bias)
 
 

@@ -672,13 +672,16 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
  * A row is live unless it is masked or its token negative; other rows are not read, and their logp and gradient
  * are 0.  A token past the vocabulary gives NaN.  grad_hidden dense [B, T, D] and grad_bias [V] of the inputs' type,
  * grad_weight dense [V, D] of that type or fp32: grad_scale * the loss's gradient; all that there are, or none of them (NULL).
- * Workspace in floats, 16-byte aligned; its size depends on whether the weight can be read as it lies. */
+ * Workspace in floats, 16-byte aligned; its size depends on whether the weight can be read as it lies.  `room` (the same in
+ * both calls): bytes that the softmax's gradient, in the products' type, and a copy of such a weight may take; of what has
+ * no room the logits are formed twice. */
 int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
-                                int with_grad);
+                                int with_grad, int64_t room);
 int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
                   const void* weight, int64_t V, int64_t ld_w, const void* bias, const void* tokens, int token_bytes,
                   const void* mask, double temperature, float grad_scale, float* logp, float* loss, void* grad_hidden,
-                  void* grad_weight, int grad_weight_elem, void* grad_bias, float* workspace, hipStream_t stream);
+                  void* grad_weight, int grad_weight_elem, void* grad_bias, float* workspace, int64_t room,
+                  hipStream_t stream);
 
 /* Dropout: out[e] = (residual[e]) + (u_e >= border ? x[e] / (1 - border / 2^16) : 0) with border = p * 2^16, rounded, in
  * fp32 and rounded once.  u_e are 16 bits of the Philox 4x32 generator of ten rounds, whose counter is (e / 8,

@@ -40,10 +40,12 @@ def tolerances(r, dtype, temperature, V, D):
     # What is below a type's normal numbers: fp16 holds 2^14 G in steps of 2^-24, so G to 2^-39.  In fp32 a probability below
     # 2^-126 is 0, and so is each of three bf16 parts (the matrix cores read subnormal bf16 as 0): 4 * 2^-126 in all.
     extra = 2.0 ** -124 if dtype == torch.float32 else 2.0 ** -39
-    return tol_lp, r["p"] * (tol_lp + 2.0 ** -21)[:, None] + r["g"].abs() * (U[dtype] + 2.0 ** -23) + extra
+    # exponentials are rounded to the type before they are scaled (but for the token's), G after it
+    return tol_lp, r["p"] * (tol_lp + 2.0 ** -21 + U[dtype])[:, None] + r["g"].abs() * (U[dtype] + 2.0 ** -23) + extra
 
 
-def check(hidden, weight, tokens, *, bias=None, mask=None, temperature=1.0, grad_scale=1.0, wide=None, on=None, what=""):
+def check(hidden, weight, tokens, *, bias=None, mask=None, temperature=1.0, grad_scale=1.0, wide=None, room=2 << 30, on=None,
+          what=""):
     """`on`: the device tensors where their layout is not that of the others."""
     dev = device()
     dtype, (V, D) = weight.dtype, weight.shape
@@ -51,7 +53,7 @@ def check(hidden, weight, tokens, *, bias=None, mask=None, temperature=1.0, grad
     args = {"hidden": hidden, "weight": weight, "tokens": tokens, "bias": bias, "mask": mask}
     args = {k: None if v is None else v.to(dev) for k, v in args.items()}
     args.update(on or {})
-    kw = dict(temperature=temperature, grad_scale=grad_scale)
+    kw = dict(temperature=temperature, grad_scale=grad_scale, room=room)
     what = f"{what or tuple(hidden.shape)} x {V} {dtype}"
     got = training.vocabulary_loss(**args, **kw, weight_grad_dtype=wide)
     tol_lp, tol_g = tolerances(r, dtype, temperature, V, D)
@@ -248,13 +250,32 @@ def test_gradients_against_differences():
         assert abs(slope - want) <= tol
 
 
-def test_pieces_of_the_vocabulary():
-    """More vocabulary than a piece holds: fp32 rows take 6 bytes of the softmax's gradient and of the packed weight each."""
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", [(5, 64, 700), (70, 40, 1003), (300, 192, 513), (90, 65, 2000)])
+@pytest.mark.parametrize("room", [0, 300_000])
+def test_pieces(dtype, N, D, V, room):
+    """No room, or a little: pieces of 256 tokens or some more, the logits of all but the first formed again."""
+    hidden, weight, tokens, bias = head(N, D, V, dtype, 17)
+    mask = torch.rand(N, generator=gen(5)) < 0.9
+    check(hidden, weight, tokens, bias=bias, mask=mask, room=room, wide=torch.float32)
+
+
+def test_room_that_is_the_products_alone():
+    """The first piece's gradient comes from rounded exponentials, the others' from logits formed again: both as close."""
+    for dtype in TYPES:
+        hidden, weight, tokens, bias = head(40, 128, 1024, dtype, 23)
+        whole = check(hidden, weight, tokens, bias=bias)
+        cut = check(hidden, weight, tokens, bias=bias, room=0)
+        assert torch.equal(whole.logp, cut.logp) and torch.equal(whole.loss, cut.loss)
+
+
+def test_many_pieces_of_a_large_vocabulary():
     dev = device()
     N, D, V = 1024, 40, 170_001
     hidden, weight, tokens, bias = head(N, D, V, torch.float32, 6)
     mask = torch.rand(N, generator=gen(4)) < 0.6
-    got = training.vocabulary_loss(hidden.to(dev), weight.to(dev), tokens.to(dev), bias=bias.to(dev), mask=mask.to(dev))
+    got = training.vocabulary_loss(hidden.to(dev), weight.to(dev), tokens.to(dev), bias=bias.to(dev), mask=mask.to(dev),
+                                   room=400 << 20)
     at = mask.nonzero()[:, 0]
     n = at.numel()
     x, w = hidden[at].double().to(dev), weight.double().to(dev)
@@ -295,6 +316,7 @@ def test_refusals():
             (HipError, "mask must be", (hidden, weight, tokens), {"mask": tokens}),
             (ValueError, "mask of shape", (hidden, weight, tokens), {"mask": tokens[:5] > 0}),
             (ValueError, "temperature", (hidden, weight, tokens), {"temperature": 0.0}),
+            (ValueError, "room must be", (hidden, weight, tokens), {"room": -1}),
             (ValueError, "weight_grad_dtype", (hidden, weight, tokens), {"weight_grad_dtype": torch.float16}),
             (HipError, "device tensor", (hidden, weight.cpu(), tokens), {}),
             (HipError, "must be float32", (hidden.double(), weight, tokens), {})):

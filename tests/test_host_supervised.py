@@ -42,11 +42,11 @@ def test_entry_points_refuse_bad_arguments(lib):
     assert p % 16 == 0
     loss = lambda **k: lib.bf_vocab_loss(*{**dict(  # noqa: E731
         hidden=p, elem=0, B=1, T=2, D=4, ld_b=8, ld_t=4, weight=p, V=3, ld_w=4, bias=p, tokens=p, token_bytes=8, mask=None,
-        temperature=1.0, scale=1.0, logp=p, loss=p, dh=p, dw=p, dw_elem=0, db=p, space=p, stream=None), **k}.values())
+        temperature=1.0, scale=1.0, logp=p, loss=p, dh=p, dw=p, dw_elem=0, db=p, space=p, room=1 << 30, stream=None), **k}.values())
     for bad in (dict(elem=5), dict(V=0), dict(D=0), dict(temperature=0.0), dict(temperature=float("nan")), dict(loss=None),
                 dict(token_bytes=1), dict(ld_t=-1), dict(ld_w=3), dict(weight=None), dict(hidden=None), dict(tokens=None),
                 dict(logp=None), dict(space=None), dict(space=p + 4), dict(dw=None), dict(dh=None), dict(db=None),
-                dict(bias=None), dict(dw_elem=1), dict(B=-1)):
+                dict(bias=None), dict(dw_elem=1), dict(B=-1), dict(room=-1)):
         assert loss(**bad) == 1, bad
     for far in (dict(T=1 << 24), dict(B=1 << 40, T=1 << 40), dict(V=1 << 31), dict(ld_w=1 << 21),
                 dict(D=1 << 21, ld_w=1 << 21), dict(T=(1 << 23) - 1, V=1 << 29)):
@@ -66,16 +66,21 @@ def test_workspaces_hold_what_their_kernels_write(lib):
     for N, D, V, elem in ((1, 1, 1, 0), (8, 2048, 32000, 1), (1003, 1025, 50001, 2), (2048, 1024, 32000, 0),
                           (8184, 4096, 128000, 1)):
         some = 1 << 20        # an address that can be read as it lies
-        alone, grad = size(N, D, V, elem, some, D, 0), size(N, D, V, elem, some, D, 1)
+        alone, grad = size(N, D, V, elem, some, D, 0, 256 << 20), size(N, D, V, elem, some, D, 1, 256 << 20)
         assert 0 < alone < grad
         # a token, a place and statistics per row and tile of the vocabulary; the packed rows
         parts = 3 if elem == 0 else 1
         assert 4 * alone >= 8 * N + 2 * parts * N * D
-        # G and the sums of the hidden rows' gradient stay bounded: the logits would be 4 N V
-        assert 4 * (grad - alone) <= (540 << 20) + 16 * 4 * (N + 64) * (D + 64)
-    assert size(0, 4, 4, 0, 0, 4, 1) == 0 and size(4, 4, 4, 7, 0, 4, 1) == 0 and size(1 << 24, 4, 4, 0, 0, 4, 1) == 0
+        # G stays within the room (the logits would be 4 N V), the sums of the hidden rows' gradient within theirs
+        assert 4 * (grad - alone) <= (256 << 20) + max(128 << 20, 4 * (N + 64) * (D + 64)) + 4096
+        # no room: a piece of 256 tokens
+        assert 4 * size(N, D, V, elem, some, D, 1, 0) < 4 * alone + 600 * parts * (N + D + 128) + \
+            max(128 << 20, 4 * (N + 64) * (D + 64)) + 4096
+    room = 1 << 30
+    assert size(0, 4, 4, 0, 0, 4, 1, room) == 0 and size(4, 4, 4, 7, 0, 4, 1, room) == 0
+    assert size(1 << 24, 4, 4, 0, 0, 4, 1, room) == 0 and size(4, 4, 4, 0, 0, 4, 1, -1) == 0
     # a weight that has to be packed takes more
-    assert size(100, 64, 1000, 1, 1 << 20, 64, 0) < size(100, 64, 1000, 1, (1 << 20) + 2, 64, 0)
+    assert size(100, 64, 1000, 1, 1 << 20, 64, 0, room) < size(100, 64, 1000, 1, (1 << 20) + 2, 64, 0, room)
 
 
 def test_requires_grad_is_refused_before_the_device_is_asked():
