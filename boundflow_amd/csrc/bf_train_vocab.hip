@@ -296,31 +296,68 @@ __global__ void __launch_bounds__(256) vocab_loss_kernel(const float* __restrict
   vocab_loss<4>(logp, N, *live, loss, red);
 }
 
-// The hidden rows' gradient where it was summed in pieces: joined, scaled and brought back to the rows that count.
+// Gradients that were summed in pieces, joined and scaled: rows of the hidden rows' (brought back to their places),
+// then of the weight's, then the bias's.  A thread takes eight elements.
+struct VocabJoin {
+  const int* live;
+  const int* source;
+  const float* dx;          // [dx_splits, rows, ld], or null
+  int64_t dx_split;
+  int dx_splits, N;
+  void* grad_hidden;
+  const float* dw;          // [dw_splits, V, ld], or null
+  int64_t dw_split, V;
+  int dw_splits;
+  void* grad_weight;
+  int dw_elem;
+  const float* db;          // [dw_splits, V], or null
+  void* grad_bias;
+  int elem, D;
+  int64_t ld;
+  float scale;
+};
+
 template <class T>
-__global__ void __launch_bounds__(256) vocab_join_kernel(const int* __restrict__ live, const int* __restrict__ place,
-                                                         const float* __restrict__ dx, int64_t dx_split, int64_t dx_ld,
-                                                         int splits, int D, float scale, T* __restrict__ grad) {
-  const int at = place[blockIdx.x];
-  if (at < 0) return;
-  T* out = grad + (int64_t)blockIdx.x * D;
-  const float factor = scale / (float)*live;
-  for (int d = 8 * threadIdx.x; d < D; d += 8 * 256) {
-    float x[8] = {};
+__device__ __forceinline__ void join_chunk(const float* from, int64_t split, int splits, int d, int D, float factor, T* out) {
+  float x[8] = {};
 #pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-      const Pack<float, 8> more = load_pack<float, 8>(dx + s * dx_split + at * dx_ld + d);
+  for (int s = 0; s < splits; ++s) {
+    const Pack<float, 8> more = load_pack<float, 8>(from + s * split + d);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] += more.v[k];
-    }
-    Pack<T, 8> y;
+    for (int k = 0; k < 8; ++k) x[k] += more.v[k];
+  }
+  Pack<T, 8> y;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y.v[k] = (T)(x[k] * factor);
-    if (d + 8 <= D) {
-      store_pack(out + d, y);
-    } else {
-      for (int k = 0; d + k < D; ++k) out[d + k] = y.v[k];
-    }
+  for (int k = 0; k < 8; ++k) y.v[k] = (T)(x[k] * factor);
+  if (d + 8 <= D) {
+    store_pack(out + d, y);
+  } else {
+    for (int k = 0; d + k < D; ++k) out[d + k] = y.v[k];
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) vocab_join_kernel(VocabJoin p) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int chunks = (p.D + 7) / 8, live = *p.live;
+  const float factor = p.scale / (float)max(live, 1);
+  int64_t row = div_rows(at, chunks, at < (1LL << 31));
+  const int d = 8 * (int)(at - row * chunks);
+  const int N = p.dx ? p.N : 0;
+  if (row < N) {
+    if (row < live)
+      join_chunk(p.dx + row * p.ld, p.dx_split, p.dx_splits, d, p.D, factor, (T*)p.grad_hidden + (int64_t)p.source[row] * p.D);
+    return;
+  }
+  row -= N;
+  if (!p.dw || row >= p.V) return;
+  const float* from = p.dw + row * p.ld;
+  if (p.dw_elem == TE_F32) join_chunk(from, p.dw_split, p.dw_splits, d, p.D, factor, (float*)p.grad_weight + row * p.D);
+  else join_chunk(from, p.dw_split, p.dw_splits, d, p.D, factor, (T*)p.grad_weight + row * p.D);
+  if (p.db && d == 0) {
+    float sum = 0.f;
+    for (int s = 0; s < p.dw_splits; ++s) sum += p.db[s * p.V + row];
+    ((T*)p.grad_bias)[row] = (T)(sum * factor);
   }
 }
 
@@ -346,20 +383,21 @@ struct VocabPlan {
   int64_t piece;             // vocabulary of a piece: what G and the packed weight have room for
   int64_t tiles;             // of the vocabulary in the first pass
   int logits_tile, grads_tile;
-  int splits;                // of the hidden rows' gradient
-  bool joined;               // it is summed in pieces first
+  int dx_splits, dw_splits;  // of the gradients' sums
+  bool dx_joined, dw_joined; // they are summed in pieces first
   // bytes from the workspace's start
-  int64_t live, source, place, token, chosen, row, part, x, w, g, dx, bytes;
+  int64_t live, source, place, token, chosen, row, part, x, w, g, dx, dw, db, bytes;
 };
 
 inline bool vocab_direct(int elem, int64_t D, const void* weight, int64_t ld) {
-  return elem != TE_F32 && D % 64 == 0 && ld % 8 == 0 && (uintptr_t)weight % 16 == 0;
+  return elem != TE_F32 && D % 8 == 0 && ld % 8 == 0 && (uintptr_t)weight % 16 == 0;
 }
 
 inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n) {
   switch (tile) {
     case VT_LARGE: return ceil_div(m, VocabLarge::BM) * ceil_div(n, VocabLarge::BN);
-    case VT_SLIM: return ceil_div(m, VocabSlim::BM) * ceil_div(n, VocabSlim::BN);
+    case VT_SLIM:
+    case VT_THIN: return ceil_div(m, VocabSlim::BM) * ceil_div(n, VocabSlim::BN);
     default: return ceil_div(m, VocabMid::BM) * ceil_div(n, VocabMid::BN);
   }
 }
@@ -386,32 +424,40 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   }
   const int64_t in_piece = p.piece < V ? p.piece : V;
   // by the whole vocabulary, so that the statistics have the same bits with and without gradients and whatever the room
-  if (N <= VocabSlim::BN) p.logits_tile = VT_SLIM;
+  if (N <= VocabSlim::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N) > 256 ? VT_SLIM : VT_THIN;
   else if (vocab_tile_count(VT_LARGE, V, N) >= 200) p.logits_tile = VT_LARGE;
   else p.logits_tile = vocab_tile_count(VT_MID, V, N) > 256 ? VT_MID : VT_DEEP;
   p.tiles = vocab_tile_count(p.logits_tile, V, 1);
   p.grads_tile = VT_SLIM;
-  p.splits = 1;
-  p.joined = false;
+  p.dx_splits = p.dw_splits = 1;
+  p.dx_joined = p.dw_joined = false;
   if (grad) {
-    if (N > VocabSlim::BN) {
+    if (N <= VocabSlim::BN) {
+      const int64_t slim = vocab_tile_count(VT_SLIM, D, N) + vocab_tile_count(VT_SLIM, D, in_piece);
+      p.grads_tile = slim > 256 ? VT_SLIM : VT_THIN;
+    } else {
       const int64_t large = vocab_tile_count(VT_LARGE, D, N) + vocab_tile_count(VT_LARGE, D, in_piece);
       const int64_t mid = vocab_tile_count(VT_MID, D, N) + vocab_tile_count(VT_MID, D, in_piece);
       p.grads_tile = large >= 200 ? VT_LARGE : mid > 256 ? VT_MID : VT_DEEP;
     }
-    // dx's sums over the vocabulary are cut so that none of them takes longer than a good part of the whole launch
-    const int64_t slots = p.grads_tile == VT_LARGE || p.grads_tile == VT_DEEP ? 256 : 512;
+    // Sums are cut along k so that none of them takes longer than a good part of the whole launch, nor than it takes to
+    // add one more piece's sums (some eight stages).
+    const int64_t slots = p.grads_tile == VT_MID || p.grads_tile == VT_SLIM ? 512 : 256;
     const int64_t dx = vocab_tile_count(p.grads_tile, D, N), dw = vocab_tile_count(p.grads_tile, D, in_piece);
-    const int64_t dx_steps = ceil_div(in_piece, 64), dw_steps = ceil_div(N, 64) + 4;
-    int64_t most = (dx * dx_steps + dw * dw_steps) / slots / 3;
-    if (most < 8) most = 8;
-    int64_t splits = ceil_div(dx_steps, most);
-    const int64_t fits = (128LL << 20) / (4 * p.rows * p.Dp);
-    if (splits > fits) splits = fits;
-    if (splits > 32) splits = 32;
-    if (splits < 1) splits = 1;
-    p.splits = (int)splits;
-    p.joined = splits > 1 || p.piece < V;
+    const int64_t dx_steps = ceil_div(in_piece, 64), dw_steps = ceil_div(N, 64);
+    int64_t most = (dx * dx_steps + dw * (dw_steps + 4)) / slots / 3;
+    const int64_t least = p.parts > 1 ? 2 : 8;      // six stages a step in parts
+    if (most < least) most = least;
+    auto cut = [&](int64_t steps, int64_t rows) {
+      int64_t splits = ceil_div(steps, most), fits = (128LL << 20) / (4 * rows * p.Dp);
+      if (splits > fits) splits = fits;
+      if (splits > 32) splits = 32;
+      return (int)(splits < 1 ? 1 : splits);
+    };
+    p.dx_splits = cut(dx_steps, p.rows);
+    p.dw_splits = p.piece < V ? 1 : cut(dw_steps, V);
+    p.dx_joined = p.dx_splits > 1 || p.piece < V;
+    p.dw_joined = p.dw_splits > 1;
   }
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -429,7 +475,9 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.x = take(2 * p.parts * p.rows * p.Dp);
   p.w = take(p.direct ? 0 : 2 * p.parts * p.piece * p.Dp);
   p.g = take(grad ? 2 * p.parts * p.rows * p.piece : 0);
-  p.dx = take(p.joined ? 4 * p.splits * p.rows * p.Dp : 0);
+  p.dx = take(p.dx_joined ? 4 * p.dx_splits * p.rows * p.Dp : 0);
+  p.dw = take(p.dw_joined ? 4 * p.dw_splits * V * p.Dp : 0);
+  p.db = take(p.dw_joined ? 4 * p.dw_splits * V : 0);
   p.bytes = at;
   return p;
 }
@@ -472,6 +520,8 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   E* w = (E*)(q.space + p.w);
   E* g = (E*)(q.space + p.g);
   float* dx = (float*)(q.space + p.dx);
+  float* dw = (float*)(q.space + p.dw);
+  float* db = (float*)(q.space + p.db);
   const int64_t x_part = p.rows * p.Dp, w_part = p.piece * p.Dp, g_part = p.rows * p.piece;
   const float c = (float)(1.4426950408889634 / q.temperature), inv_t = (float)(1.0 / q.temperature);
   const float scale = (float)((double)q.grad_scale / q.temperature) / (__is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f);
@@ -537,6 +587,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   a.N = N;
   a.b_rows = (int)p.rows;
   a.K = (int)p.Dp;
+  a.a_cols = p.direct ? D : (int)p.Dp;
   a.ldg = p.piece;
   a.g_part = g_part;
   a.g_rows = (int)p.rows;
@@ -607,20 +658,22 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     b.b_part = g_part;
     b.M = D;
     b.K = (int)(ceil_div(count, 64) * 64);
-    b.a_cols = (int)p.Dp;
-    b.splits = p.splits;
-    b.dx = p.joined ? dx : nullptr;
-    b.dx_split = p.rows * p.Dp;
-    b.dx_ld = p.Dp;
-    b.dx_add = k > 0;
+    b.splits = p.dx_splits;
+    b.sums = p.dx_joined ? dx : nullptr;
+    b.sums_split = p.rows * p.Dp;
+    b.sums_ld = p.Dp;
+    b.add = k > 0;
     b.source = source;
     b.out = q.grad_hidden;
     b.out_elem = p.elem;
     b.scale = scale;
     // dw: the hidden rows are k
     VocabArgs d = b;
-    d.splits = 1;
-    d.dx = nullptr;
+    d.splits = p.dw_splits;
+    d.sums = p.dw_joined ? dw : nullptr;
+    d.sums_split = p.V * p.Dp;
+    d.db_sums = db;
+    d.a_cols = (int)p.Dp;
     d.A = x;
     d.lda = p.Dp;
     d.a_part = x_part;
@@ -633,9 +686,30 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     vocab_grads<E, PARTS>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
-  if (p.joined) {
-    hipLaunchKernelGGL((vocab_join_kernel<T>), dim3((unsigned)N), dim3(256), 0, stream, live, place, dx, p.rows * p.Dp, p.Dp,
-                       p.splits, D, scale, (T*)q.grad_hidden);
+  if (p.dx_joined || p.dw_joined) {
+    VocabJoin j;
+    memset(&j, 0, sizeof(j));
+    j.live = live;
+    j.source = source;
+    if (p.dx_joined) j.dx = dx;
+    j.dx_split = p.rows * p.Dp;
+    j.dx_splits = p.dx_splits;
+    j.N = N;
+    j.grad_hidden = q.grad_hidden;
+    if (p.dw_joined) j.dw = dw;
+    j.dw_split = p.V * p.Dp;
+    j.V = p.V;
+    j.dw_splits = p.dw_splits;
+    j.grad_weight = q.grad_weight;
+    j.dw_elem = q.grad_weight_elem;
+    if (q.grad_bias) j.db = db;
+    j.grad_bias = q.grad_bias;
+    j.elem = p.elem;
+    j.D = D;
+    j.ld = p.Dp;
+    j.scale = scale;
+    const int64_t rows = (p.dx_joined ? N : 0) + (p.dw_joined ? p.V : 0);
+    hipLaunchKernelGGL((vocab_join_kernel<T>), dim3((unsigned)ceil_div(rows * ceil_div(D, 8), 256)), dim3(256), 0, stream, j);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
   return BF_OK;

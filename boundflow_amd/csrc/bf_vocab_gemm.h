@@ -50,7 +50,7 @@ struct VocabArgs {
   int a_rows, b_rows;        // rows of A and B that may be read: later ones give the last one's values
   int a_cols, b_cols;        // of operands with k in their rows: elements of a row that may be read
   const int* live;           // rows of X that count, on the device
-  int splits;                // VM_DX: pieces of k, each with sums of its own
+  int splits;                // VM_DX, VM_DW: pieces of k, each with sums of its own
   int elem;                  // of the call's tensors
   // softmax
   const void* bias;          // [M] or null
@@ -65,13 +65,14 @@ struct VocabArgs {
   int64_t ldg, g_part;
   int g_rows;
   // gradients
-  float* dx;                 // [splits, dx_rows, dx_ld], or null: rows are final and go to `out`
-  int64_t dx_split, dx_ld;
-  int dx_add;                // add to what is there
-  const int* source;         // VM_DX without dx: the row of out that row n is
+  float* sums;               // [splits, rows, sums_ld], to be joined later, or null: results are final and go to `out`
+  int64_t sums_split, sums_ld;
+  int add;                   // add to the sums that are there
+  const int* source;         // VM_DX without sums: the row of out that row n is
   void* out;                 // dense rows of M: VM_DX of type elem, VM_DW of type out_elem
   int out_elem;
-  void* db;                  // [N] of type elem, or null
+  void* db;                  // VM_DW: [N] of type elem, or null
+  float* db_sums;            // [splits, N] in its place, where there are sums
   float scale;               // of out and db, before the division by the rows that count
 };
 
@@ -112,8 +113,9 @@ struct Vec8<_Float16> {
 
 // One operand's stages: SIDE rows or columns of the tile.
 //
-// LDS of a stage, in slots of 16 bytes.  k contiguous: row r of 8 slots, slot s holding chunk s ^ (r % 8), so that the
-// 32 lanes which read one chunk of 32 rows meet all banks.  k in rows (TR): row k of SIDE / 8 slots, slot s holding
+// LDS of a stage, in slots of 16 bytes.  k contiguous: row r of 8 slots, slot s holding chunk s ^ (r / 2 % 8), so that the
+// 16 lanes which read one chunk of 16 rows together meet all 64 banks (r % 8 in its place: half of them, twice; the
+// reads of z took 1.3 times their cycles).  k in rows (TR): row k of SIDE / 8 slots, slot s holding
 // chunk s ^ swap(k): 32 lanes read 64 bytes of four rows of k together, which meet all banks.
 template <bool TR, int SIDE, int WAVES>
 struct VocabOperand {
@@ -125,6 +127,9 @@ struct VocabOperand {
   int krow[PER_WAVE];       // TR: the row of k that a lane copies
 
   static __device__ __forceinline__ int swap(int k) { return SIDE >= 128 ? 4 * (k & 3) : 4 * ((k >> 1) & 1); }
+
+  // k contiguous: the eight k that a lane copies
+  static __device__ __forceinline__ int chunk(int copy, int lane) { return (lane & 7) ^ ((4 * copy + (lane >> 4)) & 7); }
 
   // first: the tile's first row (k contiguous) or column (TR)
   __device__ __forceinline__ void set(int wave, int lane, int first, int rows, int cols, int64_t ld) {
@@ -141,7 +146,7 @@ struct VocabOperand {
       } else {
         int r = first + 8 * copy + (lane >> 3);
         if (r > rows - 1) r = rows - 1;
-        off[j] = (uint32_t)(2 * ((int64_t)(r - first) * ld + 8 * ((lane & 7) ^ (lane >> 3))));
+        off[j] = (uint32_t)(2 * ((int64_t)(r - first) * ld + 8 * chunk(copy, lane)));
       }
     }
   }
@@ -152,12 +157,14 @@ struct VocabOperand {
     for (int j = 0; j < PER_WAVE; ++j) copy16_to_lds(base, off[j], dst + (wave * PER_WAVE + j) * 1024);
   }
 
-  // the same of a stage that only `left` rows of k are left for: the last one stands for those that are missing
-  __device__ __forceinline__ void copy_last(const char* base, int64_t ld, int left, int wave, uint32_t dst) const {
+  // The same of a stage that only `left` k are left for: the last row of them (TR), or the last eight of a row, stand for those
+  // that are missing, whose counterparts in the other operand are zeros.
+  __device__ __forceinline__ void copy_last(const char* base, int64_t ld, int left, int wave, int lane, uint32_t dst) const {
 #pragma unroll
     for (int j = 0; j < PER_WAVE; ++j) {
-      const int past = krow[j] - (left - 1);
-      copy16_to_lds(base, off[j] - (past > 0 ? (uint32_t)(2 * past * ld) : 0), dst + (wave * PER_WAVE + j) * 1024);
+      const int past = TR ? krow[j] - (left - 1) : 8 * chunk(wave * PER_WAVE + j, lane) - (left - 8);
+      copy16_to_lds(base, off[j] - (past > 0 ? (uint32_t)(2 * past * (TR ? ld : 1)) : 0),
+                    dst + (wave * PER_WAVE + j) * 1024);
     }
   }
 
@@ -174,7 +181,7 @@ struct VocabOperand {
       return __builtin_bit_cast(V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       const int r = side + (lane & 31);
-      return *(const V*)(stage + r * 128 + (((2 * kk + (lane >> 5)) ^ (r & 7)) << 4));
+      return *(const V*)(stage + r * 128 + (((2 * kk + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4));
     }
   }
 };
@@ -239,12 +246,12 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   // Tiles in the order of groups of 8 along M, a contiguous share of them to each XCD: the 32 or 64 tiles that run on
   // one XCD at a time read 8 tiles of A and 4 or 8 of B through its L2.  Only rows that count have tiles.
   const int ntm = (p.M + T::BM - 1) / T::BM, ntn = (N + T::BN - 1) / T::BN;
-  const int splits = MODE == VM_DX ? p.splits : 1;
+  const int splits = MODE >= VM_DX ? p.splits : 1;
   const int tiles = ntm * ntn * splits, share = (tiles + 7) / 8;
   int tile = (int)(block & 7) * share + (int)(block >> 3);
   if ((int)(block >> 3) >= share || tile >= tiles) return;
   int split = 0;
-  if constexpr (MODE == VM_DX) {
+  if constexpr (MODE >= VM_DX) {
     split = tile / (ntm * ntn);
     tile -= split * (ntm * ntn);
   }
@@ -254,7 +261,7 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   const int m0 = tm * T::BM, n0 = tn * T::BN;
 
   int steps = MODE == VM_DW ? (live + VOCAB_BK - 1) / VOCAB_BK : p.K / VOCAB_BK, k_first = 0;
-  if constexpr (MODE == VM_DX) {
+  if constexpr (MODE >= VM_DX) {
     const int per = (steps + splits - 1) / splits;
     k_first = split * per;
     steps = max(0, min(per, steps - k_first));
@@ -275,9 +282,11 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
 
   auto issue = [&](int buffer) {
     const uint32_t dst = lds0 + buffer * T::STAGE;
-    // the weight ends where the vocabulary does; everything else has zeros up to a whole stage
-    const int left = MODE == VM_DX ? p.a_rows - (k_first + ks) * VOCAB_BK : VOCAB_BK;
-    if (left < VOCAB_BK) opa.copy_last(a_at, p.lda, left, wave, dst);
+    // the weight's rows end where the width does and the weight where the vocabulary does; everything else has zeros up
+    // to a whole stage
+    const int left = (MODE == VM_DX ? p.a_rows : MODE == VM_DW ? VOCAB_BK : p.a_cols) -
+                     (MODE == VM_DW ? 0 : (k_first + ks) * VOCAB_BK);
+    if (left < VOCAB_BK) opa.copy_last(a_at, p.lda, left, wave, lane, dst);
     else opa.copy(a_at, wave, dst);
     opb.copy(b_at, wave, dst + T::A_BYTES);
     a_at += a_step;
@@ -528,22 +537,26 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
         p.part[(n0 + col) * p.part_ld + (p.v0 + m0) / T::BM] = make_float2(top, sum);
       }
     }
-  } else if (MODE == VM_DX && p.dx) {
+  } else if (p.sums) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = n0 + wn + 32 * j + ln;
+      if (sum_cols) {
+        const float sum = col_sum[j] + __shfl_xor(col_sum[j], 32);
+        if (half == 0 && n < N) p.db_sums[(int64_t)split * N + n] = sum;
+      }
       if (n >= N) continue;
-      float* row = p.dx + split * p.dx_split + (int64_t)n * p.dx_ld;
+      float* row = p.sums + split * p.sums_split + (int64_t)n * p.sums_ld;
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int m = m0 + wm + 32 * i + 8 * q + 4 * half;
-          if (m >= p.dx_ld) continue;
+          if (m >= p.sums_ld) continue;
           Pack<float, 4> x;
 #pragma unroll
           for (int r = 0; r < 4; ++r) x.v[r] = acc[i][j][4 * q + r];
-          if (p.dx_add) {
+          if (p.add) {
             const Pack<float, 4> was = load_pack<float, 4>(row + m);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x.v[r] += was.v[r];
@@ -620,20 +633,22 @@ template <class T, class E, bool PARTS>
 inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                                hipStream_t stream) {
   const int64_t first = vocab_blocks(ceil_div(dx.M, T::BM) * ceil_div(dx.N, T::BN) * dx.splits);
-  const int64_t all = first + vocab_blocks(ceil_div(dw.M, T::BM) * ceil_div(dw.N, T::BN)) + (loss ? 1 : 0);
+  const int64_t all = first + vocab_blocks(ceil_div(dw.M, T::BM) * ceil_div(dw.N, T::BN) * dw.splits) + (loss ? 1 : 0);
   hipLaunchKernelGGL((vocab_grads_kernel<T, E, PARTS>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
                      logp, rows, loss);
 }
 
 // Tiles by the size of the problem.
 // Large: the products' rate.  Mid: where Large would leave CUs without a tile.  Slim: up to 64 rows, where the
-// weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU.
+// weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU.  Deep and
+// Thin are these with more stages under way for grids of at most a workgroup per CU, whose time is the copies' latency.
 typedef VocabTile<4, 2, 2, 4, 2, 1> VocabLarge;
 typedef VocabTile<2, 2, 2, 2, 2, 2> VocabMid;
 typedef VocabTile<2, 2, 2, 2, 4, 1> VocabDeep;
 typedef VocabTile<1, 2, 4, 1, 3, 2> VocabSlim;
+typedef VocabTile<1, 2, 4, 1, 6, 1> VocabThin;
 
-enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3 };
+enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4 };
 
 // Defined for each type by a file of its own (bf_vocab_*.hip).
 template <class E, bool PARTS>

@@ -11,6 +11,7 @@ void vocab_logits(int tile, const VocabArgs& p, bool stats, hipStream_t stream) 
     case VT_LARGE: launch_vocab_logits<VocabLarge, E, PARTS>(p, stats, stream); break;
     case VT_MID: launch_vocab_logits<VocabMid, E, PARTS>(p, stats, stream); break;
     case VT_DEEP: launch_vocab_logits<VocabDeep, E, PARTS>(p, stats, stream); break;
+    case VT_THIN: launch_vocab_logits<VocabThin, E, PARTS>(p, stats, stream); break;
     default: launch_vocab_logits<VocabSlim, E, PARTS>(p, stats, stream);
   }
 }
@@ -22,6 +23,7 @@ void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float
     case VT_LARGE: launch_vocab_grads<VocabLarge, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
     case VT_MID: launch_vocab_grads<VocabMid, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
     case VT_DEEP: launch_vocab_grads<VocabDeep, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    case VT_THIN: launch_vocab_grads<VocabThin, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
     default: launch_vocab_grads<VocabSlim, E, PARTS>(dx, dw, logp, rows, loss, stream);
   }
 }
