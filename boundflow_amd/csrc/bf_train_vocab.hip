@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256) vocab_pack_weight_kernel(const T* __restr
 // Statistics of the rows that count, from those of their tiles, and G from the exponentials that the first pass left, in
 // place.  A workgroup joins a row's tiles and takes VOCAB_CHUNK of its entries; the first one of a row writes what others
 // read.  The token's entry comes from its log-probability: p - 1 from a rounded p would have no digits left where p is near 1.
-// The others are rounded a second time here (half a step of their type).
+// The others are rounded a second time here (half a step of their type; fp32 ones lie here whole).
 constexpr int VOCAB_CHUNK = 8192;
 
 struct VocabSoftmax {
@@ -269,11 +269,12 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
     const float factor = __builtin_amdgcn_exp2f((part[v / p.tile].x - top) * p.c) * inv;
     Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
 #pragma unroll
-    for (int q = 0; q < (PARTS ? VOCAB_PARTS : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part + v);
+    for (int q = 0; q < (PARTS ? 2 : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part + v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float y = (float)x[0].v[e];
-      if constexpr (PARTS) y = ((float)x[2].v[e] + (float)x[1].v[e]) + y;
+      if constexpr (PARTS)      // the two halves of an fp32 number
+        y = __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, x[0].v[e]) << 16 | __builtin_bit_cast(uint16_t, x[1].v[e]));
       y = v + e == token ? at_token : y * factor;
       if constexpr (PARTS) {
         __bf16 parts[VOCAB_PARTS];

@@ -85,7 +85,7 @@ struct VocabTile {
   static constexpr int STAGE = A_BYTES + B_BYTES;
   // behind the stages: the bias of the tile's rows, two floats per column from each half of a wave along M
   static constexpr int BIAS_AT = STAGES * STAGE, RED_AT = BIAS_AT + 4 * BM, LDS = RED_AT + 2 * 4 * 2 * NWM * BN;
-  static_assert(BM * BN * 2 <= STAGES * STAGE, "a tile of G passes through the stages' memory");
+  static constexpr int TILE = 2 * BM * BN;   // of 16-bit results
 };
 
 // 16 bytes a lane from base + off to LDS at dst + 16 lane, asynchronously (vmcnt counts it)
@@ -377,15 +377,27 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   } else {
     // All but one of the stages are under way.
     constexpr int AHEAD = T::STAGES - 1, COPIES = OpA::PER_WAVE + OpB::PER_WAVE;
-    static_assert((AHEAD - 1) * COPIES < 64, "what vmcnt counts");
+    if constexpr (T::STAGES == 1) {
+      // for sums of one stage: the workgroups beside this one hide its copies
+      if (total > 0) issue(0);
+    }
+    static_assert(AHEAD * COPIES < 64 + COPIES, "what vmcnt counts");
     for (int s = 0; s < AHEAD && s < total; ++s) issue(s);
     int from = 0, to = AHEAD;   // buffers of stage s and of the stage that is started beside it
     for (int s = 0; s < total; ++s) {
       // this wave's copies of the stage are there, then everyone's; the readers of the buffer before it are done
-      if (s + AHEAD <= total) wait_copies<(AHEAD - 1) * COPIES>();
-      else wait_copies<0>();
+      if constexpr (T::STAGES == 1) {
+        if (s > 0) {
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          issue(0);
+        }
+        wait_copies<0>();
+      } else {
+        if (s + AHEAD <= total) wait_copies<AHEAD * COPIES - COPIES>();
+        else wait_copies<0>();
+      }
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + AHEAD < total) issue(to);
+      if (AHEAD > 0 && s + AHEAD < total) issue(to);
       const char* stage = smem + from * T::STAGE;
       from = from + 1 == T::STAGES ? 0 : from + 1;
       to = to + 1 == T::STAGES ? 0 : to + 1;
@@ -485,10 +497,13 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     }
     if (MODE == VM_GRAD || p.G) {
       // The tile as rows of G: a lane has four neighbours of a row, a wave 32 rows, so it passes through LDS (slot s of
-      // 16 bytes of row n at s ^ n % slots) to be written in whole lines.  fp32: part by part.
+      // 16 bytes of row n at s ^ n % slots) to be written in whole lines.  fp32: part by part; exponentials, which are not
+      // multiplied yet, as the upper and the lower 16 bits of the number.
       constexpr int SLOTS = T::BM / 8;
+      constexpr int PLANES = !PARTS ? 1 : MODE == VM_STATS ? 2 : VOCAB_PARTS;
+      static_assert(T::TILE <= T::STAGES * T::STAGE, "in the stages' memory");
 #pragma unroll 1
-      for (int part = 0; part < (PARTS ? VOCAB_PARTS : 1); ++part) {
+      for (int part = 0; part < PLANES; ++part) {
         if (part) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
@@ -503,6 +518,9 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
                 const float v = acc[i][j][4 * q + r];
                 if constexpr (__is_same(E, _Float16)) {
                   x.v[r] = (E)(v * VOCAB_F16_SCALE);
+                } else if constexpr (PARTS && MODE == VM_STATS) {
+                  const uint32_t bits = __float_as_uint(v);
+                  x.v[r] = __builtin_bit_cast(E, (uint16_t)(part ? bits : bits >> 16));
                 } else {
                   x.v[r] = (E)v;
                   if constexpr (PARTS) acc[i][j][4 * q + r] = __builtin_isfinite(v) ? v - (float)x.v[r] : 0.f;
@@ -517,9 +535,11 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
 #pragma unroll 4
         for (int at = threadIdx.x; at < T::BN * SLOTS; at += T::NT) {
           const int col = at / SLOTS, slot = at % SLOTS;
-          if (n0 + col < p.g_rows)
-            *(Words*)(g + (int64_t)(n0 + col) * p.ldg + 8 * slot) =
-                *(const Words*)(smem + col * (2 * T::BM) + 16 * (slot ^ (col % SLOTS)));
+          if (n0 + col >= p.g_rows) continue;
+          E* to = g + (int64_t)(n0 + col) * p.ldg + 8 * slot;
+          *(Words*)to = *(const Words*)(smem + col * (2 * T::BM) + 16 * (slot ^ (col % SLOTS)));
+          // no one makes the third part of rows that do not count
+          if (PARTS && MODE == VM_STATS && part == 1 && n0 + col >= N) *(Words*)(to + p.g_part) = zero_words();
         }
       }
     } else {
@@ -566,38 +586,65 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     }
   } else {
     const float scale = p.scale / (float)max(live, 1);
+    const bool wide = PARTS || p.out_elem == TE_F32;
+    if (sum_cols) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = n0 + wn + 32 * j + ln;
-      if (sum_cols) {
+      for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn + 32 * j + ln;
         const float sum = col_sum[j] + __shfl_xor(col_sum[j], 32);
         if (half == 0 && n < N) store_elem(p.db, p.elem, n, sum * scale);
       }
-      if (n >= N) continue;
-      const int64_t row = (int64_t)(MODE == VM_DX ? p.source[n] : n) * p.M;
+    }
+    // 16-bit rows pass through LDS as those of G do, fp32 ones go out four neighbours a lane
+    constexpr int SLOTS = T::BM / 8;
+    if (!wide) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int col = wn + 32 * j + ln, n = n0 + col;
+      const int64_t row = n < N ? (int64_t)(MODE == VM_DX ? p.source[n] : n) * p.M : 0;
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int m = m0 + wm + 32 * i + 8 * q + 4 * half;
-          if (m + 4 <= p.M) {
-            if (PARTS || p.out_elem == TE_F32) {
+          if (!wide) {
+            Pack<E, 4> x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x.v[r] = (E)(acc[i][j][4 * q + r] * scale);
+            const int slot = ((wm + 32 * i) / 8 + q) ^ (col % SLOTS);
+            *(Pack<E, 4>*)__builtin_assume_aligned(smem + col * (2 * T::BM) + 16 * slot + 8 * half, 8) = x;
+          } else if (n < N) {
+            const int m = m0 + wm + 32 * i + 8 * q + 4 * half;
+            float* out = (float*)p.out + row + m;
+            if (m + 4 <= p.M) {
               Pack<float, 4> x;
 #pragma unroll
               for (int r = 0; r < 4; ++r) x.v[r] = acc[i][j][4 * q + r] * scale;
-              store_pack((float*)p.out + row + m, x);
+              store_pack(out, x);
             } else {
-              Pack<E, 4> x;
 #pragma unroll
-              for (int r = 0; r < 4; ++r) x.v[r] = (E)(acc[i][j][4 * q + r] * scale);
-              store_pack((E*)p.out + row + m, x);
+              for (int r = 0; r < 4; ++r)
+                if (m + r < p.M) out[r] = acc[i][j][4 * q + r] * scale;
             }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (m + r < p.M) store_elem(p.out, p.out_elem, row + m + r, acc[i][j][4 * q + r] * scale);
           }
         }
+    }
+    if (!wide) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll 4
+      for (int at = threadIdx.x; at < T::BN * SLOTS; at += T::NT) {
+        const int col = at / SLOTS, slot = at % SLOTS, n = n0 + col, m = m0 + 8 * slot;
+        if (n >= N || m >= p.M) continue;
+        const Words x = *(const Words*)(smem + col * (2 * T::BM) + 16 * (slot ^ (col % SLOTS)));
+        E* out = (E*)p.out + (int64_t)(MODE == VM_DX ? p.source[n] : n) * p.M + m;
+        if (m + 8 <= p.M) {
+          __builtin_memcpy(out, &x, 16);
+        } else {
+          const Pack<E, 8> y = __builtin_bit_cast(Pack<E, 8>, x);
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (m + r < p.M) out[r] = y.v[r];
+        }
+      }
     }
   }
 }
@@ -608,15 +655,17 @@ __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4) vocab_logi
   vocab_tile<T, MODE, E, PARTS>(p, smem, blockIdx.x);
 }
 
-// dX and dW of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the CUs that dX's few long
+// dX (tiles T) and dW (tiles W) of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the CUs that dX's few long
 // ones leave.  dX's come first; the last workgroup takes the loss where `loss` is given.
-template <class T, class E, bool PARTS>
+template <class T, class W, class E, bool PARTS>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
     vocab_grads_kernel(VocabArgs dx, VocabArgs dw, uint32_t dx_blocks, const float* logp, int rows, float* loss) {
-  __shared__ __attribute__((aligned(1024))) char smem[T::RED_AT];
+  static_assert(T::NT == W::NT && W::STAGES * W::STAGE <= T::STAGES * T::STAGE && T::TILE <= T::STAGES * T::STAGE &&
+                    W::TILE <= T::STAGES * T::STAGE, "dX's stages hold dW's, and the tiles of both");
+  __shared__ __attribute__((aligned(1024))) char smem[T::STAGES * T::STAGE];
   if (loss && blockIdx.x + 1 == gridDim.x) vocab_loss<T::WAVES>(logp, rows, *dx.live, loss, (float*)smem);
   else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, PARTS>(dx, smem, blockIdx.x);
-  else vocab_tile<T, VM_DW, E, PARTS>(dw, smem, blockIdx.x - dx_blocks);
+  else vocab_tile<W, VM_DW, E, PARTS>(dw, smem, blockIdx.x - dx_blocks);
 }
 
 // Workgroups for `tiles` tiles at most, a whole number per XCD.
@@ -629,12 +678,12 @@ inline void launch_vocab_logits(const VocabArgs& p, bool stats, hipStream_t stre
   else hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
 }
 
-template <class T, class E, bool PARTS>
+template <class T, class W, class E, bool PARTS>
 inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                                hipStream_t stream) {
   const int64_t first = vocab_blocks(ceil_div(dx.M, T::BM) * ceil_div(dx.N, T::BN) * dx.splits);
-  const int64_t all = first + vocab_blocks(ceil_div(dw.M, T::BM) * ceil_div(dw.N, T::BN) * dw.splits) + (loss ? 1 : 0);
-  hipLaunchKernelGGL((vocab_grads_kernel<T, E, PARTS>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
+  const int64_t all = first + vocab_blocks(ceil_div(dw.M, W::BM) * ceil_div(dw.N, W::BN) * dw.splits) + (loss ? 1 : 0);
+  hipLaunchKernelGGL((vocab_grads_kernel<T, W, E, PARTS>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
                      logp, rows, loss);
 }
 
@@ -647,6 +696,8 @@ typedef VocabTile<2, 2, 2, 2, 2, 2> VocabMid;
 typedef VocabTile<2, 2, 2, 2, 4, 1> VocabDeep;
 typedef VocabTile<1, 2, 4, 1, 3, 2> VocabSlim;
 typedef VocabTile<1, 2, 4, 1, 6, 1> VocabThin;
+// dW beside Slim's dX: its rows are k, one stage of them, so that the tile's stores are its time
+typedef VocabTile<1, 8, 4, 1, 1, 2> VocabWide;
 
 enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4 };
 

@@ -20,11 +20,11 @@ template <class E, bool PARTS>
 void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                  hipStream_t stream) {
   switch (tile) {
-    case VT_LARGE: launch_vocab_grads<VocabLarge, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
-    case VT_MID: launch_vocab_grads<VocabMid, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
-    case VT_DEEP: launch_vocab_grads<VocabDeep, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
-    case VT_THIN: launch_vocab_grads<VocabThin, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
-    default: launch_vocab_grads<VocabSlim, E, PARTS>(dx, dw, logp, rows, loss, stream);
+    case VT_LARGE: launch_vocab_grads<VocabLarge, VocabLarge, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    case VT_MID: launch_vocab_grads<VocabMid, VocabMid, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    case VT_DEEP: launch_vocab_grads<VocabDeep, VocabDeep, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    case VT_THIN: launch_vocab_grads<VocabThin, VocabThin, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    default: launch_vocab_grads<VocabSlim, VocabWide, E, PARTS>(dx, dw, logp, rows, loss, stream);
   }
 }
 
