@@ -394,11 +394,12 @@ inline bool vocab_direct(int elem, int64_t D, const void* weight, int64_t ld) {
   return elem != TE_F32 && D % 8 == 0 && ld % 8 == 0 && (uintptr_t)weight % 16 == 0;
 }
 
-inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n) {
+inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
   switch (tile) {
-    case VT_LARGE: return ceil_div(m, VocabLarge::BM) * ceil_div(n, VocabLarge::BN);
+    case VT_LARGE:
+      return ceil_div(m, VocabLarge<false>::BM) * ceil_div(n, parts > 1 ? VocabLarge<true>::BN : VocabLarge<false>::BN);
     case VT_SLIM:
-    case VT_THIN: return ceil_div(m, VocabSlim::BM) * ceil_div(n, VocabSlim::BN);
+    case VT_THIN: return ceil_div(m, VocabSlim<false>::BM) * ceil_div(n, VocabSlim<false>::BN);
     default: return ceil_div(m, VocabMid::BM) * ceil_div(n, VocabMid::BN);
   }
 }
@@ -425,29 +426,29 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   }
   const int64_t in_piece = p.piece < V ? p.piece : V;
   // by the whole vocabulary, so that the statistics have the same bits with and without gradients and whatever the room
-  if (N <= VocabSlim::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N) > 256 ? VT_SLIM : VT_THIN;
-  else if (vocab_tile_count(VT_LARGE, V, N) >= 200) p.logits_tile = VT_LARGE;
-  else p.logits_tile = vocab_tile_count(VT_MID, V, N) > 256 ? VT_MID : VT_DEEP;
-  p.tiles = vocab_tile_count(p.logits_tile, V, 1);
+  if (N <= VocabSlim<false>::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N, p.parts) > 256 ? VT_SLIM : VT_THIN;
+  else if (vocab_tile_count(VT_LARGE, V, N, p.parts) >= 200) p.logits_tile = VT_LARGE;
+  else p.logits_tile = p.parts == 1 && vocab_tile_count(VT_MID, V, N, p.parts) > 256 ? VT_MID : VT_DEEP;
+  p.tiles = vocab_tile_count(p.logits_tile, V, 1, p.parts);
   p.grads_tile = VT_SLIM;
   p.dx_splits = p.dw_splits = 1;
   p.dx_joined = p.dw_joined = false;
   if (grad) {
-    if (N <= VocabSlim::BN) {
-      const int64_t slim = vocab_tile_count(VT_SLIM, D, N) + vocab_tile_count(VT_SLIM, D, in_piece);
+    if (N <= VocabSlim<false>::BN) {
+      const int64_t slim = vocab_tile_count(VT_SLIM, D, N, p.parts) + vocab_tile_count(VT_SLIM, D, in_piece, p.parts);
       p.grads_tile = slim > 256 ? VT_SLIM : VT_THIN;
     } else {
-      const int64_t large = vocab_tile_count(VT_LARGE, D, N) + vocab_tile_count(VT_LARGE, D, in_piece);
-      const int64_t mid = vocab_tile_count(VT_MID, D, N) + vocab_tile_count(VT_MID, D, in_piece);
-      p.grads_tile = large >= 200 ? VT_LARGE : mid > 256 ? VT_MID : VT_DEEP;
+      const int64_t large = vocab_tile_count(VT_LARGE, D, N, p.parts) + vocab_tile_count(VT_LARGE, D, in_piece, p.parts);
+      const int64_t mid = vocab_tile_count(VT_MID, D, N, p.parts) + vocab_tile_count(VT_MID, D, in_piece, p.parts);
+      p.grads_tile = large >= 200 ? VT_LARGE : p.parts == 1 && mid > 256 ? VT_MID : VT_DEEP;
     }
     // Sums are cut along k so that none of them takes longer than a good part of the whole launch, nor than it takes to
     // add one more piece's sums (some eight stages).
     const int64_t slots = p.grads_tile == VT_MID || p.grads_tile == VT_SLIM ? 512 : 256;
-    const int64_t dx = vocab_tile_count(p.grads_tile, D, N), dw = vocab_tile_count(p.grads_tile, D, in_piece);
+    const int64_t dx = vocab_tile_count(p.grads_tile, D, N, p.parts), dw = vocab_tile_count(p.grads_tile, D, in_piece, p.parts);
     const int64_t dx_steps = ceil_div(in_piece, 64), dw_steps = ceil_div(N, 64);
     int64_t most = (dx * dx_steps + dw * (dw_steps + 4)) / slots / 3;
-    const int64_t least = p.parts > 1 ? 2 : 8;      // six stages a step in parts
+    const int64_t least = p.parts > 1 ? 3 : 8;      // six products a step in parts
     if (most < least) most = least;
     auto cut = [&](int64_t steps, int64_t rows) {
       int64_t splits = ceil_div(steps, most), fits = (128LL << 20) / (4 * rows * p.Dp);
@@ -620,7 +621,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   soft.part = part;
   soft.part_ld = p.tiles;
   soft.tiles = (int)p.tiles;
-  soft.tile = p.logits_tile == VT_LARGE ? VocabLarge::BM : VocabMid::BM;
+  soft.tile = p.logits_tile == VT_LARGE ? VocabLarge<false>::BM : VocabMid::BM;
   soft.chosen = chosen;
   soft.token = token;
   soft.source = source;

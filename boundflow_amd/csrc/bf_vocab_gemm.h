@@ -14,8 +14,10 @@
 // k of its column, so that no operand is transposed in memory.
 //
 // fp32 values come as three bf16 parts, x = x0 + x1 + x2 (8 + 8 + 8 significant bits); a product is the sum of six
-// part products, least first: x2 y0, x0 y2, x1 y1, x1 y0, x0 y1, x0 y0, one after another along k into the same
-// fp32 sums.  What is left out is 2^-24 of a product.
+// part products, least first: x0 y2, x1 y1, x2 y0, x0 y1, x1 y0, x0 y0, into the same fp32 sums.  What is left out is
+// 2^-24 of a product.  A stage holds the three parts of both operands, each read from LDS once for two products (the six one after
+// another along k, a part of each operand in a stage: 2048 x 1024 rows over 32000 tokens 2041 us in the place of 1667, a head of eight
+// actions 45 us in the place of 40).
 #pragma once
 
 #include "bf_train.h"
@@ -36,8 +38,8 @@ enum : int { VM_STATS = 0, VM_GRAD = 1, VM_DX = 2, VM_DW = 3 };
 // given the exponentials themselves, 2^(c (z - the tile's largest)); vocab_softmax_kernel makes them G in place.  VM_GRAD, with the rows'
 // statistics known: G.
 
-constexpr int VOCAB_BK = 64;            // k of a stage
-constexpr int VOCAB_PARTS = 3, VOCAB_PAIRS = 6;
+constexpr int VOCAB_BK = 64;            // k come in multiples of this
+constexpr int VOCAB_PARTS = 3;
 // fp16 holds G times this: p - [v = y] lies within [-1, 1], and a probability below 2^-24 would be subnormal
 constexpr float VOCAB_F16_SCALE = 16384.f;
 
@@ -76,13 +78,16 @@ struct VocabArgs {
   float scale;               // of out and db, before the division by the rows that count
 };
 
-// Tiles of BM x BN, NWM x NWN waves of 32 FM x 32 FN each; STAGES of LDS, OCC workgroups on a CU.
-template <int FM_, int FN_, int NWM_, int NWN_, int STAGES_, int OCC_>
+// Tiles of BM x BN, NWM x NWN waves of 32 FM x 32 FN each; STAGES of LDS, OCC workgroups on a CU.  FUSED: three
+// parts of fp32 operands in a stage.
+template <int FM_, int FN_, int NWM_, int NWN_, int STAGES_, int OCC_, bool FUSED_>
 struct VocabTile {
   static constexpr int FM = FM_, FN = FN_, NWM = NWM_, NWN = NWN_, STAGES = STAGES_, OCC = OCC_;
+  static constexpr bool FUSED = FUSED_;
+  static constexpr int BK = FUSED ? 32 : 64, PLANES = FUSED ? VOCAB_PARTS : 1;   // k of a stage, parts in it
   static constexpr int BM = 32 * FM * NWM, BN = 32 * FN * NWN, WAVES = NWM * NWN, NT = 64 * WAVES;
-  static constexpr int A_BYTES = BM * VOCAB_BK * 2, B_BYTES = BN * VOCAB_BK * 2;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
+  static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2, A_BYTES = PLANES * A_PLANE;
+  static constexpr int STAGE = A_BYTES + PLANES * B_PLANE;
   // behind the stages: the bias of the tile's rows, two floats per column from each half of a wave along M
   static constexpr int BIAS_AT = STAGES * STAGE, RED_AT = BIAS_AT + 4 * BM, LDS = RED_AT + 2 * 4 * 2 * NWM * BN;
   static constexpr int TILE = 2 * BM * BN;   // of 16-bit results
@@ -111,43 +116,36 @@ struct Vec8<_Float16> {
   typedef f16x8v type;
 };
 
-// One operand's stages: SIDE rows or columns of the tile.
+// One operand's stages: SIDE rows or columns of the tile, BK k of them.
 //
-// LDS of a stage, in slots of 16 bytes.  k contiguous: row r of 8 slots, slot s holding chunk s ^ (r / 2 % 8), so that the
-// 16 lanes which read one chunk of 16 rows together meet all 64 banks (r % 8 in its place: half of them, twice; the
-// reads of z took 1.3 times their cycles).  k in rows (TR): row k of SIDE / 8 slots, slot s holding
+// LDS of a stage, in slots of 16 bytes.  k contiguous: row r of BK / 8 slots, slot s holding chunk s ^ swap(r), so that the
+// 16 lanes which read one chunk of 16 rows together meet all 64 banks (r % 8 in the place of r / 2 % 8 for 64 k: half of
+// them, twice; the reads of z took twice their cycles).  k in rows (TR): row k of SIDE / 8 slots, slot s holding
 // chunk s ^ swap(k): 32 lanes read 64 bytes of four rows of k together, which meet all banks.
-template <bool TR, int SIDE, int WAVES>
+template <bool TR, int SIDE, int WAVES, int BK>
 struct VocabOperand {
-  static constexpr int COPIES = SIDE * VOCAB_BK * 2 / 1024;     // of 1 KB, one wave each
+  static constexpr int COPIES = SIDE * BK * 2 / 1024;     // of 1 KB, one wave each
   static constexpr int PER_WAVE = (COPIES + WAVES - 1) / WAVES;
+  static constexpr int SLOTS = TR ? SIDE / 8 : BK / 8, ROWS = 64 / SLOTS;   // slots of a row, rows of a copy
   static_assert(!TR || SIDE >= 64, "the slots' permutation spans 8 of them, or 16");
   static_assert(COPIES % WAVES == 0, "every wave makes the same copies");
   uint32_t off[PER_WAVE];   // bytes from the stage's first k
-  int krow[PER_WAVE];       // TR: the row of k that a lane copies
 
-  static __device__ __forceinline__ int swap(int k) { return SIDE >= 128 ? 4 * (k & 3) : 4 * ((k >> 1) & 1); }
-
-  // k contiguous: the eight k that a lane copies
-  static __device__ __forceinline__ int chunk(int copy, int lane) { return (lane & 7) ^ ((4 * copy + (lane >> 4)) & 7); }
+  static __device__ __forceinline__ int swap(int row) {
+    if (TR) return SIDE >= 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1);
+    return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+  }
+  // the row and the chunk of eight elements of it that a lane copies
+  static __device__ __forceinline__ int row(int copy, int lane) { return copy * ROWS + lane / SLOTS; }
+  static __device__ __forceinline__ int chunk(int copy, int lane) { return (lane % SLOTS) ^ swap(row(copy, lane)); }
 
   // first: the tile's first row (k contiguous) or column (TR)
   __device__ __forceinline__ void set(int wave, int lane, int first, int rows, int cols, int64_t ld) {
 #pragma unroll
     for (int j = 0; j < PER_WAVE; ++j) {
-      const int copy = wave * PER_WAVE + j;
-      if constexpr (TR) {
-        constexpr int SLOTS = SIDE / 8;
-        const int k = copy * (64 / SLOTS) + lane / SLOTS;
-        int col = first + 8 * ((lane % SLOTS) ^ swap(k));
-        if (col > cols - 8) col = cols - 8;
-        krow[j] = k;
-        off[j] = (uint32_t)(2 * (k * ld + col));
-      } else {
-        int r = first + 8 * copy + (lane >> 3);
-        if (r > rows - 1) r = rows - 1;
-        off[j] = (uint32_t)(2 * ((int64_t)(r - first) * ld + 8 * chunk(copy, lane)));
-      }
+      const int copy = wave * PER_WAVE + j, r = row(copy, lane), c = 8 * chunk(copy, lane);
+      if constexpr (TR) off[j] = (uint32_t)(2 * (r * ld + min(first + c, cols - 8)));
+      else off[j] = (uint32_t)(2 * (min(r, rows - 1 - first) * ld + c));
     }
   }
 
@@ -162,9 +160,9 @@ struct VocabOperand {
   __device__ __forceinline__ void copy_last(const char* base, int64_t ld, int left, int wave, int lane, uint32_t dst) const {
 #pragma unroll
     for (int j = 0; j < PER_WAVE; ++j) {
-      const int past = TR ? krow[j] - (left - 1) : 8 * chunk(wave * PER_WAVE + j, lane) - (left - 8);
-      copy16_to_lds(base, off[j] - (past > 0 ? (uint32_t)(2 * past * (TR ? ld : 1)) : 0),
-                    dst + (wave * PER_WAVE + j) * 1024);
+      const int copy = wave * PER_WAVE + j;
+      const int past = TR ? row(copy, lane) - (left - 1) : 8 * chunk(copy, lane) - (left - 8);
+      copy16_to_lds(base, off[j] - (past > 0 ? (uint32_t)(2 * past * (TR ? ld : 1)) : 0), dst + copy * 1024);
     }
   }
 
@@ -181,7 +179,7 @@ struct VocabOperand {
       return __builtin_bit_cast(V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       const int r = side + (lane & 31);
-      return *(const V*)(stage + r * 128 + (((2 * kk + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4));
+      return *(const V*)(stage + r * (2 * BK) + (((2 * kk + (lane >> 5)) ^ swap(lane & 31)) << 4));
     }
   }
 };
@@ -235,8 +233,10 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   constexpr bool A_TR = MODE >= VM_DX, B_TR = MODE == VM_DW;
   constexpr int FM = T::FM, FN = T::FN;
   typedef typename Vec8<E>::type V8;
-  typedef VocabOperand<A_TR, T::BM, T::WAVES> OpA;
-  typedef VocabOperand<B_TR, T::BN, T::WAVES> OpB;
+  typedef VocabOperand<A_TR, T::BM, T::WAVES, T::BK> OpA;
+  typedef VocabOperand<B_TR, T::BN, T::WAVES, T::BK> OpB;
+  constexpr int BK = T::BK, PLANES = T::PLANES;
+  static_assert(PARTS == T::FUSED, "three parts in a stage");
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -260,47 +260,45 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   const int tm = 8 * group + in_group % width, tn = in_group / width;
   const int m0 = tm * T::BM, n0 = tn * T::BN;
 
-  int steps = MODE == VM_DW ? (live + VOCAB_BK - 1) / VOCAB_BK : p.K / VOCAB_BK, k_first = 0;
+  int steps = (MODE == VM_DW ? (live + VOCAB_BK - 1) / VOCAB_BK * VOCAB_BK : p.K) / BK, k_first = 0;
   if constexpr (MODE >= VM_DX) {
     const int per = (steps + splits - 1) / splits;
     k_first = split * per;
     steps = max(0, min(per, steps - k_first));
   }
-  const int total = PARTS ? steps * VOCAB_PAIRS : steps;
 
   OpA opa;
   OpB opb;
   opa.set(wave, lane, m0, p.a_rows, p.a_cols, p.lda);
   opb.set(wave, lane, n0, p.b_rows, p.b_cols, p.ldb);
-  const int64_t a_step = 2 * (A_TR ? p.lda * VOCAB_BK : VOCAB_BK), b_step = 2 * (B_TR ? p.ldb * VOCAB_BK : VOCAB_BK);
-  const char* a_first = (const char*)p.A + (A_TR ? 0 : 2 * (int64_t)m0 * p.lda) + k_first * a_step;
-  const char* b_first = (const char*)p.B + (B_TR ? 0 : 2 * (int64_t)n0 * p.ldb) + k_first * b_step;
-  const char *a_at = a_first, *b_at = b_first;
+  const int64_t a_step = 2 * (A_TR ? p.lda * BK : BK), b_step = 2 * (B_TR ? p.ldb * BK : BK);
+  const char* a_at = (const char*)p.A + (A_TR ? 0 : 2 * (int64_t)m0 * p.lda) + k_first * a_step;
+  const char* b_at = (const char*)p.B + (B_TR ? 0 : 2 * (int64_t)n0 * p.ldb) + k_first * b_step;
   const uint32_t lds0 = (uint32_t)(uintptr_t)((lds_char*)smem);
-  int pair = 0, ks = 0;
-  if constexpr (PARTS) a_at = a_first + 2 * 2 * p.a_part;   // a2 b0 first
+  int ks = 0;
 
   auto issue = [&](int buffer) {
     const uint32_t dst = lds0 + buffer * T::STAGE;
     // the weight's rows end where the width does and the weight where the vocabulary does; everything else has zeros up
     // to a whole stage
-    const int left = (MODE == VM_DX ? p.a_rows : MODE == VM_DW ? VOCAB_BK : p.a_cols) -
-                     (MODE == VM_DW ? 0 : (k_first + ks) * VOCAB_BK);
-    if (left < VOCAB_BK) opa.copy_last(a_at, p.lda, left, wave, lane, dst);
-    else opa.copy(a_at, wave, dst);
-    opb.copy(b_at, wave, dst + T::A_BYTES);
+    int left = MODE == VM_DW ? BK : (MODE == VM_DX ? p.a_rows : p.a_cols) - (k_first + ks) * BK;
+    const char* from = a_at;
+    if (MODE == VM_DX && left < 1) {      // a stage past the end, in the padding of k: the last row alone
+      from -= 2 * (1 - left) * p.lda;
+      left = 1;
+    }
+#pragma unroll
+    for (int part = 0; part < PLANES; ++part) {
+      const uint32_t to = dst + part * T::A_PLANE;
+      if (left < BK) opa.copy_last(from + 2 * part * p.a_part, p.lda, left, wave, lane, to);
+      else opa.copy(from + 2 * part * p.a_part, wave, to);
+    }
+#pragma unroll
+    for (int part = 0; part < PLANES; ++part)
+      opb.copy(b_at + 2 * part * p.b_part, wave, dst + T::A_BYTES + part * T::B_PLANE);
     a_at += a_step;
     b_at += b_step;
-    if (++ks == steps) {
-      ks = 0;
-      ++pair;
-      if constexpr (PARTS) {
-        // parts of (A, B) in turn: 2 0, 0 2, 1 1, 1 0, 0 1, 0 0
-        const int pa = (0b000001010010 >> (2 * pair)) & 3, pb = (0b000100011000 >> (2 * pair)) & 3;
-        a_at = a_first + 2 * pa * p.a_part;
-        b_at = b_first + 2 * pb * p.b_part;
-      }
-    }
+    ++ks;
   };
 
   float* bias = (float*)(smem + T::BIAS_AT);
@@ -322,9 +320,9 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   const bool sum_cols = MODE == VM_DW && p.db && tm == 0 && wave % T::NWM == 0;
 #pragma unroll
   for (int j = 0; j < FN; ++j) col_sum[j] = 0.f;
-  // G's column sums, the bias's gradient: every part of G once, beside the first part of X
-  auto column_sums = [&](int s, const V8* x) {
-    if (sum_cols && (!PARTS || (s >= steps && s < 2 * steps) || s >= 4 * steps)) {
+  // G's column sums, the bias's gradient
+  auto column_sums = [&](const V8* x) {
+    if (sum_cols) {
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -332,41 +330,55 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     }
   };
 
+  auto multiply = [&](const V8 (&a)[PLANES][FM], const V8 (&b)[PLANES][FN]) {
+#pragma unroll
+    for (int sum = PLANES - 1; sum >= 0; --sum)     // the least products first
+#pragma unroll
+      for (int part = 0; part <= sum; ++part)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[part][i], b[sum - part][j], acc[i][j]);
+    if constexpr (MODE == VM_DW) {
+#pragma unroll
+      for (int part = 0; part < PLANES; ++part) column_sums(b[part]);
+    }
+  };
+
   if constexpr (T::WAVES == 8) {
     // Two groups of four waves, one wave of each on a SIMD, take turns: while one multiplies what it has in registers
-    // (half a stage, 16 products in 512 cycles) the other reads its next half stage from LDS and starts the copies
+    // (half a stage, 16 products in 512 cycles; fp32: 24 in 768) the other reads its next half stage from LDS and starts the copies
     // of the next stage.  A buffer is written again when the second group has read its last half, and has to be there
     // three turns later.
     static_assert(T::STAGES == 2, "two buffers in turn");
     const bool second = wave >= 4;
-    if (total > 0) issue(0);
+    if (steps > 0) issue(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (second) asm volatile("s_barrier" ::: "memory");
-    for (int s = 0; s < total; ++s) {
+    for (int s = 0; s < steps; ++s) {
       const char* stage = smem + (s & 1) * T::STAGE;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        V8 a[2][FM], b[2][FN];
+        constexpr int KK = BK / 32;     // 16 k each, of half a stage
+        V8 a[KK][PLANES][FM], b[KK][PLANES][FN];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < KK; ++k)
 #pragma unroll
-          for (int i = 0; i < FM; ++i) a[k][i] = OpA::template read<V8>(stage, wm + 32 * i, 2 * h + k, lane);
+          for (int part = 0; part < PLANES; ++part) {
 #pragma unroll
-          for (int j = 0; j < FN; ++j) b[k][j] = OpB::template read<V8>(stage + T::A_BYTES, wn + 32 * j, 2 * h + k, lane);
-        }
-        if (h == 0 && s + 1 < total) issue((s + 1) & 1);
+            for (int i = 0; i < FM; ++i)
+              a[k][part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, KK * h + k, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+              b[k][part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, KK * h + k, lane);
+          }
+        if (h == 0 && s + 1 < steps) issue((s + 1) & 1);
         if (h == 1 && second) wait_copies<0>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[k][i], b[k][j], acc[i][j]);
-          if constexpr (MODE == VM_DW) column_sums(s, b[k]);
-        }
+        for (int k = 0; k < KK; ++k) multiply(a[k], b[k]);
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
         if (h == 1 && !second) wait_copies<0>();
@@ -376,15 +388,15 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     if (!second) asm volatile("s_barrier" ::: "memory");
   } else {
     // All but one of the stages are under way.
-    constexpr int AHEAD = T::STAGES - 1, COPIES = OpA::PER_WAVE + OpB::PER_WAVE;
+    constexpr int AHEAD = T::STAGES - 1, COPIES = PLANES * (OpA::PER_WAVE + OpB::PER_WAVE);
     if constexpr (T::STAGES == 1) {
       // for sums of one stage: the workgroups beside this one hide its copies
-      if (total > 0) issue(0);
+      if (steps > 0) issue(0);
     }
     static_assert(AHEAD * COPIES < 64 + COPIES, "what vmcnt counts");
-    for (int s = 0; s < AHEAD && s < total; ++s) issue(s);
+    for (int s = 0; s < AHEAD && s < steps; ++s) issue(s);
     int from = 0, to = AHEAD;   // buffers of stage s and of the stage that is started beside it
-    for (int s = 0; s < total; ++s) {
+    for (int s = 0; s < steps; ++s) {
       // this wave's copies of the stage are there, then everyone's; the readers of the buffer before it are done
       if constexpr (T::STAGES == 1) {
         if (s > 0) {
@@ -393,26 +405,27 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
         }
         wait_copies<0>();
       } else {
-        if (s + AHEAD <= total) wait_copies<AHEAD * COPIES - COPIES>();
+        if (s + AHEAD <= steps) wait_copies<AHEAD * COPIES - COPIES>();
         else wait_copies<0>();
       }
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (AHEAD > 0 && s + AHEAD < total) issue(to);
+      if (AHEAD > 0 && s + AHEAD < steps) issue(to);
       const char* stage = smem + from * T::STAGE;
       from = from + 1 == T::STAGES ? 0 : from + 1;
       to = to + 1 == T::STAGES ? 0 : to + 1;
 #pragma unroll
-      for (int kk = 0; kk < VOCAB_BK / 16; ++kk) {
-        V8 a[FM], b[FN];
+      for (int kk = 0; kk < BK / 16; ++kk) {
+        V8 a[PLANES][FM], b[PLANES][FN];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) a[i] = OpA::template read<V8>(stage, wm + 32 * i, kk, lane);
+        for (int part = 0; part < PLANES; ++part) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) b[j] = OpB::template read<V8>(stage + T::A_BYTES, wn + 32 * j, kk, lane);
+          for (int i = 0; i < FM; ++i)
+            a[part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, kk, lane);
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[i], b[j], acc[i][j]);
-        if constexpr (MODE == VM_DW) column_sums(s, b);
+          for (int j = 0; j < FN; ++j)
+            b[part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, kk, lane);
+        }
+        multiply(a, b);
       }
     }
   }
@@ -687,17 +700,22 @@ inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const f
                      logp, rows, loss);
 }
 
-// Tiles by the size of the problem.
+// Tiles by the size of the problem (P: for fp32 in parts).
 // Large: the products' rate.  Mid: where Large would leave CUs without a tile.  Slim: up to 64 rows, where the
 // weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU.  Deep and
 // Thin are these with more stages under way for grids of at most a workgroup per CU, whose time is the copies' latency.
-typedef VocabTile<4, 2, 2, 4, 2, 1> VocabLarge;
-typedef VocabTile<2, 2, 2, 2, 2, 2> VocabMid;
-typedef VocabTile<2, 2, 2, 2, 4, 1> VocabDeep;
-typedef VocabTile<1, 2, 4, 1, 3, 2> VocabSlim;
-typedef VocabTile<1, 2, 4, 1, 6, 1> VocabThin;
+template <bool P>
+using VocabLarge = VocabTile<P ? 2 : 4, 2, P ? 4 : 2, P ? 2 : 4, 2, 1, P>;
+template <bool P>
+using VocabDeep = VocabTile<2, 2, 2, 2, P ? 3 : 4, 1, P>;
+template <bool P>
+using VocabThin = VocabTile<1, 2, 4, 1, P ? 4 : 6, 1, P>;
+template <bool P>
+using VocabSlim = VocabTile<1, 2, 4, 1, P ? 2 : 3, 2, P>;
+typedef VocabTile<2, 2, 2, 2, 2, 2, false> VocabMid;      // in parts it would be Deep
 // dW beside Slim's dX: its rows are k, one stage of them, so that the tile's stores are its time
-typedef VocabTile<1, 8, 4, 1, 1, 2> VocabWide;
+template <bool P>
+using VocabWide = VocabTile<1, 8, 4, 1, 1, 2, P>;
 
 enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4 };
 
