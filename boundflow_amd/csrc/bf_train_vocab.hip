@@ -333,7 +333,9 @@ __device__ __forceinline__ void join_chunk(const float* from, int64_t split, int
   if (d + 8 <= D) {
     store_pack(out + d, y);
   } else {
-    for (int k = 0; d + k < D; ++k) out[d + k] = y.v[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)     // unrolled: an array that is indexed by a loop lies in LDS, which took 15 us in the place of 5
+      if (d + k < D) out[d + k] = y.v[k];
   }
 }
 
@@ -450,14 +452,15 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
     int64_t most = (dx * dx_steps + dw * (dw_steps + 4)) / slots / 3;
     const int64_t least = p.parts > 1 ? 3 : 8;      // six products a step in parts
     if (most < least) most = least;
-    auto cut = [&](int64_t steps, int64_t rows) {
+    auto cut = [&](int64_t steps, int64_t rows, int64_t limit) {
       int64_t splits = ceil_div(steps, most), fits = (128LL << 20) / (4 * rows * p.Dp);
       if (splits > fits) splits = fits;
-      if (splits > 32) splits = 32;
+      if (splits > limit) splits = limit;
       return (int)(splits < 1 ? 1 : splits);
     };
-    p.dx_splits = cut(dx_steps, p.rows);
-    p.dw_splits = p.piece < V ? 1 : cut(dw_steps, V);
+    p.dx_splits = cut(dx_steps, p.rows, 32);
+    // dw's pieces are rows of the vocabulary each: only where it leaves CUs without a tile
+    p.dw_splits = p.piece < V ? 1 : cut(dw_steps, V, slots / dw < 32 ? slots / dw : 32);
     p.dx_joined = p.dx_splits > 1 || p.piece < V;
     p.dw_joined = p.dw_splits > 1;
   }

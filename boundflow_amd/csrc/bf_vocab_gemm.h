@@ -330,6 +330,20 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     }
   };
 
+  auto fragments = [&](const char* stage, int first, auto& a, auto& b) {
+    constexpr int KK = sizeof(a) / sizeof(a[0]);
+#pragma unroll
+    for (int k = 0; k < KK; ++k)
+#pragma unroll
+      for (int part = 0; part < PLANES; ++part) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+          a[k][part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, first + k, lane);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          b[k][part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, first + k, lane);
+      }
+  };
   auto multiply = [&](const V8 (&a)[PLANES][FM], const V8 (&b)[PLANES][FN]) {
 #pragma unroll
     for (int sum = PLANES - 1; sum >= 0; --sum)     // the least products first
@@ -361,17 +375,7 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
       for (int h = 0; h < 2; ++h) {
         constexpr int KK = BK / 32;     // 16 k each, of half a stage
         V8 a[KK][PLANES][FM], b[KK][PLANES][FN];
-#pragma unroll
-        for (int k = 0; k < KK; ++k)
-#pragma unroll
-          for (int part = 0; part < PLANES; ++part) {
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-              a[k][part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, KK * h + k, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-              b[k][part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, KK * h + k, lane);
-          }
+        fragments(stage, KK * h, a, b);
         if (h == 0 && s + 1 < steps) issue((s + 1) & 1);
         if (h == 1 && second) wait_copies<0>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -413,19 +417,18 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
       const char* stage = smem + from * T::STAGE;
       from = from + 1 == T::STAGES ? 0 : from + 1;
       to = to + 1 == T::STAGES ? 0 : to + 1;
+      // a stage's fragments are on their way together where they fit the registers, or the products would wait for LDS
+      // at every 16 k
+      constexpr int KK = PLANES * (FM + FN) * (BK / 16) <= 24 ? BK / 16 : BK / 32;
+      constexpr bool TOGETHER = PLANES * (FM + FN) * KK <= 24;
 #pragma unroll
-      for (int kk = 0; kk < BK / 16; ++kk) {
-        V8 a[PLANES][FM], b[PLANES][FN];
+      for (int h = 0; h < BK / 16 / KK; ++h) {
+        V8 a[KK][PLANES][FM], b[KK][PLANES][FN];
+        fragments(stage, KK * h, a, b);
+        if constexpr (TOGETHER) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int part = 0; part < PLANES; ++part) {
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-            a[part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, kk, lane);
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-            b[part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, kk, lane);
-        }
-        multiply(a, b);
+        for (int k = 0; k < KK; ++k) multiply(a[k], b[k]);
+        if constexpr (TOGETHER) __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -715,7 +718,7 @@ using VocabSlim = VocabTile<1, 2, 4, 1, P ? 2 : 3, 2, P>;
 typedef VocabTile<2, 2, 2, 2, 2, 2, false> VocabMid;      // in parts it would be Deep
 // dW beside Slim's dX: its rows are k, one stage of them, so that the tile's stores are its time
 template <bool P>
-using VocabWide = VocabTile<1, 8, 4, 1, 1, 2, P>;
+using VocabWide = VocabTile<1, P ? 4 : 8, 4, 1, 1, 2, P>;
 
 enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4 };
 
