@@ -44,9 +44,8 @@ __device__ __forceinline__ Philox philox(uint64_t block, uint64_t counter, uint3
 }
 
 // A thread per eight elements; eight that span rows (a width that is no multiple of eight, in rows with gaps) are addressed one by
-// one.  Bound by memory: 16384 x 4096 bf16 46 us (268 MB at 5.8 TB/s), with a residual 70 us (403 MB at 5.7 TB/s); one call of ten rounds
-// gives eight elements their 16 bits each, where one of 32 bits each would take two, and the rounds' 20 wide products as long as the
-// memory.  A small tensor takes the host's call, 8 us.
+// one.  Bound by memory: 16384 x 4096 bf16 46 us (268 MB at 5.8 TB/s), with a residual 70 us (403 MB at 5.7 TB/s); rows
+// with gaps, of an odd width, the same.  A small tensor takes the host's call, 8 us.
 template <class T, bool FLAT>
 __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs p) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -290,6 +290,102 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
   }
 }
 
+// The same from logits that were summed in pieces (VM_SUMS): a workgroup joins a row, whose logits it holds, and leaves its G,
+// rounded once, and zeros in G's rows behind the last that counts.
+constexpr int VOCAB_HELD = 8192;
+
+struct VocabSoftmaxSums {
+  VocabSoftmax s;
+  const float* sums;          // [splits, rows, ld]
+  int64_t split, ld;
+  int splits;
+  const void* bias;           // or null
+  int elem;
+};
+
+template <class E, bool PARTS>
+__global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSums q) {
+  const VocabSoftmax& p = q.s;
+  const int n = blockIdx.x, live = *p.live, t = threadIdx.x, wave = t >> 6;
+  constexpr int HELD = VOCAB_HELD / 2048;
+  E* g = p.G ? (E*)p.G + n * p.ldg : nullptr;
+  if (n >= live) {
+    if (!g || n >= (live + 63) / 64 * 64) return;
+    for (int v = 8 * t; v < p.held; v += 2048)
+#pragma unroll
+      for (int k = 0; k < (PARTS ? VOCAB_PARTS : 1); ++k) *(Words*)(g + k * p.g_part + v) = zero_words();
+    return;
+  }
+  __shared__ float red[9];
+  const int token = p.token[n];
+  float z[HELD][8];
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int v = 2048 * k + 8 * t;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[k][e] = 0.f;
+    if (v < p.vocab) {
+#pragma unroll 4
+      for (int s = 0; s < q.splits; ++s) {
+        const Pack<float, 8> more = load_pack<float, 8>(q.sums + s * q.split + n * q.ld + v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[k][e] += more.v[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (q.bias && v + e < p.vocab) z[k][e] += load_elem(q.bias, q.elem, v + e);
+      if (v + e >= p.vocab) z[k][e] = -INFINITY;
+      if (v + e == token) red[8] = z[k][e];
+      top = fmaxf(top, z[k][e]);
+    }
+  }
+  top = wave_max(top);
+  if ((t & 63) == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      z[k][e] = __builtin_amdgcn_exp2f((z[k][e] - top) * p.c);
+      sum += z[k][e];
+    }
+  sum = block_sum<4>(sum, red + 4);
+  float lp = (red[8] - top) * p.inv_t - logf(sum);
+  float inv = 1.f / sum;
+  if (token >= p.vocab) lp = inv = __int_as_float(0x7fc00000);
+  if (t == 0) {
+    p.row[n] = make_float2(top, inv);
+    p.logp[p.source[n]] = lp;
+  }
+  if (!g) return;
+  constexpr float SCALE = __is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f;
+  const float at_token = (expf(lp) - 1.f) * SCALE;
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int v = 2048 * k + 8 * t;
+    if (v >= p.held) break;
+    Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = v + e == token ? at_token : z[k][e] * inv * SCALE;
+      if constexpr (PARTS) {
+        __bf16 parts[VOCAB_PARTS];
+        split_parts(y, parts);
+#pragma unroll
+        for (int m = 0; m < VOCAB_PARTS; ++m) x[m].v[e] = parts[m];
+      } else {
+        x[0].v[e] = (E)y;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < (PARTS ? VOCAB_PARTS : 1); ++m) store_pack(g + m * p.g_part + v, x[m]);
+  }
+}
+
 // The loss alone.
 __global__ void __launch_bounds__(256) vocab_loss_kernel(const float* __restrict__ logp, int N, const int* __restrict__ live,
                                                           float* __restrict__ loss) {
@@ -386,10 +482,11 @@ struct VocabPlan {
   int64_t piece;             // vocabulary of a piece: what G and the packed weight have room for
   int64_t tiles;             // of the vocabulary in the first pass
   int logits_tile, grads_tile;
+  int logits_splits;         // of the logits' sums; 1: they are not cut
   int dx_splits, dw_splits;  // of the gradients' sums
   bool dx_joined, dw_joined; // they are summed in pieces first
   // bytes from the workspace's start
-  int64_t live, source, place, token, chosen, row, part, x, w, g, dx, dw, db, bytes;
+  int64_t live, source, place, token, chosen, row, part, x, w, g, sums, dx, dw, db, bytes;
 };
 
 inline bool vocab_direct(int elem, int64_t D, const void* weight, int64_t ld) {
@@ -432,6 +529,17 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   else if (vocab_tile_count(VT_LARGE, V, N, p.parts) >= 200) p.logits_tile = VT_LARGE;
   else p.logits_tile = p.parts == 1 && vocab_tile_count(VT_MID, V, N, p.parts) > 256 ? VT_MID : VT_DEEP;
   p.tiles = vocab_tile_count(p.logits_tile, V, 1, p.parts);
+  // Few tiles are cut along the width, to some two stages at least and a workgroup for every CU at most; the joining
+  // workgroup has to hold a row.
+  p.logits_splits = 1;
+  if ((p.logits_tile == VT_DEEP || p.logits_tile == VT_THIN) && V <= VOCAB_HELD) {
+    const int64_t tiles = vocab_tile_count(p.logits_tile, V, N, p.parts);
+    int64_t splits = 256 / tiles, most = p.Dp / (p.parts > 1 ? 64 : 128);
+    if (splits > most) splits = most;
+    if (splits > 16) splits = 16;
+    if (splits > 1) p.logits_splits = (int)splits;
+  }
+  const int64_t sums_ld = ceil_div(V, 256) * 256;
   p.grads_tile = VT_SLIM;
   p.dx_splits = p.dw_splits = 1;
   p.dx_joined = p.dw_joined = false;
@@ -476,7 +584,8 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.token = take(4 * N);
   p.chosen = take(4 * N);
   p.row = take(8 * N);
-  p.part = take(8 * p.tiles * N);
+  p.part = take(p.logits_splits > 1 ? 0 : 8 * p.tiles * N);
+  p.sums = take(p.logits_splits > 1 ? 4 * p.logits_splits * N * sums_ld : 0);
   p.x = take(2 * p.parts * p.rows * p.Dp);
   p.w = take(p.direct ? 0 : 2 * p.parts * p.piece * p.Dp);
   p.g = take(grad ? 2 * p.parts * p.rows * p.piece : 0);
@@ -616,7 +725,13 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   for (int64_t k = pieces - 1; k >= 0; --k) {
     weight_rows(k * first_piece, count_of(k), k < pieces - 1);
     a.G = p.grad && k == 0 ? g : nullptr;
-    vocab_logits<E, PARTS>(p.logits_tile, a, true, stream);
+    if (p.logits_splits > 1) {
+      a.splits = p.logits_splits;
+      a.sums_ld = ceil_div(p.V, 256) * 256;
+      a.sums_split = N * a.sums_ld;
+      a.sums = (float*)(q.space + p.sums) + k * first_piece;
+    }
+    vocab_logits<E, PARTS>(p.logits_tile, a, p.logits_splits > 1 ? VM_SUMS : VM_STATS, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
 
@@ -639,7 +754,15 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   soft.g_part = g_part;
   soft.held = p.grad ? (int)(ceil_div(count_of(0), 64) * 64) : 0;
   soft.chunks = p.grad ? (int)ceil_div(soft.held, VOCAB_CHUNK) : 1;
-  hipLaunchKernelGGL((vocab_softmax_kernel<E, PARTS>), dim3((unsigned)((int64_t)N * soft.chunks)), dim3(256), 0, stream, soft);
+  if (p.logits_splits > 1) {
+    const VocabSoftmaxSums joined = {soft, (const float*)(q.space + p.sums), a.sums_split, a.sums_ld, p.logits_splits, q.bias,
+                                     p.elem};
+    hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, PARTS>), dim3((unsigned)p.rows), dim3(256), 0, stream, joined);
+    a.splits = 1;
+    a.sums = nullptr;
+  } else {
+    hipLaunchKernelGGL((vocab_softmax_kernel<E, PARTS>), dim3((unsigned)((int64_t)N * soft.chunks)), dim3(256), 0, stream, soft);
+  }
   BF_LAUNCH_CHECK("bf_vocab_loss");
   if (!p.grad) {
     hipLaunchKernelGGL(vocab_loss_kernel, dim3(1), dim3(256), 0, stream, q.logp, N, live, q.loss);
@@ -653,7 +776,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     weight_rows(v0, count, k > 0);
     if (k > 0) {
       a.G = g;
-      vocab_logits<E, PARTS>(p.logits_tile, a, false, stream);
+      vocab_logits<E, PARTS>(p.logits_tile, a, VM_GRAD, stream);
       BF_LAUNCH_CHECK("bf_vocab_loss");
     }
     // dx: the weight's rows are k

@@ -32,11 +32,12 @@ typedef short short8v __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
 typedef __attribute__((address_space(3))) char lds_char;
 
-enum : int { VM_STATS = 0, VM_GRAD = 1, VM_DX = 2, VM_DW = 3 };
+enum : int { VM_STATS = 0, VM_GRAD = 1, VM_SUMS = 2, VM_DX = 3, VM_DW = 4 };
 
-// z's tiles end in one of two ways.  VM_STATS: the tile's largest logit and sum of exponentials per token, and where G is
+// z's tiles end in one of three ways.  VM_STATS: the tile's largest logit and sum of exponentials per token, and where G is
 // given the exponentials themselves, 2^(c (z - the tile's largest)); vocab_softmax_kernel makes them G in place.  VM_GRAD, with the rows'
-// statistics known: G.
+// statistics known: G.  VM_SUMS: sums over a part of k each, of a problem with so few tiles that they are cut along k (a CU
+// takes 40 GB/s from memory, so few CUs take long); vocab_softmax_sums_kernel joins them.
 
 constexpr int VOCAB_BK = 64;            // k come in multiples of this
 constexpr int VOCAB_PARTS = 3;
@@ -52,7 +53,7 @@ struct VocabArgs {
   int a_rows, b_rows;        // rows of A and B that may be read: later ones give the last one's values
   int a_cols, b_cols;        // of operands with k in their rows: elements of a row that may be read
   const int* live;           // rows of X that count, on the device
-  int splits;                // VM_DX, VM_DW: pieces of k, each with sums of its own
+  int splits;                // VM_SUMS, VM_DX, VM_DW: pieces of k, each with sums of its own
   int elem;                  // of the call's tensors
   // softmax
   const void* bias;          // [M] or null
@@ -246,12 +247,12 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   // Tiles in the order of groups of 8 along M, a contiguous share of them to each XCD: the 32 or 64 tiles that run on
   // one XCD at a time read 8 tiles of A and 4 or 8 of B through its L2.  Only rows that count have tiles.
   const int ntm = (p.M + T::BM - 1) / T::BM, ntn = (N + T::BN - 1) / T::BN;
-  const int splits = MODE >= VM_DX ? p.splits : 1;
+  const int splits = MODE >= VM_SUMS ? p.splits : 1;
   const int tiles = ntm * ntn * splits, share = (tiles + 7) / 8;
   int tile = (int)(block & 7) * share + (int)(block >> 3);
   if ((int)(block >> 3) >= share || tile >= tiles) return;
   int split = 0;
-  if constexpr (MODE >= VM_DX) {
+  if constexpr (MODE >= VM_SUMS) {
     split = tile / (ntm * ntn);
     tile -= split * (ntm * ntn);
   }
@@ -261,7 +262,7 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   const int m0 = tm * T::BM, n0 = tn * T::BN;
 
   int steps = (MODE == VM_DW ? (live + VOCAB_BK - 1) / VOCAB_BK * VOCAB_BK : p.K) / BK, k_first = 0;
-  if constexpr (MODE >= VM_DX) {
+  if constexpr (MODE >= VM_SUMS) {
     const int per = (steps + splits - 1) / splits;
     k_first = split * per;
     steps = max(0, min(per, steps - k_first));
@@ -573,11 +574,11 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
         p.part[(n0 + col) * p.part_ld + (p.v0 + m0) / T::BM] = make_float2(top, sum);
       }
     }
-  } else if (p.sums) {
+  } else if (MODE == VM_SUMS || p.sums) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
       const int n = n0 + wn + 32 * j + ln;
-      if (sum_cols) {
+      if (MODE == VM_DW && sum_cols) {
         const float sum = col_sum[j] + __shfl_xor(col_sum[j], 32);
         if (half == 0 && n < N) p.db_sums[(int64_t)split * N + n] = sum;
       }
@@ -688,9 +689,13 @@ __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
 inline int64_t vocab_blocks(int64_t tiles) { return 8 * ceil_div(tiles, 8); }
 
 template <class T, class E, bool PARTS>
-inline void launch_vocab_logits(const VocabArgs& p, bool stats, hipStream_t stream) {
-  const dim3 grid((unsigned)vocab_blocks(ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN)));
-  if (stats) hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
+inline void launch_vocab_logits(const VocabArgs& p, int mode, hipStream_t stream) {
+  const dim3 grid((unsigned)vocab_blocks(ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN) * p.splits));
+  if (mode == VM_SUMS) {
+    // only small grids are cut
+    if constexpr (T::OCC == 1 && T::WAVES == 4)
+      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_SUMS, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
+  } else if (mode == VM_STATS) hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
   else hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
 }
 
@@ -724,7 +729,7 @@ enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4 };
 
 // Defined for each type by a file of its own (bf_vocab_*.hip).
 template <class E, bool PARTS>
-void vocab_logits(int tile, const VocabArgs& p, bool stats, hipStream_t stream);
+void vocab_logits(int tile, const VocabArgs& p, int mode, hipStream_t stream);
 template <class E, bool PARTS>
 void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                  hipStream_t stream);

@@ -6,15 +6,15 @@
 namespace bf {
 
 template <class E, bool PARTS>
-void vocab_logits(int tile, const VocabArgs& p, bool stats, hipStream_t stream) {
+void vocab_logits(int tile, const VocabArgs& p, int mode, hipStream_t stream) {
   switch (tile) {
-    case VT_LARGE: launch_vocab_logits<VocabLarge<PARTS>, E, PARTS>(p, stats, stream); break;
+    case VT_LARGE: launch_vocab_logits<VocabLarge<PARTS>, E, PARTS>(p, mode, stream); break;
     case VT_MID:
-      if constexpr (!PARTS) launch_vocab_logits<VocabMid, E, PARTS>(p, stats, stream);
+      if constexpr (!PARTS) launch_vocab_logits<VocabMid, E, PARTS>(p, mode, stream);
       break;
-    case VT_DEEP: launch_vocab_logits<VocabDeep<PARTS>, E, PARTS>(p, stats, stream); break;
-    case VT_THIN: launch_vocab_logits<VocabThin<PARTS>, E, PARTS>(p, stats, stream); break;
-    default: launch_vocab_logits<VocabSlim<PARTS>, E, PARTS>(p, stats, stream);
+    case VT_DEEP: launch_vocab_logits<VocabDeep<PARTS>, E, PARTS>(p, mode, stream); break;
+    case VT_THIN: launch_vocab_logits<VocabThin<PARTS>, E, PARTS>(p, mode, stream); break;
+    default: launch_vocab_logits<VocabSlim<PARTS>, E, PARTS>(p, mode, stream);
   }
 }
 

@@ -96,6 +96,18 @@ def test_vocabulary_loss(dtype, N, D, V):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,D,V", [(3, 4090, 600), (190, 2552, 904), (1, 2048, 8192), (70, 1024, 8193), (2000, 520, 7)])
+def test_vocabulary_loss_of_long_rows(dtype, N, D, V):
+    """Few tiles, whose sums are cut along the width (up to 8192 tokens)."""
+    hidden, weight, tokens, bias = head(N, D, V, dtype, N + D)
+    mask = torch.rand(N, generator=gen(1)) < 0.8
+    mask[0] = True
+    bias[V // 2:V // 2 + 2] = float("-inf")
+    tokens = torch.where((tokens >= V // 2) & (tokens < V // 2 + 2), 0, tokens)
+    check(hidden, weight, tokens, bias=bias, mask=mask, temperature=1.2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N,D,V", [(700, 192, 1500), (1500, 64, 700), (40, 64, 9000), (513, 1100, 520)])
 def test_vocabulary_loss_of_many_tiles(dtype, N, D, V):
     hidden, weight, tokens, bias = head(N, D, V, dtype, N + D)
@@ -251,7 +263,7 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("N,D,V", [(5, 64, 700), (70, 40, 1003), (300, 192, 513), (90, 65, 2000)])
+@pytest.mark.parametrize("N,D,V", [(5, 64, 700), (70, 40, 1003), (300, 192, 513), (90, 65, 2000), (90, 520, 700), (6, 1000, 2051)])
 @pytest.mark.parametrize("room", [0, 300_000])
 def test_pieces(dtype, N, D, V, room):
     """No room, or a little: pieces of 256 tokens or some more, the logits of all but the first formed again."""
