@@ -846,10 +846,22 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
 constexpr int64_t VOCAB_ROWS = 1LL << 23, VOCAB_DIM = 1LL << 20, VOCAB_TOKENS = 1LL << 30;
 
 inline bool vocab_sizes_ok(int64_t N, int64_t D, int64_t V, int64_t ld_w) {
-  if (!(N < VOCAB_ROWS && D <= VOCAB_DIM && V <= VOCAB_TOKENS && ld_w <= VOCAB_DIM)) return false;
-  // tiles of a launch (its workgroups of 512 work-items have to stay below 2^32)
-  return ceil_div(V, 128) * ceil_div(N, 128) < (1LL << 22) && ceil_div(V, 128) * ceil_div(D, 128) < (1LL << 22) &&
-         ceil_div(N, 128) * ceil_div(D, 128) < (1LL << 22);
+  return N < VOCAB_ROWS && D <= VOCAB_DIM && V <= VOCAB_TOKENS && ld_w <= VOCAB_DIM;
+}
+
+// Every launch of a call stays below 2^32 work-items (asked before the first of them).
+inline bool vocab_launches_ok(const VocabPlan& p) {
+  auto products = [&](int tile, int64_t tiles) { return launch_fits(tiles + 16, tile == VT_LARGE ? 512 : 256); };
+  const int64_t packed = p.direct ? 0 : ceil_div(p.piece * (p.Dp / 8), 256);
+  if (!launch_fits(p.N + 64 + packed, 256) ||
+      !products(p.logits_tile, vocab_tile_count(p.logits_tile, p.V, p.N, p.parts) * p.logits_splits))
+    return false;
+  if (!p.grad) return true;
+  const int64_t tiles = vocab_tile_count(p.grads_tile, p.D, p.N, p.parts) * p.dx_splits +
+                        vocab_tile_count(p.grads_tile, p.D, p.piece, p.parts) * p.dw_splits;
+  const int64_t joined = (p.dx_joined ? p.N : 0) + (p.dw_joined ? p.V : 0);
+  return products(p.grads_tile, tiles) && launch_fits(p.N * ceil_div(p.piece, VOCAB_CHUNK), 256) &&
+         launch_fits(ceil_div(joined * ceil_div(p.D, 8), 256), 256);
 }
 
 }  // namespace bf
@@ -859,7 +871,8 @@ using namespace bf;
 extern "C" int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
                                            int with_grad, int64_t room) {
   if (!elem_ok(elem) || N <= 0 || D <= 0 || V <= 0 || ld_w < D || room < 0 || !vocab_sizes_ok(N, D, V, ld_w)) return 0;
-  return vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0, room).bytes / 4;
+  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0, room);
+  return vocab_launches_ok(p) ? p.bytes / 4 : 0;
 }
 
 extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
@@ -878,9 +891,12 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
              "bf_vocab_loss: gradients of hidden rows and weight, and of the bias where there is one, come together");
   BF_REQUIRE(!grad || grad_weight_elem == elem || grad_weight_elem == TE_F32,
              "bf_vocab_loss: weight gradient of element type %d", grad_weight_elem);
-  if (B > VOCAB_ROWS || T > VOCAB_ROWS || !vocab_sizes_ok(B * T, D, V, ld_w)) {
-    set_error("bf_vocab_loss: %lld x %lld rows, width %lld, vocabulary %lld are more than it takes", (long long)B,
-              (long long)T, (long long)D, (long long)V);
+  const bool sizes = B <= VOCAB_ROWS && T <= VOCAB_ROWS && vocab_sizes_ok(B * T, D, V, ld_w);
+  VocabPlan p;
+  if (sizes && B * T > 0) p = vocab_plan(B * T, D, V, elem, weight, ld_w, grad, room);
+  if (!sizes || (B * T > 0 && !vocab_launches_ok(p))) {
+    set_error("bf_vocab_loss: %lld x %lld rows, width %lld, vocabulary %lld, weight rows %lld apart are more than it takes",
+              (long long)B, (long long)T, (long long)D, (long long)V, (long long)ld_w);
     return BF_ERANGE;
   }
   const int64_t N = B * T;
@@ -894,7 +910,6 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
     BF_LAUNCH_CHECK("bf_vocab_loss");
     return BF_OK;
   }
-  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, grad, room);
   const VocabCall q = {hidden, T, ld_b, ld_t, weight, ld_w, bias, tokens, token_bytes, mask, temperature, grad_scale, logp,
                        loss, grad_hidden, grad_weight, grad_weight_elem, grad_bias, (char*)workspace, stream};
   switch (elem) {

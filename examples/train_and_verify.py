@@ -3,11 +3,12 @@
 A policy reads a context of four tokens and answers with one of eight actions; the right one
 follows from the context.  It is trained in two stages, as such policies are: sampled actions and the
 clipped policy loss, then pairs of a right and a wrong action and the preference loss, with AdamW and its
-moments in 8 bits.  Before and after, the same contexts are verified: every perturbation of the embedded
+moments in 8 bits.  Before them it may imitate right actions (--imitate), with dropout of the hidden layer and the
+cross entropy of its head.  Before and after, the same contexts are verified: every perturbation of the embedded
 context within a Linf ball has to leave the right action's logit the largest (CROWN bounds of
 its margins).
 
-    python examples/train_and_verify.py [--steps 120] [--contexts 512] [--eps 0.05]
+    python examples/train_and_verify.py [--steps 120] [--contexts 512] [--eps 0.05] [--imitate 0]
 
 Needs an MI355X and the built library (python -m boundflow_amd.build).
 """
@@ -56,6 +57,22 @@ class Policy:
         table_grad = training.embed_tokens_grad(grads[0].view(-1, CONTEXT, DIM), contexts, VOCAB, scale=SCALE)
         self.optimizer.step([table_grad, *grads[1:]])
         return result
+
+    def imitate(self, contexts, actions, drop: float):
+        """One supervised step: the layers before the head through autograd, the dropped hidden layer and the head through
+        the package.  (the loss result, the gradients in the parameters' order)"""
+        x = self.embed(contexts).requires_grad_(True)
+        *body, head = self.net
+        hidden = torch.nn.Sequential(*body)(x)
+        mask = {"seed": 7, "counter": self.optimizer.t}      # another mask each step
+        result = training.vocabulary_loss(training.dropout(hidden.detach(), drop, **mask), head.weight.detach(), actions,
+                                          bias=head.bias.detach())
+        through = training.dropout_grad(result.grad_hidden, drop, **mask)
+        grads = torch.autograd.grad(hidden, [x, *(p for layer in body for p in layer.parameters())], through)
+        table_grad = training.embed_tokens_grad(grads[0].view(-1, CONTEXT, DIM), contexts, VOCAB, scale=SCALE)
+        grads = [table_grad, *grads[1:], result.grad_weight, result.grad_bias]
+        self.optimizer.step(grads)
+        return result, grads
 
     def planned(self, example) -> BFTaskModule:
         """The MLP as the bound queries take it."""
@@ -112,24 +129,34 @@ def train(policy: Policy, contexts, steps: int, g):
     return float(reinforced.loss), float(preferred.loss)
 
 
+def imitate(policy: Policy, contexts, steps: int, drop: float = 0.1):
+    """The losses of a supervised stage."""
+    label = right_action(contexts)
+    return [policy.imitate(contexts, label, drop)[0].loss for _ in range(steps)]
+
+
 def main(argv=None) -> dict:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--steps", type=int, default=120)
     ap.add_argument("--contexts", type=int, default=512)
     ap.add_argument("--eps", type=float, default=0.05)
+    ap.add_argument("--imitate", type=int, default=0, help="supervised steps before the two stages")
     a = ap.parse_args(argv)
     device = torch.device("cuda:0")
     g = torch.Generator(device=device).manual_seed(1)
     contexts = torch.randint(0, VOCAB, (a.contexts, CONTEXT), device=device, generator=g)
     policy = Policy(device)
     before = verify(policy, contexts, a.eps)
+    imitated = [float(loss) for loss in imitate(policy, contexts, a.imitate)]
     losses = train(policy, contexts, a.steps, g)
     after = verify(policy, contexts, a.eps)
     for name, (right, certified, margin) in (("before", before), ("after", after)):
         print(f"{name:>6}: {100 * right:5.1f} % answered rightly, {100 * certified:5.1f} % certified within {a.eps}, "
               f"mean lower margin {margin:+.3f}", flush=True)
+    if imitated:
+        print(f"imitation: loss {imitated[0]:.4f} at first, {imitated[-1]:.4f} at last")
     print(f"last losses: policy {losses[0]:.4f}, preference {losses[1]:.4f}")
-    return {"before": before, "after": after, "losses": losses}
+    return {"before": before, "after": after, "losses": losses, "imitated": imitated}
 
 
 if __name__ == "__main__":

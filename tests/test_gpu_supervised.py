@@ -7,7 +7,10 @@ magnitudes, as is a gradient's sum over its rows or its vocabulary.  A log-proba
 leave.  The softmax's gradient is rounded to the inputs' type between the products (fp32: to three bf16 parts, 2^-24),
 and results are rounded once."""
 
+import copy
+import importlib.util
 import math
+import os
 
 import pytest
 import torch
@@ -480,3 +483,115 @@ def test_scores_feed_the_other_losses():
     tol = (2 * 128 * 2.0 ** -24 * float((hidden.abs() @ weight.abs().t()).max() + 3) * 2 + 2.0 ** -17)
     assert float((r.logp - scored).abs().max()) < tol
     assert abs(float(r.loss) - math.log(2)) < 0.1 * 24 * tol
+
+
+def test_calls_on_two_streams():
+    """Two calls under way at once, and the same call twice: the bits of calls one after another."""
+    dev = device()
+    cases = [tuple(t.to(dev) for t in head(n, 256, 9000, torch.bfloat16, n)) for n in (300, 50)]
+    run = lambda c: training.vocabulary_loss(c[0], c[1], c[2], bias=c[3])  # noqa: E731
+    want = [run(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(run(c))
+    torch.cuda.synchronize()
+    for k, r in enumerate(got):
+        for a, b in zip(r, want[k % 2]):
+            assert torch.equal(a, b), k
+
+
+def test_more_than_four_gigabytes():
+    """A weight of 4.6 GB, and a softmax gradient of 8.7 GB where there is room: offsets past 32 bits."""
+    dev = device()
+    g = torch.Generator(device=dev).manual_seed(3)
+
+    def check_rows(hidden, weight, tokens, got, rows, words, dtype):
+        n = tokens.numel()
+        size, tops = 0.0, []
+        for i in rows:
+            z = torch.mv(weight.float(), hidden[i].float()).double()      # fp32 sums of D products
+            q = torch.log_softmax(z, 0)
+            D = hidden.shape[1]
+            size = (D + 8) * 2.0 ** -23 * float(torch.mv(weight.float().abs(), hidden[i].float().abs()).max())
+            assert abs(float(got.logp[i]) - float(q[tokens[i]])) <= 4 * size + 2.0 ** -20 * (40 + z.numel() / 4096), i
+            p = q.exp()
+            p[tokens[i]] -= 1.0
+            want = torch.mv(weight.t().float(), p.float()).double() / n
+            bound = torch.mv(weight.t().float().abs(), p.float().abs()).double() / n
+            tops.append((i, got.grad_hidden[i].double(), want, bound * (2 * U[dtype] + 4 * size + 2.0 ** -16)))
+        for i, have, want, tol in tops:
+            close(have.cpu(), want.cpu(), (tol + rounded(want, dtype)).cpu(), f"grad hidden of row {i}")
+        # the weight's rows that are asked for, from all rows' probabilities of those tokens
+        for v in words:
+            z = torch.mv(hidden.float(), weight[v].float()).double()
+            # the row's normaliser from its own token
+            own = torch.stack([torch.dot(hidden[i].float(), weight[tokens[i]].float()) for i in range(n)]).double() \
+                if n <= 100 else (hidden.float() * weight[tokens].float()).sum(1).double()
+            p = torch.exp(z - (own - got.logp.double())) - (tokens == v).double()
+            want = torch.mv(hidden.t().double(), p) / n
+            bound = torch.mv(hidden.t().double().abs(), p.abs()) / n
+            close(got.grad_weight[v].cpu(), want.cpu(), (bound * (2 * U[dtype] + 2.0 ** -12) + rounded(want, dtype)).cpu(),
+                  f"grad weight of token {v}")
+
+    V, D = 140_000, 16_384
+    weight = torch.empty(V, D, device=dev, dtype=torch.bfloat16).normal_(0.0, 2.0 / math.sqrt(D), generator=g)
+    tokens = torch.tensor([0, V - 1, 131_071, 131_073, 5], device=dev)
+    hidden = torch.randn(5, D, device=dev, generator=g).bfloat16()
+    got = training.vocabulary_loss(hidden, weight, tokens)
+    check_rows(hidden, weight, tokens, got, range(5), (0, V - 1, 131_072, 131_073), torch.bfloat16)
+    del weight, got
+    N, V, D = 33_000, 131_072, 64
+    weight = torch.empty(V, D, device=dev, dtype=torch.bfloat16).normal_(0.0, 0.25, generator=g)
+    hidden = torch.randn(N, D, device=dev, generator=g).bfloat16()
+    tokens = torch.randint(0, V, (N,), device=dev, generator=g)
+    got = training.vocabulary_loss(hidden, weight, tokens, room=16 << 30)
+    check_rows(hidden, weight, tokens, got, (0, 1, 32_767, 32_768, N - 1), (0, 65_536, V - 1, int(tokens[-1])), torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------
+# the example
+
+def example():
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "train_and_verify.py")
+    spec = importlib.util.spec_from_file_location("train_and_verify", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def test_a_supervised_step_against_autograd():
+    """The step's gradients, chained through lookup, layers, dropout and loss, against float64 autograd with the oracle's
+    mask.  fp32 throughout: products of up to 160 terms, a mean over 64 rows."""
+    dev = device()
+    ex = example()
+    contexts = torch.randint(0, ex.VOCAB, (64, ex.CONTEXT), generator=gen(1)).to(dev)
+    policy = ex.Policy(dev, seed=3)
+    label = ex.right_action(contexts)
+    params = [p.detach().double().cpu().requires_grad_(True) for p in policy.params]
+    result, grads = policy.imitate(contexts, label, 0.25)
+    net = copy.deepcopy(policy.net).double().cpu()
+    table, w0, b0, w1, b1 = params
+    x = (table[contexts.cpu()] * ex.SCALE).flatten(1)
+    hidden = torch.relu(torch.nn.functional.linear(x, w0, b0))
+    _, kept = ref.dropout(hidden.detach(), 0.25, 7, 0)
+    logits = torch.nn.functional.linear(torch.where(kept, hidden / 0.75, 0.0), w1, b1)
+    loss = torch.nn.functional.cross_entropy(logits, label.cpu())
+    want = torch.autograd.grad(loss, params)
+    assert len(list(net.parameters())) == 4
+    # hidden and logits are sums of up to 160 products in fp32, off by 168 2^-24 of their magnitudes, some 1e-5 of
+    # the values; gradients are means of 64 such terms, whose magnitudes are some ten times their sum
+    assert abs(float(result.loss) - float(loss.detach())) < 2.0 ** -15
+    for name, a, b in zip(("table", "w0", "b0", "w1", "b1"), grads, want):
+        err = float((a.double().cpu() - b).abs().max())
+        announce(f"supervised step: gradient of {name} off by {err:.2e} of {float(b.abs().max()):.2e}")
+        assert err <= 2.0 ** -13 * float(b.abs().max()), name
+
+
+def test_example_with_a_supervised_stage():
+    got = example().main(["--steps", "2", "--contexts", "64", "--eps", "0.02", "--imitate", "5"])
+    assert len(got["imitated"]) == 5 and all(math.isfinite(x) for x in (*got["imitated"], *got["losses"]))
+    assert 0.0 <= got["after"][1] <= got["after"][0] <= 1.0

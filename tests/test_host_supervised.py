@@ -7,6 +7,7 @@ import torch
 from boundflow_amd import _lib, training
 from boundflow_amd._lib import HipError
 from oracle import training_ref as ref
+from tests.test_host_training_memory import default_type, fp32, recorded  # noqa: F401
 
 
 @pytest.fixture(scope="module")
@@ -49,7 +50,7 @@ def test_entry_points_refuse_bad_arguments(lib):
                 dict(bias=None), dict(dw_elem=1), dict(B=-1), dict(room=-1)):
         assert loss(**bad) == 1, bad
     for far in (dict(T=1 << 24), dict(B=1 << 40, T=1 << 40), dict(V=1 << 31), dict(ld_w=1 << 21),
-                dict(D=1 << 21, ld_w=1 << 21), dict(T=(1 << 23) - 1, V=1 << 29)):
+                dict(D=1 << 21, ld_w=1 << 21), dict(T=(1 << 23) - 1, V=1 << 29), dict(T=(1 << 23) - 1, V=1 << 28, room=1 << 60)):
         assert loss(**far) == 3, far
     drop = lambda **k: lib.bf_dropout(*{**dict(  # noqa: E731
         x=p, ld=4, residual=None, r_ld=0, elem=0, rows=2, dim=4, p=0.5, seed=1, counter=0, counter_dev=None, out=p,
@@ -87,3 +88,40 @@ def test_requires_grad_is_refused_before_the_device_is_asked():
     x = torch.zeros(3, requires_grad=True)
     with pytest.raises(HipError, match="dropout_grad"):
         training.dropout(x, 0.5, seed=1)
+
+
+def test_buffers_follow_the_inputs_whatever_the_default_type(recorded, default_type):  # noqa: F811
+    made, calls = recorded
+    tokens = torch.ones(300, dtype=torch.int64)
+    for dtype in (torch.float32, torch.bfloat16):
+        r = training.vocabulary_loss(torch.ones(300, 24, dtype=dtype), torch.ones(70, 24, dtype=dtype), tokens,
+                                     bias=torch.ones(70, dtype=dtype))
+        assert r.loss.dtype == r.logp.dtype == torch.float32
+        assert r.grad_hidden.dtype == r.grad_weight.dtype == r.grad_bias.dtype == dtype
+        r = training.vocabulary_loss(torch.ones(300, 24, dtype=dtype), torch.ones(70, 24, dtype=dtype), tokens,
+                                     weight_grad_dtype=torch.float32)
+        assert r.grad_weight.dtype == torch.float32 and r.grad_bias is None
+        assert training.dropout(torch.ones(5, 3, dtype=dtype), 0.5, seed=1).dtype == dtype
+    assert [name for name, _ in calls] == ["bf_vocab_loss", "bf_vocab_loss", "bf_dropout"] * 2
+    assert {t.dtype for t in made} == {torch.float32, torch.bfloat16}
+
+
+@pytest.mark.parametrize("rows,V", [(4, 5), (300, 700), (2000, 40)])
+def test_results_do_not_keep_the_workspace(recorded, rows, V):  # noqa: F811
+    _made, calls = recorded
+    r = training.vocabulary_loss(fp32(rows, 24), fp32(V, 24), torch.zeros(rows, dtype=torch.int64))
+    held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in r if t is not None}
+    assert sum(held.values()) <= 4 * (1 + rows + 24 * (rows + V)) + 64
+    need = _lib.load().bf_vocab_loss_workspace(rows, 24, V, 0, calls[0][1][7], 24, 1, 2 << 30)
+    space = calls[0][1][-3]
+    base = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in recorded[0]}
+    assert base[space] >= 4 * need
+
+
+def test_seeds_and_counters_reach_the_library_whole(recorded):  # noqa: F811
+    _made, calls = recorded
+    training.dropout(fp32(6), 0.25, seed=(1 << 64) - 1, counter=(1 << 63) - 1)
+    training.dropout(fp32(2, 3, 4)[:, 1:], 0.25, seed=5, counter=torch.tensor(9), residual=fp32(2, 2, 4))
+    (_, a), (_, b) = calls
+    assert a[8] == -1 and a[9] == (1 << 63) - 1 and a[10] is None and a[5:7] == (1, 6)
+    assert b[8] == 5 and b[9] == 0 and b[10] is not None and b[5:7] == (4, 4)
