@@ -29,41 +29,46 @@ __global__ void __launch_bounds__(1024) vocab_rows_kernel(const void* __restrict
                                                           int* __restrict__ token, float* __restrict__ logp) {
   __shared__ int sums[16];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  constexpr int HELD = 4;
+  constexpr int HELD = 8;      // neighbours a thread: their places follow from one sum over the threads before it
   int done = 0;
   for (int base = 0; base < N; base += 1024 * HELD) {
-    int tok[HELD];
+    const int first = base + HELD * t;
+    int tok[HELD], mine = 0;
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
-      const int n = base + 1024 * k + t;
+      const int n = first + k;
       tok[k] = n < N && (!mask || mask[n]) ? load_token(tokens, token_bytes, n) : -1;
+      mine += tok[k] >= 0;
+    }
+    int upto = mine;           // over this lane and those before it
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+      const int other = __shfl_up(upto, step);
+      if (lane >= step) upto += other;
+    }
+    if (lane == 63) sums[wave] = upto;
+    __syncthreads();
+    int at = done + upto - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      at += w < wave ? sums[w] : 0;
+      all += sums[w];
     }
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
-      const int n = base + 1024 * k + t;
-      const uint64_t votes = __ballot(tok[k] >= 0);
-      if (lane == 0) sums[wave] = __popcll(votes);
-      __syncthreads();
-      int before = done, all = 0;
-#pragma unroll
-      for (int w = 0; w < 16; ++w) {
-        before += w < wave ? sums[w] : 0;
-        all += sums[w];
+      const int n = first + k;
+      if (n >= N) break;
+      if (tok[k] >= 0) {
+        source[at] = n;
+        token[at] = tok[k];
+        place[n] = at++;
+      } else {
+        place[n] = -1;
+        logp[n] = 0.f;
       }
-      const int at = before + __popcll(votes & ((1ull << lane) - 1));
-      if (n < N) {
-        if (tok[k] >= 0) {
-          source[at] = n;
-          token[at] = tok[k];
-          place[n] = at;
-        } else {
-          place[n] = -1;
-          logp[n] = 0.f;
-        }
-      }
-      done += all;
-      __syncthreads();
     }
+    done += all;
+    __syncthreads();
   }
   if (t == 0) *live = done;
 }
@@ -207,7 +212,8 @@ __global__ void __launch_bounds__(256) vocab_pack_weight_kernel(const T* __restr
 // Statistics of the rows that count, from those of their tiles, and G from the exponentials that the first pass left, in
 // place.  A workgroup joins a row's tiles and takes VOCAB_CHUNK of its entries; the first one of a row writes what others
 // read.  The token's entry comes from its log-probability: p - 1 from a rounded p would have no digits left where p is near 1.
-// The others are rounded a second time here (half a step of their type; fp32 ones lie here whole).
+// The others are rounded a second time here.  They lie here with 11 bits (fp32: whole), so that the gradients of bf16 feel
+// that rounding alone.
 constexpr int VOCAB_CHUNK = 8192;
 
 struct VocabSoftmax {
@@ -266,14 +272,16 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
   for (int k = 0; k < VOCAB_CHUNK / 2048; ++k) {
     const int v = chunk * VOCAB_CHUNK + 2048 * k + 8 * t;
     if (v >= p.held) break;
-    const float factor = __builtin_amdgcn_exp2f((part[v / p.tile].x - top) * p.c) * inv;
+    const float factor = __builtin_amdgcn_exp2f((part[v / p.tile].x - top) * p.c) * inv * (PARTS ? 1.f : SCALE / VOCAB_E_SCALE);
     Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
 #pragma unroll
     for (int q = 0; q < (PARTS ? 2 : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part + v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float y = (float)x[0].v[e];
-      if constexpr (PARTS)      // the two halves of an fp32 number
+      float y;
+      if constexpr (!PARTS)
+        y = (float)__builtin_bit_cast(_Float16, x[0].v[e]);
+      else                      // the two halves of an fp32 number
         y = __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, x[0].v[e]) << 16 | __builtin_bit_cast(uint16_t, x[1].v[e]));
       y = v + e == token ? at_token : y * factor;
       if constexpr (PARTS) {
@@ -477,7 +485,7 @@ __global__ void __launch_bounds__(256) vocab_nothing_kernel(float* loss, void* d
 struct VocabPlan {
   int64_t N, D, V;
   int elem, parts;
-  bool direct, grad;
+  bool direct, regs, grad;   // the weight is read as it lies: copied to LDS, or through registers
   int64_t rows, Dp;          // padded
   int64_t piece;             // vocabulary of a piece: what G and the packed weight have room for
   int64_t tiles;             // of the vocabulary in the first pass
@@ -498,10 +506,17 @@ inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
     case VT_LARGE:
       return ceil_div(m, VocabLarge<false>::BM) * ceil_div(n, parts > 1 ? VocabLarge<true>::BN : VocabLarge<false>::BN);
     case VT_SLIM:
+    case VT_REGS:
     case VT_THIN: return ceil_div(m, VocabSlim<false>::BM) * ceil_div(n, VocabSlim<false>::BN);
     default: return ceil_div(m, VocabMid::BM) * ceil_div(n, VocabMid::BN);
   }
 }
+
+// Rows up to which a weight that cannot be copied to LDS as it lies passes through registers, where a packed copy of it would be
+// most of the bytes.  fp32 (us, packed / through registers; rows of 2048 over 32000 tokens): 8 rows 399 / 265, 128 rows 529 / 401, 192 rows
+// 620 / 567, scored alone 212 / 91, 252 / 126, 271 / 195.  16-bit rows of an odd width, scored: 64 rows of 2049 over 50001 tokens
+// 119 / 77, 128 rows 131 / 137; with gradients, whose product along the vocabulary is read two bytes aside, 227 / 277.
+constexpr int64_t VOCAB_REGS_FP32 = 192, VOCAB_REGS_SCORED = 64;
 
 inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld, bool grad,
                             int64_t room) {
@@ -513,9 +528,10 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.grad = grad;
   p.parts = elem == TE_F32 ? VOCAB_PARTS : 1;
   p.direct = vocab_direct(elem, D, weight, ld);
+  p.regs = !p.direct && (elem == TE_F32 ? N <= VOCAB_REGS_FP32 : !grad && N <= VOCAB_REGS_SCORED);
   p.rows = ceil_div(N, 64) * 64;
   p.Dp = ceil_div(D, 64) * 64;
-  const int64_t per_token = 2 * p.parts * ((grad ? p.rows : 0) + (p.direct ? 0 : p.Dp));
+  const int64_t per_token = 2 * p.parts * ((grad ? p.rows : 0) + (p.direct || p.regs ? 0 : p.Dp));
   const int64_t whole = ceil_div(V, 256) * 256;
   p.piece = whole;
   if (per_token > 0) {
@@ -525,14 +541,15 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   }
   const int64_t in_piece = p.piece < V ? p.piece : V;
   // by the whole vocabulary, so that the statistics have the same bits with and without gradients and whatever the room
-  if (N <= VocabSlim<false>::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N, p.parts) > 256 ? VT_SLIM : VT_THIN;
+  if (p.regs) p.logits_tile = VT_REGS;
+  else if (N <= VocabSlim<false>::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N, p.parts) > 256 ? VT_SLIM : VT_THIN;
   else if (vocab_tile_count(VT_LARGE, V, N, p.parts) >= 200) p.logits_tile = VT_LARGE;
   else p.logits_tile = p.parts == 1 && vocab_tile_count(VT_MID, V, N, p.parts) > 256 ? VT_MID : VT_DEEP;
   p.tiles = vocab_tile_count(p.logits_tile, V, 1, p.parts);
   // Few tiles are cut along the width, to some two stages at least and a workgroup for every CU at most; the joining
   // workgroup has to hold a row.
   p.logits_splits = 1;
-  if ((p.logits_tile == VT_DEEP || p.logits_tile == VT_THIN) && V <= VOCAB_HELD) {
+  if ((p.logits_tile == VT_DEEP || p.logits_tile == VT_THIN || p.logits_tile == VT_REGS) && V <= VOCAB_HELD) {
     const int64_t tiles = vocab_tile_count(p.logits_tile, V, N, p.parts);
     int64_t splits = 256 / tiles, most = p.Dp / (p.parts > 1 ? 64 : 128);
     if (splits > most) splits = most;
@@ -544,7 +561,9 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.dx_splits = p.dw_splits = 1;
   p.dx_joined = p.dw_joined = false;
   if (grad) {
-    if (N <= VocabSlim<false>::BN) {
+    if (p.regs) {
+      p.grads_tile = VT_REGS;
+    } else if (N <= VocabSlim<false>::BN) {
       const int64_t slim = vocab_tile_count(VT_SLIM, D, N, p.parts) + vocab_tile_count(VT_SLIM, D, in_piece, p.parts);
       p.grads_tile = slim > 256 ? VT_SLIM : VT_THIN;
     } else {
@@ -554,7 +573,7 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
     }
     // Sums are cut along k so that none of them takes longer than a good part of the whole launch, nor than it takes to
     // add one more piece's sums (some eight stages).
-    const int64_t slots = p.grads_tile == VT_MID || p.grads_tile == VT_SLIM ? 512 : 256;
+    const int64_t slots = p.grads_tile == VT_LARGE || p.grads_tile == VT_DEEP || p.grads_tile == VT_THIN ? 256 : 512;
     const int64_t dx = vocab_tile_count(p.grads_tile, D, N, p.parts), dw = vocab_tile_count(p.grads_tile, D, in_piece, p.parts);
     const int64_t dx_steps = ceil_div(in_piece, 64), dw_steps = ceil_div(N, 64);
     int64_t most = (dx * dx_steps + dw * (dw_steps + 4)) / slots / 3;
@@ -587,7 +606,7 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.part = take(p.logits_splits > 1 ? 0 : 8 * p.tiles * N);
   p.sums = take(p.logits_splits > 1 ? 4 * p.logits_splits * N * sums_ld : 0);
   p.x = take(2 * p.parts * p.rows * p.Dp);
-  p.w = take(p.direct ? 0 : 2 * p.parts * p.piece * p.Dp);
+  p.w = take(p.direct || p.regs ? 0 : 2 * p.parts * p.piece * p.Dp);
   p.g = take(grad ? 2 * p.parts * p.rows * p.piece : 0);
   p.dx = take(p.dx_joined ? 4 * p.dx_splits * p.rows * p.Dp : 0);
   p.dw = take(p.dw_joined ? 4 * p.dw_splits * V * p.Dp : 0);
@@ -642,7 +661,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   const T* weight = (const T*)q.weight;
   // Without G in the way the first pass takes a weight that can be read as it lies whole; otherwise the pieces from
   // the last to the first, whose packed weight and exponentials are then there for the second pass.
-  const int64_t first_piece = p.direct && !p.grad ? ceil_div(p.V, 256) * 256 : p.piece;
+  const int64_t first_piece = (p.direct || p.regs) && !p.grad ? ceil_div(p.V, 256) * 256 : p.piece;
   const int64_t pieces = ceil_div(p.V, first_piece);
   auto count_of = [&](int64_t k) { return (int)(p.V - k * first_piece < first_piece ? p.V - k * first_piece : first_piece); };
 
@@ -666,7 +685,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   pre.x = x;
   pre.x_part = x_part;
   pre.grad_hidden = q.grad_hidden;
-  if (!p.direct) {
+  if (!p.direct && !p.regs) {
     pre.weight = weight + (pieces - 1) * first_piece * q.ld_w;
     pre.ld_w = q.ld_w;
     pre.weight_rows = count_of(pieces - 1);
@@ -701,7 +720,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   a.N = N;
   a.b_rows = (int)p.rows;
   a.K = (int)p.Dp;
-  a.a_cols = p.direct ? D : (int)p.Dp;
+  a.a_cols = p.direct || p.regs ? D : (int)p.Dp;
   a.ldg = p.piece;
   a.g_part = g_part;
   a.g_rows = (int)p.rows;
@@ -710,7 +729,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     a.v0 = (int)v0;
     a.M = a.a_rows = count;
     a.bias = q.bias ? (const T*)q.bias + v0 : nullptr;
-    if (p.direct) {
+    if (p.direct || p.regs) {
       a.A = weight + v0 * q.ld_w;
       a.lda = q.ld_w;
       return;
@@ -852,7 +871,7 @@ inline bool vocab_sizes_ok(int64_t N, int64_t D, int64_t V, int64_t ld_w) {
 // Every launch of a call stays below 2^32 work-items (asked before the first of them).
 inline bool vocab_launches_ok(const VocabPlan& p) {
   auto products = [&](int tile, int64_t tiles) { return launch_fits(tiles + 16, tile == VT_LARGE ? 512 : 256); };
-  const int64_t packed = p.direct ? 0 : ceil_div(p.piece * (p.Dp / 8), 256);
+  const int64_t packed = p.direct || p.regs ? 0 : ceil_div(p.piece * (p.Dp / 8), 256);
   if (!launch_fits(p.N + 64 + packed, 256) ||
       !products(p.logits_tile, vocab_tile_count(p.logits_tile, p.V, p.N, p.parts) * p.logits_splits))
     return false;

@@ -43,6 +43,9 @@ constexpr int VOCAB_BK = 64;            // k come in multiples of this
 constexpr int VOCAB_PARTS = 3;
 // fp16 holds G times this: p - [v = y] lies within [-1, 1], and a probability below 2^-24 would be subnormal
 constexpr float VOCAB_F16_SCALE = 16384.f;
+// Exponentials, at most 1, wait for their row's statistics as fp16 times this, whichever 16-bit type G has: 11 bits down to
+// 2^-29, and 0 below 2^-40.
+constexpr float VOCAB_E_SCALE = 32768.f;
 
 struct VocabArgs {
   const void* A;
@@ -229,7 +232,80 @@ __device__ __forceinline__ void wait_copies() {
 }
 
 // One tile's sums.  `block` of `share * 8` workgroups: XCD block % 8's share-th of the tiles.
-template <class T, int MODE, class E, bool PARTS>
+// Stages that pass through registers, for a weight of type S that cannot be copied as it lies (rows that do not start at 16
+// bytes, fp32 that is split into parts on the way): where few rows use it, a packed copy of it would take longer than
+// everything else.  The layout in LDS is VocabOperand's; what is past the end of rows or columns is zeros.
+template <bool TR, int SIDE, int NT, int BK, int PLANES, class S>
+struct VocabWeightChunks {
+  typedef VocabOperand<TR, SIDE, NT / 64, BK> Op;
+  static constexpr int COUNT = SIDE * BK / 8 / NT;
+  Pack<S, 8> x[COUNT];
+
+  __device__ __forceinline__ void load(const S* base, int64_t ld, int k0, int first, int rows, int cols) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int id = threadIdx.x + NT * j, along = id / Op::SLOTS, at = 8 * (id % Op::SLOTS);
+      const int r = TR ? k0 + along : min(first + along, rows - 1), c = TR ? first + at : k0 + at;
+      if (r < rows && c + 8 <= cols) {
+        x[j] = load_pack<S, 8>(base + r * ld + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[j].v[e] = r < rows && c + e < cols ? base[r * ld + c + e] : (S)0.f;
+      }
+    }
+  }
+
+  template <class E>
+  __device__ __forceinline__ void put(char* stage, int plane) const {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int id = threadIdx.x + NT * j, row = id / Op::SLOTS, slot = (id % Op::SLOTS) ^ Op::swap(row);
+      char* to = stage + 16 * (row * Op::SLOTS + slot);
+      if constexpr (sizeof(S) == 2) {
+        *(Words*)to = __builtin_bit_cast(Words, x[j]);
+      } else {
+        Pack<__bf16, 8> y[VOCAB_PARTS];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          __bf16 parts[VOCAB_PARTS];
+          split_parts(x[j].v[e], parts);
+#pragma unroll
+          for (int q = 0; q < VOCAB_PARTS; ++q) y[q].v[e] = parts[q];
+        }
+#pragma unroll
+        for (int q = 0; q < VOCAB_PARTS; ++q) *(Words*)(to + q * plane) = __builtin_bit_cast(Words, y[q]);
+      }
+    }
+  }
+};
+
+// The other operand beside it: packed rows with k contiguous.
+template <int SIDE, int NT, int BK, int PLANES>
+struct VocabRowChunks {
+  typedef VocabOperand<false, SIDE, NT / 64, BK> Op;
+  static constexpr int EACH = SIDE * BK / 8, COUNT = PLANES * EACH / NT;
+  static_assert(COUNT * NT == PLANES * EACH, "whole chunks a thread");
+  Words x[COUNT];
+
+  __device__ __forceinline__ void load(const char* base, int64_t ld, int64_t part, int k0, int first, int rows) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int id = threadIdx.x + NT * j, q = id / EACH, at = id % EACH;
+      const int r = min(first + at / Op::SLOTS, rows - 1);
+      x[j] = *(const Words*)(base + 2 * (q * part + r * ld + k0 + 8 * (at % Op::SLOTS)));
+    }
+  }
+  __device__ __forceinline__ void put(char* stage) const {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int id = threadIdx.x + NT * j, q = id / EACH, at = id % EACH, row = at / Op::SLOTS;
+      *(Words*)(stage + 2 * SIDE * BK * q + 16 * (row * Op::SLOTS + ((at % Op::SLOTS) ^ Op::swap(row)))) = x[j];
+    }
+  }
+};
+
+// S: the type of a weight that passes through registers, or void.
+template <class T, int MODE, class E, bool PARTS, class S = void>
 __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint32_t block) {
   constexpr bool A_TR = MODE >= VM_DX, B_TR = MODE == VM_DW;
   constexpr int FM = T::FM, FN = T::FN;
@@ -360,7 +436,40 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     }
   };
 
-  if constexpr (T::WAVES == 8) {
+  if constexpr (!__is_same(S, void)) {
+    static_assert(MODE != VM_DW && T::STAGES >= 2 && T::WAVES == 4, "the weight is the first operand; two buffers");
+    constexpr int AHEAD = 3;      // stages under way in registers
+    VocabWeightChunks<A_TR, T::BM, T::NT, BK, PLANES, S> wa[AHEAD];
+    VocabRowChunks<T::BN, T::NT, BK, PLANES> xb[AHEAD];
+    auto load = [&](int s, int to) {
+      const int k0 = (k_first + s) * BK;
+      wa[to].load((const S*)p.A, p.lda, k0, m0, p.a_rows, p.a_cols);
+      xb[to].load((const char*)p.B, p.ldb, p.b_part, k0, n0, p.b_rows);
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d)
+      if (d < steps) load(d, d);
+    for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        const int s = s0 + d;
+        if (s < steps) {
+          char* stage = smem + (s & 1) * T::STAGE;
+          wa[d].template put<E>(stage, T::A_PLANE);
+          xb[d].put(stage + T::A_BYTES);
+          // everyone has read the other buffer when everyone is here
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          if (s + AHEAD < steps) load(s + AHEAD, d);
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            V8 a[1][PLANES][FM], b[1][PLANES][FN];
+            fragments(stage, kk, a, b);
+            multiply(a[0], b[0]);
+          }
+        }
+      }
+    }
+  } else if constexpr (T::WAVES == 8) {
     // Two groups of four waves, one wave of each on a SIMD, take turns: while one multiplies what it has in registers
     // (half a stage, 16 products in 512 cycles; fp32: 24 in 768) the other reads its next half stage from LDS and starts the copies
     // of the next stage.  A buffer is written again when the second group has read its last half, and has to be there
@@ -533,7 +642,9 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float v = acc[i][j][4 * q + r];
-                if constexpr (__is_same(E, _Float16)) {
+                if constexpr (!PARTS && MODE == VM_STATS) {
+                  x.v[r] = __builtin_bit_cast(E, (_Float16)(v * VOCAB_E_SCALE));
+                } else if constexpr (__is_same(E, _Float16)) {
                   x.v[r] = (E)(v * VOCAB_F16_SCALE);
                 } else if constexpr (PARTS && MODE == VM_STATS) {
                   const uint32_t bits = __float_as_uint(v);
@@ -666,45 +777,45 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   }
 }
 
-template <class T, int MODE, class E, bool PARTS>
+template <class T, int MODE, class E, bool PARTS, class S = void>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4) vocab_logits_kernel(VocabArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[T::LDS];
-  vocab_tile<T, MODE, E, PARTS>(p, smem, blockIdx.x);
+  vocab_tile<T, MODE, E, PARTS, S>(p, smem, blockIdx.x);
 }
 
 // dX (tiles T) and dW (tiles W) of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the CUs that dX's few long
 // ones leave.  dX's come first; the last workgroup takes the loss where `loss` is given.
-template <class T, class W, class E, bool PARTS>
+template <class T, class W, class E, bool PARTS, class S = void>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
     vocab_grads_kernel(VocabArgs dx, VocabArgs dw, uint32_t dx_blocks, const float* logp, int rows, float* loss) {
   static_assert(T::NT == W::NT && W::STAGES * W::STAGE <= T::STAGES * T::STAGE && T::TILE <= T::STAGES * T::STAGE &&
                     W::TILE <= T::STAGES * T::STAGE, "dX's stages hold dW's, and the tiles of both");
   __shared__ __attribute__((aligned(1024))) char smem[T::STAGES * T::STAGE];
   if (loss && blockIdx.x + 1 == gridDim.x) vocab_loss<T::WAVES>(logp, rows, *dx.live, loss, (float*)smem);
-  else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, PARTS>(dx, smem, blockIdx.x);
+  else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, PARTS, S>(dx, smem, blockIdx.x);
   else vocab_tile<W, VM_DW, E, PARTS>(dw, smem, blockIdx.x - dx_blocks);
 }
 
 // Workgroups for `tiles` tiles at most, a whole number per XCD.
 inline int64_t vocab_blocks(int64_t tiles) { return 8 * ceil_div(tiles, 8); }
 
-template <class T, class E, bool PARTS>
+template <class T, class E, bool PARTS, class S = void>
 inline void launch_vocab_logits(const VocabArgs& p, int mode, hipStream_t stream) {
   const dim3 grid((unsigned)vocab_blocks(ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN) * p.splits));
   if (mode == VM_SUMS) {
     // only small grids are cut
-    if constexpr (T::OCC == 1 && T::WAVES == 4)
-      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_SUMS, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
-  } else if (mode == VM_STATS) hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
-  else hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, PARTS>), grid, dim3(T::NT), 0, stream, p);
+    if constexpr ((T::OCC == 1 && T::WAVES == 4) || !__is_same(S, void))
+      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_SUMS, E, PARTS, S>), grid, dim3(T::NT), 0, stream, p);
+  } else if (mode == VM_STATS) hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, PARTS, S>), grid, dim3(T::NT), 0, stream, p);
+  else hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, PARTS, S>), grid, dim3(T::NT), 0, stream, p);
 }
 
-template <class T, class W, class E, bool PARTS>
+template <class T, class W, class E, bool PARTS, class S = void>
 inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                                hipStream_t stream) {
   const int64_t first = vocab_blocks(ceil_div(dx.M, T::BM) * ceil_div(dx.N, T::BN) * dx.splits);
   const int64_t all = first + vocab_blocks(ceil_div(dw.M, W::BM) * ceil_div(dw.N, W::BN) * dw.splits) + (loss ? 1 : 0);
-  hipLaunchKernelGGL((vocab_grads_kernel<T, W, E, PARTS>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
+  hipLaunchKernelGGL((vocab_grads_kernel<T, W, E, PARTS, S>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
                      logp, rows, loss);
 }
 
@@ -725,7 +836,7 @@ typedef VocabTile<2, 2, 2, 2, 2, 2, false> VocabMid;      // in parts it would b
 template <bool P>
 using VocabWide = VocabTile<1, P ? 4 : 8, 4, 1, 1, 2, P>;
 
-enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4 };
+enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4, VT_REGS = 5 };   // REGS: Slim through registers
 
 // Defined for each type by a file of its own (bf_vocab_*.hip).
 template <class E, bool PARTS>

@@ -40,11 +40,13 @@ def tolerances(r, dtype, temperature, V, D):
     dz = (count * 2.0 ** -24 * r["size"]).amax(1) / temperature + 2.0 ** -22 * r["size"].amax(1) * (
         dtype == torch.float32)
     tol_lp = 2 * dz + logp_tol(r["z"] / temperature, V)
-    # What is below a type's normal numbers: fp16 holds 2^14 G in steps of 2^-24, so G to 2^-39.  In fp32 a probability below
-    # 2^-126 is 0, and so is each of three bf16 parts (the matrix cores read subnormal bf16 as 0): 4 * 2^-126 in all.
-    extra = 2.0 ** -124 if dtype == torch.float32 else 2.0 ** -39
-    # exponentials are rounded to the type before they are scaled (but for the token's), G after it
-    return tol_lp, r["p"] * (tol_lp + 2.0 ** -21 + U[dtype])[:, None] + r["g"].abs() * (U[dtype] + 2.0 ** -23) + extra
+    # What is below a type's normal numbers: fp16 holds 2^14 G in steps of 2^-24, so G to 2^-39, and 2^15 times the exponentials
+    # of 16-bit types, so these to 2^-40.  In fp32 a probability below 2^-126 is 0, and so is each of three bf16 parts (the
+    # matrix cores read subnormal bf16 as 0): 4 * 2^-126 in all.
+    extra = 2.0 ** -124 if dtype == torch.float32 else 2.0 ** -38
+    # exponentials are rounded to 11 bits before they are scaled (but for the token's; fp32 not at all), G to its type after it
+    early = 0.0 if dtype == torch.float32 else 2.0 ** -11
+    return tol_lp, r["p"] * (tol_lp + 2.0 ** -21 + early)[:, None] + r["g"].abs() * (U[dtype] + 2.0 ** -23) + extra
 
 
 def check(hidden, weight, tokens, *, bias=None, mask=None, temperature=1.0, grad_scale=1.0, wide=None, room=2 << 30, on=None,
