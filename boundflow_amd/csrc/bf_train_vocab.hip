@@ -21,56 +21,51 @@ namespace bf {
 // ---------------------------------------------------------------------------
 // Rows that count
 
-// One workgroup: the rows that count in their order.  live[0] their number, source[i] row i's place, place[n] the
-// inverse (-1: does not count), token[i] its token; logp is 0 where a row does not count.
+// The rows that count in their order: live[0] their number, source[i] row i's place, place[n] the inverse (-1: does not
+// count), token[i] its token; logp is 0 where a row does not count.  A workgroup takes VOCAB_COUNTED rows and counts those
+// before them for itself, which for many rows would be most of the work: past VOCAB_COUNTED_ROWS one workgroup takes
+// all (8000 rows: 15 us by one workgroup, 8 by eight).
+constexpr int VOCAB_COUNTED = 1024, VOCAB_COUNTED_ROWS = 64 * VOCAB_COUNTED;
+
 __global__ void __launch_bounds__(1024) vocab_rows_kernel(const void* __restrict__ tokens, int token_bytes,
                                                           const uint8_t* __restrict__ mask, int N, int* __restrict__ live,
                                                           int* __restrict__ source, int* __restrict__ place,
                                                           int* __restrict__ token, float* __restrict__ logp) {
   __shared__ int sums[16];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  constexpr int HELD = 8;      // neighbours a thread: their places follow from one sum over the threads before it
+  auto token_of = [&](int n) { return n < N && (!mask || mask[n]) ? load_token(tokens, token_bytes, n) : -1; };
+  const int from = blockIdx.x * VOCAB_COUNTED, to = gridDim.x == 1 ? N : min(N, from + VOCAB_COUNTED);
+  int before = 0;      // of this wave's share of the rows before
+#pragma unroll 8
+  for (int n = t; n < from; n += 1024) before += __popcll(__ballot(token_of(n) >= 0));
+  if (lane == 0) sums[wave] = before;
+  __syncthreads();
   int done = 0;
-  for (int base = 0; base < N; base += 1024 * HELD) {
-    const int first = base + HELD * t;
-    int tok[HELD], mine = 0;
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      const int n = first + k;
-      tok[k] = n < N && (!mask || mask[n]) ? load_token(tokens, token_bytes, n) : -1;
-      mine += tok[k] >= 0;
-    }
-    int upto = mine;           // over this lane and those before it
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-      const int other = __shfl_up(upto, step);
-      if (lane >= step) upto += other;
-    }
-    if (lane == 63) sums[wave] = upto;
+  for (int w = 0; w < 16; ++w) done += sums[w];
+  for (int base = from; base < to; base += 1024) {
+    const int n = base + t, tok = token_of(n);
+    const uint64_t votes = __ballot(tok >= 0);
     __syncthreads();
-    int at = done + upto - mine, all = 0;
+    if (lane == 0) sums[wave] = __popcll(votes);
+    __syncthreads();
+    int at = done + __popcll(votes & ((1ull << lane) - 1));
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
       at += w < wave ? sums[w] : 0;
-      all += sums[w];
+      done += sums[w];
     }
-#pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-      const int n = first + k;
-      if (n >= N) break;
-      if (tok[k] >= 0) {
+    if (n < N) {
+      place[n] = tok >= 0 ? at : -1;
+      if (tok >= 0) {
         source[at] = n;
-        token[at] = tok[k];
-        place[n] = at++;
+        token[at] = tok;
       } else {
-        place[n] = -1;
         logp[n] = 0.f;
       }
     }
-    done += all;
-    __syncthreads();
   }
-  if (t == 0) *live = done;
+  if (blockIdx.x + 1 == gridDim.x && t == 0) *live = done;
 }
 
 // Eight elements of a row from column d on, zeros past the row's end.
@@ -298,39 +293,42 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
   }
 }
 
-// The same from logits that were summed in pieces (VM_SUMS): a workgroup joins a row, whose logits it holds, and leaves its G,
-// rounded once, and zeros in G's rows behind the last that counts.
-constexpr int VOCAB_HELD = 8192;
+// The same from logits that were summed in pieces (VM_SUMS): a row is joined by a workgroup, which holds its logits, or up to
+// VOCAB_HELD_WAVE entries by one of four waves (8000 rows of 20 tokens: 5 us against 19).  It leaves the row's G, rounded once,
+// and zeros in G's rows behind the last that counts.
+constexpr int VOCAB_HELD = 8192, VOCAB_HELD_WAVE = 512;
 
 struct VocabSoftmaxSums {
   VocabSoftmax s;
   const float* sums;          // [splits, rows, ld]
   int64_t split, ld;
   int splits;
+  int rows;                   // of G
   const void* bias;           // or null
   int elem;
 };
 
-template <class E, bool PARTS>
+template <class E, bool PARTS, bool WAVE>
 __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSums q) {
+  constexpr int THREADS = WAVE ? 64 : 256, HELD = (WAVE ? VOCAB_HELD_WAVE : VOCAB_HELD) / (8 * THREADS);
   const VocabSoftmax& p = q.s;
-  const int n = blockIdx.x, live = *p.live, t = threadIdx.x, wave = t >> 6;
-  constexpr int HELD = VOCAB_HELD / 2048;
+  const int live = *p.live, wave = threadIdx.x >> 6, t = threadIdx.x % THREADS;
+  const int n = WAVE ? blockIdx.x * 4 + wave : blockIdx.x;
   E* g = p.G ? (E*)p.G + n * p.ldg : nullptr;
   if (n >= live) {
-    if (!g || n >= (live + 63) / 64 * 64) return;
-    for (int v = 8 * t; v < p.held; v += 2048)
+    if (!g || n >= min(q.rows, (live + 63) / 64 * 64)) return;
+    for (int v = 8 * t; v < p.held; v += 8 * THREADS)
 #pragma unroll
       for (int k = 0; k < (PARTS ? VOCAB_PARTS : 1); ++k) *(Words*)(g + k * p.g_part + v) = zero_words();
     return;
   }
-  __shared__ float red[9];
+  __shared__ float red[12];
   const int token = p.token[n];
   float z[HELD][8];
-  float top = -INFINITY;
+  float top = -INFINITY, chosen = -INFINITY;
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
-    const int v = 2048 * k + 8 * t;
+    const int v = 8 * (THREADS * k + t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) z[k][e] = 0.f;
     if (v < p.vocab) {
@@ -345,14 +343,21 @@ __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSum
     for (int e = 0; e < 8; ++e) {
       if (q.bias && v + e < p.vocab) z[k][e] += load_elem(q.bias, q.elem, v + e);
       if (v + e >= p.vocab) z[k][e] = -INFINITY;
-      if (v + e == token) red[8] = z[k][e];
+      if (v + e == token) chosen = z[k][e];
       top = fmaxf(top, z[k][e]);
     }
   }
   top = wave_max(top);
-  if ((t & 63) == 0) red[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  chosen = wave_max(chosen);
+  if constexpr (!WAVE) {
+    if ((threadIdx.x & 63) == 0) {
+      red[wave] = top;
+      red[4 + wave] = chosen;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    chosen = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+  }
   float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < HELD; ++k)
@@ -361,8 +366,9 @@ __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSum
       z[k][e] = __builtin_amdgcn_exp2f((z[k][e] - top) * p.c);
       sum += z[k][e];
     }
-  sum = block_sum<4>(sum, red + 4);
-  float lp = (red[8] - top) * p.inv_t - logf(sum);
+  if constexpr (WAVE) sum = wave_sum(sum);
+  else sum = block_sum<4>(sum, red + 8);
+  float lp = (chosen - top) * p.inv_t - logf(sum);
   float inv = 1.f / sum;
   if (token >= p.vocab) lp = inv = __int_as_float(0x7fc00000);
   if (t == 0) {
@@ -374,7 +380,7 @@ __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSum
   const float at_token = (expf(lp) - 1.f) * SCALE;
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
-    const int v = 2048 * k + 8 * t;
+    const int v = 8 * (THREADS * k + t);
     if (v >= p.held) break;
     Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
 #pragma unroll
@@ -490,7 +496,8 @@ struct VocabPlan {
   int64_t piece;             // vocabulary of a piece: what G and the packed weight have room for
   int64_t tiles;             // of the vocabulary in the first pass
   int logits_tile, grads_tile;
-  int logits_splits;         // of the logits' sums; 1: they are not cut
+  bool logits_summed;        // the logits of a row are joined by one workgroup
+  int logits_splits;         // from sums over pieces of the width
   int dx_splits, dw_splits;  // of the gradients' sums
   bool dx_joined, dw_joined; // they are summed in pieces first
   // bytes from the workspace's start
@@ -547,14 +554,16 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   else p.logits_tile = p.parts == 1 && vocab_tile_count(VT_MID, V, N, p.parts) > 256 ? VT_MID : VT_DEEP;
   p.tiles = vocab_tile_count(p.logits_tile, V, 1, p.parts);
   // Few tiles are cut along the width, to some two stages at least and a workgroup for every CU at most; the joining
-  // workgroup has to hold a row.
+  // workgroup has to hold a row.  Short rows, which a wave joins, go that way cut or not.
   p.logits_splits = 1;
+  p.logits_summed = false;
   if ((p.logits_tile == VT_DEEP || p.logits_tile == VT_THIN || p.logits_tile == VT_REGS) && V <= VOCAB_HELD) {
     const int64_t tiles = vocab_tile_count(p.logits_tile, V, N, p.parts);
     int64_t splits = 256 / tiles, most = p.Dp / (p.parts > 1 ? 64 : 128);
     if (splits > most) splits = most;
     if (splits > 16) splits = 16;
     if (splits > 1) p.logits_splits = (int)splits;
+    p.logits_summed = splits > 1 || V <= VOCAB_HELD_WAVE;
   }
   const int64_t sums_ld = ceil_div(V, 256) * 256;
   p.grads_tile = VT_SLIM;
@@ -603,8 +612,8 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.token = take(4 * N);
   p.chosen = take(4 * N);
   p.row = take(8 * N);
-  p.part = take(p.logits_splits > 1 ? 0 : 8 * p.tiles * N);
-  p.sums = take(p.logits_splits > 1 ? 4 * p.logits_splits * N * sums_ld : 0);
+  p.part = take(p.logits_summed ? 0 : 8 * p.tiles * N);
+  p.sums = take(p.logits_summed ? 4 * p.logits_splits * N * sums_ld : 0);
   p.x = take(2 * p.parts * p.rows * p.Dp);
   p.w = take(p.direct || p.regs ? 0 : 2 * p.parts * p.piece * p.Dp);
   p.g = take(grad ? 2 * p.parts * p.rows * p.piece : 0);
@@ -696,7 +705,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   if (N <= VOCAB_SCAN) {
     hipLaunchKernelGGL((vocab_prepare_kernel<T, E, true>), prepare, dim3(256), 0, stream, pre);
   } else {
-    hipLaunchKernelGGL(vocab_rows_kernel, dim3(1), dim3(1024), 0, stream, q.tokens, q.token_bytes, (const uint8_t*)q.mask, N,
+    hipLaunchKernelGGL(vocab_rows_kernel, dim3(N > VOCAB_COUNTED_ROWS ? 1 : (unsigned)ceil_div(N, VOCAB_COUNTED)), dim3(1024), 0, stream, q.tokens, q.token_bytes, (const uint8_t*)q.mask, N,
                        live, source, place, token, q.logp);
     BF_LAUNCH_CHECK("bf_vocab_loss");
     hipLaunchKernelGGL((vocab_prepare_kernel<T, E, false>), prepare, dim3(256), 0, stream, pre);
@@ -744,13 +753,13 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   for (int64_t k = pieces - 1; k >= 0; --k) {
     weight_rows(k * first_piece, count_of(k), k < pieces - 1);
     a.G = p.grad && k == 0 ? g : nullptr;
-    if (p.logits_splits > 1) {
+    if (p.logits_summed) {
       a.splits = p.logits_splits;
       a.sums_ld = ceil_div(p.V, 256) * 256;
       a.sums_split = N * a.sums_ld;
       a.sums = (float*)(q.space + p.sums) + k * first_piece;
     }
-    vocab_logits<E, PARTS>(p.logits_tile, a, p.logits_splits > 1 ? VM_SUMS : VM_STATS, stream);
+    vocab_logits<E, PARTS>(p.logits_tile, a, p.logits_summed ? VM_SUMS : VM_STATS, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
 
@@ -773,10 +782,14 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   soft.g_part = g_part;
   soft.held = p.grad ? (int)(ceil_div(count_of(0), 64) * 64) : 0;
   soft.chunks = p.grad ? (int)ceil_div(soft.held, VOCAB_CHUNK) : 1;
-  if (p.logits_splits > 1) {
-    const VocabSoftmaxSums joined = {soft, (const float*)(q.space + p.sums), a.sums_split, a.sums_ld, p.logits_splits, q.bias,
-                                     p.elem};
-    hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, PARTS>), dim3((unsigned)p.rows), dim3(256), 0, stream, joined);
+  if (p.logits_summed) {
+    const VocabSoftmaxSums joined = {soft, (const float*)(q.space + p.sums), a.sums_split, a.sums_ld, p.logits_splits,
+                                     (int)p.rows, q.bias, p.elem};
+    if (p.V <= VOCAB_HELD_WAVE)
+      hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, PARTS, true>), dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, stream,
+                         joined);
+    else
+      hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, PARTS, false>), dim3((unsigned)p.rows), dim3(256), 0, stream, joined);
     a.splits = 1;
     a.sums = nullptr;
   } else {
