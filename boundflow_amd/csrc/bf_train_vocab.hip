@@ -204,11 +204,35 @@ __global__ void __launch_bounds__(256) vocab_pack_weight_kernel(const T* __restr
   pack_chunk<T, E>(row_chunk(weight + v * ld, d, D), out + v * Dp + d, part);
 }
 
+// Eight numbers, G's or what G is scaled by, in its parts.
+template <class E, int GP>
+__device__ __forceinline__ void put_parts(float y, Pack<E, 8>* x, int e) {
+  if constexpr (GP == VOCAB_PARTS) {
+    __bf16 parts[VOCAB_PARTS];
+    split_parts(y, parts);
+#pragma unroll
+    for (int q = 0; q < VOCAB_PARTS; ++q) x[q].v[e] = parts[q];
+  } else {
+    x[0].v[e] = (E)y;
+    if constexpr (GP == 2) x[1].v[e] = (E)(__builtin_isfinite(y) ? y - (float)x[0].v[e] : 0.f);
+  }
+}
+
+// Exponential e of eight as the first pass left them: fp16, or the two halves of an fp32 number.
+template <class E, int GP>
+__device__ __forceinline__ float held_exponential(const Pack<E, 8>* x, int e) {
+  if constexpr (GP == 1) return (float)__builtin_bit_cast(_Float16, x[0].v[e]) * (1.f / VOCAB_E_SCALE);
+  else
+    return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, x[0].v[e]) << 16 | __builtin_bit_cast(uint16_t, x[1].v[e]));
+}
+
+template <class E>
+constexpr float vocab_g_scale() { return __is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f; }
+
 // Statistics of the rows that count, from those of their tiles, and G from the exponentials that the first pass left, in
 // place.  A workgroup joins a row's tiles and takes VOCAB_CHUNK of its entries; the first one of a row writes what others
 // read.  The token's entry comes from its log-probability: p - 1 from a rounded p would have no digits left where p is near 1.
-// The others are rounded a second time here.  They lie here with 11 bits (fp32: whole), so that the gradients of bf16 feel
-// that rounding alone.
+// The others are rounded a second time here: they lie here with 11 bits (where G has parts, whole).
 constexpr int VOCAB_CHUNK = 8192;
 
 struct VocabSoftmax {
@@ -229,7 +253,7 @@ struct VocabSoftmax {
   int chunks;                 // workgroups of a row
 };
 
-template <class E, bool PARTS>
+template <class E, int GP>
 __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
   const int n = blockIdx.x / p.chunks, chunk = blockIdx.x - n * p.chunks;
   if (n >= *p.live) return;
@@ -260,37 +284,83 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
     p.logp[p.source[n]] = lp;
   }
   if (!p.G) return;
-  constexpr float SCALE = __is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f;
+  constexpr float SCALE = vocab_g_scale<E>();
   const float at_token = (expf(lp) - 1.f) * SCALE;
   E* g = (E*)p.G + n * p.ldg;
 #pragma unroll
   for (int k = 0; k < VOCAB_CHUNK / 2048; ++k) {
     const int v = chunk * VOCAB_CHUNK + 2048 * k + 8 * t;
     if (v >= p.held) break;
-    const float factor = __builtin_amdgcn_exp2f((part[v / p.tile].x - top) * p.c) * inv * (PARTS ? 1.f : SCALE / VOCAB_E_SCALE);
-    Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
+    const float factor = __builtin_amdgcn_exp2f((part[v / p.tile].x - top) * p.c) * inv * SCALE;
+    Pack<E, 8> x[GP];
 #pragma unroll
-    for (int q = 0; q < (PARTS ? 2 : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part + v);
+    for (int q = 0; q < (GP > 1 ? 2 : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part + v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float y;
-      if constexpr (!PARTS)
-        y = (float)__builtin_bit_cast(_Float16, x[0].v[e]);
-      else                      // the two halves of an fp32 number
-        y = __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, x[0].v[e]) << 16 | __builtin_bit_cast(uint16_t, x[1].v[e]));
-      y = v + e == token ? at_token : y * factor;
-      if constexpr (PARTS) {
-        __bf16 parts[VOCAB_PARTS];
-        split_parts(y, parts);
+    for (int e = 0; e < 8; ++e)
+      put_parts<E, GP>(v + e == token ? at_token : held_exponential<E, GP>(x, e) * factor, x, e);
 #pragma unroll
-        for (int q = 0; q < VOCAB_PARTS; ++q) x[q].v[e] = parts[q];
-      } else {
-        x[0].v[e] = (E)y;
-      }
+    for (int q = 0; q < GP; ++q) store_pack(g + q * p.g_part + v, x[q]);
+  }
+}
+
+// G in place where the bias's gradient is asked for too, from statistics that vocab_softmax_kernel has left: a workgroup takes
+// 2048 columns of 64 rows and leaves their sums, of what G is before it is rounded (a token's column cancels: the sums of
+// a rounded G were up to 1.9 times as far from 64 bits as those of fp32).
+constexpr int VOCAB_GROUP = 64;
+
+template <class E, int GP>
+__global__ void __launch_bounds__(256) vocab_softmax_columns_kernel(VocabSoftmax p, int chunks, float* __restrict__ sums) {
+  const int group = blockIdx.x / chunks, chunk = blockIdx.x - group * chunks, live = *p.live;
+  const int v = 2048 * chunk + 8 * threadIdx.x;
+  const int first = VOCAB_GROUP * group, last = min(first + VOCAB_GROUP, live);
+  if (first >= live || v >= p.held) return;
+  constexpr float SCALE = vocab_g_scale<E>();
+  float sum[8] = {};
+#pragma unroll 2
+  for (int n = first; n < last; ++n) {
+    const float2 row = p.row[n];
+    const int token = p.token[n] - v;
+    E* g = (E*)p.G + n * p.ldg + v;
+    const float factor = __builtin_amdgcn_exp2f((p.part[n * p.part_ld + v / p.tile].x - row.x) * p.c) * row.y * SCALE;
+    Pack<E, 8> x[GP];
+#pragma unroll
+    for (int q = 0; q < (GP > 1 ? 2 : 1); ++q) x[q] = load_pack<E, 8>(g + q * p.g_part);
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = held_exponential<E, GP>(x, e) * factor;
+    if (token >= 0 && token < 8) {
+      const float at_token = (expf(p.logp[p.source[n]]) - 1.f) * SCALE;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = e == token ? at_token : y[e];
     }
 #pragma unroll
-    for (int q = 0; q < (PARTS ? VOCAB_PARTS : 1); ++q) store_pack(g + q * p.g_part + v, x[q]);
+    for (int e = 0; e < 8; ++e) {
+      sum[e] += y[e];
+      put_parts<E, GP>(y[e], x, e);
+    }
+#pragma unroll
+    for (int q = 0; q < GP; ++q) store_pack(g + q * p.g_part, x[q]);
   }
+  Pack<float, 8> out;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out.v[e] = sum[e];
+  store_pack(sums + group * p.ldg + v, out);
+}
+
+// The bias's gradient from those sums; what a sum rounds away is kept and added again.
+template <class T>
+__global__ void __launch_bounds__(256) vocab_bias_kernel(const float* __restrict__ sums, int64_t ld, int columns,
+                                                         const int* __restrict__ live, float scale, T* __restrict__ grad) {
+  const int v = blockIdx.x * 256 + threadIdx.x, groups = (*live + VOCAB_GROUP - 1) / VOCAB_GROUP;
+  if (v >= columns) return;
+  float sum = 0.f, left = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < groups; ++k) {
+    const float more = sums[k * ld + v] - left, all = sum + more;
+    left = (all - sum) - more;
+    sum = all;
+  }
+  grad[v] = (T)(sum * scale / (float)max(*live, 1));
 }
 
 // The same from logits that were summed in pieces (VM_SUMS): a row is joined by a workgroup, which holds its logits, or up to
@@ -308,7 +378,7 @@ struct VocabSoftmaxSums {
   int elem;
 };
 
-template <class E, bool PARTS, bool WAVE>
+template <class E, int GP, bool WAVE>
 __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSums q) {
   constexpr int THREADS = WAVE ? 64 : 256, HELD = (WAVE ? VOCAB_HELD_WAVE : VOCAB_HELD) / (8 * THREADS);
   const VocabSoftmax& p = q.s;
@@ -319,7 +389,7 @@ __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSum
     if (!g || n >= min(q.rows, (live + 63) / 64 * 64)) return;
     for (int v = 8 * t; v < p.held; v += 8 * THREADS)
 #pragma unroll
-      for (int k = 0; k < (PARTS ? VOCAB_PARTS : 1); ++k) *(Words*)(g + k * p.g_part + v) = zero_words();
+      for (int k = 0; k < GP; ++k) *(Words*)(g + k * p.g_part + v) = zero_words();
     return;
   }
   __shared__ float red[12];
@@ -376,27 +446,17 @@ __global__ void __launch_bounds__(256) vocab_softmax_sums_kernel(VocabSoftmaxSum
     p.logp[p.source[n]] = lp;
   }
   if (!g) return;
-  constexpr float SCALE = __is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f;
+  constexpr float SCALE = vocab_g_scale<E>();
   const float at_token = (expf(lp) - 1.f) * SCALE;
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     const int v = 8 * (THREADS * k + t);
     if (v >= p.held) break;
-    Pack<E, 8> x[PARTS ? VOCAB_PARTS : 1];
+    Pack<E, 8> x[GP];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = v + e == token ? at_token : z[k][e] * inv * SCALE;
-      if constexpr (PARTS) {
-        __bf16 parts[VOCAB_PARTS];
-        split_parts(y, parts);
+    for (int e = 0; e < 8; ++e) put_parts<E, GP>(v + e == token ? at_token : z[k][e] * inv * SCALE, x, e);
 #pragma unroll
-        for (int m = 0; m < VOCAB_PARTS; ++m) x[m].v[e] = parts[m];
-      } else {
-        x[0].v[e] = (E)y;
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < (PARTS ? VOCAB_PARTS : 1); ++m) store_pack(g + m * p.g_part + v, x[m]);
+    for (int m = 0; m < GP; ++m) store_pack(g + m * p.g_part + v, x[m]);
   }
 }
 
@@ -490,18 +550,19 @@ __global__ void __launch_bounds__(256) vocab_nothing_kernel(float* loss, void* d
 
 struct VocabPlan {
   int64_t N, D, V;
-  int elem, parts;
+  int elem, parts, g_parts;  // parts of the weight and the rows, parts of G
   bool direct, regs, grad;   // the weight is read as it lies: copied to LDS, or through registers
   int64_t rows, Dp;          // padded
   int64_t piece;             // vocabulary of a piece: what G and the packed weight have room for
   int64_t tiles;             // of the vocabulary in the first pass
   int logits_tile, grads_tile;
+  bool columns;              // the bias's gradient is summed beside the softmax
   bool logits_summed;        // the logits of a row are joined by one workgroup
   int logits_splits;         // from sums over pieces of the width
   int dx_splits, dw_splits;  // of the gradients' sums
   bool dx_joined, dw_joined; // they are summed in pieces first
   // bytes from the workspace's start
-  int64_t live, source, place, token, chosen, row, part, x, w, g, sums, dx, dw, db, bytes;
+  int64_t live, source, place, token, chosen, row, part, x, w, g, cols, sums, dx, dw, db, bytes;
 };
 
 inline bool vocab_direct(int elem, int64_t D, const void* weight, int64_t ld) {
@@ -511,10 +572,10 @@ inline bool vocab_direct(int elem, int64_t D, const void* weight, int64_t ld) {
 inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
   switch (tile) {
     case VT_LARGE:
-      return ceil_div(m, VocabLarge<false>::BM) * ceil_div(n, parts > 1 ? VocabLarge<true>::BN : VocabLarge<false>::BN);
+      return ceil_div(m, VocabLarge<1>::BM) * ceil_div(n, parts > 1 ? VocabLarge<3>::BN : VocabLarge<1>::BN);
     case VT_SLIM:
     case VT_REGS:
-    case VT_THIN: return ceil_div(m, VocabSlim<false>::BM) * ceil_div(n, VocabSlim<false>::BN);
+    case VT_THIN: return ceil_div(m, VocabSlim<1>::BM) * ceil_div(n, VocabSlim<1>::BN);
     default: return ceil_div(m, VocabMid::BM) * ceil_div(n, VocabMid::BN);
   }
 }
@@ -526,7 +587,7 @@ inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
 constexpr int64_t VOCAB_REGS_FP32 = 192, VOCAB_REGS_SCORED = 64;
 
 inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld, bool grad,
-                            int64_t room) {
+                            bool bias, int64_t room) {
   VocabPlan p;
   p.N = N;
   p.D = D;
@@ -538,18 +599,9 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.regs = !p.direct && (elem == TE_F32 ? N <= VOCAB_REGS_FP32 : !grad && N <= VOCAB_REGS_SCORED);
   p.rows = ceil_div(N, 64) * 64;
   p.Dp = ceil_div(D, 64) * 64;
-  const int64_t per_token = 2 * p.parts * ((grad ? p.rows : 0) + (p.direct || p.regs ? 0 : p.Dp));
-  const int64_t whole = ceil_div(V, 256) * 256;
-  p.piece = whole;
-  if (per_token > 0) {
-    p.piece = room / per_token / 256 * 256;
-    if (p.piece < 256) p.piece = 256;
-    if (p.piece > whole) p.piece = whole;
-  }
-  const int64_t in_piece = p.piece < V ? p.piece : V;
   // by the whole vocabulary, so that the statistics have the same bits with and without gradients and whatever the room
   if (p.regs) p.logits_tile = VT_REGS;
-  else if (N <= VocabSlim<false>::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N, p.parts) > 256 ? VT_SLIM : VT_THIN;
+  else if (N <= VocabSlim<1>::BN) p.logits_tile = vocab_tile_count(VT_SLIM, V, N, p.parts) > 256 ? VT_SLIM : VT_THIN;
   else if (vocab_tile_count(VT_LARGE, V, N, p.parts) >= 200) p.logits_tile = VT_LARGE;
   else p.logits_tile = p.parts == 1 && vocab_tile_count(VT_MID, V, N, p.parts) > 256 ? VT_MID : VT_DEEP;
   p.tiles = vocab_tile_count(p.logits_tile, V, 1, p.parts);
@@ -565,6 +617,19 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
     if (splits > 1) p.logits_splits = (int)splits;
     p.logits_summed = splits > 1 || V <= VOCAB_HELD_WAVE;
   }
+  // Rounded to one 16-bit part, G's error is as large as that of the rounded gradients, and few rows do not average it out
+  // (2-norm of all errors against 64 bits over that of one rounding: one to eight rows 1.3 to 1.7, thousands 1.1 to 1.2).
+  p.g_parts = p.parts > 1 ? p.parts : grad && (N <= VocabSlim<1>::BN || (p.logits_summed && bias)) ? 2 : 1;
+  p.columns = grad && bias && !p.logits_summed && p.g_parts != 2;
+  const int64_t per_token = 2 * ((grad ? p.g_parts * p.rows : 0) + (p.direct || p.regs ? 0 : p.parts * p.Dp));
+  const int64_t whole = ceil_div(V, 256) * 256;
+  p.piece = whole;
+  if (per_token > 0) {
+    p.piece = room / per_token / 256 * 256;
+    if (p.piece < 256) p.piece = 256;
+    if (p.piece > whole) p.piece = whole;
+  }
+  const int64_t in_piece = p.piece < V ? p.piece : V;
   const int64_t sums_ld = ceil_div(V, 256) * 256;
   p.grads_tile = VT_SLIM;
   p.dx_splits = p.dw_splits = 1;
@@ -572,7 +637,7 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   if (grad) {
     if (p.regs) {
       p.grads_tile = VT_REGS;
-    } else if (N <= VocabSlim<false>::BN) {
+    } else if (N <= VocabSlim<1>::BN) {
       const int64_t slim = vocab_tile_count(VT_SLIM, D, N, p.parts) + vocab_tile_count(VT_SLIM, D, in_piece, p.parts);
       p.grads_tile = slim > 256 ? VT_SLIM : VT_THIN;
     } else {
@@ -580,6 +645,7 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
       const int64_t mid = vocab_tile_count(VT_MID, D, N, p.parts) + vocab_tile_count(VT_MID, D, in_piece, p.parts);
       p.grads_tile = large >= 200 ? VT_LARGE : p.parts == 1 && mid > 256 ? VT_MID : VT_DEEP;
     }
+    if (p.g_parts == 2 && (p.grads_tile == VT_LARGE || p.grads_tile == VT_MID)) p.grads_tile = VT_DEEP;
     // Sums are cut along k so that none of them takes longer than a good part of the whole launch, nor than it takes to
     // add one more piece's sums (some eight stages).
     const int64_t slots = p.grads_tile == VT_LARGE || p.grads_tile == VT_DEEP || p.grads_tile == VT_THIN ? 256 : 512;
@@ -616,7 +682,8 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   p.sums = take(p.logits_summed ? 4 * p.logits_splits * N * sums_ld : 0);
   p.x = take(2 * p.parts * p.rows * p.Dp);
   p.w = take(p.direct || p.regs ? 0 : 2 * p.parts * p.piece * p.Dp);
-  p.g = take(grad ? 2 * p.parts * p.rows * p.piece : 0);
+  p.g = take(grad ? 2 * p.g_parts * p.rows * p.piece : 0);
+  p.cols = take(p.columns ? 4 * ceil_div(N, VOCAB_GROUP) * p.piece : 0);
   p.dx = take(p.dx_joined ? 4 * p.dx_splits * p.rows * p.Dp : 0);
   p.dw = take(p.dw_joined ? 4 * p.dw_splits * V * p.Dp : 0);
   p.db = take(p.dw_joined ? 4 * p.dw_splits * V : 0);
@@ -645,8 +712,8 @@ struct VocabCall {
   hipStream_t stream;
 };
 
-// T: the tensors' type, E: the matrix products'
-template <class T, class E>
+// T: the tensors' type, E: the matrix products', GP: the parts of G
+template <class T, class E, int GP>
 int vocab_run(const VocabPlan& p, const VocabCall& q) {
   constexpr bool PARTS = sizeof(T) == 4;
   hipStream_t stream = q.stream;
@@ -759,7 +826,8 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
       a.sums_split = N * a.sums_ld;
       a.sums = (float*)(q.space + p.sums) + k * first_piece;
     }
-    vocab_logits<E, PARTS>(p.logits_tile, a, p.logits_summed ? VM_SUMS : VM_STATS, stream);
+    if (p.logits_summed) vocab_logits<E, PARTS ? GP : 1>(p.logits_tile, a, VM_SUMS, stream);
+    else vocab_logits<E, GP>(p.logits_tile, a, VM_STATS, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
 
@@ -767,7 +835,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   soft.part = part;
   soft.part_ld = p.tiles;
   soft.tiles = (int)p.tiles;
-  soft.tile = p.logits_tile == VT_LARGE ? VocabLarge<false>::BM : VocabMid::BM;
+  soft.tile = p.logits_tile == VT_LARGE ? VocabLarge<1>::BM : VocabMid::BM;
   soft.chosen = chosen;
   soft.token = token;
   soft.source = source;
@@ -786,14 +854,27 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     const VocabSoftmaxSums joined = {soft, (const float*)(q.space + p.sums), a.sums_split, a.sums_ld, p.logits_splits,
                                      (int)p.rows, q.bias, p.elem};
     if (p.V <= VOCAB_HELD_WAVE)
-      hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, PARTS, true>), dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, stream,
+      hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, GP, true>), dim3((unsigned)ceil_div(p.rows, 4)), dim3(256), 0, stream,
                          joined);
     else
-      hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, PARTS, false>), dim3((unsigned)p.rows), dim3(256), 0, stream, joined);
+      hipLaunchKernelGGL((vocab_softmax_sums_kernel<E, GP, false>), dim3((unsigned)p.rows), dim3(256), 0, stream, joined);
     a.splits = 1;
     a.sums = nullptr;
+  } else if (p.columns) {
+    VocabSoftmax stats = soft;
+    stats.G = nullptr;
+    stats.chunks = 1;
+    hipLaunchKernelGGL((vocab_softmax_kernel<E, GP>), dim3((unsigned)N), dim3(256), 0, stream, stats);
+    BF_LAUNCH_CHECK("bf_vocab_loss");
+    const int chunks = (int)ceil_div(soft.held, 2048);
+    float* cols = (float*)(q.space + p.cols);
+    hipLaunchKernelGGL((vocab_softmax_columns_kernel<E, GP>), dim3((unsigned)(ceil_div(N, VOCAB_GROUP) * chunks)), dim3(256), 0,
+                       stream, soft, chunks, cols);
+    BF_LAUNCH_CHECK("bf_vocab_loss");
+    hipLaunchKernelGGL((vocab_bias_kernel<T>), dim3((unsigned)ceil_div(count_of(0), 256)), dim3(256), 0, stream, cols, p.piece,
+                       count_of(0), live, scale, (T*)q.grad_bias);
   } else {
-    hipLaunchKernelGGL((vocab_softmax_kernel<E, PARTS>), dim3((unsigned)((int64_t)N * soft.chunks)), dim3(256), 0, stream, soft);
+    hipLaunchKernelGGL((vocab_softmax_kernel<E, GP>), dim3((unsigned)((int64_t)N * soft.chunks)), dim3(256), 0, stream, soft);
   }
   BF_LAUNCH_CHECK("bf_vocab_loss");
   if (!p.grad) {
@@ -808,7 +889,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     weight_rows(v0, count, k > 0);
     if (k > 0) {
       a.G = g;
-      vocab_logits<E, PARTS>(p.logits_tile, a, VM_GRAD, stream);
+      vocab_logits<E, GP>(p.logits_tile, a, VM_GRAD, stream);
       BF_LAUNCH_CHECK("bf_vocab_loss");
     }
     // dx: the weight's rows are k
@@ -842,8 +923,8 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     d.b_cols = (int)p.piece;
     d.out = (char*)q.grad_weight + v0 * D * elem_bytes(q.grad_weight_elem);
     d.out_elem = q.grad_weight_elem;
-    d.db = q.grad_bias ? (T*)q.grad_bias + v0 : nullptr;
-    vocab_grads<E, PARTS>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream);
+    d.db = q.grad_bias && !(p.columns && k == 0) ? (T*)q.grad_bias + v0 : nullptr;
+    vocab_grads<E, GP>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
   if (p.dx_joined || p.dw_joined) {
@@ -862,7 +943,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     j.dw_splits = p.dw_splits;
     j.grad_weight = q.grad_weight;
     j.dw_elem = q.grad_weight_elem;
-    if (q.grad_bias) j.db = db;
+    if (q.grad_bias && !p.columns) j.db = db;
     j.grad_bias = q.grad_bias;
     j.elem = p.elem;
     j.D = D;
@@ -893,6 +974,7 @@ inline bool vocab_launches_ok(const VocabPlan& p) {
                         vocab_tile_count(p.grads_tile, p.D, p.piece, p.parts) * p.dw_splits;
   const int64_t joined = (p.dx_joined ? p.N : 0) + (p.dw_joined ? p.V : 0);
   return products(p.grads_tile, tiles) && launch_fits(p.N * ceil_div(p.piece, VOCAB_CHUNK), 256) &&
+         launch_fits(ceil_div(p.N, VOCAB_GROUP) * ceil_div(p.piece, 2048), 256) &&
          launch_fits(ceil_div(joined * ceil_div(p.D, 8), 256), 256);
 }
 
@@ -901,9 +983,9 @@ inline bool vocab_launches_ok(const VocabPlan& p) {
 using namespace bf;
 
 extern "C" int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
-                                           int with_grad, int64_t room) {
+                                           int with_grad, int with_bias, int64_t room) {
   if (!elem_ok(elem) || N <= 0 || D <= 0 || V <= 0 || ld_w < D || room < 0 || !vocab_sizes_ok(N, D, V, ld_w)) return 0;
-  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0, room);
+  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0, with_bias != 0, room);
   return vocab_launches_ok(p) ? p.bytes / 4 : 0;
 }
 
@@ -925,7 +1007,7 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
              "bf_vocab_loss: weight gradient of element type %d", grad_weight_elem);
   const bool sizes = B <= VOCAB_ROWS && T <= VOCAB_ROWS && vocab_sizes_ok(B * T, D, V, ld_w);
   VocabPlan p;
-  if (sizes && B * T > 0) p = vocab_plan(B * T, D, V, elem, weight, ld_w, grad, room);
+  if (sizes && B * T > 0) p = vocab_plan(B * T, D, V, elem, weight, ld_w, grad, bias != nullptr, room);
   if (!sizes || (B * T > 0 && !vocab_launches_ok(p))) {
     set_error("bf_vocab_loss: %lld x %lld rows, width %lld, vocabulary %lld, weight rows %lld apart are more than it takes",
               (long long)B, (long long)T, (long long)D, (long long)V, (long long)ld_w);
@@ -945,8 +1027,8 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
   const VocabCall q = {hidden, T, ld_b, ld_t, weight, ld_w, bias, tokens, token_bytes, mask, temperature, grad_scale, logp,
                        loss, grad_hidden, grad_weight, grad_weight_elem, grad_bias, (char*)workspace, stream};
   switch (elem) {
-    case TE_F32: return vocab_run<float, __bf16>(p, q);
-    case TE_BF16: return vocab_run<__bf16, __bf16>(p, q);
-    default: return vocab_run<_Float16, _Float16>(p, q);
+    case TE_F32: return vocab_run<float, __bf16, VOCAB_PARTS>(p, q);
+    case TE_BF16: return p.g_parts == 2 ? vocab_run<__bf16, __bf16, 2>(p, q) : vocab_run<__bf16, __bf16, 1>(p, q);
+    default: return p.g_parts == 2 ? vocab_run<_Float16, _Float16, 2>(p, q) : vocab_run<_Float16, _Float16, 1>(p, q);
   }
 }

@@ -13,6 +13,9 @@
 // otherwise (W in dX, both in dW) a stage is held as rows of k and read by ds_read_b64_tr_b16, which hands a lane four
 // k of its column, so that no operand is transposed in memory.
 //
+// Up to 64 rows, and where a bias's gradient is asked for of few tiles, G comes as two 16-bit parts: a rounding of it to one
+// would not average out over the rows, and the products are not the time.
+//
 // fp32 values come as three bf16 parts, x = x0 + x1 + x2 (8 + 8 + 8 significant bits); a product is the sum of six
 // part products, least first: x0 y2, x1 y1, x2 y0, x0 y1, x1 y0, x0 y0, into the same fp32 sums.  What is left out is
 // 2^-24 of a product.  A stage holds the three parts of both operands, each read from LDS once for two products (the six one after
@@ -82,16 +85,15 @@ struct VocabArgs {
   float scale;               // of out and db, before the division by the rows that count
 };
 
-// Tiles of BM x BN, NWM x NWN waves of 32 FM x 32 FN each; STAGES of LDS, OCC workgroups on a CU.  FUSED: three
-// parts of fp32 operands in a stage.
-template <int FM_, int FN_, int NWM_, int NWN_, int STAGES_, int OCC_, bool FUSED_>
+// Tiles of BM x BN, NWM x NWN waves of 32 FM x 32 FN each; STAGES of LDS, OCC workgroups on a CU; parts of A and of B in a
+// stage, whose products with parts i and j of i + j < max(PA, PB) are summed.
+template <int FM_, int FN_, int NWM_, int NWN_, int STAGES_, int OCC_, int PA_, int PB_>
 struct VocabTile {
-  static constexpr int FM = FM_, FN = FN_, NWM = NWM_, NWN = NWN_, STAGES = STAGES_, OCC = OCC_;
-  static constexpr bool FUSED = FUSED_;
-  static constexpr int BK = FUSED ? 32 : 64, PLANES = FUSED ? VOCAB_PARTS : 1;   // k of a stage, parts in it
+  static constexpr int FM = FM_, FN = FN_, NWM = NWM_, NWN = NWN_, STAGES = STAGES_, OCC = OCC_, PA = PA_, PB = PB_;
+  static constexpr int BK = PA == VOCAB_PARTS ? 32 : 64;   // k of a stage
   static constexpr int BM = 32 * FM * NWM, BN = 32 * FN * NWN, WAVES = NWM * NWN, NT = 64 * WAVES;
-  static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2, A_BYTES = PLANES * A_PLANE;
-  static constexpr int STAGE = A_BYTES + PLANES * B_PLANE;
+  static constexpr int A_PLANE = BM * BK * 2, B_PLANE = BN * BK * 2, A_BYTES = PA * A_PLANE;
+  static constexpr int STAGE = A_BYTES + PB * B_PLANE;
   // behind the stages: the bias of the tile's rows, two floats per column from each half of a wave along M
   static constexpr int BIAS_AT = STAGES * STAGE, RED_AT = BIAS_AT + 4 * BM, LDS = RED_AT + 2 * 4 * 2 * NWM * BN;
   static constexpr int TILE = 2 * BM * BN;   // of 16-bit results
@@ -235,7 +237,7 @@ __device__ __forceinline__ void wait_copies() {
 // Stages that pass through registers, for a weight of type S that cannot be copied as it lies (rows that do not start at 16
 // bytes, fp32 that is split into parts on the way): where few rows use it, a packed copy of it would take longer than
 // everything else.  The layout in LDS is VocabOperand's; what is past the end of rows or columns is zeros.
-template <bool TR, int SIDE, int NT, int BK, int PLANES, class S>
+template <bool TR, int SIDE, int NT, int BK, class S>
 struct VocabWeightChunks {
   typedef VocabOperand<TR, SIDE, NT / 64, BK> Op;
   static constexpr int COUNT = SIDE * BK / 8 / NT;
@@ -304,16 +306,17 @@ struct VocabRowChunks {
   }
 };
 
-// S: the type of a weight that passes through registers, or void.
-template <class T, int MODE, class E, bool PARTS, class S = void>
+// GP: the parts of G.  S: the type of a weight that passes through registers, or void.
+template <class T, int MODE, class E, int GP, class S = void>
 __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint32_t block) {
   constexpr bool A_TR = MODE >= VM_DX, B_TR = MODE == VM_DW;
   constexpr int FM = T::FM, FN = T::FN;
   typedef typename Vec8<E>::type V8;
   typedef VocabOperand<A_TR, T::BM, T::WAVES, T::BK> OpA;
   typedef VocabOperand<B_TR, T::BN, T::WAVES, T::BK> OpB;
-  constexpr int BK = T::BK, PLANES = T::PLANES;
-  static_assert(PARTS == T::FUSED, "three parts in a stage");
+  constexpr int BK = T::BK, PA = T::PA, PB = T::PB;
+  constexpr bool PARTS = GP == VOCAB_PARTS;
+  static_assert(PA == (PARTS ? VOCAB_PARTS : 1) && PB == (MODE >= VM_DX || PARTS ? GP : 1), "the operands' parts");
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -365,13 +368,13 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
       left = 1;
     }
 #pragma unroll
-    for (int part = 0; part < PLANES; ++part) {
+    for (int part = 0; part < PA; ++part) {
       const uint32_t to = dst + part * T::A_PLANE;
       if (left < BK) opa.copy_last(from + 2 * part * p.a_part, p.lda, left, wave, lane, to);
       else opa.copy(from + 2 * part * p.a_part, wave, to);
     }
 #pragma unroll
-    for (int part = 0; part < PLANES; ++part)
+    for (int part = 0; part < PB; ++part)
       opb.copy(b_at + 2 * part * p.b_part, wave, dst + T::A_BYTES + part * T::B_PLANE);
     a_at += a_step;
     b_at += b_step;
@@ -393,54 +396,63 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  float col_sum[FN];
+  float col_sum[FN], col_left[FN];
   const bool sum_cols = MODE == VM_DW && p.db && tm == 0 && wave % T::NWM == 0;
 #pragma unroll
-  for (int j = 0; j < FN; ++j) col_sum[j] = 0.f;
-  // G's column sums, the bias's gradient
-  auto column_sums = [&](const V8* x) {
+  for (int j = 0; j < FN; ++j) col_sum[j] = col_left[j] = 0.f;
+  // G's column sums, the bias's gradient: they cancel (a token's are one less than its probability), so what a sum rounds
+  // away is kept and added again
+  auto column_sums = [&](const V8 (&x)[PB][FN]) {
     if (sum_cols) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+      for (int j = 0; j < FN; ++j) {
+        float more = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) col_sum[j] += (float)x[j][e];
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int part = PB - 1; part >= 0; --part) more += (float)x[part][j][e];
+        more -= col_left[j];
+        const float all = col_sum[j] + more;
+        col_left[j] = (all - col_sum[j]) - more;
+        col_sum[j] = all;
+      }
     }
   };
-
   auto fragments = [&](const char* stage, int first, auto& a, auto& b) {
     constexpr int KK = sizeof(a) / sizeof(a[0]);
 #pragma unroll
     for (int k = 0; k < KK; ++k)
 #pragma unroll
-      for (int part = 0; part < PLANES; ++part) {
+      for (int part = 0; part < (PA > PB ? PA : PB); ++part) {
+        if (part < PA)
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-          a[k][part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, first + k, lane);
+          for (int i = 0; i < FM; ++i)
+            a[k][part][i] = OpA::template read<V8>(stage + part * T::A_PLANE, wm + 32 * i, first + k, lane);
+        if (part < PB)
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-          b[k][part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, first + k, lane);
+          for (int j = 0; j < FN; ++j)
+            b[k][part][j] = OpB::template read<V8>(stage + T::A_BYTES + part * T::B_PLANE, wn + 32 * j, first + k, lane);
       }
   };
-  auto multiply = [&](const V8 (&a)[PLANES][FM], const V8 (&b)[PLANES][FN]) {
+  auto multiply = [&](const V8 (&a)[PA][FM], const V8 (&b)[PB][FN]) {
 #pragma unroll
-    for (int sum = PLANES - 1; sum >= 0; --sum)     // the least products first
+    for (int sum = (PA > PB ? PA : PB) - 1; sum >= 0; --sum)     // the least products first
 #pragma unroll
-      for (int part = 0; part <= sum; ++part)
+      for (int part = 0; part <= sum; ++part) {
+        if (part >= PA || sum - part >= PB) continue;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int j = 0; j < FN; ++j) acc[i][j] = mfma16(a[part][i], b[sum - part][j], acc[i][j]);
-    if constexpr (MODE == VM_DW) {
-#pragma unroll
-      for (int part = 0; part < PLANES; ++part) column_sums(b[part]);
-    }
+      }
+    if constexpr (MODE == VM_DW) column_sums(b);
   };
 
   if constexpr (!__is_same(S, void)) {
     static_assert(MODE != VM_DW && T::STAGES >= 2 && T::WAVES == 4, "the weight is the first operand; two buffers");
     constexpr int AHEAD = 3;      // stages under way in registers
-    VocabWeightChunks<A_TR, T::BM, T::NT, BK, PLANES, S> wa[AHEAD];
-    VocabRowChunks<T::BN, T::NT, BK, PLANES> xb[AHEAD];
+    VocabWeightChunks<A_TR, T::BM, T::NT, BK, S> wa[AHEAD];
+    VocabRowChunks<T::BN, T::NT, BK, PB> xb[AHEAD];
     auto load = [&](int s, int to) {
       const int k0 = (k_first + s) * BK;
       wa[to].load((const S*)p.A, p.lda, k0, m0, p.a_rows, p.a_cols);
@@ -462,7 +474,7 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
           if (s + AHEAD < steps) load(s + AHEAD, d);
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {
-            V8 a[1][PLANES][FM], b[1][PLANES][FN];
+            V8 a[1][PA][FM], b[1][PB][FN];
             fragments(stage, kk, a, b);
             multiply(a[0], b[0]);
           }
@@ -484,7 +496,7 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         constexpr int KK = BK / 32;     // 16 k each, of half a stage
-        V8 a[KK][PLANES][FM], b[KK][PLANES][FN];
+        V8 a[KK][PA][FM], b[KK][PB][FN];
         fragments(stage, KK * h, a, b);
         if (h == 0 && s + 1 < steps) issue((s + 1) & 1);
         if (h == 1 && second) wait_copies<0>();
@@ -502,7 +514,7 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     if (!second) asm volatile("s_barrier" ::: "memory");
   } else {
     // All but one of the stages are under way.
-    constexpr int AHEAD = T::STAGES - 1, COPIES = PLANES * (OpA::PER_WAVE + OpB::PER_WAVE);
+    constexpr int AHEAD = T::STAGES - 1, COPIES = PA * OpA::PER_WAVE + PB * OpB::PER_WAVE;
     if constexpr (T::STAGES == 1) {
       // for sums of one stage: the workgroups beside this one hide its copies
       if (steps > 0) issue(0);
@@ -529,11 +541,11 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
       to = to + 1 == T::STAGES ? 0 : to + 1;
       // a stage's fragments are on their way together where they fit the registers, or the products would wait for LDS
       // at every 16 k
-      constexpr int KK = PLANES * (FM + FN) * (BK / 16) <= 24 ? BK / 16 : BK / 32;
-      constexpr bool TOGETHER = PLANES * (FM + FN) * KK <= 24;
+      constexpr int KK = (PA * FM + PB * FN) * (BK / 16) <= 24 ? BK / 16 : BK / 32;
+      constexpr bool TOGETHER = (PA * FM + PB * FN) * KK <= 24;
 #pragma unroll
       for (int h = 0; h < BK / 16 / KK; ++h) {
-        V8 a[KK][PLANES][FM], b[KK][PLANES][FN];
+        V8 a[KK][PA][FM], b[KK][PB][FN];
         fragments(stage, KK * h, a, b);
         if constexpr (TOGETHER) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -623,10 +635,10 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
     }
     if (MODE == VM_GRAD || p.G) {
       // The tile as rows of G: a lane has four neighbours of a row, a wave 32 rows, so it passes through LDS (slot s of
-      // 16 bytes of row n at s ^ n % slots) to be written in whole lines.  fp32: part by part; exponentials, which are not
-      // multiplied yet, as the upper and the lower 16 bits of the number.
+      // 16 bytes of row n at s ^ n % slots) to be written in whole lines.  In parts: one by one; exponentials, which are not
+      // multiplied yet, as the upper and the lower 16 bits of an fp32 number.
       constexpr int SLOTS = T::BM / 8;
-      constexpr int PLANES = !PARTS ? 1 : MODE == VM_STATS ? 2 : VOCAB_PARTS;
+      constexpr int PLANES = GP > 1 && MODE == VM_STATS ? 2 : GP;
       static_assert(T::TILE <= T::STAGES * T::STAGE, "in the stages' memory");
 #pragma unroll 1
       for (int part = 0; part < PLANES; ++part) {
@@ -642,16 +654,15 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float v = acc[i][j][4 * q + r];
-                if constexpr (!PARTS && MODE == VM_STATS) {
+                if constexpr (GP == 1 && MODE == VM_STATS) {
                   x.v[r] = __builtin_bit_cast(E, (_Float16)(v * VOCAB_E_SCALE));
-                } else if constexpr (__is_same(E, _Float16)) {
-                  x.v[r] = (E)(v * VOCAB_F16_SCALE);
-                } else if constexpr (PARTS && MODE == VM_STATS) {
+                } else if constexpr (MODE == VM_STATS) {
                   const uint32_t bits = __float_as_uint(v);
                   x.v[r] = __builtin_bit_cast(E, (uint16_t)(part ? bits : bits >> 16));
                 } else {
-                  x.v[r] = (E)v;
-                  if constexpr (PARTS) acc[i][j][4 * q + r] = __builtin_isfinite(v) ? v - (float)x.v[r] : 0.f;
+                  constexpr float SCALE = __is_same(E, _Float16) ? VOCAB_F16_SCALE : 1.f;
+                  x.v[r] = (E)(v * SCALE);
+                  if constexpr (GP > 1) acc[i][j][4 * q + r] = __builtin_isfinite(v) ? v - (float)x.v[r] * (1.f / SCALE) : 0.f;
                 }
               }
               const int slot = ((wm + 32 * i) / 8 + q) ^ (col % SLOTS);
@@ -777,71 +788,78 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
   }
 }
 
-template <class T, int MODE, class E, bool PARTS, class S = void>
+template <class T, int MODE, class E, int GP, class S = void>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4) vocab_logits_kernel(VocabArgs p) {
   __shared__ __attribute__((aligned(1024))) char smem[T::LDS];
-  vocab_tile<T, MODE, E, PARTS, S>(p, smem, blockIdx.x);
+  vocab_tile<T, MODE, E, GP, S>(p, smem, blockIdx.x);
 }
 
 // dX (tiles T) and dW (tiles W) of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the CUs that dX's few long
 // ones leave.  dX's come first; the last workgroup takes the loss where `loss` is given.
-template <class T, class W, class E, bool PARTS, class S = void>
+template <class T, class W, class E, int GP, class S = void>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
     vocab_grads_kernel(VocabArgs dx, VocabArgs dw, uint32_t dx_blocks, const float* logp, int rows, float* loss) {
   static_assert(T::NT == W::NT && W::STAGES * W::STAGE <= T::STAGES * T::STAGE && T::TILE <= T::STAGES * T::STAGE &&
                     W::TILE <= T::STAGES * T::STAGE, "dX's stages hold dW's, and the tiles of both");
   __shared__ __attribute__((aligned(1024))) char smem[T::STAGES * T::STAGE];
   if (loss && blockIdx.x + 1 == gridDim.x) vocab_loss<T::WAVES>(logp, rows, *dx.live, loss, (float*)smem);
-  else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, PARTS, S>(dx, smem, blockIdx.x);
-  else vocab_tile<W, VM_DW, E, PARTS>(dw, smem, blockIdx.x - dx_blocks);
+  else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, GP, S>(dx, smem, blockIdx.x);
+  else vocab_tile<W, VM_DW, E, GP>(dw, smem, blockIdx.x - dx_blocks);
 }
 
 // Workgroups for `tiles` tiles at most, a whole number per XCD.
 inline int64_t vocab_blocks(int64_t tiles) { return 8 * ceil_div(tiles, 8); }
 
-template <class T, class E, bool PARTS, class S = void>
+template <class T, class E, int GP, class S = void>
 inline void launch_vocab_logits(const VocabArgs& p, int mode, hipStream_t stream) {
   const dim3 grid((unsigned)vocab_blocks(ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN) * p.splits));
+  // what no call asks for is not compiled: only small grids are cut, whatever G has; few rows have G in parts, many in one
+  constexpr bool FEW = T::BN == 64;
   if (mode == VM_SUMS) {
-    // only small grids are cut
-    if constexpr ((T::OCC == 1 && T::WAVES == 4) || !__is_same(S, void))
-      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_SUMS, E, PARTS, S>), grid, dim3(T::NT), 0, stream, p);
-  } else if (mode == VM_STATS) hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, PARTS, S>), grid, dim3(T::NT), 0, stream, p);
-  else hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, PARTS, S>), grid, dim3(T::NT), 0, stream, p);
+    if constexpr (GP != 2 && ((T::OCC == 1 && T::WAVES == 4) || !__is_same(S, void)))
+      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_SUMS, E, GP, S>), grid, dim3(T::NT), 0, stream, p);
+  } else if (mode == VM_STATS) {
+    if constexpr (GP != 2 || FEW)
+      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, GP, S>), grid, dim3(T::NT), 0, stream, p);
+  } else {
+    if constexpr (GP != 1 || !FEW)
+      hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, GP, S>), grid, dim3(T::NT), 0, stream, p);
+  }
 }
 
-template <class T, class W, class E, bool PARTS, class S = void>
+template <class T, class W, class E, int GP, class S = void>
 inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                                hipStream_t stream) {
   const int64_t first = vocab_blocks(ceil_div(dx.M, T::BM) * ceil_div(dx.N, T::BN) * dx.splits);
   const int64_t all = first + vocab_blocks(ceil_div(dw.M, W::BM) * ceil_div(dw.N, W::BN) * dw.splits) + (loss ? 1 : 0);
-  hipLaunchKernelGGL((vocab_grads_kernel<T, W, E, PARTS, S>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
+  hipLaunchKernelGGL((vocab_grads_kernel<T, W, E, GP, S>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
                      logp, rows, loss);
 }
 
-// Tiles by the size of the problem (P: for fp32 in parts).
+// Tiles by the size of the problem; G: the parts of G (3: of everything, fp32), for the gradients PB of them.
 // Large: the products' rate.  Mid: where Large would leave CUs without a tile.  Slim: up to 64 rows, where the
 // weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU.  Deep and
 // Thin are these with more stages under way for grids of at most a workgroup per CU, whose time is the copies' latency.
-template <bool P>
-using VocabLarge = VocabTile<P ? 2 : 4, 2, P ? 4 : 2, P ? 2 : 4, 2, 1, P>;
-template <bool P>
-using VocabDeep = VocabTile<2, 2, 2, 2, P ? 3 : 4, 1, P>;
-template <bool P>
-using VocabThin = VocabTile<1, 2, 4, 1, P ? 4 : 6, 1, P>;
-template <bool P>
-using VocabSlim = VocabTile<1, 2, 4, 1, P ? 2 : 3, 2, P>;
-typedef VocabTile<2, 2, 2, 2, 2, 2, false> VocabMid;      // in parts it would be Deep
+constexpr int vocab_pa(int g) { return g == VOCAB_PARTS ? g : 1; }
+template <int G>
+using VocabLarge = VocabTile<G == 3 ? 2 : 4, 2, G == 3 ? 4 : 2, G == 3 ? 2 : 4, 2, 1, vocab_pa(G), G>;
+template <int G>
+using VocabDeep = VocabTile<2, 2, 2, 2, G == 1 ? 4 : 3, 1, vocab_pa(G), G>;
+template <int G>
+using VocabThin = VocabTile<1, 2, 4, 1, G == 1 ? 6 : 4, 1, vocab_pa(G), G>;
+template <int G>
+using VocabSlim = VocabTile<1, 2, 4, 1, G == 1 ? 3 : 2, 2, vocab_pa(G), G>;
+typedef VocabTile<2, 2, 2, 2, 2, 2, 1, 1> VocabMid;      // in parts it would be Deep
 // dW beside Slim's dX: its rows are k, one stage of them, so that the tile's stores are its time
-template <bool P>
-using VocabWide = VocabTile<1, P ? 4 : 8, 4, 1, 1, 2, P>;
+template <int G>
+using VocabWide = VocabTile<1, 4, 4, 1, 1, 2, vocab_pa(G), G>;
 
 enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4, VT_REGS = 5 };   // REGS: Slim through registers
 
 // Defined for each type by a file of its own (bf_vocab_*.hip).
-template <class E, bool PARTS>
+template <class E, int GP>
 void vocab_logits(int tile, const VocabArgs& p, int mode, hipStream_t stream);
-template <class E, bool PARTS>
+template <class E, int GP>
 void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                  hipStream_t stream);
 

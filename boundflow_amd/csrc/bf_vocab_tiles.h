@@ -5,49 +5,60 @@
 
 namespace bf {
 
-template <class E, bool PARTS>
+// The type of a weight that passes through registers.
+template <class E, int GP>
 struct WeightType {
   typedef E type;
 };
 template <class E>
-struct WeightType<E, true> {
+struct WeightType<E, VOCAB_PARTS> {
   typedef float type;
 };
 
-template <class E, bool PARTS>
+// Of the logits' products: of 16-bit types one part of each operand, whatever G has.
+template <class E, int GP>
 void vocab_logits(int tile, const VocabArgs& p, int mode, hipStream_t stream) {
+  constexpr int P = vocab_pa(GP);
+  typedef typename WeightType<E, GP>::type S;
   switch (tile) {
-    case VT_LARGE: launch_vocab_logits<VocabLarge<PARTS>, E, PARTS>(p, mode, stream); break;
+    case VT_LARGE:
+      if constexpr (GP != 2) launch_vocab_logits<VocabLarge<P>, E, GP>(p, mode, stream);
+      break;
     case VT_MID:
-      if constexpr (!PARTS) launch_vocab_logits<VocabMid, E, PARTS>(p, mode, stream);
+      if constexpr (GP == 1) launch_vocab_logits<VocabMid, E, GP>(p, mode, stream);
       break;
-    case VT_DEEP: launch_vocab_logits<VocabDeep<PARTS>, E, PARTS>(p, mode, stream); break;
-    case VT_THIN: launch_vocab_logits<VocabThin<PARTS>, E, PARTS>(p, mode, stream); break;
+    case VT_DEEP: launch_vocab_logits<VocabDeep<P>, E, GP>(p, mode, stream); break;
+    case VT_THIN: launch_vocab_logits<VocabThin<P>, E, GP>(p, mode, stream); break;
     case VT_REGS:
-      launch_vocab_logits<VocabSlim<PARTS>, E, PARTS, typename WeightType<E, PARTS>::type>(p, mode, stream);
+      if constexpr (GP != 2) launch_vocab_logits<VocabSlim<P>, E, GP, S>(p, mode, stream);
       break;
-    default: launch_vocab_logits<VocabSlim<PARTS>, E, PARTS>(p, mode, stream);
+    default: launch_vocab_logits<VocabSlim<P>, E, GP>(p, mode, stream);
   }
 }
 
-template <class E, bool PARTS>
+template <class E, int GP>
 void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                  hipStream_t stream) {
-  typedef VocabLarge<PARTS> Large;
-  typedef VocabDeep<PARTS> Deep;
-  typedef VocabThin<PARTS> Thin;
+  typedef VocabLarge<GP> Large;
+  typedef VocabDeep<GP> Deep;
+  typedef VocabThin<GP> Thin;
+  typedef typename WeightType<E, GP>::type S;
   switch (tile) {
-    case VT_LARGE: launch_vocab_grads<Large, Large, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    case VT_LARGE:
+      if constexpr (GP != 2) launch_vocab_grads<Large, Large, E, GP>(dx, dw, logp, rows, loss, stream);
+      break;
     case VT_MID:
-      if constexpr (!PARTS) launch_vocab_grads<VocabMid, VocabMid, E, PARTS>(dx, dw, logp, rows, loss, stream);
+      if constexpr (GP == 1) launch_vocab_grads<VocabMid, VocabMid, E, GP>(dx, dw, logp, rows, loss, stream);
       break;
-    case VT_DEEP: launch_vocab_grads<Deep, Deep, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
-    case VT_THIN: launch_vocab_grads<Thin, Thin, E, PARTS>(dx, dw, logp, rows, loss, stream); break;
+    case VT_DEEP: launch_vocab_grads<Deep, Deep, E, GP>(dx, dw, logp, rows, loss, stream); break;
+    case VT_THIN:
+      if constexpr (GP != 1) launch_vocab_grads<Thin, Thin, E, GP>(dx, dw, logp, rows, loss, stream);
+      break;
     case VT_REGS:
-      launch_vocab_grads<VocabSlim<PARTS>, VocabWide<PARTS>, E, PARTS, typename WeightType<E, PARTS>::type>(
-          dx, dw, logp, rows, loss, stream);
+      if constexpr (GP == 3) launch_vocab_grads<VocabSlim<GP>, VocabWide<GP>, E, GP, S>(dx, dw, logp, rows, loss, stream);
       break;
-    default: launch_vocab_grads<VocabSlim<PARTS>, VocabWide<PARTS>, E, PARTS>(dx, dw, logp, rows, loss, stream);
+    default:
+      if constexpr (GP != 1) launch_vocab_grads<VocabSlim<GP>, VocabWide<GP>, E, GP>(dx, dw, logp, rows, loss, stream);
   }
 }
 

@@ -472,7 +472,7 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     if wide not in (weight.dtype, torch.float32):
         raise ValueError(f"weight_grad_dtype must be {weight.dtype} or float32, got {wide}")
     N = B * T
-    need = _lib.load().bf_vocab_loss_workspace(N, D, V, elem, weight.data_ptr(), ld, with_grad, room)
+    need = _lib.load().bf_vocab_loss_workspace(N, D, V, elem, weight.data_ptr(), ld, with_grad, bias is not None, room)
     out = torch.empty(1 + N, dtype=torch.float32, device=hidden.device)      # loss, logp
     space = torch.empty(need, dtype=torch.float32, device=hidden.device) if need else None
     grad_hidden = grad_weight = grad_bias = None

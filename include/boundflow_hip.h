@@ -676,7 +676,7 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
  * both calls): bytes that the softmax's gradient, in the products' type, and a copy of such a weight may take; of what has
  * no room the logits are formed twice. */
 int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
-                                int with_grad, int64_t room);
+                                int with_grad, int with_bias, int64_t room);
 int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
                   const void* weight, int64_t V, int64_t ld_w, const void* bias, const void* tokens, int token_bytes,
                   const void* mask, double temperature, float grad_scale, float* logp, float* loss, void* grad_hidden,

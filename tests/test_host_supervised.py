@@ -67,7 +67,7 @@ def test_workspaces_hold_what_their_kernels_write(lib):
     for N, D, V, elem in ((1, 1, 1, 0), (8, 2048, 32000, 1), (1003, 1025, 50001, 2), (2048, 1024, 32000, 0),
                           (8184, 4096, 128000, 1)):
         some = 1 << 20        # an address that can be read as it lies
-        alone, grad = size(N, D, V, elem, some, D, 0, 256 << 20), size(N, D, V, elem, some, D, 1, 256 << 20)
+        alone, grad = size(N, D, V, elem, some, D, 0, 0, 256 << 20), size(N, D, V, elem, some, D, 1, 0, 256 << 20)
         assert 0 < alone < grad
         # a token, a place and statistics per row and tile of the vocabulary; the packed rows
         parts = 3 if elem == 0 else 1
@@ -75,13 +75,13 @@ def test_workspaces_hold_what_their_kernels_write(lib):
         # G stays within the room (the logits would be 4 N V), the sums of the hidden rows' gradient within theirs
         assert 4 * (grad - alone) <= (256 << 20) + max(128 << 20, 4 * (N + 64) * (D + 64)) + 4096
         # no room: a piece of 256 tokens
-        assert 4 * size(N, D, V, elem, some, D, 1, 0) < 4 * alone + 600 * parts * (N + D + 128) + \
+        assert 4 * size(N, D, V, elem, some, D, 1, 0, 0) < 4 * alone + 600 * parts * (N + D + 128) + \
             max(128 << 20, 4 * (N + 64) * (D + 64)) + 4096
     room = 1 << 30
-    assert size(0, 4, 4, 0, 0, 4, 1, room) == 0 and size(4, 4, 4, 7, 0, 4, 1, room) == 0
-    assert size(1 << 24, 4, 4, 0, 0, 4, 1, room) == 0 and size(4, 4, 4, 0, 0, 4, 1, -1) == 0
+    assert size(0, 4, 4, 0, 0, 4, 1, 1, room) == 0 and size(4, 4, 4, 7, 0, 4, 1, 1, room) == 0
+    assert size(1 << 24, 4, 4, 0, 0, 4, 1, 1, room) == 0 and size(4, 4, 4, 0, 0, 4, 1, 1, -1) == 0
     # a weight that has to be packed takes more
-    assert size(100, 64, 1000, 1, 1 << 20, 64, 0, room) < size(100, 64, 1000, 1, (1 << 20) + 2, 64, 0, room)
+    assert size(100, 64, 1000, 1, 1 << 20, 64, 0, 0, room) < size(100, 64, 1000, 1, (1 << 20) + 2, 64, 0, 0, room)
 
 
 def test_requires_grad_is_refused_before_the_device_is_asked():
@@ -112,7 +112,7 @@ def test_results_do_not_keep_the_workspace(recorded, rows, V):  # noqa: F811
     r = training.vocabulary_loss(fp32(rows, 24), fp32(V, 24), torch.zeros(rows, dtype=torch.int64))
     held = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in r if t is not None}
     assert sum(held.values()) <= 4 * (1 + rows + 24 * (rows + V)) + 64
-    need = _lib.load().bf_vocab_loss_workspace(rows, 24, V, 0, calls[0][1][7], 24, 1, 2 << 30)
+    need = _lib.load().bf_vocab_loss_workspace(rows, 24, V, 0, calls[0][1][7], 24, 1, 0, 2 << 30)
     space = calls[0][1][-3]
     base = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in recorded[0]}
     assert base[space] >= 4 * need
