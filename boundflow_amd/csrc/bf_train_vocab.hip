@@ -304,9 +304,9 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
 }
 
 // G in place where the bias's gradient is asked for too, from statistics that vocab_softmax_kernel has left: a workgroup takes
-// 2048 columns of 64 rows and leaves their sums, of what G is before it is rounded (a token's column cancels: the sums of
+// 2048 columns of 32 rows and leaves their sums, of what G is before it is rounded (a token's column cancels: the sums of
 // a rounded G were up to 1.9 times as far from 64 bits as those of fp32).
-constexpr int VOCAB_GROUP = 64;
+constexpr int VOCAB_GROUP = 32;
 
 template <class E, int GP>
 __global__ void __launch_bounds__(256) vocab_softmax_columns_kernel(VocabSoftmax p, int chunks, float* __restrict__ sums) {
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256) vocab_softmax_columns_kernel(VocabSoftmax
   if (first >= live || v >= p.held) return;
   constexpr float SCALE = vocab_g_scale<E>();
   float sum[8] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int n = first; n < last; ++n) {
     const float2 row = p.row[n];
     const int token = p.token[n] - v;

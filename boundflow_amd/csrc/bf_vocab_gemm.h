@@ -541,16 +541,16 @@ __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint3
       to = to + 1 == T::STAGES ? 0 : to + 1;
       // a stage's fragments are on their way together where they fit the registers, or the products would wait for LDS
       // at every 16 k
-      constexpr int KK = (PA * FM + PB * FN) * (BK / 16) <= 24 ? BK / 16 : BK / 32;
-      constexpr bool TOGETHER = (PA * FM + PB * FN) * KK <= 24;
+      constexpr int EACH = PA * FM + PB * FN;
+      constexpr int KK = EACH * (BK / 16) <= 24 ? BK / 16 : EACH * (BK / 32) <= 24 ? BK / 32 : 1;
 #pragma unroll
       for (int h = 0; h < BK / 16 / KK; ++h) {
         V8 a[KK][PA][FM], b[KK][PB][FN];
         fragments(stage, KK * h, a, b);
-        if constexpr (TOGETHER) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < KK; ++k) multiply(a[k], b[k]);
-        if constexpr (TOGETHER) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -799,9 +799,10 @@ __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4) vocab_logi
 template <class T, class W, class E, int GP, class S = void>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
     vocab_grads_kernel(VocabArgs dx, VocabArgs dw, uint32_t dx_blocks, const float* logp, int rows, float* loss) {
-  static_assert(T::NT == W::NT && W::STAGES * W::STAGE <= T::STAGES * T::STAGE && T::TILE <= T::STAGES * T::STAGE &&
-                    W::TILE <= T::STAGES * T::STAGE, "dX's stages hold dW's, and the tiles of both");
-  __shared__ __attribute__((aligned(1024))) char smem[T::STAGES * T::STAGE];
+  static_assert(T::NT == W::NT, "one launch");
+  constexpr int LDS = T::STAGES * T::STAGE > W::STAGES * W::STAGE ? T::STAGES * T::STAGE : W::STAGES * W::STAGE;
+  static_assert(T::TILE <= LDS && W::TILE <= LDS, "tiles of results pass through the stages' memory");
+  __shared__ __attribute__((aligned(1024))) char smem[LDS];
   if (loss && blockIdx.x + 1 == gridDim.x) vocab_loss<T::WAVES>(logp, rows, *dx.live, loss, (float*)smem);
   else if (blockIdx.x < dx_blocks) vocab_tile<T, VM_DX, E, GP, S>(dx, smem, blockIdx.x);
   else vocab_tile<W, VM_DW, E, GP>(dw, smem, blockIdx.x - dx_blocks);
