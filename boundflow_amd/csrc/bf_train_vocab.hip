@@ -586,6 +586,9 @@ inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
 // 119 / 77, 128 rows 131 / 137; with gradients, whose product along the vocabulary is read two bytes aside, 227 / 277.
 constexpr int64_t VOCAB_REGS_FP32 = 192, VOCAB_REGS_SCORED = 64;
 
+// The copies to LDS address G from a tile's first row by 32 bits of bytes: 256 rows of so many tokens at most.
+constexpr int64_t VOCAB_PIECE = 1LL << 23;
+
 inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld, bool grad,
                             bool bias, int64_t room) {
   VocabPlan p;
@@ -627,6 +630,7 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
   if (per_token > 0) {
     p.piece = room / per_token / 256 * 256;
     if (p.piece < 256) p.piece = 256;
+    if (p.piece > VOCAB_PIECE) p.piece = VOCAB_PIECE;
     if (p.piece > whole) p.piece = whole;
   }
   const int64_t in_piece = p.piece < V ? p.piece : V;

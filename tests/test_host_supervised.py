@@ -84,6 +84,15 @@ def test_workspaces_hold_what_their_kernels_write(lib):
     assert size(100, 64, 1000, 1, 1 << 20, 64, 0, 0, room) < size(100, 64, 1000, 1, (1 << 20) + 2, 64, 0, 0, room)
 
 
+def test_rows_of_the_softmax_stay_within_32_bit_offsets(lib):
+    """The products address a tile of up to 256 rows of G by 32 bits of bytes, however much room there is: 2^23 tokens."""
+    for N, parts in ((64, 2), (256, 1)):
+        V, D = 1 << 27, 8
+        stats = 8 * (V // 128) * N + (1 << 24)      # per row and tile; dx's sums of 128 MB, dw's none
+        got = 4 * lib.bf_vocab_loss_workspace(N, D, V, 1, 1 << 20, D, 1, 0, 1 << 60)
+        assert 2 * parts * N * (1 << 23) <= got <= 2 * parts * N * (1 << 23) + stats + (128 << 20)
+
+
 def test_requires_grad_is_refused_before_the_device_is_asked():
     x = torch.zeros(3, requires_grad=True)
     with pytest.raises(HipError, match="dropout_grad"):
