@@ -1009,7 +1009,9 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
              "bf_vocab_loss: gradients of hidden rows and weight, and of the bias where there is one, come together");
   BF_REQUIRE(!grad || grad_weight_elem == elem || grad_weight_elem == TE_F32,
              "bf_vocab_loss: weight gradient of element type %d", grad_weight_elem);
-  const bool sizes = B <= VOCAB_ROWS && T <= VOCAB_ROWS && vocab_sizes_ok(B * T, D, V, ld_w);
+  bool sizes = B <= VOCAB_ROWS && T <= VOCAB_ROWS && vocab_sizes_ok(B * T, D, V, ld_w);
+  const int64_t cleared = sizes && grad ? ceil_div(V * D, 256 * 16) : 1;      // workgroups of a call without rows
+  if (sizes && B * T == 0) sizes = launch_fits(cleared, 256);
   VocabPlan p;
   if (sizes && B * T > 0) p = vocab_plan(B * T, D, V, elem, weight, ld_w, grad, bias != nullptr, room);
   if (!sizes || (B * T > 0 && !vocab_launches_ok(p))) {
@@ -1021,10 +1023,8 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
   BF_REQUIRE(weight && (N == 0 || (hidden && tokens && logp && workspace)), "bf_vocab_loss: null pointer");
   BF_REQUIRE((uintptr_t)workspace % 16 == 0, "bf_vocab_loss: workspace not aligned to 16 bytes");
   if (N == 0) {
-    const int64_t weights = grad ? V * D : 0, biases = grad_bias ? V : 0;
-    const int64_t blocks = ceil_div(weights > biases ? weights : biases, 256 * 16);
-    hipLaunchKernelGGL(vocab_nothing_kernel, dim3(blocks ? (unsigned)blocks : 1), dim3(256), 0, stream, loss, grad_weight,
-                       weights, grad_weight_elem, grad_bias, biases, elem);
+    hipLaunchKernelGGL(vocab_nothing_kernel, dim3((unsigned)cleared), dim3(256), 0, stream, loss, grad_weight, grad ? V * D : 0,
+                       grad_weight_elem, grad_bias, grad_bias ? V : 0, elem);
     BF_LAUNCH_CHECK("bf_vocab_loss");
     return BF_OK;
   }

@@ -93,6 +93,14 @@ def test_rows_of_the_softmax_stay_within_32_bit_offsets(lib):
         assert 2 * parts * N * (1 << 23) <= got <= 2 * parts * N * (1 << 23) + stats + (128 << 20)
 
 
+def test_an_empty_batch_over_a_vocabulary_past_a_launch_is_refused(lib):
+    p = torch.zeros(64).data_ptr()
+    args = lambda V, D: (None, 1, 0, 2, D, 0, 0, p, V, D, None, None, 8, None, 1.0, 1.0, None, p, None, p, 1, None, None,  # noqa: E731
+                         1 << 30, None)
+    assert lib.bf_vocab_loss(*args(1 << 30, 1 << 20)) == 3
+    assert lib.bf_vocab_loss(*args(1 << 25, 1 << 11)) == 3
+
+
 def test_requires_grad_is_refused_before_the_device_is_asked():
     x = torch.zeros(3, requires_grad=True)
     with pytest.raises(HipError, match="dropout_grad"):
