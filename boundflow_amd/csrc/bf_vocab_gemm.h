@@ -31,7 +31,6 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
-typedef short short8v __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) short4v lds_short4;
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -233,7 +232,6 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
 }
 
-// One tile's sums.  `block` of `share * 8` workgroups: XCD block % 8's share-th of the tiles.
 // Stages that pass through registers, for a weight of type S that cannot be copied as it lies (rows that do not start at 16
 // bytes, fp32 that is split into parts on the way): where few rows use it, a packed copy of it would take longer than
 // everything else.  The layout in LDS is VocabOperand's; what is past the end of rows or columns is zeros.
@@ -306,7 +304,8 @@ struct VocabRowChunks {
   }
 };
 
-// GP: the parts of G.  S: the type of a weight that passes through registers, or void.
+// One tile.  `block`: XCD block % 8 takes a share of neighbouring tiles.  GP: the parts of G.  S: the type of a weight that
+// passes through registers, or void.
 template <class T, int MODE, class E, int GP, class S = void>
 __device__ __forceinline__ void vocab_tile(const VocabArgs& p, char* smem, uint32_t block) {
   constexpr bool A_TR = MODE >= VM_DX, B_TR = MODE == VM_DW;
