@@ -20,6 +20,7 @@ No counterpart in the reference, which bounds networks and does not train them.
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -203,6 +204,7 @@ def _dropout(x, name, p, seed, counter, residual) -> torch.Tensor:
     elem = _elem(x, name)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p must be in [0, 1], got {p}")
+    seed = operator.index(seed)
     if not 0 <= seed < 1 << 64:
         raise ValueError(f"seed must be in [0, 2^64), got {seed}")
     at, counter_dev = 0, None
@@ -212,7 +214,7 @@ def _dropout(x, name, p, seed, counter, residual) -> torch.Tensor:
             raise HipError("counter must be a number or an int64 tensor of one element")
         counter_dev = counter.data_ptr()
     else:
-        at = int(counter)
+        at = operator.index(counter)
         if not 0 <= at < 1 << 63:
             raise ValueError(f"counter must be in [0, 2^63), got {counter}")
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)

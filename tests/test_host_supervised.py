@@ -142,3 +142,11 @@ def test_seeds_and_counters_reach_the_library_whole(recorded):  # noqa: F811
     (_, a), (_, b) = calls
     assert a[8] == -1 and a[9] == (1 << 63) - 1 and a[10] is None and a[5:7] == (1, 6)
     assert b[8] == 5 and b[9] == 0 and b[10] is not None and b[5:7] == (4, 4)
+
+
+def test_a_seed_or_counter_that_is_no_integer_is_refused(recorded):  # noqa: F811
+    _made, calls = recorded
+    for kw in ({"seed": 1, "counter": 1.5}, {"seed": 1.0}, {"seed": 1, "counter": 2.0}):
+        with pytest.raises(TypeError):
+            training.dropout(fp32(6), 0.25, **kw)
+    assert not calls
