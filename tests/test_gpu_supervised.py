@@ -120,6 +120,17 @@ def test_vocabulary_loss_of_many_tiles(dtype, N, D, V):
     check(hidden, weight, tokens, bias=bias, mask=mask, wide=torch.float32)
 
 
+@pytest.mark.parametrize("N,D,V,dtype", [(1025, 24, 60, torch.float32), (5000, 40, 9, torch.bfloat16), (66_000, 16, 530, torch.bfloat16),
+                                         (70_000, 8, 5, torch.float32)])
+def test_rows_that_are_counted_by_many(N, D, V, dtype):
+    """More rows than one workgroup counts, and than many do, of 32-bit tokens, long stretches of them not counting."""
+    hidden, weight, tokens, bias = head(N, D, V, dtype, 3)
+    mask = torch.rand(N, generator=gen(6)) < 0.7
+    mask[: N // 9] = False
+    mask[N // 3: N // 2] = False
+    check(hidden, weight, tokens, bias=bias, mask=mask, on={"tokens": tokens.int().to(device())})
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["some", "sequence", "first", "empty", "negative"])
 @pytest.mark.parametrize("B,T", [(3, 2), (5, 77)])
@@ -472,6 +483,31 @@ def test_on_another_stream_and_in_a_graph():
             assert torch.equal(a, b), turn
         seen.append(captured[2].clone())
     assert not torch.equal(seen[0], seen[1])
+
+
+def test_two_graphs():
+    """Two captured calls of different sizes, replayed in turn beside eager ones: neither's workspace is the other's."""
+    dev = device()
+    cases = [[t.to(dev) for t in head(n, 128, v, dtype, n)] for n, v, dtype in
+             ((150, 2000, torch.bfloat16), (7, 9000, torch.bfloat16), (100, 40, torch.float32))]
+    run = lambda c: training.vocabulary_loss(c[0], c[1], c[2], bias=c[3], room=1 << 20)  # noqa: E731
+    for c in cases:
+        run(c)
+    graphs, results = [], []
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(run(c))
+    for turn in range(3):
+        for c in cases:
+            c[0].copy_(torch.randn(c[0].shape, generator=gen(turn)))
+        for k in (0, 1, 2, 1, 0):
+            graphs[k].replay()
+        want = [run(c) for c in cases]
+        torch.cuda.synchronize()
+        for a, b in zip(results, want):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y), turn
 
 
 def test_scores_feed_the_other_losses():
