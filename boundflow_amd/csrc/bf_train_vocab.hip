@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
   __shared__ float red[8];
   const int t = threadIdx.x, wave = t >> 6;
   const float2* part = p.part + n * p.part_ld;
-  // the exponentials are on their way while the tiles are joined (3150 rows of 32000 tokens 76 us in the place of 93, 5.3 TB/s; 6500 of
-  // 128000 693 in the place of 750, 4.8 TB/s)
+  // the exponentials are on their way while the tiles are joined (3150 rows of 32000 tokens 76 us in the place of 93,
+  // 5.3 TB/s; 6500 of 128000 693 in the place of 750, 4.8 TB/s)
   constexpr int PLANES = GP > 1 ? 2 : 1, COUNT = VOCAB_CHUNK / 2048;
   E* g = p.G ? (E*)p.G + n * p.ldg + chunk * VOCAB_CHUNK + 8 * t : nullptr;
   const int first = chunk * VOCAB_CHUNK + 8 * t;
@@ -589,9 +589,10 @@ inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
 }
 
 // Rows up to which a weight that cannot be copied to LDS as it lies passes through registers, where a packed copy of it would be
-// most of the bytes.  fp32 (us, packed / through registers; rows of 2048 over 32000 tokens): 8 rows 399 / 265, 128 rows 529 / 401, 192 rows
-// 620 / 567, scored alone 212 / 91, 252 / 126, 271 / 195.  16-bit rows of an odd width, scored: 64 rows of 2049 over 50001 tokens
-// 119 / 77, 128 rows 131 / 137; with gradients, whose product along the vocabulary is read two bytes aside, 227 / 277.
+// most of the bytes.  fp32 (us, packed / through registers; rows of 2048 over 32000 tokens): 8 rows 399 / 265, 128 rows
+// 529 / 401, 192 rows 620 / 567, scored alone 212 / 91, 252 / 126, 271 / 195.  16-bit rows of an odd width, scored: 64 rows
+// of 2049 over 50001 tokens 119 / 77, 128 rows 131 / 137; with gradients, whose product along the vocabulary is read two
+// bytes aside, 227 / 277.
 constexpr int64_t VOCAB_REGS_FP32 = 192, VOCAB_REGS_SCORED = 64;
 
 // The copies to LDS address G from a tile's first row by 32 bits of bytes: 256 rows of so many tokens at most.

@@ -18,9 +18,9 @@
 //
 // fp32 values come as three bf16 parts, x = x0 + x1 + x2 (8 + 8 + 8 significant bits); a product is the sum of six
 // part products, least first: x0 y2, x1 y1, x2 y0, x0 y1, x1 y0, x0 y0, into the same fp32 sums.  What is left out is
-// 2^-24 of a product.  A stage holds the three parts of both operands, each read from LDS once for two products (the six one after
-// another along k, a part of each operand in a stage: 2048 x 1024 rows over 32000 tokens 2041 us in the place of 1667, a head of eight
-// actions 45 us in the place of 40).
+// 2^-24 of a product.  A stage holds the three parts of both operands, each read from LDS once for two products (the six
+// one after another along k, a part of each operand in a stage: 2048 x 1024 rows over 32000 tokens 2041 us in the place
+// of 1667, a head of eight actions 45 us in the place of 40).
 #pragma once
 
 #include "bf_train.h"
@@ -37,9 +37,9 @@ typedef __attribute__((address_space(3))) char lds_char;
 enum : int { VM_STATS = 0, VM_GRAD = 1, VM_SUMS = 2, VM_DX = 3, VM_DW = 4 };
 
 // z's tiles end in one of three ways.  VM_STATS: the tile's largest logit and sum of exponentials per token, and where G is
-// given the exponentials themselves, 2^(c (z - the tile's largest)); vocab_softmax_kernel makes them G in place.  VM_GRAD, with the rows'
-// statistics known: G.  VM_SUMS: sums over a part of k each, of a problem with so few tiles that they are cut along k (a CU
-// takes 40 GB/s from memory, so few CUs take long); vocab_softmax_sums_kernel joins them.
+// given the exponentials themselves, 2^(c (z - the tile's largest)); vocab_softmax_kernel makes them G in place.  VM_GRAD,
+// with the rows' statistics known: G.  VM_SUMS: sums over a part of k each, of a problem with so few tiles that they are
+// cut along k (a CU takes 40 GB/s from memory, so few CUs take long); vocab_softmax_sums_kernel joins them.
 
 constexpr int VOCAB_BK = 64;            // k come in multiples of this
 constexpr int VOCAB_PARTS = 3;
@@ -793,8 +793,8 @@ __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4) vocab_logi
   vocab_tile<T, MODE, E, GP, S>(p, smem, blockIdx.x);
 }
 
-// dX (tiles T) and dW (tiles W) of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the CUs that dX's few long
-// ones leave.  dX's come first; the last workgroup takes the loss where `loss` is given.
+// dX (tiles T) and dW (tiles W) of a piece, in one launch: neither needs the other, and the many short tiles of dW fill the
+// CUs that dX's few long ones leave.  dX's come first; the last workgroup takes the loss where `loss` is given.
 template <class T, class W, class E, int GP, class S = void>
 __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
     vocab_grads_kernel(VocabArgs dx, VocabArgs dw, uint32_t dx_blocks, const float* logp, int rows, float* loss) {
@@ -837,9 +837,11 @@ inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const f
 }
 
 // Tiles by the size of the problem; G: the parts of G (3: of everything, fp32), for the gradients PB of them.
-// Large: the products' rate.  Mid: where Large would leave CUs without a tile.  Slim: up to 64 rows, where the
-// weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU.  Deep and
-// Thin are these with more stages under way for grids of at most a workgroup per CU, whose time is the copies' latency.
+// Large: the products' rate, 1.2 PFLOP/s over 128000 tokens of 4096 (the matrix cores busy in 68 to 72 % of the cycles, whose
+// clock falls to 1.4 to 1.65 GHz meanwhile).  Mid: where Large would leave CUs without a tile.  Slim: up to 64 rows, where
+// the weight's bytes are the time: 16 KB of it in a stage and two stages of two workgroups under way on a CU (44 rows
+// scored over 50001 tokens of 2048: 6.3 TB/s).  Deep and Thin are these with more stages under way for grids of at most a
+// workgroup per CU, whose time is the copies' latency.
 constexpr int vocab_pa(int g) { return g == VOCAB_PARTS ? g : 1; }
 template <int G>
 using VocabLarge = VocabTile<G == 3 ? 2 : 4, 2, G == 3 ? 4 : 2, G == 3 ? 2 : 4, 2, 1, vocab_pa(G), G>;
