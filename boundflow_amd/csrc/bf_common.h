@@ -122,6 +122,12 @@ __device__ __forceinline__ float wave_max_nonneg(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// A copy from memory to LDS in inline assembly (asynchronous; vmcnt counts it): M0 takes the LDS address, operand `dst`, and
+// has to be written one wait state before the copy reads it, which the compiler sees to in its own code and not in an
+// assembly block.  The block clobbers M0.
+#define BF_COPY_TO_LDS(op, address, dst) "s_mov_b32 m0, " dst "\n\ts_nop 0\n\t" op " " address
+#pragma clang diagnostic ignored "-Winline-asm"   // M0 in a clobber list, once per use: reserved, so never allocated
+
 // m / d for 0 <= m, d > 0, in 32-bit arithmetic when both fit (uniform over a launch)
 __device__ __forceinline__ int64_t div_rows(int64_t m, int64_t d, bool fits32) {
   return fits32 ? (int64_t)((uint32_t)m / (uint32_t)d) : m / d;

@@ -98,12 +98,11 @@ constexpr int gemm_waves_per_simd() {
 // One global_load_lds_dwordx4: lane l's 16 bytes at src land at lds_dst + 16 l
 // (lds_dst wave-uniform).  Issued as inline assembly so that the compiler does
 // not track the copy and adds no wait before the LDS reads of other stages; the
-// loop orders it with wait_vmem and lds_barrier.  M0 holds the LDS address (no
-// other code of the kernel uses M0).
+// loop orders it with wait_vmem and lds_barrier.  M0 holds the LDS address.
 typedef __attribute__((address_space(3))) float lds_float;
 __device__ __forceinline__ void lds_copy16(const float* src, float* lds_dst) {
   const uint32_t off = (uint32_t)(uintptr_t)((lds_float*)lds_dst);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(off) : "memory");
+  asm volatile(BF_COPY_TO_LDS("global_load_lds_dwordx4", "%0, off", "%1") ::"v"(src), "s"(off) : "memory", "m0");
 }
 
 template <int N>

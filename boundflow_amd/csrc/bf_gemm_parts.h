@@ -63,17 +63,17 @@ struct TileParts {
 // lds_copy16 from a scalar base and a byte offset per lane.
 __device__ __forceinline__ void lds_copy16_at(const float* base, uint32_t byte_off, float* lds_dst) {
   const uint32_t off = (uint32_t)(uintptr_t)((lds_float*)lds_dst);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(byte_off), "s"(base), "s"(off) : "memory");
+  asm volatile(BF_COPY_TO_LDS("global_load_lds_dwordx4", "%0, %1", "%2") ::"v"(byte_off), "s"(base), "s"(off) : "memory", "m0");
 }
 
 // The same, four bytes a lane (256 of LDS in a row), from a scalar base or a lane's own address.
 __device__ __forceinline__ void lds_copy4_at(const float* base, uint32_t byte_off, float* lds_dst) {
   const uint32_t off = (uint32_t)(uintptr_t)((lds_float*)lds_dst);
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(byte_off), "s"(base), "s"(off) : "memory");
+  asm volatile(BF_COPY_TO_LDS("global_load_lds_dword", "%0, %1", "%2") ::"v"(byte_off), "s"(base), "s"(off) : "memory", "m0");
 }
 __device__ __forceinline__ void lds_copy4(const float* src, float* lds_dst) {
   const uint32_t off = (uint32_t)(uintptr_t)((lds_float*)lds_dst);
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(off) : "memory");
+  asm volatile(BF_COPY_TO_LDS("global_load_lds_dword", "%0, off", "%1") ::"v"(src), "s"(off) : "memory", "m0");
 }
 
 // (x, y) -> the packed bf16 pair nearest to it, and what the pair leaves of both.

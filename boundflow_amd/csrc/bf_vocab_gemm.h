@@ -100,7 +100,7 @@ struct VocabTile {
 
 // 16 bytes a lane from base + off to LDS at dst + 16 lane, asynchronously (vmcnt counts it)
 __device__ __forceinline__ void copy16_to_lds(const void* base, uint32_t off, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory");
+  asm volatile(BF_COPY_TO_LDS("global_load_lds_dwordx4", "%0, %1", "%2") ::"v"(off), "s"(base), "s"(dst) : "memory", "m0");
 }
 
 __device__ __forceinline__ floatx16 mfma16(bf16x8v a, bf16x8v b, floatx16 c) {
