@@ -976,6 +976,10 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   return BF_OK;
 }
 
+// Beyond, log2(e) / temperature would leave fp32's normal numbers, and 0 or infinity times the -inf of a tile's padding, or
+// of a barred token, is no number.
+constexpr double VOCAB_TEMPERATURE = 0x1p120;
+
 constexpr int64_t VOCAB_ROWS = 1LL << 23, VOCAB_DIM = 1LL << 20, VOCAB_TOKENS = 1LL << 30;
 
 inline bool vocab_sizes_ok(int64_t N, int64_t D, int64_t V, int64_t ld_w) {
@@ -1018,7 +1022,8 @@ extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T,
              elem, token_bytes);
   BF_REQUIRE(B >= 0 && T >= 0 && D > 0 && V > 0 && ld_b >= 0 && ld_t >= 0 && ld_w >= D && room >= 0,
              "bf_vocab_loss: bad sizes");
-  BF_REQUIRE(temperature > 0.0, "bf_vocab_loss: temperature %g", temperature);
+  BF_REQUIRE(temperature >= 1.0 / VOCAB_TEMPERATURE && temperature <= VOCAB_TEMPERATURE, "bf_vocab_loss: temperature %g",
+             temperature);
   BF_REQUIRE(loss, "bf_vocab_loss: null pointer");
   const bool grad = grad_hidden || grad_weight || grad_bias;
   BF_REQUIRE(!grad || (grad_weight && (B * T == 0 || grad_hidden) && !bias == !grad_bias),

@@ -436,8 +436,8 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     dims = len(shape)
     if dims not in (2, 3) or shape[-1] < 1:
         raise ValueError(f"hidden must be [B, T, D] or [N, D] with D >= 1, got {tuple(shape)}")
-    if not temperature > 0.0:
-        raise ValueError(f"temperature must be >0, got {temperature}")
+    if not 2.0 ** -120 <= temperature <= 2.0 ** 120:
+        raise ValueError(f"temperature must be in [2^-120, 2^120], got {temperature}")
     lead, D = shape[:-1], shape[-1]
     strides = hidden.stride()
     if strides[-1] != 1 and D > 1:

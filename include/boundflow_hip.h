@@ -667,7 +667,8 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
 
 /* Softmax cross entropy of a head over a vocabulary, with its gradients; the logits are not kept.  Hidden rows
  * [B, T, D], row (b, t) at b * ld_b + t * ld_t; weight [V, D] with row stride ld_w, bias [V] (NULL: none) of the same type;
- * tokens and mask (bytes; NULL: all ones) dense [B, T].  With z = hidden . weight + bias over the temperature:
+ * tokens and mask (bytes; NULL: all ones) dense [B, T].  With z = hidden . weight + bias over the temperature
+ * (between 2^-120 and 2^120):
  *   logp = z[token] - log(sum of exp(z)),  loss = the mean of -logp over the live rows (0 without one).
  * A row is live unless it is masked or its token negative; other rows are not read, and their logp and gradient
  * are 0.  A token past the vocabulary gives NaN.  grad_hidden dense [B, T, D] and grad_bias [V] of the inputs' type,

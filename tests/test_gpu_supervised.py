@@ -633,3 +633,22 @@ def test_example_with_a_supervised_stage():
     got = example().main(["--steps", "2", "--contexts", "64", "--eps", "0.02", "--imitate", "5"])
     assert len(got["imitated"]) == 5 and all(math.isfinite(x) for x in (*got["imitated"], *got["losses"]))
     assert 0.0 <= got["after"][1] <= got["after"][0] <= 1.0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V", [(6, 130), (6, 33_001), (100, 130), (100, 8300)])
+def test_far_temperatures(dtype, N, V):
+    """The largest temperature leaves all tokens alike, the least the largest logit alone; padded entries stay out of both."""
+    dev = device()
+    hidden, weight, tokens, bias = (t.to(dev) for t in head(N, 64, V, dtype, 2))
+    bias[1] = float("-inf")
+    tokens = torch.where(tokens == 1, 2, tokens)
+    got = training.vocabulary_loss(hidden, weight, tokens, bias=bias, temperature=2.0 ** 120)
+    # a sum of V - 1 equal terms in fp32, V / 256 of them one after another, and its logarithm
+    tol = (V / 256 + 16) * 2.0 ** -24 + 2.0 ** -23 * math.log(V)
+    close(got.logp, torch.full((N,), -math.log(V - 1), dtype=torch.float64), tol, "all alike")
+    assert all(bool(torch.isfinite(t).all()) for t in got)
+    z = torch.mm(hidden.float(), weight.float().t()) + bias.float()
+    top = z.argmax(1)
+    got = training.vocabulary_loss(hidden, weight, top, bias=bias, temperature=2.0 ** -120)
+    assert not bool(got.logp.any()), "the largest logit has all the probability"

@@ -150,3 +150,14 @@ def test_a_seed_or_counter_that_is_no_integer_is_refused(recorded):  # noqa: F81
         with pytest.raises(TypeError):
             training.dropout(fp32(6), 0.25, **kw)
     assert not calls
+
+
+@pytest.mark.parametrize("value", [float("inf"), 1e39, 2.0 ** 121, 2.0 ** -121, 1e-39, 5e-324])
+def test_temperatures_that_fp32_does_not_hold_are_refused(lib, recorded, value):  # noqa: F811
+    """Their inverse would be 0 or infinite in fp32, and that times a padded entry's -inf is no number."""
+    _made, calls = recorded
+    p = torch.zeros(64).data_ptr()
+    assert lib.bf_vocab_loss(p, 0, 1, 2, 4, 8, 4, p, 3, 4, p, p, 8, None, value, 1.0, p, p, p, p, 0, p, p, 1 << 30, None) == 1
+    with pytest.raises(ValueError, match="temperature"):
+        training.vocabulary_loss(fp32(2, 4), fp32(3, 4), torch.zeros(2, dtype=torch.int64), temperature=value)
+    assert not calls
