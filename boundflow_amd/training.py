@@ -423,6 +423,7 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     gives NaN.  The gradients are ``grad_scale`` times the loss's, of the inputs' type, the weight's also in float32
     (``weight_grad_dtype``; ``embed_tokens_grad`` can then add that of a tied table to it).  ``with_grad=False`` gives loss
     and log-probabilities alone: those that ``policy_loss`` and ``preference_loss`` take as an old or a reference policy's.
+    The result comes without a graph: a hidden, weight or bias that requires grad is refused while gradients are recorded.
 
     Products of 16-bit inputs are summed in fp32; between them the softmax's gradient is held in the inputs' type, up to 64 rows
     (with a bias and a small vocabulary: more) in two parts of it, so with twice the digits; fp32 in 24 bits.  The bias's
@@ -430,6 +431,11 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     what is not shows as NaN.  ``room`` bytes of that gradient (and of a copy of a weight whose rows cannot be read as they
     lie) are held at a time, for as many tokens of the vocabulary as fit; the logits of the others are formed twice, which
     takes up to a third longer."""
+    if torch.is_grad_enabled():
+        for t, name in ((hidden, "hidden"), (weight, "weight"), (bias, "bias")):
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise HipError(f"{name} requires grad, but the loss comes without a graph: pass {name}.detach() and take its "
+                               "gradient from the result")
     dev = _current_device(hidden, "hidden")
     elem = _elem(hidden, "hidden")
     shape = hidden.shape

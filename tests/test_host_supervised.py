@@ -161,3 +161,20 @@ def test_temperatures_that_fp32_does_not_hold_are_refused(lib, recorded, value):
     with pytest.raises(ValueError, match="temperature"):
         training.vocabulary_loss(fp32(2, 4), fp32(3, 4), torch.zeros(2, dtype=torch.int64), temperature=value)
     assert not calls
+
+
+@pytest.mark.parametrize("with_grad", [True, False])
+@pytest.mark.parametrize("name", ["hidden", "weight", "bias"])
+def test_tensors_that_require_grad_are_refused_where_their_gradient_would_be_lost(recorded, name, with_grad):  # noqa: F811
+    """The loss has no graph: a backward() of a sum that it is part of would leave the head untrained without an error."""
+    _made, calls = recorded
+    args = {"hidden": fp32(2, 4), "weight": fp32(3, 4), "bias": fp32(3)}
+    args[name].requires_grad_(True)
+    kw = {"tokens": torch.zeros(2, dtype=torch.int64), "with_grad": with_grad}
+    with pytest.raises(HipError, match=f"{name}.detach()"):
+        training.vocabulary_loss(**args, **kw)
+    assert not calls
+    with torch.no_grad():
+        assert not training.vocabulary_loss(**args, **kw).loss.requires_grad
+    training.vocabulary_loss(**{**args, name: args[name].detach()}, **kw)
+    assert len(calls) == 2
