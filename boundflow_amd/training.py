@@ -477,8 +477,9 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
             raise ValueError(f"mask of shape {tuple(mask.shape)}, expected {tuple(lead)}")
         if not mask.is_contiguous():
             mask = mask.contiguous()
-    if room < 0:
-        raise ValueError(f"room must be >=0, got {room}")
+    room = operator.index(room)
+    if not 0 <= room < 1 << 63:
+        raise ValueError(f"room must be >=0 and below 2^63, got {room}")
     wide = weight.dtype if weight_grad_dtype is None else weight_grad_dtype
     if wide not in (weight.dtype, torch.float32):
         raise ValueError(f"weight_grad_dtype must be {weight.dtype} or float32, got {wide}")

@@ -178,3 +178,17 @@ def test_tensors_that_require_grad_are_refused_where_their_gradient_would_be_los
         assert not training.vocabulary_loss(**args, **kw).loss.requires_grad
     training.vocabulary_loss(**{**args, name: args[name].detach()}, **kw)
     assert len(calls) == 2
+
+
+def test_room_reaches_the_library_whole(recorded):  # noqa: F811
+    """A number past 63 bits would arrive cut to 64: 2^64 + 256 as 256, 2^63 as a negative one."""
+    _made, calls = recorded
+    args = (fp32(2, 4), fp32(3, 4), torch.zeros(2, dtype=torch.int64))
+    for room in ((1 << 64) + 256, 1 << 63, -1):
+        with pytest.raises(ValueError, match="room must be"):
+            training.vocabulary_loss(*args, room=room)
+    with pytest.raises(TypeError):
+        training.vocabulary_loss(*args, room=2e9)
+    assert not calls
+    training.vocabulary_loss(*args, room=(1 << 63) - 1)
+    assert calls[0][1][-2] == (1 << 63) - 1
