@@ -355,11 +355,13 @@ __global__ void __launch_bounds__(256) vocab_softmax_columns_kernel(VocabSoftmax
   store_pack(sums + group * p.ldg + v, out);
 }
 
-// The bias's gradient from those sums; what a sum rounds away is kept and added again.
+// The bias's gradient from those sums, of `group` rows each (a tile's, where the logits were formed again); what a sum rounds
+// away is kept and added again.
 template <class T>
 __global__ void __launch_bounds__(256) vocab_bias_kernel(const float* __restrict__ sums, int64_t ld, int columns,
-                                                         const int* __restrict__ live, float scale, T* __restrict__ grad) {
-  const int v = blockIdx.x * 256 + threadIdx.x, groups = (*live + VOCAB_GROUP - 1) / VOCAB_GROUP;
+                                                         const int* __restrict__ live, int group, float scale,
+                                                         T* __restrict__ grad) {
+  const int v = blockIdx.x * 256 + threadIdx.x, groups = (*live + group - 1) / group;
   if (v >= columns) return;
   float sum = 0.f, left = 0.f;
 #pragma unroll 8
@@ -588,6 +590,17 @@ inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
   }
 }
 
+// Rows of X in a tile of the logits.
+inline int vocab_tile_rows(int tile, int parts) {
+  switch (tile) {
+    case VT_LARGE: return parts > 1 ? VocabLarge<3>::BN : VocabLarge<1>::BN;
+    case VT_SLIM:
+    case VT_REGS:
+    case VT_THIN: return VocabSlim<1>::BN;
+    default: return VocabMid::BN;
+  }
+}
+
 // Rows up to which a weight that cannot be copied to LDS as it lies passes through registers, where a packed copy of it would be
 // most of the bytes.  fp32 (us, packed / through registers; rows of 2048 over 32000 tokens): 8 rows 399 / 265, 128 rows
 // 529 / 401, 192 rows 620 / 567, scored alone 212 / 91, 252 / 126, 271 / 195.  16-bit rows of an odd width, scored: 64 rows
@@ -748,6 +761,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
   E* x = (E*)(q.space + p.x);
   E* w = (E*)(q.space + p.w);
   E* g = (E*)(q.space + p.g);
+  float* cols = (float*)(q.space + p.cols);
   float* dx = (float*)(q.space + p.dx);
   float* dw = (float*)(q.space + p.dw);
   float* db = (float*)(q.space + p.db);
@@ -888,12 +902,11 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     hipLaunchKernelGGL((vocab_softmax_kernel<E, GP>), dim3((unsigned)N), dim3(256), 0, stream, stats);
     BF_LAUNCH_CHECK("bf_vocab_loss");
     const int chunks = (int)ceil_div(soft.held, 2048);
-    float* cols = (float*)(q.space + p.cols);
     hipLaunchKernelGGL((vocab_softmax_columns_kernel<E, GP>), dim3((unsigned)(ceil_div(N, VOCAB_GROUP) * chunks)), dim3(256), 0,
                        stream, soft, chunks, cols);
     BF_LAUNCH_CHECK("bf_vocab_loss");
     hipLaunchKernelGGL((vocab_bias_kernel<T>), dim3((unsigned)ceil_div(count_of(0), 256)), dim3(256), 0, stream, cols, p.piece,
-                       count_of(0), live, scale, (T*)q.grad_bias);
+                       count_of(0), live, VOCAB_GROUP, scale, (T*)q.grad_bias);
   } else {
     hipLaunchKernelGGL((vocab_softmax_kernel<E, GP>), dim3((unsigned)((int64_t)N * soft.chunks)), dim3(256), 0, stream, soft);
   }
@@ -910,8 +923,14 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     weight_rows(v0, count, k > 0);
     if (k > 0) {
       a.G = g;
+      a.cols = p.columns ? cols : nullptr;
       vocab_logits<E, GP>(p.logits_tile, a, VM_GRAD, stream);
       BF_LAUNCH_CHECK("bf_vocab_loss");
+      if (p.columns) {
+        hipLaunchKernelGGL((vocab_bias_kernel<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, cols, p.piece,
+                           count, live, vocab_tile_rows(p.logits_tile, p.parts), scale, (T*)q.grad_bias + v0);
+        BF_LAUNCH_CHECK("bf_vocab_loss");
+      }
     }
     // dx: the weight's rows are k
     VocabArgs b = a;
@@ -944,7 +963,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     d.b_cols = (int)p.piece;
     d.out = (char*)q.grad_weight + v0 * D * elem_bytes(q.grad_weight_elem);
     d.out_elem = q.grad_weight_elem;
-    d.db = q.grad_bias && !(p.columns && k == 0) ? (T*)q.grad_bias + v0 : nullptr;
+    d.db = q.grad_bias && !p.columns ? (T*)q.grad_bias + v0 : nullptr;
     vocab_grads<E, GP>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }

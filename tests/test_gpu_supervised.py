@@ -652,3 +652,28 @@ def test_far_temperatures(dtype, N, V):
     top = z.argmax(1)
     got = training.vocabulary_loss(hidden, weight, top, bias=bias, temperature=2.0 ** -120)
     assert not bool(got.logp.any()), "the largest logit has all the probability"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V", [(128, 9000), (200, 9000), (600, 10_001), (600, 20_001)])
+def test_bias_gradient_of_every_piece_is_summed_before_rounding(dtype, N, V):
+    """Rows that answer tokens as often as their probabilities say: a token's column of G cancels to what the bias's rounding
+    leaves, and G's own rounding, the same in all rows, would be as large as that.  So it has no place in the tolerance: the
+    exponentials of the first piece are rounded to 11 bits in 16-bit types, what follows is formed in fp32."""
+    dev = device()
+    D = 72
+    ids = torch.tensor([3, 70, 255, 256, 700, 2049, 4100, 4101, 5000, 8000, V - 257, V - 1])
+    share = torch.rand(len(ids), generator=gen(3)) + 0.2
+    tokens = ids[torch.multinomial(share, N, replacement=True, generator=gen(4))]
+    often = torch.bincount(tokens, minlength=V).double() / N
+    bias = often.log().to(dtype)
+    weight = torch.randn(V, D, generator=gen(5)).to(dtype)
+    hidden = torch.zeros(N, D, dtype=dtype)
+    r = ref.vocabulary_loss(hidden, weight, tokens, bias=bias)
+    got = training.vocabulary_loss(hidden.to(dev), weight.to(dev), tokens.to(dev), bias=bias.to(dev), room=0)
+    tol_lp = 2.0 ** -23 * float(r["size"].max()) + logp_tol(r["z"], V)
+    tol_g = r["p"] * (tol_lp + 2.0 ** -21)[:, None] + r["g"].abs() * 2.0 ** -23
+    if dtype != torch.float32:
+        tol_g[:, :256] += r["p"][:, :256] * 2.0 ** -11       # the first piece: what is left of no room
+    tol = r["factor"] * (tol_g.sum(0) + (N + 8) * 2.0 ** -24 * r["g"].abs().sum(0))
+    close(got.grad_bias, r["bias"], tol + rounded(r["bias"], dtype), f"grad bias of pieces {N} x {V} {dtype}")
