@@ -125,6 +125,7 @@ SIGNATURES = {
     "bf_preference_loss": (I32, [P, I32, I64, I64, I64, P, I32, P, P, I64, F32, F32, F32, P, P, P, P, P, P]),
     "bf_adamw_multi": (I32, [I32, P, P, P, I32, I32, P, P, P, P, P, F64, F64, F64, F64, F64, I64, F32, P, P]),
     "bf_vocab_loss_workspace": (I64, [I64, I64, I64, I32, P, I64, I32, I32, I64]),
+    "bf_vocab_loss_plan": (I32, [I64, I64, I64, I32, P, I64, I32, I32, I64, P]),
     "bf_vocab_loss": (I32, [P, I32, I64, I64, I64, I64, I64, P, I64, I64, P, P, I32, P, F64, F32, P, P, P, P, I32, P, P,
                             I64, P]),
     "bf_dropout": (I32, [P, I64, P, I64, I32, I64, I64, F64, I64, I64, P, P, P]),

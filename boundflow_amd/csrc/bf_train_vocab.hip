@@ -1032,6 +1032,23 @@ extern "C" int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int 
   return vocab_launches_ok(p) ? p.bytes / 4 : 0;
 }
 
+extern "C" int bf_vocab_loss_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
+                                  int with_grad, int with_bias, int64_t room, int64_t* plan) {
+  BF_REQUIRE(elem_ok(elem) && N > 0 && D > 0 && V > 0 && ld_w >= D && room >= 0 && plan, "bf_vocab_loss_plan: bad arguments");
+  if (!vocab_sizes_ok(N, D, V, ld_w)) {
+    set_error("bf_vocab_loss_plan: more than bf_vocab_loss takes");
+    return BF_ERANGE;
+  }
+  const VocabPlan p = vocab_plan(N, D, V, elem, weight, ld_w, with_grad != 0, with_bias != 0, room);
+  plan[0] = ceil_div(V, p.piece);
+  plan[1] = p.logits_tile;
+  plan[2] = p.grad ? p.grads_tile : -1;
+  plan[3] = p.g_parts;
+  plan[4] = p.logits_summed ? p.logits_splits : 0;
+  plan[5] = p.columns;
+  return BF_OK;
+}
+
 extern "C" int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
                              const void* weight, int64_t V, int64_t ld_w, const void* bias, const void* tokens,
                              int token_bytes, const void* mask, double temperature, float grad_scale, float* logp,

@@ -678,6 +678,12 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
  * no room the logits are formed twice. */
 int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
                                 int with_grad, int with_bias, int64_t room);
+/* What a call of these sizes does, for tests and traces: plan[6] = pieces of the vocabulary, tile of the logits (0 large,
+ * 1 mid, 2 deep, 3 slim, 4 thin, 5 slim through registers), tile of the gradients (-1: none), parts that the softmax's
+ * gradient is held in, cuts of the logits along the width where a row's are joined by one workgroup (0: they are not), whether
+ * the bias's gradient is summed beside the softmax. */
+int bf_vocab_loss_plan(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w, int with_grad,
+                       int with_bias, int64_t room, int64_t* plan);
 int bf_vocab_loss(const void* hidden, int elem, int64_t B, int64_t T, int64_t D, int64_t ld_b, int64_t ld_t,
                   const void* weight, int64_t V, int64_t ld_w, const void* bias, const void* tokens, int token_bytes,
                   const void* mask, double temperature, float grad_scale, float* logp, float* loss, void* grad_hidden,
