@@ -18,6 +18,7 @@ import torch
 from boundflow_amd import training
 from boundflow_amd._lib import HipError
 from oracle import training_ref as ref
+from tests import vocab_cases
 from tests.gpu_util import announce, device
 from tests.test_gpu_training import TINY, TYPES, U, close, gen, logp_tol, rounded
 
@@ -677,3 +678,25 @@ def test_bias_gradient_of_every_piece_is_summed_before_rounding(dtype, N, V):
         tol_g[:, :256] += r["p"][:, :256] * 2.0 ** -11       # the first piece: what is left of no room
     tol = r["factor"] * (tol_g.sum(0) + (N + 8) * 2.0 ** -24 * r["g"].abs().sum(0))
     close(got.grad_bias, r["bias"], tol + rounded(r["bias"], dtype), f"grad bias of pieces {N} x {V} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_exponentials_kept_and_logits_formed_again(dtype):
+    """G in one part.  Where the exponentials are kept, in the first piece, they have 11 bits before G is rounded; in the others,
+    whose logits are formed again, G is rounded alone: the weight's gradient there is held to the lesser error."""
+    dev = device()
+    N, D, V = 100, 128, 9000
+    for room, border in ((2 << 30, V), (0, 256)):
+        pieces, _, _, parts, summed, _ = vocab_cases.plan(N, D, V, 0, True, room, dtype)
+        assert (pieces > 1, parts, summed) == (border < V, 1, 0)
+    hidden, weight, tokens, bias = head(N, D, V, dtype, 23)
+    r = ref.vocabulary_loss(hidden, weight, tokens, bias=bias)
+    whole = check(hidden, weight, tokens, bias=bias)
+    cut = check(hidden, weight, tokens, bias=bias, room=0)
+    assert torch.equal(whole.logp, cut.logp) and torch.equal(whole.loss, cut.loss)
+    assert torch.equal(whole.grad_weight[:256], cut.grad_weight[:256]) and torch.equal(whole.grad_bias[:256], cut.grad_bias[:256])
+    _, tol_g = tolerances(r, dtype, 1.0, V, D)
+    tol_g = tol_g - r["p"] * 2.0 ** -11
+    g, x = r["g"].abs(), r["x"].abs()
+    tol = r["factor"] * (torch.mm(tol_g.t(), x) + (N + 8) * 2.0 ** -24 * torch.mm(g.t(), x)) + rounded(r["weight"], dtype)
+    close(cut.grad_weight[256:], r["weight"][256:], tol[256:], f"grad weight past the first piece {dtype}")
