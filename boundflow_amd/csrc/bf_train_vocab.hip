@@ -745,6 +745,12 @@ struct VocabCall {
   hipStream_t stream;
 };
 
+// A rule of the plan that asks for what is not compiled is an error, not a result that is missing.
+inline int vocab_no_kernel(const VocabPlan& p) {
+  set_error("bf_vocab_loss: no kernel for tiles %d and %d with %d parts", p.logits_tile, p.grads_tile, p.g_parts);
+  return BF_ELAUNCH;
+}
+
 // T: the tensors' type, E: the matrix products', GP: the parts of G
 template <class T, class E, int GP>
 int vocab_run(const VocabPlan& p, const VocabCall& q) {
@@ -861,8 +867,9 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
       a.sums_split = N * a.sums_ld;
       a.sums = (float*)(q.space + p.sums) + k * first_piece;
     }
-    if (p.logits_summed) vocab_logits<E, PARTS ? GP : 1>(p.logits_tile, a, VM_SUMS, stream);
-    else vocab_logits<E, GP>(p.logits_tile, a, VM_STATS, stream);
+    const bool launched = p.logits_summed ? vocab_logits<E, PARTS ? GP : 1>(p.logits_tile, a, VM_SUMS, stream)
+                                          : vocab_logits<E, GP>(p.logits_tile, a, VM_STATS, stream);
+    if (!launched) return vocab_no_kernel(p);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
 
@@ -902,8 +909,10 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     hipLaunchKernelGGL((vocab_softmax_kernel<E, GP>), dim3((unsigned)N), dim3(256), 0, stream, stats);
     BF_LAUNCH_CHECK("bf_vocab_loss");
     const int chunks = (int)ceil_div(soft.held, 2048);
-    hipLaunchKernelGGL((vocab_softmax_columns_kernel<E, GP>), dim3((unsigned)(ceil_div(N, VOCAB_GROUP) * chunks)), dim3(256), 0,
-                       stream, soft, chunks, cols);
+    if constexpr (GP == 2) return vocab_no_kernel(p);      // two parts are summed beside dw's products
+    else
+      hipLaunchKernelGGL((vocab_softmax_columns_kernel<E, GP>), dim3((unsigned)(ceil_div(N, VOCAB_GROUP) * chunks)), dim3(256), 0,
+                         stream, soft, chunks, cols);
     BF_LAUNCH_CHECK("bf_vocab_loss");
     hipLaunchKernelGGL((vocab_bias_kernel<T>), dim3((unsigned)ceil_div(count_of(0), 256)), dim3(256), 0, stream, cols, p.piece,
                        count_of(0), live, VOCAB_GROUP, scale, (T*)q.grad_bias);
@@ -924,7 +933,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     if (k > 0) {
       a.G = g;
       a.cols = p.columns ? cols : nullptr;
-      vocab_logits<E, GP>(p.logits_tile, a, VM_GRAD, stream);
+      if (!vocab_logits<E, GP>(p.logits_tile, a, VM_GRAD, stream)) return vocab_no_kernel(p);
       BF_LAUNCH_CHECK("bf_vocab_loss");
       if (p.columns) {
         hipLaunchKernelGGL((vocab_bias_kernel<T>), dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, stream, cols, p.piece,
@@ -964,7 +973,7 @@ int vocab_run(const VocabPlan& p, const VocabCall& q) {
     d.out = (char*)q.grad_weight + v0 * D * elem_bytes(q.grad_weight_elem);
     d.out_elem = q.grad_weight_elem;
     d.db = q.grad_bias && !p.columns ? (T*)q.grad_bias + v0 : nullptr;
-    vocab_grads<E, GP>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream);
+    if (!vocab_grads<E, GP>(p.grads_tile, b, d, q.logp, N, k == 0 ? q.loss : nullptr, stream)) return vocab_no_kernel(p);
     BF_LAUNCH_CHECK("bf_vocab_loss");
   }
   if (p.dx_joined || p.dw_joined) {

@@ -3,9 +3,9 @@
 
 namespace bf {
 
-template void vocab_logits<_Float16, 1>(int, const VocabArgs&, int, hipStream_t);
-template void vocab_grads<_Float16, 1>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
-template void vocab_logits<_Float16, 2>(int, const VocabArgs&, int, hipStream_t);
-template void vocab_grads<_Float16, 2>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
+template bool vocab_logits<_Float16, 1>(int, const VocabArgs&, int, hipStream_t);
+template bool vocab_grads<_Float16, 1>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
+template bool vocab_logits<_Float16, 2>(int, const VocabArgs&, int, hipStream_t);
+template bool vocab_grads<_Float16, 2>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
 
 }  // namespace bf

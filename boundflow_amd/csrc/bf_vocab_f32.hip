@@ -3,7 +3,7 @@
 
 namespace bf {
 
-template void vocab_logits<__bf16, 3>(int, const VocabArgs&, int, hipStream_t);
-template void vocab_grads<__bf16, 3>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
+template bool vocab_logits<__bf16, 3>(int, const VocabArgs&, int, hipStream_t);
+template bool vocab_grads<__bf16, 3>(int, const VocabArgs&, const VocabArgs&, const float*, int, float*, hipStream_t);
 
 }  // namespace bf

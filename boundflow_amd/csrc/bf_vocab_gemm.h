@@ -837,29 +837,37 @@ __global__ void __launch_bounds__(T::NT, (T::OCC * T::WAVES + 3) / 4)
 inline int64_t vocab_blocks(int64_t tiles) { return 8 * ceil_div(tiles, 8); }
 
 template <class T, class E, int GP, class S = void>
-inline void launch_vocab_logits(const VocabArgs& p, int mode, hipStream_t stream) {
+inline bool launch_vocab_logits(const VocabArgs& p, int mode, hipStream_t stream) {
   const dim3 grid((unsigned)vocab_blocks(ceil_div(p.M, T::BM) * ceil_div(p.N, T::BN) * p.splits));
   // what no call asks for is not compiled: only small grids are cut, whatever G has; few rows have G in parts, many in one
   constexpr bool FEW = T::BN == 64;
   if (mode == VM_SUMS) {
-    if constexpr (GP != 2 && ((T::OCC == 1 && T::WAVES == 4) || !__is_same(S, void)))
+    if constexpr (GP != 2 && ((T::OCC == 1 && T::WAVES == 4) || !__is_same(S, void))) {
       hipLaunchKernelGGL((vocab_logits_kernel<T, VM_SUMS, E, GP, S>), grid, dim3(T::NT), 0, stream, p);
+      return true;
+    }
   } else if (mode == VM_STATS) {
-    if constexpr (GP != 2 || FEW)
+    if constexpr (GP != 2 || FEW) {
       hipLaunchKernelGGL((vocab_logits_kernel<T, VM_STATS, E, GP, S>), grid, dim3(T::NT), 0, stream, p);
+      return true;
+    }
   } else {
-    if constexpr (GP != 1 || !FEW)
+    if constexpr (GP != 1 || !FEW) {
       hipLaunchKernelGGL((vocab_logits_kernel<T, VM_GRAD, E, GP, S>), grid, dim3(T::NT), 0, stream, p);
+      return true;
+    }
   }
+  return false;
 }
 
 template <class T, class W, class E, int GP, class S = void>
-inline void launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
+inline bool launch_vocab_grads(const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                                hipStream_t stream) {
   const int64_t first = vocab_blocks(ceil_div(dx.M, T::BM) * ceil_div(dx.N, T::BN) * dx.splits);
   const int64_t all = first + vocab_blocks(ceil_div(dw.M, W::BM) * ceil_div(dw.N, W::BN) * dw.splits) + (loss ? 1 : 0);
   hipLaunchKernelGGL((vocab_grads_kernel<T, W, E, GP, S>), dim3((unsigned)all), dim3(T::NT), 0, stream, dx, dw, (uint32_t)first,
                      logp, rows, loss);
+  return true;
 }
 
 // Tiles by the size of the problem; G: the parts of G (3: of everything, fp32), for the gradients PB of them.
@@ -873,8 +881,8 @@ template <int G>
 using VocabLarge = VocabTile<G == 3 ? 2 : 4, 2, G == 3 ? 4 : 2, G == 3 ? 2 : 4, 2, 1, vocab_pa(G), G>;
 template <int G>
 using VocabDeep = VocabTile<2, 2, 2, 2, G == 1 ? 4 : 3, 1, vocab_pa(G), G>;
-template <int G>
-using VocabThin = VocabTile<1, 2, 4, 1, G == 1 ? 6 : 4, 1, vocab_pa(G), G>;
+typedef VocabTile<1, 2, 4, 1, 6, 1, 1, 1> VocabThin;
+typedef VocabTile<1, 2, 4, 1, 4, 1, 1, 2> VocabThinG;    // of G in two parts
 template <int G>
 using VocabSlim = VocabTile<1, 2, 4, 1, G == 1 ? 3 : 2, 2, vocab_pa(G), G>;
 typedef VocabTile<2, 2, 2, 2, 2, 2, 1, 1> VocabMid;      // in parts it would be Deep
@@ -884,11 +892,11 @@ using VocabWide = VocabTile<1, 4, 4, 1, 1, 2, vocab_pa(G), G>;
 
 enum : int { VT_LARGE = 0, VT_MID = 1, VT_DEEP = 2, VT_SLIM = 3, VT_THIN = 4, VT_REGS = 5 };   // REGS: Slim through registers
 
-// Defined for each type by a file of its own (bf_vocab_*.hip).
+// Defined for each type by a file of its own (bf_vocab_*.hip).  False: there is no such kernel, and nothing was launched.
 template <class E, int GP>
-void vocab_logits(int tile, const VocabArgs& p, int mode, hipStream_t stream);
+bool vocab_logits(int tile, const VocabArgs& p, int mode, hipStream_t stream);
 template <class E, int GP>
-void vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
+bool vocab_grads(int tile, const VocabArgs& dx, const VocabArgs& dw, const float* logp, int rows, float* loss,
                  hipStream_t stream);
 
 }  // namespace bf
