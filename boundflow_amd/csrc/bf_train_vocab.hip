@@ -590,6 +590,12 @@ inline int64_t vocab_tile_count(int tile, int64_t m, int64_t n, int parts) {
   }
 }
 
+// The same of dW, whose tiles beside Slim's dX are Wide.
+inline int64_t vocab_dw_tile_count(int tile, int64_t m, int64_t n, int parts) {
+  if (tile == VT_SLIM || tile == VT_REGS) return ceil_div(m, VocabWide<1>::BM) * ceil_div(n, VocabWide<1>::BN);
+  return vocab_tile_count(tile, m, n, parts);
+}
+
 // Rows of X in a tile of the logits.
 inline int vocab_tile_rows(int tile, int parts) {
   switch (tile) {
@@ -675,6 +681,7 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
     // Sums are cut along k so that none of them takes longer than a good part of the whole launch, nor than it takes to
     // add one more piece's sums (some eight stages).
     const int64_t slots = p.grads_tile == VT_LARGE || p.grads_tile == VT_DEEP || p.grads_tile == VT_THIN ? 256 : 512;
+    // (dw's in Slim's tiles: of work, not of workgroups)
     const int64_t dx = vocab_tile_count(p.grads_tile, D, N, p.parts), dw = vocab_tile_count(p.grads_tile, D, in_piece, p.parts);
     const int64_t dx_steps = ceil_div(in_piece, 64), dw_steps = ceil_div(N, 64);
     const int64_t most = (dx * dx_steps + dw * (dw_steps + 4)) / slots / 3;
@@ -686,13 +693,14 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
       return (int)(splits < 1 ? 1 : ceil_div(steps, ceil_div(steps, splits)));      // none without a step
     };
     p.dx_splits = cut(dx_steps, least, p.rows, 32);
+    const int64_t dw_tiles = vocab_dw_tile_count(p.grads_tile, D, in_piece, p.parts);
     // dw's pieces are rows of the vocabulary each: only where it leaves CUs without a tile.  Where a piece's sums are few
     // (512 KB), shorter ones fill the CUs that dx leaves (us; rows of 512 over 100 tokens, bf16: 512 rows 29.7 / 25.2, 2000 rows
     // 37.6 / 34.1; over 500 tokens 300 rows 27 / 30, with the join that it then takes)
-    const int64_t most_dw = slots / dw < 32 ? slots / dw : 32;
+    const int64_t most_dw = slots / dw_tiles < 32 ? slots / dw_tiles : 32;
     p.dw_splits = p.piece < V ? 1 : cut(dw_steps, least, V, most_dw);
     if (p.piece >= V && 4 * V * p.Dp <= (512 << 10)) {
-      const int64_t left = (slots - dx * p.dx_splits) / dw;
+      const int64_t left = (slots - dx * p.dx_splits) / dw_tiles;
       const int shorter = cut(dw_steps, p.parts > 1 ? 2 : 3, V, left < most_dw ? left : most_dw);
       if (shorter > p.dw_splits) p.dw_splits = shorter;
     }
@@ -1023,7 +1031,7 @@ inline bool vocab_launches_ok(const VocabPlan& p) {
     return false;
   if (!p.grad) return true;
   const int64_t tiles = vocab_tile_count(p.grads_tile, p.D, p.N, p.parts) * p.dx_splits +
-                        vocab_tile_count(p.grads_tile, p.D, p.piece, p.parts) * p.dw_splits;
+                        vocab_dw_tile_count(p.grads_tile, p.D, p.piece, p.parts) * p.dw_splits;
   const int64_t joined = (p.dx_joined ? p.N : 0) + (p.dw_joined ? p.V : 0);
   return products(p.grads_tile, tiles) && launch_fits(p.N * ceil_div(p.piece, VOCAB_CHUNK), 256) &&
          launch_fits(ceil_div(p.N, VOCAB_GROUP) * ceil_div(p.piece, 2048), 256) &&

@@ -192,3 +192,11 @@ def test_room_reaches_the_library_whole(recorded):  # noqa: F811
     assert not calls
     training.vocabulary_loss(*args, room=(1 << 63) - 1)
     assert calls[0][1][-2] == (1 << 63) - 1
+
+
+def test_what_fits_a_launch_is_counted_in_the_tiles_that_are_made(lib):
+    """Beside few rows the weight's gradient runs in tiles of 128 x 128: of 2^20 columns and 140000 tokens 2^13 x 1094 of 256
+    threads, of which 2^24 are a launch of 2^32.  Counted in tiles of half the size they would be refused."""
+    size = lib.bf_vocab_loss_workspace
+    assert size(8, 1 << 20, 140_000, 1, 1 << 20, 1 << 20, 1, 0, 1 << 40) > 0
+    assert size(8, 1 << 20, 270_000, 1, 1 << 20, 1 << 20, 1, 0, 1 << 40) == 0
