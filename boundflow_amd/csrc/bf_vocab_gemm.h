@@ -18,7 +18,7 @@
 //
 // fp32 values come as three bf16 parts, x = x0 + x1 + x2 (8 + 8 + 8 significant bits); a product is the sum of six
 // part products, least first: x0 y2, x1 y1, x2 y0, x0 y1, x1 y0, x0 y0, into the same fp32 sums.  What is left out is
-// 2^-24 of a product.  A stage holds the three parts of both operands, each read from LDS once for two products (the six
+// 2^-24 of a product, for values from 2^-103 up: of smaller ones what lies below 2^-126 counts as 0.  A stage holds the three parts of both operands, each read from LDS once for two products (the six
 // one after another along k, a part of each operand in a stage: 2048 x 1024 rows over 32000 tokens 2041 us in the place
 // of 1667, a head of eight actions 45 us in the place of 40).
 #pragma once
@@ -206,12 +206,16 @@ __device__ __forceinline__ void store_elem(void* p, int elem, int64_t i, float x
   }
 }
 
-// x in its three bf16 parts, each the nearest to what those before it leave (infinite and NaN: the first alone)
+// x in its three bf16 parts, each the nearest to what those before it leave.  The first is at most the largest bf16, past which
+// it would round to infinity; the second has what that leaves, and is NaN or infinite where x is.  Parts below 2^-126 are zeros to
+// the matrix cores, so x keeps all its bits from 2^-103 up.
 __device__ __forceinline__ void split_parts(float x, __bf16 part[VOCAB_PARTS]) {
+  constexpr float MOST = 0x1.fep127f;
+  part[0] = (__bf16)__builtin_amdgcn_fmed3f(x, -MOST, MOST);
 #pragma unroll
-  for (int k = 0; k < VOCAB_PARTS; ++k) {
+  for (int k = 1; k < VOCAB_PARTS; ++k) {
+    x -= (float)part[k - 1];
     part[k] = (__bf16)x;
-    x = __builtin_isfinite(x) ? x - (float)part[k] : 0.f;
   }
 }
 

@@ -700,3 +700,36 @@ def test_exponentials_kept_and_logits_formed_again(dtype):
     g, x = r["g"].abs(), r["x"].abs()
     tol = r["factor"] * (torch.mm(tol_g.t(), x) + (N + 8) * 2.0 ** -24 * torch.mm(g.t(), x)) + rounded(r["weight"], dtype)
     close(cut.grad_weight[256:], r["weight"][256:], tol[256:], f"grad weight past the first piece {dtype}")
+
+
+@pytest.mark.parametrize("N,V", [(5, 300), (5, 40_001), (200, 300), (200, 9000)])
+def test_the_largest_fp32_values(N, V):
+    """Finite values past the largest bf16, 3.39e38, whose first of three bf16 parts would round to infinity: in a hidden row
+    and in a weight's, against 2^-100, at a temperature that brings their logits down to a few."""
+    hidden, weight, tokens, bias = head(N, 72, V, torch.float32, 15)
+    most = torch.finfo(torch.float32).max
+    weight[:, 3] = torch.randn(V, generator=gen(1)) * 2.0 ** -100
+    hidden[:, 5] = torch.randn(N, generator=gen(2)) * 2.0 ** -100
+    hidden[1, 3], hidden[2, 3] = most, -3.395e38
+    weight[7, 5], weight[V - 1, 5] = -most, 3.4e38
+    dev, T, dtype = device(), 2.0 ** 26, torch.float32
+    r = ref.vocabulary_loss(hidden, weight, tokens, bias=bias, temperature=T)
+    got = training.vocabulary_loss(*(t.to(dev) for t in (hidden, weight, tokens)), bias=bias.to(dev), temperature=T)
+    tol_lp, tol_g = tolerances(r, dtype, T, V, 72)
+    close(got.logp, r["logp"], tol_lp + 2.0 ** -23 * r["logp"].abs(), f"logp of the largest values {N} x {V}")
+    g = r["g"].abs()
+
+    def held(have, want, a, b, terms, name):
+        """A gradient's sum is multiplied by 1 / (T N) at its end.  No partial sum is past the sum of the magnitudes and the
+        roundings, terms 2^-24 of it, so below 2^128 (1 - 2^-9) of that nothing is infinite; of the few entries beyond, two
+        rows or tokens of 2^128 in one sum, nothing is said."""
+        size = torch.mm(a.abs(), b.abs())
+        tol = r["factor"] * (torch.mm(tol_g if a is g else tol_g.t(), b.abs()) + terms * 2.0 ** -24 * size)
+        beyond = size * (1 + terms * 2.0 ** -24) > most * (1 - 2.0 ** -9)
+        assert int(beyond.sum()) <= max(N, V) // 4, "the test has nothing to look at"
+        close(torch.where(beyond.to(dev), 0.0, have), torch.where(beyond, 0.0, want), tol + rounded(want, dtype), name)
+
+    held(got.grad_hidden, r["hidden"], g, r["w"], 6 * V + 8, f"grad hidden of the largest values {N} x {V}")
+    held(got.grad_weight, r["weight"], g.t(), r["x"], 6 * N + 8, f"grad weight of the largest values {N} x {V}")
+    close(got.grad_bias, r["bias"], r["factor"] * (tol_g.sum(0) + (6 * N + 8) * 2.0 ** -24 * g.sum(0)) + rounded(r["bias"], dtype),
+          f"grad bias of the largest values {N} x {V}")
