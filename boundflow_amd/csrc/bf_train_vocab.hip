@@ -5,7 +5,7 @@
 //   G_nv   = exp(z_nv / t) / sum - [v = y_n],      s = grad_scale / (t rows)
 //   dx_n   = s sum_v G_nv w_v,   dw_v = s sum_n G_nv x_n,   db_v = s sum_n G_nv
 //
-// The logits are never stored.  A first pass over the vocabulary (vocab_logits_kernel) leaves each row's largest logit and
+// The logits are not kept.  A first pass over the vocabulary (vocab_logits_kernel) leaves each row's largest logit and
 // sum of exponentials per tile, and of as much of the vocabulary as the workspace has room for the exponentials in the type
 // of the matrix products (fp32: in three parts).  vocab_softmax_kernel joins the tiles' statistics and makes those exponentials
 // G; dx and dw follow from it (vocab_grads_kernel).  For what has no room, the logits are formed again, a
@@ -608,9 +608,9 @@ inline int vocab_tile_rows(int tile, int parts) {
 }
 
 // Rows up to which a weight that cannot be copied to LDS as it lies passes through registers, where a packed copy of it would be
-// most of the bytes.  fp32 (us, packed / through registers; rows of 2048 over 32000 tokens): 8 rows 399 / 265, 128 rows
-// 529 / 401, 192 rows 620 / 567, scored alone 212 / 91, 252 / 126, 271 / 195.  16-bit rows of an odd width, scored: 64 rows
-// of 2049 over 50001 tokens 119 / 77, 128 rows 131 / 137; with gradients, whose product along the vocabulary is read two
+// most of the bytes.  fp32 (us, packed / through registers; rows of 2048 over 32000 tokens): 8 rows 399 / 262, 128 rows
+// 542 / 413, 192 rows 650 / 567, scored alone 212 / 85, 261 / 148, 285 / 191.  16-bit rows of an odd width, scored: 64 rows
+// of 2049 over 50001 tokens 119 / 80, 128 rows 133 / 137; with gradients, whose product along the vocabulary is read two
 // bytes aside, 227 / 277.
 constexpr int64_t VOCAB_REGS_FP32 = 192, VOCAB_REGS_SCORED = 64;
 
@@ -648,8 +648,11 @@ inline VocabPlan vocab_plan(int64_t N, int64_t D, int64_t V, int elem, const voi
     if (splits > 1) p.logits_splits = (int)splits;
     p.logits_summed = splits > 1 || V <= VOCAB_HELD_WAVE;
   }
-  // Rounded to one 16-bit part, G's error is as large as that of the rounded gradients, and few rows do not average it out
-  // (2-norm of all errors against 64 bits over that of one rounding: one to eight rows 1.3 to 1.7, thousands 1.1 to 1.2).
+  // Rounded to one 16-bit part, G adds to the gradients' own rounding (2-norm of all errors against 64 bits over that of one
+  // rounding; rows of 512 over 9000 tokens): one to eight rows 1.3 to 1.7, 65 to 8000 rows 1.12 to 1.23, bf16 and fp16, since each
+  // of its errors is relative to an entry.  Two parts leave 1.00.  They are taken where they cost next to nothing, and with a
+  // bias, whose columns cancel, wherever rows are joined; without one the joined ones' would take 0 to 40 % longer (us, one part /
+  // two: 512 rows of 160 over 8 tokens 28 / 28, 1000 of 1024 over 1000 45 / 48, 400 of 4096 over 2000 61 / 85).
   p.g_parts = p.parts > 1 ? p.parts : grad && (N <= VocabSlim<1>::BN || (p.logits_summed && bias)) ? 2 : 1;
   p.columns = grad && bias && !p.logits_summed && p.g_parts != 2;
   const int64_t per_token = 2 * ((grad ? p.g_parts * p.rows : 0) + (p.direct || p.regs ? 0 : p.parts * p.Dp));

@@ -1,6 +1,6 @@
 // The three products of a head's softmax cross entropy (bf_train_vocab.hip) on the 16-bit matrix cores:
 //
-//   z[v, n]  = W[v, :] . X[n, :]      logits, never stored: their softmax statistics, or its gradient G
+//   z[v, n]  = W[v, :] . X[n, :]      logits, not kept: their softmax statistics and exponentials, or the softmax's gradient G
 //   dX[n, d] = sum over v of G[n, v] W[v, d]
 //   dW[v, d] = sum over n of G[n, v] X[n, d]
 //
@@ -13,8 +13,8 @@
 // otherwise (W in dX, both in dW) a stage is held as rows of k and read by ds_read_b64_tr_b16, which hands a lane four
 // k of its column, so that no operand is transposed in memory.
 //
-// Up to 64 rows, and where a bias's gradient is asked for of few tiles, G comes as two 16-bit parts: a rounding of it to one
-// would not average out over the rows, and the products are not the time.
+// Up to 64 rows, and where a bias's gradient is asked for of few tiles, G comes as two 16-bit parts: the products are not the
+// time there, and a rounding of it to one adds to the results' own (vocab_plan has the figures).
 //
 // fp32 values come as three bf16 parts, x = x0 + x1 + x2 (8 + 8 + 8 significant bits); a product is the sum of six
 // part products, least first: x0 y2, x1 y1, x2 y0, x0 y1, x1 y0, x0 y0, into the same fp32 sums.  What is left out is

@@ -431,7 +431,7 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     gradient is summed before that rounding (of two parts: of both).  Rows that count and weights are finite (a bias may be -inf, and bars its token);
     what is not shows as NaN.  Gradients' sums are scaled at their end: one that passes fp32's range before is infinite.  ``room`` bytes of that gradient (and of a copy of a weight whose rows cannot be read as they
     lie) are held at a time, for as many tokens of the vocabulary as fit; the logits of the others are formed twice, which
-    takes up to a third longer."""
+    takes up to a third longer.  The rows, their statistics and the gradients' sums take memory beside it."""
     if torch.is_grad_enabled():
         for t, name in ((hidden, "hidden"), (weight, "weight"), (bias, "bias")):
             if isinstance(t, torch.Tensor) and t.requires_grad:

@@ -675,7 +675,7 @@ int bf_adamw_multi(int count, void* const* p, const void* const* g, const int64_
  * grad_weight dense [V, D] of that type or fp32: grad_scale * the loss's gradient; all that there are, or none of them (NULL).
  * Workspace in floats, 16-byte aligned; its size depends on whether the weight can be read as it lies.  `room` (the same in
  * both calls): bytes that the softmax's gradient, in the products' type, and a copy of such a weight may take; of what has
- * no room the logits are formed twice. */
+ * no room the logits are formed twice.  Rows, statistics and sums of the gradients lie in the workspace beside it. */
 int64_t bf_vocab_loss_workspace(int64_t N, int64_t D, int64_t V, int elem, const void* weight, int64_t ld_w,
                                 int with_grad, int with_bias, int64_t room);
 /* What a call of these sizes does, for tests and traces: plan[6] = pieces of the vocabulary, tile of the logits (0 large,
