@@ -312,8 +312,9 @@ __global__ void __launch_bounds__(256) vocab_softmax_kernel(VocabSoftmax p) {
 }
 
 // G in place where the bias's gradient is asked for too, from statistics that vocab_softmax_kernel has left: a workgroup takes
-// 2048 columns of 32 rows and leaves their sums, of what G is before it is rounded (a token's column cancels: the sums of
-// a rounded G were up to 1.9 times as far from 64 bits as those of fp32).  841 rows of 50001 tokens 33 us (168 MB at 5.1 TB/s).
+// 2048 columns of 32 rows and leaves their sums, of what G is before it is rounded (of exponentials of 11 bits where G has
+// one part, the tokens' own entries from fp32; a token's column cancels: the sums of a rounded G were up to 1.9 times as far
+// from 64 bits as those of fp32).  841 rows of 50001 tokens 33 us (168 MB at 5.1 TB/s).
 constexpr int VOCAB_GROUP = 32;
 
 template <class E, int GP>

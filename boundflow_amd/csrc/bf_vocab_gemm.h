@@ -18,9 +18,10 @@
 //
 // fp32 values come as three bf16 parts, x = x0 + x1 + x2 (8 + 8 + 8 significant bits); a product is the sum of six
 // part products, least first: x0 y2, x1 y1, x2 y0, x0 y1, x1 y0, x0 y0, into the same fp32 sums.  What is left out is
-// 2^-24 of a product, for values from 2^-103 up: of smaller ones what lies below 2^-126 counts as 0.  A stage holds the three parts of both operands, each read from LDS once for two products (the six
-// one after another along k, a part of each operand in a stage: 2048 x 1024 rows over 32000 tokens 2041 us in the place
-// of 1667, a head of eight actions 45 us in the place of 40).
+// 2^-24 of a product, for values from 2^-103 up: of smaller ones what lies below 2^-126 counts as 0.  A stage holds the
+// three parts of both operands, each read from LDS once for two products (the six one after another along k, a part of
+// each operand in a stage: 2048 x 1024 rows over 32000 tokens 2041 us in the place of 1667, a head of eight actions 45 us
+// in the place of 40).
 #pragma once
 
 #include "bf_train.h"
