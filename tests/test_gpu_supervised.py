@@ -733,3 +733,30 @@ def test_the_largest_fp32_values(N, V):
     held(got.grad_weight, r["weight"], g.t(), r["x"], 6 * N + 8, f"grad weight of the largest values {N} x {V}")
     close(got.grad_bias, r["bias"], r["factor"] * (tol_g.sum(0) + (6 * N + 8) * 2.0 ** -24 * g.sum(0)) + rounded(r["bias"], dtype),
           f"grad bias of the largest values {N} x {V}")
+
+
+@pytest.mark.parametrize("N,dtype", [(300, torch.bfloat16), (600, torch.float32)])
+def test_a_captured_call_past_the_room(N, dtype):
+    """Pieces of the vocabulary with the bias's columns summed in each: replays between eager calls, other inputs each time."""
+    dev = device()
+    V = 9000
+    inputs = [t.to(dev) for t in head(N, 72, V, dtype, 21)]
+    call = lambda: training.vocabulary_loss(*inputs[:3], bias=inputs[3], room=1 << 20)  # noqa: E731
+    pieces, _, _, _, _, columns = vocab_cases.plan(N, 72, V, 0, True, 1 << 20, dtype)
+    assert pieces > 1 and columns
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = call()
+    for turn in range(3):
+        for t, other in zip(inputs, head(N, 72, V, dtype, turn)):
+            t.copy_(other)
+        inputs[2][turn::5] = -1
+        want = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, want):
+            assert torch.equal(a, b), turn
+        again = call()
+        for a, b in zip(again, want):
+            assert torch.equal(a, b), turn

@@ -12,11 +12,8 @@ from tests.test_gpu_training import gen
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("dtype", list(vc.ELEM))
-@pytest.mark.parametrize("case,narrow,wide", vc.CASES)
-def test_vocabulary_loss_through_every_tile(case, narrow, wide, dtype):
-    if (wide if dtype == torch.float32 else narrow) is None:
-        pytest.skip("for 16-bit types")
+@pytest.mark.parametrize("case,dtype,_ways", vc.RUNS)
+def test_vocabulary_loss_through_every_tile(case, dtype, _ways):
     N, D, V, gap, with_bias, room = case
     hidden, weight, tokens, bias = head(N, D, V, dtype, N + D + V)
     mask = torch.rand(N, generator=gen(1)) < 0.9

@@ -13,12 +13,8 @@ from tests import vocab_cases as vc
 pytestmark = pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="library not built (run python -m boundflow_amd.build)")
 
 
-@pytest.mark.parametrize("dtype", list(vc.ELEM))
-@pytest.mark.parametrize("case,narrow,wide", vc.CASES)
-def test_cases_take_the_ways_that_they_are_there_for(case, narrow, wide, dtype):
-    want = wide if dtype == torch.float32 else narrow
-    if want is None:
-        pytest.skip("for 16-bit types")
+@pytest.mark.parametrize("case,dtype,want", vc.RUNS)
+def test_cases_take_the_ways_that_they_are_there_for(case, dtype, want):
     pieces, logits, grads, *_ = vc.plan(*case, dtype)
     assert (logits, grads, pieces > 1) == want
 
@@ -27,8 +23,8 @@ def test_every_tile_is_taken_both_ways():
     """Logits formed once and formed again, in each tile that there is for a type."""
     for dtype in vc.ELEM:
         ways = set()
-        for case, narrow, wide in vc.CASES:
-            if (wide if dtype == torch.float32 else narrow) is not None:
+        for case, of, _ in vc.RUNS:
+            if of == dtype:
                 ways |= vc.kernels(case, dtype, True) | vc.kernels(case, dtype, False)
         tiles = ("large", "deep", "registers") if dtype == torch.float32 else ("large", "mid", "deep", "slim", "thin")
         for tile in tiles:
@@ -60,12 +56,10 @@ def test_no_kernel_is_compiled_that_no_call_reaches():
     assert sum(built.values()) == len(set(re.findall(
         r"\S*__device_stub__vocab_(?:logits|grads|softmax_columns)_kernel\S*", names))), "a name that was not understood"
     reached = set()
-    for dtype in vc.ELEM:
+    for case, dtype, _ in vc.RUNS:
         e = "DF16_" if dtype == torch.float16 else "DF16b"
-        for case, narrow, wide in vc.CASES:
-            if (wide if dtype == torch.float32 else narrow) is not None:
-                ways = vc.kernels(case, dtype, True) | vc.kernels(case, dtype, False)
-                reached |= {(what, mode, parts, e, tile) for what, mode, parts, tile in ways}
-                *_, parts, _, columns = vc.plan(*case, dtype)
-                reached |= {("columns", None, parts, e, None)} if columns else set()
+        ways = vc.kernels(case, dtype, True) | vc.kernels(case, dtype, False)
+        reached |= {(what, mode, parts, e, tile) for what, mode, parts, tile in ways}
+        *_, parts, _, columns = vc.plan(*case, dtype)
+        reached |= {("columns", None, parts, e, None)} if columns else set()
     assert collections.Counter(w[:4] for w in reached) == built

@@ -36,6 +36,10 @@ CASES = [
     ((7, 521, 700, 0, True, ROOM), ("thin", "thin", False), ("registers", "registers", False)),
 ]
 
+# (case, type, what it takes)
+RUNS = [(case, dtype, wide if dtype == torch.float32 else narrow) for case, narrow, wide in CASES for dtype in ELEM
+        if (wide if dtype == torch.float32 else narrow) is not None]
+
 
 def plan(N, D, V, gap, bias, room, dtype, with_grad=True, address=1 << 20):
     """(pieces, tile of the logits, tile of the gradients, parts of G, cuts of joined logits or 0, columns beside the softmax)"""
