@@ -425,14 +425,15 @@ def vocabulary_loss(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Te
     and log-probabilities alone: those that ``policy_loss`` and ``preference_loss`` take as an old or a reference policy's.
     The result comes without a graph: a hidden, weight or bias that requires grad is refused while gradients are recorded.
 
-    Products of 16-bit inputs are summed in fp32; between them the softmax's gradient is held in the inputs' type, up to 64 rows
-    (with a bias and a small vocabulary: more) in two parts of it, so with twice the digits; fp32 in 24 bits (of values
-    and gradients below 2^-103: what they have below 2^-126 counts as 0).  The bias's
-    gradient is summed before that rounding (of two parts: of both).  Where it has one part, exponentials wait with 11 bits for
-    their rows' sums, but for the token's own.  Rows that count and weights are finite (a bias may be -inf, and bars its token);
-    what is not shows as NaN.  Gradients' sums are scaled at their end: one that passes fp32's range before is infinite.  ``room`` bytes of that gradient (and of a copy of a weight whose rows cannot be read as they
-    lie) are held at a time, for as many tokens of the vocabulary as fit; the logits of the others are formed twice, which
-    takes up to a third longer.  The rows, their statistics and the gradients' sums take memory beside it."""
+    Products of 16-bit inputs are summed in fp32; between them the softmax's gradient is held in the inputs' type, up
+    to 64 rows (with a bias and a small vocabulary: more) in two parts of it, so with twice the digits; fp32 in 24
+    bits (of values and gradients below 2^-103: what they have below 2^-126 counts as 0).  The bias's gradient is
+    summed before that rounding (of two parts: of both).  Where it has one part, exponentials wait with 11 bits for
+    their rows' sums, but for the token's own.  Rows that count and weights are finite (a bias may be -inf, and bars
+    its token); what is not shows as NaN.  Gradients' sums are scaled at their end: one that passes fp32's range
+    before is infinite.  ``room`` bytes of that gradient (and of a copy of a weight whose rows cannot be read as they
+    lie) are held at a time, for as many tokens of the vocabulary as fit; the logits of the others are formed twice,
+    which takes up to a third longer.  The rows, their statistics and the gradients' sums take memory beside it."""
     if torch.is_grad_enabled():
         for t, name in ((hidden, "hidden"), (weight, "weight"), (bias, "bias")):
             if isinstance(t, torch.Tensor) and t.requires_grad:
